@@ -327,6 +327,92 @@ LDN_API int ldn_bound_inf_dist_forward_nograd_shifted(const float* inputL, const
                                                       float* outputU, const float* sub, const float* add,
                                                       ldn_stream_t stream);
 
+/* ---- a head behind the distance layers: layer norm, dropout, the product in 8-bit integers ------------------------- */
+/* None of these has a counterpart in the reference.  Activations are rows of C elements of one `type`; a pitch is the distance
+ * of two rows in elements, and rows that the library writes without a pitch are contiguous.  Pointers need the alignment of
+ * their elements only (16-byte aligned rows are faster). */
+#define LDN_F32 0
+#define LDN_F16 1
+#define LDN_BF16 2
+
+/*
+ * y = (x - mean) * rstd * weight + bias per row, rstd = 1 / sqrt(mean((x - mean)^2) + eps); weight and bias (either may be NULL)
+ * have C elements of param_type: LDN_F32, or the rows' type.  mean and rstd: `rows` floats each for the backward pass, or both
+ * NULL.  Statistics and all arithmetic have 32 bits; y is rounded once.
+ */
+LDN_API int ldn_layer_norm(const void* x, long long pitch, long long rows, int C, int type, const void* weight, const void* bias,
+                           int param_type, float eps, void* y, float* mean, float* rstd, ldn_stream_t stream);
+
+/*
+ * Gradients of ldn_layer_norm: with a = grad_y * weight and z = (x - mean) * rstd,
+ *   grad_x = rstd * (a - mean(a) - z * mean(a z)),  grad_weight = sum over rows of grad_y z,  grad_bias = sum over rows of grad_y.
+ * grad_y and grad_x are contiguous; any of the three results may be NULL; grad_weight and grad_bias have param_type.  The sums
+ * are taken in a fixed order (no atomics).  rows == 0 sets them to zero.
+ */
+LDN_API int ldn_layer_norm_backward(const void* grad_y, const void* x, long long pitch, long long rows, int C, int type,
+                                    const float* mean, const float* rstd, const void* weight, int param_type, void* grad_x,
+                                    void* grad_weight, void* grad_bias, ldn_stream_t stream);
+
+/*
+ * out = [residual +] (x / (1 - p) where element i = row * C + column is kept, else 0); out is contiguous, residual may be NULL.
+ * Element i is kept if word i % 4 of Philox4x32-10 with key `seed` and counter (i / 4, offset), low words first, is at least
+ * round(p * 2^32) (p = 1: never).  The mask is not stored: the gradient of x is the same call on the gradient of out.
+ * state: two 64-bit words on the device, a seed that is taken in place of `seed` and an offset that is added to `offset`
+ * (so that a recorded graph can draw another mask per replay), or NULL.
+ */
+LDN_API int ldn_dropout(const void* x, long long pitch, const void* residual, long long pitch_residual, long long rows, int C,
+                        int type, double p, unsigned long long seed, unsigned long long offset, const unsigned long long* state,
+                        void* out, ldn_stream_t stream);
+
+/*
+ * h = residual + dropout(x) as above, rounded to the rows' type, and y = layer norm of h, in one kernel.
+ */
+LDN_API int ldn_dropout_add_layer_norm(const void* x, long long pitch, const void* residual, long long pitch_residual,
+                                       long long rows, int C, int type, const void* weight, const void* bias, int param_type,
+                                       float eps, double p, unsigned long long seed, unsigned long long offset,
+                                       const unsigned long long* state, void* h, void* y, float* mean, float* rstd,
+                                       ldn_stream_t stream);
+
+/*
+ * Its gradients: grad_residual = grad_h (may be NULL: none) + the norm's gradient of h, grad_x = dropout of that before it is
+ * rounded.  All rows are contiguous; any result may be NULL.
+ */
+LDN_API int ldn_dropout_add_layer_norm_backward(const void* grad_y, const void* grad_h, const void* h, long long rows, int C,
+                                                int type, const float* mean, const float* rstd, const void* weight, int param_type,
+                                                double p, unsigned long long seed, unsigned long long offset,
+                                                const unsigned long long* state, void* grad_x, void* grad_residual,
+                                                void* grad_weight, void* grad_bias, ldn_stream_t stream);
+
+/*
+ * Rows as 8-bit integers: scale = max(largest |x| of the row / 127, 2^-126), q = round(x * (1 / scale)), ties to even, in 32-bit
+ * floating point.  A row with a value that is not finite gets a scale that is not, and integers whose products with it are
+ * not-a-number.
+ */
+LDN_API int ldn_quantize_rows(const void* x, long long pitch, long long rows, int C, int type, signed char* q, long long pitch_q,
+                              float* scale, ldn_stream_t stream);
+
+/* ldn_layer_norm whose rows leave as ldn_quantize_rows of y before it is rounded. */
+LDN_API int ldn_layer_norm_quantized(const void* x, long long pitch, long long rows, int C, int type, const void* weight,
+                                     const void* bias, int param_type, float eps, signed char* q, long long pitch_q, float* scale,
+                                     ldn_stream_t stream);
+
+#define LDN_NO_ACTIVATION 0
+#define LDN_RELU 1
+#define LDN_TANH 2
+
+/*
+ * out[m, n] = act((sum_k q[m, k] w[n, k]) * scale[m] * w_scale[n] + bias[n]) for M tokens, K terms (at most 131071) and N outputs;
+ * the sums are exact.  bias (N floats) may be NULL; out is contiguous, of `type`.
+ */
+LDN_API int ldn_int8_linear(const signed char* q, long long pitch_q, const float* scale, const signed char* w, long long pitch_w,
+                            const float* w_scale, const float* bias, long long M, int N, int K, int activation, void* out,
+                            int type, ldn_stream_t stream);
+
+/* The same behind ldn_quantize_rows of x (rows of K elements of x_type); the integers are scratch. */
+LDN_API int ldn_int8_linear_float(const void* x, long long pitch, int x_type, const signed char* w, long long pitch_w,
+                                  const float* w_scale, const float* bias, long long M, int N, int K, int activation, void* out,
+                                  int type, ldn_stream_t stream);
+
 /* ---- allocation-free variant ------------------------------------------------------------------ */
 
 /*

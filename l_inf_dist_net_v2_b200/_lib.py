@@ -14,6 +14,9 @@ _c_int_p = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
 _s = ctypes.c_void_p
+_p = ctypes.c_void_p
+_l = ctypes.c_longlong
+_u = ctypes.c_ulonglong
 
 # name -> argument types, exactly as declared in include/ldn_b200.h
 SIGNATURES = {
@@ -49,6 +52,15 @@ SIGNATURES = {
                                     ctypes.c_void_p, _f, _f, _f, _f, ctypes.c_void_p, _f, _s],
     "ldn_sgd_update": [_i, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                        _f, _f, _f, _f, _i, _i, _f, _s],
+    "ldn_layer_norm": [_p, _l, _l, _i, _i, _p, _p, _i, _f, _p, _p, _p, _s],
+    "ldn_layer_norm_backward": [_p, _p, _l, _l, _i, _i, _p, _p, _p, _i, _p, _p, _p, _s],
+    "ldn_dropout": [_p, _l, _p, _l, _l, _i, _i, ctypes.c_double, _u, _u, _p, _p, _s],
+    "ldn_dropout_add_layer_norm": [_p, _l, _p, _l, _l, _i, _i, _p, _p, _i, _f, ctypes.c_double, _u, _u, _p, _p, _p, _p, _p, _s],
+    "ldn_dropout_add_layer_norm_backward": [_p, _p, _p, _l, _i, _i, _p, _p, _p, _i, ctypes.c_double, _u, _u, _p, _p, _p, _p, _p, _s],
+    "ldn_quantize_rows": [_p, _l, _l, _i, _i, _p, _l, _p, _s],
+    "ldn_layer_norm_quantized": [_p, _l, _l, _i, _i, _p, _p, _i, _f, _p, _l, _p, _s],
+    "ldn_int8_linear": [_p, _l, _p, _p, _l, _p, _p, _l, _i, _i, _i, _p, _i, _s],
+    "ldn_int8_linear_float": [_p, _l, _i, _p, _l, _p, _p, _l, _i, _i, _i, _p, _i, _s],
     "ldn_check_status": [_s],
     "ldn_noalloc_check_status": [_s],
     "ldn_release_scratch": [],

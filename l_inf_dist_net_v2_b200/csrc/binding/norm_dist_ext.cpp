@@ -490,7 +490,10 @@ void check_status() { check(ldn_check_status(stream()), "device status check"); 
 
 }  // namespace
 
+void register_head(pybind11::module& m);  // head_ext.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    register_head(m);
     m.def("norm_dist_forward", &norm_dist_forward);
     m.def("norm_dist_forward_with_max", &norm_dist_forward_with_max);
     m.def("norm_dist_backward_input", &norm_dist_backward_input);
