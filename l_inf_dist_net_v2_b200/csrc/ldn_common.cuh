@@ -253,6 +253,10 @@ inline size_t pad256(size_t bytes) { return (bytes + 255) & ~size_t(255); }
 int make_tensor_map(CUtensorMap* map, const float* base, const unsigned long long dims[3],
                     const unsigned long long strides_elems[2], const unsigned box[3], bool swizzle128);
 
+// Tiled 2-D tensor map over rows of bytes that start at multiples of 16 bytes: boxes of 128 bytes x box_rows, 128-byte swizzle.
+int make_byte_map(CUtensorMap* map, const void* base, unsigned long long columns, unsigned long long rows, unsigned long long pitch,
+                  unsigned box_rows);
+
 // optional CUDA-event pair around the most recent tile-kernel launch (ldn_diag.cu); no-ops unless enabled
 void timing_before(cudaStream_t st);
 void timing_after(cudaStream_t st);

@@ -183,8 +183,7 @@ int release_arenas() {
     return kOk;
 }
 
-int make_tensor_map(CUtensorMap* map, const float* base, const unsigned long long dims[3],
-                    const unsigned long long strides_elems[2], const unsigned box[3], bool swizzle128) {
+static int find_encode() {
     if (!g_encode) {
         std::lock_guard<std::mutex> lock(g_mutex);
         if (!g_encode) {
@@ -195,6 +194,13 @@ int make_tensor_map(CUtensorMap* map, const float* base, const unsigned long lon
             g_encode = reinterpret_cast<EncodeTiledFn>(fn);
         }
     }
+    return kOk;
+}
+
+int make_tensor_map(CUtensorMap* map, const float* base, const unsigned long long dims[3],
+                    const unsigned long long strides_elems[2], const unsigned box[3], bool swizzle128) {
+    const int found = find_encode();
+    if (found != kOk) return found;
     cuuint64_t gdim[3] = {dims[0], dims[1], dims[2]};
     cuuint64_t gstr[2] = {strides_elems[0] * 4ull, strides_elems[1] * 4ull};
     cuuint32_t bdim[3] = {box[0], box[1], box[2]};
@@ -203,6 +209,18 @@ int make_tensor_map(CUtensorMap* map, const float* base, const unsigned long lon
                           CU_TENSOR_MAP_INTERLEAVE_NONE,
                           swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? kOk : kTensorMap;
+}
+
+int make_byte_map(CUtensorMap* map, const void* base, unsigned long long columns, unsigned long long rows, unsigned long long pitch,
+                  unsigned box_rows) {
+    const int found = find_encode();
+    if (found != kOk) return found;
+    cuuint64_t gdim[2] = {columns, rows}, gstr[1] = {pitch};
+    cuuint32_t bdim[2] = {128, box_rows}, estr[2] = {1, 1};
+    CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), gdim, gstr, bdim, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? kOk : kTensorMap;
 }
 

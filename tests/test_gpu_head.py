@@ -279,7 +279,7 @@ def _weight(N, K, seed):
 # one token; around the smallest tiles; around a tile of each kind; odd everything; lengths below 16 bytes; the longest sums
 SHAPES = [(1, 1, 1), (1, 5120, 5120), (1, 10, 512), (2, 33, 15), (3, 128, 128), (8, 257, 1000), (9, 96, 272), (16, 512, 5119), (17, 130, 127),
           (33, 1000, 784), (64, 512, 5120), (100, 10, 5120), (129, 129, 129), (200, 777, 1001), (257, 384, 640), (300, 2049, 333),
-          (512, 512, 2048), (1000, 5120, 160), (5, 40, 131071)]
+          (512, 512, 2048), (1000, 5120, 160), (5, 40, 131071), (3000, 1100, 333), (4000, 2700, 200)]
 
 
 @pytest.mark.parametrize("M, N, K", SHAPES)
