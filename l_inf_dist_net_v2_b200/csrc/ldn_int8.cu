@@ -2,32 +2,12 @@
 //     out[m, n] = act(sum_k q[m, k] w[n, k] * scale[m] * w_scale[n] + bias[n]),
 // the sums exact in 32-bit integers, the rest in 32-bit floating point; and rows as such integers.
 #include "ldn_int8.cuh"
+#include "ldn_norm.cuh"
 
 namespace ldn {
 namespace {
 
 constexpr int kMostTerms = 131071;  // 2^31 / 2^14: sums of products of two values of -128 .. 127 stay in 32 bits
-
-// A block per row: the largest magnitude, then the integers.
-template <class T>
-__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const void* x, long long pitch, long long rows, int C, signed char* q,
-                                                                 long long pitch_q, float* scale) {
-    stream_order_begin();
-    __shared__ unsigned all;
-    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-        const T* v = static_cast<const T*>(x) + row * pitch;
-        unsigned largest = 0;
-        for (int c = threadIdx.x; c < C; c += kThreads) largest = max(largest, magnitude(to_float(v[c])));
-        __syncthreads();
-        if (threadIdx.x == 0) all = 0;
-        __syncthreads();
-        atomicMax(&all, largest);
-        __syncthreads();
-        const float step = step_of(all), inverse = __frcp_rn(step);
-        for (int c = threadIdx.x; c < C; c += kThreads) q[row * pitch_q + c] = static_cast<signed char>(steps(to_float(v[c]), inverse));
-        if (threadIdx.x == 0) scale[row] = step;
-    }
-}
 
 // Rows of bytes that start anywhere as rows that start at multiples of 16 bytes
 __global__ void __launch_bounds__(kThreads) align_rows_kernel(const signed char* from, long long pitch, long long rows, int C,
@@ -38,13 +18,11 @@ __global__ void __launch_bounds__(kThreads) align_rows_kernel(const signed char*
 }
 
 int launch_quantize(const void* x, long long pitch, long long rows, int C, int type, signed char* q, long long pitch_q, float* scale,
-                    const DeviceCtx* ctx, cudaStream_t st) {
-    return with_type(type, [&](auto t) {
-        using T = decltype(t);
-        const long long most = 32LL * ctx->sm_count;
-        return launch_after(quantize_rows_kernel<T>, static_cast<unsigned>(rows < most ? rows : most), kThreads, 0, st, x, pitch, rows,
-                            C, q, pitch_q, scale);
-    });
+                    cudaStream_t st) {
+    NormArgs a = {};
+    a.x = x; a.pitch = pitch; a.rows = rows; a.C = C;
+    a.q = q; a.pitch_q = pitch_q; a.scale = scale;
+    return norm_forward<Form::Quantised>(a, type, st);
 }
 
 long long padded16(long long bytes) { return (bytes + 15) / 16 * 16; }
@@ -93,10 +71,7 @@ extern "C" LDN_API int ldn_quantize_rows(const void* x, long long pitch, long lo
     if (rows < 0 || C <= 0 || !known_type(type) || pitch_q < C) return kBadArgument;
     if (rows == 0) return kOk;
     if (!x || !q || !scale) return kBadArgument;
-    const DeviceCtx* ctx;
-    const int r = get_device_ctx(&ctx);
-    if (r != kOk) return r;
-    return launch_quantize(x, pitch, rows, C, type, q, pitch_q, scale, ctx, reinterpret_cast<cudaStream_t>(stream));
+    return launch_quantize(x, pitch, rows, C, type, q, pitch_q, scale, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" LDN_API int ldn_int8_linear(const signed char* q, long long pitch_q, const float* scale, const signed char* w,
@@ -134,7 +109,7 @@ extern "C" LDN_API int ldn_int8_linear_float(const void* x, long long pitch, int
     if ((r = scratch.take(st, bytes_q + bytes_scale + o.bytes_w)) != kOk) return r;
     signed char* q = reinterpret_cast<signed char*>(scratch.base);
     float* scale = reinterpret_cast<float*>(scratch.base + bytes_q);
-    if ((r = launch_quantize(x, pitch, M, K, x_type, q, pitch_q, scale, ctx, st)) != kOk) return r;
+    if ((r = launch_quantize(x, pitch, M, K, x_type, q, pitch_q, scale, st)) != kOk) return r;
     a.q = q;
     a.scale = scale;
     return launch_product(a, type, o, scratch.base + bytes_q + bytes_scale, scratch.status, ctx, st);

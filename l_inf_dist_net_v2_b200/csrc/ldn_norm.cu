@@ -5,28 +5,10 @@
 // Statistics are those of two passes (the mean first, then the squares of what is left), in 32 bits: rows with a large mean lose
 // nothing.  h is held in the type of the activations, and what is held is what is normalised, so the backward pass sees the
 // numbers that the forward pass used.
-#include "ldn_head.cuh"
+#include "ldn_norm.cuh"
 
 namespace ldn {
 namespace {
-
-struct NormArgs {
-    const void* x;
-    const void* residual;  // joined form only
-    long long pitch, pitch_residual, rows;
-    int C;
-    const void *weight, *bias;  // may be null
-    bool wide;                  // they have 32 bits
-    float eps;
-    DropoutArgs drop;
-    void *h, *y;
-    float *mean, *rstd;  // may be null
-    signed char* q;      // integer form only
-    long long pitch_q;
-    float* scale;
-};
-
-enum class Form { Plain, Joined, Integers };
 
 constexpr int kRowThreads = 256;
 
@@ -52,23 +34,27 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows_kernel(NormArgs a) {
             sum += v;
         }
         if constexpr (F == Form::Joined) x = static_cast<const T*>(a.h) + at;  // (a thread reads back what it wrote)
-        const float mean = block_sum(sum, slots) / a.C;
-        float squares = 0.0f;
-        for (int c = threadIdx.x; c < a.C; c += kRowThreads) {
-            const float d = to_float(x[c]) - mean;
-            squares += d * d;
+        float mean = 0.0f, rstd = 0.0f;
+        if constexpr (F != Form::Quantised) {
+            mean = block_sum(sum, slots) / a.C;
+            float squares = 0.0f;
+            for (int c = threadIdx.x; c < a.C; c += kRowThreads) {
+                const float d = to_float(x[c]) - mean;
+                squares += d * d;
+            }
+            rstd = 1.0f / sqrtf(block_sum(squares, slots) / a.C + a.eps);
         }
-        const float rstd = 1.0f / sqrtf(block_sum(squares, slots) / a.C + a.eps);
         if (threadIdx.x == 0 && a.mean) {
             a.mean[row] = mean;
             a.rstd[row] = rstd;
         }
         auto normed = [&](int c) {
+            if (F == Form::Quantised) return to_float(x[c]);
             float v = (to_float(x[c]) - mean) * rstd;
             if (a.weight) v *= param_at<T>(a.weight, a.wide, c);
             return a.bias ? v + param_at<T>(a.bias, a.wide, c) : v;
         };
-        if constexpr (F == Form::Integers) {
+        if constexpr (F == Form::Integers || F == Form::Quantised) {
             unsigned largest = 0;
             for (int c = threadIdx.x; c < a.C; c += kRowThreads) largest = max(largest, magnitude(normed(c)));
             __shared__ unsigned all;
@@ -86,21 +72,6 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows_kernel(NormArgs a) {
         }
     }
 }
-
-struct NormGradArgs {
-    const void* grad_y;  // rows of C
-    const void* grad_h;  // joined form only, may be null
-    const void* x;       // what was normalised
-    long long pitch, rows;
-    int C;
-    const float *mean, *rstd;
-    const void* weight;
-    bool wide;
-    DropoutArgs drop;
-    void* grad_x;         // may be null
-    void* grad_residual;  // joined form only: the gradient of h; may be null
-    float* parts;         // [block of rows][2][C]: sums for the weight and the bias
-};
 
 // a = grad_y * weight, z = (x - mean) rstd:  grad_x = rstd (a - mean(a) - z mean(a z))
 template <class T, bool JOINED>
@@ -161,41 +132,48 @@ __global__ void __launch_bounds__(kColumns * kColumnLanes) norm_grad_columns_ker
     }
 }
 
-// The parts in order: a thread has a column of one of the two sums and every eighth part.
+// The parts in order: a thread has a column of one of the two sums and every 32nd part.
+constexpr int kFoldLanes = 32;
 template <class T>
-__global__ void __launch_bounds__(kColumns * kColumnLanes) norm_grad_fold_kernel(const float* parts, int count, int C, bool wide,
-                                                                                 void* grad_weight, void* grad_bias) {
+__global__ void __launch_bounds__(kColumns * kFoldLanes) norm_grad_fold_kernel(const float* parts, int count, int C, bool wide,
+                                                                               void* grad_weight, void* grad_bias) {
     stream_order_begin();
-    __shared__ float sums[kColumnLanes][kColumns];
+    __shared__ float sums[kFoldLanes][kColumns + 1];
     const int lane = threadIdx.x % kColumns, part = threadIdx.x / kColumns, c = blockIdx.x * kColumns + lane;
     float s = 0.0f;
     if (c < C)
-        for (int i = part; i < count; i += kColumnLanes) s += parts[(static_cast<long long>(i) * 2 + blockIdx.y) * C + c];
+#pragma unroll 4
+        for (int i = part; i < count; i += kFoldLanes) s += parts[(static_cast<long long>(i) * 2 + blockIdx.y) * C + c];
     sums[part][lane] = s;
     __syncthreads();
+    // a warp adds up a column's sums
+    s = warp_sum(sums[lane][part]);
     void* to = blockIdx.y == 0 ? grad_weight : grad_bias;
-    if (part == 0 && c < C && to) {
-        s = 0.0f;
-        for (int i = 0; i < kColumnLanes; ++i) s += sums[i][lane];
-        set_param<T>(to, wide, c, s);
-    }
+    if (lane == 0 && blockIdx.x * kColumns + part < C && to) set_param<T>(to, wide, blockIdx.x * kColumns + part, s);
 }
 
 bool params_fit(int type, int param_type, const void* weight, const void* bias) {
     return (!weight && !bias) || param_type == LDN_F32 || param_type == type;
 }
 
+}  // namespace
+
 template <Form F>
 int norm_forward(const NormArgs& a, int type, cudaStream_t st) {
     const DeviceCtx* ctx;
-    const int r = get_device_ctx(&ctx);
+    int r = get_device_ctx(&ctx);
     if (r != kOk) return r;
+    if (norm_in_registers(F, a, type, ctx, st, &r)) return r;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         const long long most = 32LL * ctx->sm_count;
         return launch_after(norm_rows_kernel<T, F>, static_cast<unsigned>(a.rows < most ? a.rows : most), kRowThreads, 0, st, a);
     });
 }
+
+template int norm_forward<Form::Quantised>(const NormArgs& a, int type, cudaStream_t st);
+
+namespace {
 
 int zero_param(void* p, bool wide, int type, int C, cudaStream_t st) {
     return p ? cuda_status(cudaMemsetAsync(p, 0, static_cast<size_t>(C) * (wide ? 4 : size_of(type)), st)) : kOk;
@@ -211,27 +189,34 @@ int norm_backward(NormGradArgs a, int type, void* grad_weight, void* grad_bias, 
         return r == kOk ? zero_param(grad_bias, a.wide, type, a.C, st) : r;
     }
     const int columns = (a.C + kColumns - 1) / kColumns;
-    long long blocks = (4LL * ctx->sm_count + columns - 1) / columns;
-    if (blocks > (a.rows + 63) / 64) blocks = (a.rows + 63) / 64;
-    Scratch scratch;
     const bool sums = grad_weight || grad_bias;
+    int blocks = 0;
+    const bool registers = norm_grad_in_registers(JOINED, a, type, ctx, &blocks);
+    if (!registers) {
+        const long long most = (4LL * ctx->sm_count + columns - 1) / columns, needed = (a.rows + 63) / 64;
+        blocks = static_cast<int>(most < needed ? most : needed);
+    }
+    Scratch scratch;
     if (sums) {
         r = scratch.take(st, static_cast<size_t>(blocks) * 2 * a.C * sizeof(float));
         if (r != kOk) return r;
         a.parts = reinterpret_cast<float*>(scratch.base);
     }
+    if (registers) r = launch_norm_grad_in_registers(JOINED, a, type, ctx, st);
+    if (r != kOk) return r;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         const long long most = 32LL * ctx->sm_count;
         int r = kOk;
-        if (a.grad_x || a.grad_residual)
+        if (!registers && (a.grad_x || a.grad_residual))
             r = launch_after(norm_grad_rows_kernel<T, JOINED>, static_cast<unsigned>(a.rows < most ? a.rows : most), kRowThreads, 0,
                              st, a);
         if (!sums || r != kOk) return r;
-        r = launch_after(norm_grad_columns_kernel<T>, dim3(columns, static_cast<unsigned>(blocks)), kColumns * kColumnLanes, 0, st, a);
+        if (!registers)
+            r = launch_after(norm_grad_columns_kernel<T>, dim3(columns, static_cast<unsigned>(blocks)), kColumns * kColumnLanes, 0, st, a);
         if (r != kOk) return r;
-        return launch_after(norm_grad_fold_kernel<T>, dim3(columns, 2), kColumns * kColumnLanes, 0, st, a.parts,
-                            static_cast<int>(blocks), a.C, a.wide, grad_weight, grad_bias);
+        return launch_after(norm_grad_fold_kernel<T>, dim3(columns, 2), kColumns * kFoldLanes, 0, st, a.parts, blocks, a.C, a.wide,
+                            grad_weight, grad_bias);
     });
 }
 
