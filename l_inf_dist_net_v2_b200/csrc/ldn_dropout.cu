@@ -1,6 +1,6 @@
 // Dropout with a counter-based generator: out = [residual +] (x / (1 - p) where its word says so, else 0).  No mask is stored;
 // the backward pass is the same kernel on the gradient with the same seed and offset.
-#include "ldn_head.cuh"
+#include "ldn_rows.cuh"
 
 namespace ldn {
 namespace {
@@ -13,7 +13,47 @@ struct DropoutCall {
     void* out;
 };
 
-// A thread has the four elements of a block of words, wherever the rows break.
+// Contiguous tensors that start at multiples of 16 bytes: 16-byte pieces, the next one under way while a thread has this one's words
+// made.
+template <class T, bool ONTO>
+__global__ void __launch_bounds__(kThreads) dropout_pieces_kernel(DropoutCall a, long long n) {
+    stream_order_begin();
+    constexpr int V = kPiece<T>;
+    const Generator gen = generator_of(a.drop);
+    const T *x = static_cast<const T*>(a.x), *onto = static_cast<const T*>(a.residual);
+    T* out = static_cast<T*>(a.out);
+    const long long pieces = n / V, step = static_cast<long long>(gridDim.x) * kThreads;
+    long long piece = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
+    uint4 next = make_uint4(0u, 0u, 0u, 0u), next_onto = next;
+    auto fetch = [&](long long i) {
+        if (i < pieces) {
+            next = *reinterpret_cast<const uint4*>(x + i * V);
+            if (ONTO) next_onto = *reinterpret_cast<const uint4*>(onto + i * V);
+        }
+    };
+    fetch(piece);
+    for (; piece < pieces; piece += step) {
+        const uint4 raw = next, raw_onto = next_onto;
+        fetch(piece + step);
+        float v[V], r[V];
+        unpack<T>(raw, v);
+        if (ONTO) unpack<T>(raw_onto, r);
+        drop_piece<V>(a.drop, gen, piece * V, v);
+        if (ONTO)
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = __fadd_rn(r[e], v[e]);
+        *reinterpret_cast<uint4*>(out + piece * V) = pack<T>(v);
+    }
+    // what is left behind the last whole piece
+    const long long i = pieces * V + threadIdx.x;
+    if (blockIdx.x == 0 && i < n) {
+        float v = dropped(a.drop, random_word(gen, i), to_float(x[i]));
+        if (ONTO) v = __fadd_rn(to_float(onto[i]), v);
+        out[i] = from_float<T>(v);
+    }
+}
+
+// Any pitch and alignment: a thread has the four elements of a block of words, wherever the rows break.
 template <class T>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(DropoutCall a) {
     stream_order_begin();
@@ -58,6 +98,14 @@ extern "C" LDN_API int ldn_dropout(const void* x, long long pitch, const void* r
     a.x = x; a.pitch = pitch; a.residual = residual; a.pitch_residual = pitch_residual; a.rows = rows; a.C = C; a.out = out;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
+        const long long n = rows * C;
+        if (pitch == C && (!residual || pitch_residual == C) && on16(x) && on16(residual) && on16(out)) {
+            const long long blocks = (n / kPiece<T> + kThreads - 1) / kThreads + (n < kPiece<T>), most = 6LL * ctx->sm_count;
+            const unsigned grid = static_cast<unsigned>(blocks < most ? blocks : most);
+            const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+            return residual ? launch_after(dropout_pieces_kernel<T, true>, grid, kThreads, 0, st, a, n)
+                            : launch_after(dropout_pieces_kernel<T, false>, grid, kThreads, 0, st, a, n);
+        }
         const long long blocks = ((rows * C + 3) / 4 + kThreads - 1) / kThreads, most = 32LL * ctx->sm_count;
         return launch_after(dropout_kernel<T>, static_cast<unsigned>(blocks < most ? blocks : most), kThreads, 0,
                             reinterpret_cast<cudaStream_t>(stream), a);
