@@ -35,13 +35,13 @@ __global__ void __launch_bounds__(kThreads) dropout_pieces_kernel(DropoutCall a,
     for (; piece < pieces; piece += step) {
         const uint4 raw = next, raw_onto = next_onto;
         fetch(piece + step);
-        float v[V], r[V];
+        float2 v[V / 2], r[V / 2];
         unpack<T>(raw, v);
         if (ONTO) unpack<T>(raw_onto, r);
-        drop_piece<V>(a.drop, gen, piece * V, v);
+        drop_piece(a.drop, gen, piece * V, v);
         if (ONTO)
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = __fadd_rn(r[e], v[e]);
+            for (int e = 0; e < V / 2; ++e) v[e] = __fadd2_rn(r[e], v[e]);
         *reinterpret_cast<uint4*>(out + piece * V) = pack<T>(v);
     }
     // what is left behind the last whole piece

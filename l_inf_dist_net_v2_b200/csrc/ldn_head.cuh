@@ -169,16 +169,14 @@ __device__ __forceinline__ float dropped(const DropoutArgs& d, unsigned word, fl
     return word >= d.threshold && !d.all ? __fmul_rn(v, d.scale) : 0.0f;
 }
 
-// The same for N neighbouring elements from `at` on, a multiple of four (N is one, too)
+// The same for 2 N neighbouring elements from `at` on, a multiple of four (2 N is one, too)
 template <int N>
-__device__ __forceinline__ void drop_piece(const DropoutArgs& d, const Generator& gen, long long at, float (&v)[N]) {
+__device__ __forceinline__ void drop_piece(const DropoutArgs& d, const Generator& gen, long long at, float2 (&v)[N]) {
 #pragma unroll
-    for (int e = 0; e < N; e += 4) {
-        const uint4 w = random_words(gen, static_cast<unsigned long long>(at + e) >> 2);
-        v[e] = dropped(d, w.x, v[e]);
-        v[e + 1] = dropped(d, w.y, v[e + 1]);
-        v[e + 2] = dropped(d, w.z, v[e + 2]);
-        v[e + 3] = dropped(d, w.w, v[e + 3]);
+    for (int e = 0; e < N; e += 2) {
+        const uint4 w = random_words(gen, static_cast<unsigned long long>(at + 2 * e) >> 2);
+        v[e] = make_float2(dropped(d, w.x, v[e].x), dropped(d, w.y, v[e].y));
+        v[e + 1] = make_float2(dropped(d, w.z, v[e + 1].x), dropped(d, w.w, v[e + 1].y));
     }
 }
 
@@ -203,13 +201,41 @@ __device__ __forceinline__ float block_sum(float v, float* slots) {
 // The bits of |v|: their order is that of the magnitudes, with infinity above all numbers and what is not a number above that.
 __device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 // A row's step: its largest magnitude is 127 steps, and no step is below the smallest normal number, so that its reciprocal is
-// finite; a row with a value that is not finite has such a step, and all its products are not-a-number.
+// finite; a row with a value that is not finite has a step that is not a number, and so are all its products
 __device__ __forceinline__ float step_of(unsigned largest) {
+    if (largest >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
     const float s = __fdiv_rn(__uint_as_float(largest), 127.0f);
     return s < 1.17549435e-38f ? 1.17549435e-38f : s;
 }
-// The nearest integer number of steps, ties to even: |v| <= 127 step (1 + 2^-24), so it has 8 bits; 0 for what is not a number
+// The nearest integer number of steps, ties to even: |v| <= 127 step (1 + 2^-24), so it has 8 bits (any 8 for what is not a number)
 __device__ __forceinline__ int steps(float v, float inverse) { return __float2int_rn(__fmul_rn(v, inverse)); }
+// The product of two values with one, rounded (the compiler's packed product may join an addition behind it)
+__device__ __forceinline__ float2 rounded_product(float2 v, float s) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmul.rn.f32x2 c, a, b;\n\tmov.b64 {%0, %1}, c;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(v.x), "f"(v.y), "f"(s));
+    return r;
+}
+// The same of four values as bytes: 1.5 2^23 more, the nearest integer is what a number's last bits hold
+__device__ __forceinline__ unsigned steps4(float2 a, float2 b, float inverse) {
+    a = rounded_product(a, inverse);
+    b = rounded_product(b, inverse);
+    constexpr float kMagic = 12582912.0f;
+    return __byte_perm(__byte_perm(__float_as_uint(__fadd_rn(a.x, kMagic)), __float_as_uint(__fadd_rn(a.y, kMagic)), 0x0040),
+                       __byte_perm(__float_as_uint(__fadd_rn(b.x, kMagic)), __float_as_uint(__fadd_rn(b.y, kMagic)), 0x0040), 0x5410);
+}
+// Largest of two magnitudes, or of one and two values' magnitudes; what is not a number wins
+__device__ __forceinline__ float larger(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float larger(float top, float2 v) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(top), "f"(fabsf(v.x)), "f"(fabsf(v.y)));
+    return r;
+}
 #endif  // __CUDACC__
 
 }  // namespace ldn

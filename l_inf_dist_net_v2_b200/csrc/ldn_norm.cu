@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kColumns * kColumnLanes) norm_grad_columns_ker
     }
 }
 
-// The parts in order: a thread has a column of one of the two sums and every 32nd part.
+// The parts in order: a thread has a column of one of the two sums and every 32nd part, eight of them under way.
 constexpr int kFoldLanes = 32;
 template <class T>
 __global__ void __launch_bounds__(kColumns * kFoldLanes) norm_grad_fold_kernel(const float* parts, int count, int C, bool wide,
@@ -140,10 +140,19 @@ __global__ void __launch_bounds__(kColumns * kFoldLanes) norm_grad_fold_kernel(c
     stream_order_begin();
     __shared__ float sums[kFoldLanes][kColumns + 1];
     const int lane = threadIdx.x % kColumns, part = threadIdx.x / kColumns, c = blockIdx.x * kColumns + lane;
+    const float* from = parts + static_cast<long long>(blockIdx.y) * C + c;
     float s = 0.0f;
     if (c < C)
-#pragma unroll 4
-        for (int i = part; i < count; i += kFoldLanes) s += parts[(static_cast<long long>(i) * 2 + blockIdx.y) * C + c];
+        for (int i = part; i < count; i += 8 * kFoldLanes) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int k = i + u * kFoldLanes;
+                v[u] = k < count ? from[2LL * k * C] : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
     sums[part][lane] = s;
     __syncthreads();
     // a warp adds up a column's sums

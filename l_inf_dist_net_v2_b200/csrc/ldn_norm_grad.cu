@@ -1,26 +1,35 @@
-// Layer norm's gradient with the row in registers: one read of x and of the incoming gradients, both sums over a row at once, and
-// the column sums for the weight and the bias carried in the threads that have those columns, from row to row.
+// Layer norm's gradient with the row on the SM: one read of x and of the incoming gradients, both sums over a row at once, and the
+// column sums for the weight and the bias carried in the threads that have those columns, from row to row.
 //
 // A block takes every gridDim-th row, so its threads' columns stay (rows that start anywhere in 16 bytes: the grid is a multiple of
-// eight, and rows that far apart start alike).  The next row is under way while this one is summed.  Bound by memory: x, the incoming
-// and the outgoing gradients once.
+// eight, and rows that far apart start alike).  Rows are under way into shared memory while others are summed, as in the forward
+// pass, and are read there twice: in front of the sums and behind them.  Bound by memory: x, the incoming and the outgoing gradients
+// once; joined, also by the words of the dropout.
 #include "ldn_norm.cuh"
 #include "ldn_rows.cuh"
 
 namespace ldn {
 namespace {
 
-// 16 elements per thread, whose 32 column sums stay in registers: rows of up to 8192
-constexpr int kMostThreads = 512;
-template <class T>
-constexpr int kMostItems = 16 / kPiece<T>;
+// Rows that a block takes at a time, so that their sums share their barriers
+__host__ __device__ constexpr int rows_at_once(bool joined, int elements, bool group) {
+    return group || elements > 16 ? 1 : elements > 8 || joined ? 2 : 4;
+}
+template <bool JOINED>
+constexpr int kStreams = JOINED ? 3 : 2;
+
+template <int N>
+__device__ __forceinline__ float at_of(const float2 (&v)[N], int e) {
+    return e % 2 ? v[e / 2].y : v[e / 2].x;
+}
 
 template <class T, bool JOINED, int ITEMS, bool GROUP, bool SHIFT>
-__global__ void __launch_bounds__(GROUP ? kGroupThreads : kMostThreads) norm_grad_registers_kernel(NormGradArgs a, int lanes) {
+__global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPiece<T>), !GROUP && ITEMS * kPiece<T> == 16 ? 2 : 1) norm_grad_registers_kernel(NormGradArgs a, int lanes, int depth) {
     stream_order_begin();
-    constexpr int V = kPiece<T>;
-    __shared__ float slots[128];
-    extern __shared__ float columns[];  // groups: [warp][2][C]
+    constexpr int V = kPiece<T>, S = kStreams<JOINED>, R = rows_at_once(JOINED, ITEMS * V, GROUP);
+    constexpr bool kKeep = ITEMS * V <= 16;  // the columns' weights stay in registers, too
+    __shared__ float slots[2 * RowSum::kSlots];
+    extern __shared__ uint4 ring[];  // [depth][row][stream][item][thread]; at the end, groups: [warp][2][C] floats
     RowSum reduce{lanes, slots, 0};
     Generator gen;
     if constexpr (JOINED) gen = generator_of(a.drop);
@@ -31,97 +40,113 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : kMostThreads) norm_gra
     const float inv_C = 1.0f / a.C;
     // (the same for all rows of this thread)
     const int shift = SHIFT ? shift_of(static_cast<const T*>(a.x) + (mine < a.rows ? mine : 0) * a.pitch) : 0;
-    float sum_w[ITEMS][V], sum_b[ITEMS][V];
+    auto column = [&](int i) { return (lane + i * lanes) * V - shift; };
+    float2 sum_w[ITEMS][V / 2], sum_b[ITEMS][V / 2], w[ITEMS][V / 2];
+    uint4 mask[ITEMS];
+    int bytes[ITEMS];
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
+    for (int i = 0; i < ITEMS; ++i) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) sum_w[i][e] = sum_b[i][e] = 0.0f;
-
-    uint4 next_x[ITEMS], next_g[ITEMS];
-    float next_mean = 0.0f, next_rstd = 0.0f;
-    auto fetch = [&](long long row) {
-        const bool live = row < a.rows;
-        const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.pitch;
-        const T* g = static_cast<const T*>(a.grad_y) + (live ? row : 0) * a.C;
-        const int C = live ? a.C : 0;
+        for (int e = 0; e < V / 2; ++e) sum_w[i][e] = sum_b[i][e] = both(0.0f);
+        mask[i] = mask_of<T, SHIFT>(column(i), a.C);
+        bytes[i] = piece_bytes<T>(column(i), a.C);
+        if constexpr (kKeep) load_params<T, SHIFT>(a.weight, a.wide, column(i), a.C, 1.0f, w[i]);
+    }
+    uint4* own = ring + threadIdx.x;
+    auto slot_of = [&](int stage, int j, int stream, int i) { return own + (((stage * R + j) * S + stream) * ITEMS + i) * blockDim.x; };
+    auto fetch = [&](long long row, int stage) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            next_x[i] = load_piece<T, SHIFT>(x, (lane + i * lanes) * V - shift, C);
-            next_g[i] = load_piece<T, SHIFT>(g, (lane + i * lanes) * V - shift, C);
-        }
-        next_mean = live ? a.mean[row] : 0.0f;
-        next_rstd = live ? a.rstd[row] : 0.0f;
-    };
-    fetch(mine);
-    // (a warp's groups take part in its shuffles whether they have a row or not)
-    for (long long first = static_cast<long long>(blockIdx.x) * per_block; first < a.rows; first += step) {
-        const long long row = GROUP ? first + threadIdx.x / lanes : first;
-        const bool live = !GROUP || row < a.rows;
-        const long long at = (live ? row : 0) * a.C;
-        const int C = live ? a.C : 0;
-        uint4 x[ITEMS], g[ITEMS], more[ITEMS];
-        const float mean = next_mean, rstd = next_rstd;
+        for (int j = 0; j < R; ++j, row += step)
+            if (row < a.rows) {
+                const T *x = static_cast<const T*>(a.x) + row * a.pitch, *g = static_cast<const T*>(a.grad_y) + row * a.C;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            x[i] = next_x[i];
-            g[i] = next_g[i];
-        }
-        if constexpr (JOINED) {
-            if (a.grad_h)
-#pragma unroll
-                for (int i = 0; i < ITEMS; ++i)
-                    more[i] = load_piece<T, SHIFT>(static_cast<const T*>(a.grad_h) + at, (lane + i * lanes) * V - shift, C);
-        }
-        fetch(row + step);
-        float s[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int c0 = (lane + i * lanes) * V - shift;
-            float vx[V], vg[V], w[V];
-            unpack<T>(x[i], vx);
-            unpack<T>(g[i], vg);
-            load_params<T, SHIFT>(a.weight, a.wide, c0, C, 1.0f, w);
-#pragma unroll
-            for (int e = 0; e < V; ++e) {  // (outside the row the gradient is 0)
-                const float z = (vx[e] - mean) * rstd;
-                sum_w[i][e] = fmaf(vg[e], z, sum_w[i][e]);
-                sum_b[i][e] += vg[e];
-                const float p = vg[e] * w[e];
-                s[0] += p;
-                s[1] = fmaf(p, z, s[1]);
-            }
-        }
-        reduce.template sum<2, GROUP>(s);
-        const float m1 = s[0] * inv_C, m2 = s[1] * inv_C;
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int c0 = (lane + i * lanes) * V - shift;
-            float vx[V], vg[V], w[V];
-            unpack<T>(x[i], vx);
-            unpack<T>(g[i], vg);
-            load_params<T, SHIFT>(a.weight, a.wide, c0, C, 1.0f, w);
-#pragma unroll
-            for (int e = 0; e < V; ++e) vg[e] = rstd * (vg[e] * w[e] - m1 - (vx[e] - mean) * rstd * m2);
-            if constexpr (JOINED) {
-                if (a.grad_h) {
-                    float vh[V];
-                    unpack<T>(more[i], vh);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) vg[e] += vh[e];
+                for (int i = 0; i < ITEMS; ++i) {
+                    copy_piece<T, SHIFT>(slot_of(stage, j, 0, i), x, column(i), bytes[i], row == 0);
+                    copy_piece<T, SHIFT>(slot_of(stage, j, 1, i), g, column(i), bytes[i], row == 0);
+                    if constexpr (JOINED)
+                        if (a.grad_h)
+                            copy_piece<T, SHIFT>(slot_of(stage, j, 2, i), static_cast<const T*>(a.grad_h) + row * a.C, column(i), bytes[i], row == 0);
                 }
-                if (a.grad_residual) store_piece<T, SHIFT>(static_cast<T*>(a.grad_residual) + at, c0, C, pack<T>(vg));
-                if (a.grad_x)
-#pragma unroll
-                    for (int e = 0; e < V; e += 4) {  // (pieces start at multiples of four elements of the whole tensor)
-                        const uint4 r = random_words(gen, static_cast<unsigned long long>(at + c0 + e) >> 2);
-                        vg[e] = dropped(a.drop, r.x, vg[e]);
-                        vg[e + 1] = dropped(a.drop, r.y, vg[e + 1]);
-                        vg[e + 2] = dropped(a.drop, r.z, vg[e + 2]);
-                        vg[e + 3] = dropped(a.drop, r.w, vg[e + 3]);
-                    }
             }
-            if (a.grad_x) store_piece<T, SHIFT>(static_cast<T*>(a.grad_x) + at, c0, C, pack<T>(vg));
+        copies_commit();
+    };
+    for (int d = 0; d < depth * R * S; ++d)
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (!bytes[i]) own[(d * ITEMS + i) * blockDim.x] = make_uint4(0u, 0u, 0u, 0u);
+    for (int d = 0; d < depth; ++d) fetch(mine + d * R * step, d);
+    int stage = 0;
+    // (a warp's groups take part in its shuffles whether they have a row or not)
+    for (long long first = static_cast<long long>(blockIdx.x) * per_block; first < a.rows; first += R * step) {
+        const long long row0 = GROUP ? first + threadIdx.x / lanes : first;
+        auto live = [&](int j) { return row0 + j * step < a.rows; };
+        float mean[R], rstd[R], s[2 * R];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            mean[j] = live(j) ? a.mean[row0 + j * step] : 0.0f;
+            rstd[j] = live(j) ? a.rstd[row0 + j * step] : 0.0f;
         }
+        copies_wait(depth);
+        // (outside the row the gradient is 0, and x a number; where there is no row, all is 0)
+        auto piece_of = [&](int j, int stream, int i) {
+            uint4 raw = live(j) ? *slot_of(stage, j, stream, i) : make_uint4(0u, 0u, 0u, 0u);
+            return SHIFT ? masked(raw, mask[i]) : raw;
+        };
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            float2 s0 = both(0.0f), s1 = both(0.0f);
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                float2 vx[V / 2], vg[V / 2];
+                unpack<T>(piece_of(j, 0, i), vx);
+                unpack<T>(piece_of(j, 1, i), vg);
+                if constexpr (!kKeep) load_params<T, SHIFT>(a.weight, a.wide, column(i), a.C, 1.0f, w[i]);
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) {
+                    const float2 z = __fmul2_rn(__fadd2_rn(vx[e], both(-mean[j])), both(rstd[j]));
+                    sum_w[i][e] = __ffma2_rn(vg[e], z, sum_w[i][e]);
+                    sum_b[i][e] = __fadd2_rn(sum_b[i][e], vg[e]);
+                    const float2 p = __fmul2_rn(vg[e], w[i][e]);
+                    s0 = __fadd2_rn(s0, p);
+                    s1 = __ffma2_rn(p, z, s1);
+                }
+            }
+            s[2 * j] = s0.x + s0.y;
+            s[2 * j + 1] = s1.x + s1.y;
+        }
+        reduce.template sum<GROUP>(s, [&](float all) { return all * inv_C; });
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            if (!live(j)) continue;
+            const long long at = (row0 + j * step) * a.C;
+            const float m1 = s[2 * j], m2 = s[2 * j + 1] * rstd[j];
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int c0 = column(i);
+                float2 vx[V / 2], vg[V / 2];
+                unpack<T>(piece_of(j, 0, i), vx);
+                unpack<T>(piece_of(j, 1, i), vg);
+                if constexpr (!kKeep) load_params<T, SHIFT>(a.weight, a.wide, c0, a.C, 1.0f, w[i]);
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) {
+                    const float2 p = __ffma2_rn(vg[e], w[i][e], both(-m1));
+                    vg[e] = __fmul2_rn(__ffma2_rn(__fadd2_rn(vx[e], both(-mean[j])), both(-m2), p), both(rstd[j]));
+                }
+                if constexpr (JOINED) {
+                    if (a.grad_h) {
+                        float2 vh[V / 2];
+                        unpack<T>(piece_of(j, 2, i), vh);
+#pragma unroll
+                        for (int e = 0; e < V / 2; ++e) vg[e] = __fadd2_rn(vg[e], vh[e]);
+                    }
+                    if (a.grad_residual) store_piece<T, SHIFT>(static_cast<T*>(a.grad_residual) + at, c0, a.C, pack<T>(vg));
+                    if (a.grad_x) drop_piece(a.drop, gen, at + c0, vg);  // (pieces start at multiples of four elements of the tensor)
+                }
+                if (a.grad_x) store_piece<T, SHIFT>(static_cast<T*>(a.grad_x) + at, c0, a.C, pack<T>(vg));
+            }
+        }
+        fetch(row0 + depth * R * step, stage);
+        stage = stage + 1 == depth ? 0 : stage + 1;
     }
     if (!a.parts) return;
     float* part = a.parts + static_cast<long long>(blockIdx.x) * 2 * a.C;
@@ -132,12 +157,15 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : kMostThreads) norm_gra
 #pragma unroll
             for (int e = 0; e < V; ++e)
                 if (static_cast<unsigned>(c0 + e) < static_cast<unsigned>(a.C)) {
-                    part[c0 + e] = sum_w[i][e];
-                    part[a.C + c0 + e] = sum_b[i][e];
+                    part[c0 + e] = at_of(sum_w[i], e);
+                    part[a.C + c0 + e] = at_of(sum_b[i], e);
                 }
         }
     } else {
         // a warp's groups add to its columns in turn, then the warps' are added up
+        float* columns = reinterpret_cast<float*>(ring);
+        copies_wait(1);
+        __syncthreads();  // (all have read their rows)
         float* own = columns + (threadIdx.x >> 5) * 2 * a.C;
         const int turn = (threadIdx.x & 31) / lanes;
         for (int k = 0; k < 32 / lanes; ++k) {
@@ -148,8 +176,8 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : kMostThreads) norm_gra
 #pragma unroll
                     for (int e = 0; e < V; ++e)
                         if (static_cast<unsigned>(c0 + e) < static_cast<unsigned>(a.C)) {
-                            own[c0 + e] = sum_w[i][e] + (k ? own[c0 + e] : 0.0f);
-                            own[a.C + c0 + e] = sum_b[i][e] + (k ? own[a.C + c0 + e] : 0.0f);
+                            own[c0 + e] = at_of(sum_w[i], e) + (k ? own[c0 + e] : 0.0f);
+                            own[a.C + c0 + e] = at_of(sum_b[i], e) + (k ? own[a.C + c0 + e] : 0.0f);
                         }
                 }
             __syncwarp();
@@ -164,67 +192,78 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : kMostThreads) norm_gra
     }
 }
 
-int smem_of(const RowPlan& p, int C) { return p.group ? kGroupThreads / 32 * 2 * C * static_cast<int>(sizeof(float)) : 0; }
+struct GradShape {
+    RowPlan p;
+    int blocks, depth;
+    size_t smem;
+};
 
-template <class T, bool JOINED, int ITEMS, bool GROUP, bool SHIFT>
-int run(const NormGradArgs& a, const RowPlan& p, const DeviceCtx* ctx, cudaStream_t st, int blocks) {
-    // groups keep up to 1024 columns' sums per warp
-    constexpr int kMostSmem = kGroupThreads / 32 * 2 * 32 * 16 * static_cast<int>(sizeof(float));
-    static OncePerDevice once;
-    if (GROUP) {
-        const int r = once([] { return allow_smem(norm_grad_registers_kernel<T, JOINED, ITEMS, GROUP, SHIFT>, kMostSmem); });
-        if (r != kOk) return r;
-    }
-    return launch_after(norm_grad_registers_kernel<T, JOINED, ITEMS, GROUP, SHIFT>, blocks, p.threads, smem_of(p, a.C), st, a, p.lanes);
-}
-template <class T, bool JOINED, int ITEMS>
-int run(const NormGradArgs& a, const RowPlan& p, const DeviceCtx* ctx, cudaStream_t st, int blocks) {
-    if (p.group)
-        return p.shift ? run<T, JOINED, ITEMS, true, true>(a, p, ctx, st, blocks) : run<T, JOINED, ITEMS, true, false>(a, p, ctx, st, blocks);
-    return p.shift ? run<T, JOINED, ITEMS, false, true>(a, p, ctx, st, blocks) : run<T, JOINED, ITEMS, false, false>(a, p, ctx, st, blocks);
-}
-
-bool plan_of(bool joined, const NormGradArgs& a, int type, RowPlan* p) {
+bool plan_of(bool joined, const NormGradArgs& a, int type, const DeviceCtx* ctx, GradShape* s) {
     const int size = size_of(type);
     const bool aligned = on16(a.x) && on16(a.grad_y) && on16(a.grad_h) && on16(a.grad_x) && on16(a.grad_residual);
     const bool shift = rows_shift(size, a.C) || !on16(a.weight);
-    return rows_match(size, a.C, a.pitch, aligned) && plan_rows(a.C, 16 / size, shift, size, kMostThreads, 1, p);
-}
-int blocks_of(const RowPlan& p, const NormGradArgs& a, const DeviceCtx* ctx) {
+    RowPlan& p = s->p;
+    if (!rows_match(size, a.C, a.pitch, aligned) ||
+        !plan_elements(a.C, size, shift, joined, &p))
+        return false;
+    const int elements = p.items * (16 / size), R = rows_at_once(joined, elements, p.group);
+    const long long row_bytes = static_cast<long long>(R) * (joined ? 3 : 2) * p.items * p.threads * 16, most_smem = ctx->max_smem_optin - 2560;
+    // blocks per SM: up to 102 registers per thread, 128 with 32 elements, and rows under way behind those that are summed
+    int per_sm = 65536 / (p.threads * (elements <= 16 ? 102 : 128));
+    if (per_sm > 4) per_sm = 4;
+    if (per_sm < 1) per_sm = 1;
+    s->depth = ring_depth(row_bytes, most_smem / per_sm - 1024);
+    while (s->depth < 2 && per_sm > 1) s->depth = ring_depth(row_bytes, most_smem / --per_sm - 1024);
+    if (s->depth < 1) s->depth = 1;  // (rows of 16384 in 32 bits: 128 KB, joined 192 KB)
     const long long needed = (a.rows + p.rows_per_block() - 1) / p.rows_per_block();
-    const int per_sm = p.threads <= 192 ? 4 : p.threads <= 256 ? 3 : p.threads <= 384 ? 2 : 1;
-    long long most = static_cast<long long>(per_sm) * ctx->sm_count;
-    if (p.shift && !p.group) {
-        most = most / 8 * 8;
-        return static_cast<int>(needed < most ? (needed + 7) / 8 * 8 : most);  // (blocks without rows give parts of zeros)
-    }
-    return static_cast<int>(needed < most ? needed : most);
+    long long blocks = static_cast<long long>(per_sm) * ctx->sm_count;
+    if (p.shift && !p.group) blocks = blocks / 8 * 8;
+    if (needed < blocks) blocks = needed;
+    const long long turns = (needed + R * blocks - 1) / (R * blocks);
+    if (turns < s->depth) s->depth = static_cast<int>(turns);
+    s->blocks = static_cast<int>(blocks);
+    s->smem = static_cast<size_t>(s->depth) * row_bytes;
+    const size_t columns = p.group ? static_cast<size_t>(kGroupThreads / 32) * 2 * a.C * sizeof(float) : 0;
+    if (s->smem < columns) s->smem = columns;
+    return true;
+}
+
+template <class T, bool JOINED, int ITEMS, bool GROUP, bool SHIFT>
+int run(const NormGradArgs& a, const GradShape& s, const DeviceCtx* ctx, cudaStream_t st) {
+    constexpr auto kernel = norm_grad_registers_kernel<T, JOINED, ITEMS, GROUP, SHIFT>;
+    static OncePerDevice once;
+    const int r = once([&] { return allow_smem(kernel, ctx->max_smem_optin - 2560); });
+    if (r != kOk) return r;
+    return launch_after(kernel, s.blocks, s.p.threads, s.smem, st, a, s.p.lanes, s.depth);
+}
+template <class T, bool JOINED>
+int run(const NormGradArgs& a, const GradShape& s, const DeviceCtx* ctx, cudaStream_t st) {
+    constexpr int k8 = 8 / kPiece<T>, k16 = 16 / kPiece<T>, k32 = 32 / kPiece<T>;
+    constexpr int kBlock = JOINED || sizeof(T) == 4 ? k8 : k16;  // (as plan_elements has it)
+    const RowPlan& p = s.p;
+    if (p.group && p.items == k8)
+        return p.shift ? run<T, JOINED, k8, true, true>(a, s, ctx, st) : run<T, JOINED, k8, true, false>(a, s, ctx, st);
+    if (p.group) return p.shift ? run<T, JOINED, k16, true, true>(a, s, ctx, st) : run<T, JOINED, k16, true, false>(a, s, ctx, st);
+    if (p.items == kBlock)
+        return p.shift ? run<T, JOINED, kBlock, false, true>(a, s, ctx, st) : run<T, JOINED, kBlock, false, false>(a, s, ctx, st);
+    return p.shift ? run<T, JOINED, k32, false, true>(a, s, ctx, st) : run<T, JOINED, k32, false, false>(a, s, ctx, st);
 }
 
 }  // namespace
 
 bool norm_grad_in_registers(bool joined, const NormGradArgs& a, int type, const DeviceCtx* ctx, int* blocks) {
-    RowPlan p;
-    if (!plan_of(joined, a, type, &p)) return false;
-    *blocks = blocks_of(p, a, ctx);
+    GradShape s;
+    if (!plan_of(joined, a, type, ctx, &s)) return false;
+    *blocks = s.blocks;
     return true;
 }
 
 int launch_norm_grad_in_registers(bool joined, const NormGradArgs& a, int type, const DeviceCtx* ctx, cudaStream_t st) {
-    RowPlan p;
-    if (!plan_of(joined, a, type, &p)) return kBadArgument;
-    const int blocks = blocks_of(p, a, ctx);
+    GradShape s;
+    if (!plan_of(joined, a, type, ctx, &s)) return kBadArgument;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        auto by_items = [&](auto j) {
-            constexpr bool J = decltype(j)::value;
-            switch (p.items) {
-                case 1: return run<T, J, 1>(a, p, ctx, st, blocks);
-                case 2: return run<T, J, 2>(a, p, ctx, st, blocks);
-                default: return run<T, J, kMostItems<T>>(a, p, ctx, st, blocks);
-            }
-        };
-        return joined ? by_items(std::true_type()) : by_items(std::false_type());
+        return joined ? run<T, true>(a, s, ctx, st) : run<T, false>(a, s, ctx, st);
     });
 }
 

@@ -1,132 +1,215 @@
-// Layer norm forward (and rows as integers) with the row in registers: one read of the row, two sums over it (the mean, then the
-// squares of what is left), one write.  Bound by memory: what a call cannot do without is x and y once.
+// Layer norm forward (and rows as integers) with rows in registers: one read of a row, two sums over it (the mean, then the squares of
+// what is left), one write.
+//
+// Bound by memory: what a call cannot do without is x and y once (joined: x, the residual, h and y).  So a block always has rows
+// under way, into shared memory without registers, and takes several rows at a time, whose sums share their barriers: with one row
+// that was loaded when the one before was done, a 16384 x 5120 bf16 norm took 104 us at 49 % of the copy rate, with rows under
+// way 72 - 84.  A thread keeps its columns' weight and bias from row to row (a block takes every gridDim-th row; where rows
+// start anywhere in 16 bytes the grid is a multiple of eight, and rows that far apart start alike).  Rows of 8192 to 16384 have no
+// registers for that and read them again.
 #include "ldn_norm.cuh"
 #include "ldn_rows.cuh"
 
 namespace ldn {
 namespace {
 
-// 32 elements per thread, so that 128 registers hold them beside the rest: rows of up to 16384
-constexpr int kMostThreads = 512;
-template <class T>
-constexpr int kMostItems = 32 / kPiece<T>;
+// Rows that a block takes at a time
+__host__ __device__ constexpr int rows_at_once(Form f, int elements, bool group) {
+    return group || elements > 16 ? 1 : elements > 8 || f == Form::Joined ? 2 : 4;
+}
+template <Form F>
+constexpr int kStreams = F == Form::Joined ? 2 : 1;
+
+// The integers of a piece, whose columns start at c0: words of four where memory allows, as pieces that are cut do not start at
+// multiples of four bytes of the integers' row: the last `ahead` bytes of a word come from the next lane's piece.
+template <int V, bool SHIFT>
+__device__ __forceinline__ void store_integers(signed char* q, int c0, int C, const unsigned (&word)[V / 4], int lane_in_warp, int lanes) {
+    if (!SHIFT) {  // (rows start at multiples of 16 bytes then)
+        if (c0 < C) {
+            if constexpr (V == 8) *reinterpret_cast<uint2*>(q + c0) = make_uint2(word[0], word[1]);
+            else *reinterpret_cast<unsigned*>(q + c0) = word[0];
+        }
+        return;
+    }
+    const unsigned next = __shfl_down_sync(0xffffffffu, word[0], 1);
+    const int ahead = (4 - static_cast<int>((reinterpret_cast<uintptr_t>(q) + c0) & 3u)) & 3;
+    const bool last = lane_in_warp == (lanes < 32 ? lanes : 32) - 1, begins = lane_in_warp == 0;
+    if (c0 >= 0 && c0 + V + 4 <= C && !last) {
+        unsigned w[V / 4 + 1];
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) w[i] = word[i];
+        w[V / 4] = next;
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) *reinterpret_cast<unsigned*>(q + c0 + ahead + 4 * i) = __funnelshift_r(w[i], w[i + 1], 8 * ahead);
+        if (!begins && c0 >= V) return;  // (its first bytes are the lane's in front)
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            if (e < ahead) q[c0 + e] = static_cast<signed char>(word[0] >> 8 * e);
+    } else {
+        // (those that the lane in front has stored are stored again: the same bytes)
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (static_cast<unsigned>(c0 + e) < static_cast<unsigned>(C)) q[c0 + e] = static_cast<signed char>(word[e / 4] >> 8 * (e % 4));
+    }
+}
 
 template <class T, Form F, int ITEMS, bool GROUP, bool SHIFT>
-__global__ void __launch_bounds__(GROUP ? kGroupThreads : kMostThreads) norm_registers_kernel(NormArgs a, int lanes) {
+__global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPiece<T>), !GROUP && ITEMS * kPiece<T> == 16 ? 2 : 1)
+norm_registers_kernel(NormArgs a, int lanes, int depth) {
     stream_order_begin();
-    constexpr int V = kPiece<T>;
-    __shared__ float slots[128];
+    constexpr int V = kPiece<T>, S = kStreams<F>, R = rows_at_once(F, ITEMS * V, GROUP);
+    constexpr bool kParams = F != Form::Quantised, kKeep = kParams && ITEMS * V <= 16;
+    __shared__ float slots[2 * RowSum::kSlots];
+    extern __shared__ uint4 ring[];  // [depth][row][stream][item][thread]
     RowSum reduce{lanes, slots, 0};
     Generator gen;
     if constexpr (F == Form::Joined) gen = generator_of(a.drop);
     const int lane = GROUP ? threadIdx.x & (lanes - 1) : threadIdx.x;
     const int per_block = GROUP ? kGroupThreads / lanes : 1;
     const long long step = static_cast<long long>(gridDim.x) * per_block;
+    const long long mine = static_cast<long long>(blockIdx.x) * per_block + (GROUP ? threadIdx.x / lanes : 0);
     const float inv_C = 1.0f / a.C;
-    // (a warp's groups take part in its shuffles whether they have a row or not)
-    for (long long first = static_cast<long long>(blockIdx.x) * per_block; first < a.rows; first += step) {
-        const long long row = GROUP ? first + threadIdx.x / lanes : first;
-        const bool live = !GROUP || row < a.rows;
-        const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.pitch;
-        const long long at = (live ? row : 0) * a.C;
-        const int C = live ? a.C : 0, shift = SHIFT ? shift_of(x) : 0;
-        float v[ITEMS][V];
-        {
-            uint4 raw[ITEMS], onto[ITEMS];
+    // (the same for all rows of this thread)
+    const int shift = SHIFT ? shift_of(static_cast<const T*>(a.x) + (mine < a.rows ? mine : 0) * a.pitch) : 0;
+    auto column = [&](int i) { return (lane + i * lanes) * V - shift; };
+    float2 w[ITEMS][V / 2], b[ITEMS][V / 2];
+    uint4 mask[ITEMS];
+    int bytes[ITEMS];
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) raw[i] = load_piece<T, SHIFT>(x, (lane + i * lanes) * V - shift, C);
-            if constexpr (F == Form::Joined) {
-                const T* res = static_cast<const T*>(a.residual) + (live ? row : 0) * a.pitch_residual;
-#pragma unroll
-                for (int i = 0; i < ITEMS; ++i) onto[i] = load_piece<T, SHIFT>(res, (lane + i * lanes) * V - shift, C);
-            }
-#pragma unroll
-            for (int i = 0; i < ITEMS; ++i) {
-                unpack<T>(raw[i], v[i]);
-                if constexpr (F == Form::Joined) {
-                    const int c0 = (lane + i * lanes) * V - shift;
-                    float r[V];
-                    unpack<T>(onto[i], r);
-                    // (pieces start at multiples of four elements of the whole tensor)
-#pragma unroll
-                    for (int e = 0; e < V; e += 4) {
-                        const uint4 w = random_words(gen, static_cast<unsigned long long>(at + c0 + e) >> 2);
-                        v[i][e] = __fadd_rn(r[e], dropped(a.drop, w.x, v[i][e]));
-                        v[i][e + 1] = __fadd_rn(r[e + 1], dropped(a.drop, w.y, v[i][e + 1]));
-                        v[i][e + 2] = __fadd_rn(r[e + 2], dropped(a.drop, w.z, v[i][e + 2]));
-                        v[i][e + 3] = __fadd_rn(r[e + 3], dropped(a.drop, w.w, v[i][e + 3]));
-                    }
-                    const uint4 h = pack<T>(v[i]);
-                    store_piece<T, SHIFT>(static_cast<T*>(a.h) + at, c0, C, h);
-                    unpack<T>(h, v[i]);
-                    if (SHIFT) {  // (dropout of nothing is the residual's nothing: 0)
-#pragma unroll
-                        for (int e = 0; e < V; ++e) v[i][e] = in_row<SHIFT>(c0, e, C) ? v[i][e] : 0.0f;
-                    }
-                }
-            }
+    for (int i = 0; i < ITEMS; ++i) {
+        mask[i] = mask_of<T, SHIFT>(column(i), a.C);
+        bytes[i] = piece_bytes<T>(column(i), a.C);
+        if constexpr (kKeep) {
+            load_params<T, SHIFT>(a.weight, a.wide, column(i), a.C, 1.0f, w[i]);
+            load_params<T, SHIFT>(a.bias, a.wide, column(i), a.C, 0.0f, b[i]);
         }
-        if constexpr (F != Form::Quantised) {
-            float s[1] = {0.0f};
+    }
+    uint4* own = ring + threadIdx.x;
+    auto slot_of = [&](int stage, int j, int stream, int i) { return own + (((stage * R + j) * S + stream) * ITEMS + i) * blockDim.x; };
+    auto fetch = [&](long long row, int stage) {
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i)
+        for (int j = 0; j < R; ++j, row += step)
+            if (row < a.rows) {
 #pragma unroll
-                for (int e = 0; e < V; ++e) s[0] += v[i][e];
-            reduce.template sum<1, GROUP>(s);
-            const float mean = s[0] * inv_C;
-            s[0] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < ITEMS; ++i) {
-                const int c0 = (lane + i * lanes) * V - shift;
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    v[i][e] = in_row<SHIFT>(c0, e, C) ? v[i][e] - mean : 0.0f;
-                    s[0] += v[i][e] * v[i][e];
+                for (int i = 0; i < ITEMS; ++i) {
+                    copy_piece<T, SHIFT>(slot_of(stage, j, 0, i), static_cast<const T*>(a.x) + row * a.pitch, column(i), bytes[i],
+                                         row * a.pitch < V);
+                    if constexpr (S == 2)
+                        copy_piece<T, SHIFT>(slot_of(stage, j, 1, i), static_cast<const T*>(a.residual) + row * a.pitch_residual, column(i),
+                                             bytes[i], row == 0);
                 }
             }
-            reduce.template sum<1, GROUP>(s);
-            const float rstd = 1.0f / sqrtf(s[0] * inv_C + a.eps);
-            if (lane == 0 && live && a.mean) {
-                a.mean[row] = mean;
-                a.rstd[row] = rstd;
-            }
+        copies_commit();
+    };
+    for (int d = 0; d < depth * R * S; ++d)
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (!bytes[i]) own[(d * ITEMS + i) * blockDim.x] = make_uint4(0u, 0u, 0u, 0u);
+    for (int d = 0; d < depth; ++d) fetch(mine + d * R * step, d);
+    int stage = 0;
+    // (a warp's groups take part in its shuffles whether they have a row or not)
+    for (long long first = static_cast<long long>(blockIdx.x) * per_block; first < a.rows; first += R * step) {
+        const long long row0 = GROUP ? first + threadIdx.x / lanes : first;
+        auto live = [&](int j) { return row0 + j * step < a.rows; };
+        copies_wait(depth);
+        float2 v[R][ITEMS][V / 2];
+#pragma unroll
+        for (int j = 0; j < R; ++j)
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
-                const int c0 = (lane + i * lanes) * V - shift;
-                float w[V], b[V];
-                load_params<T, SHIFT>(a.weight, a.wide, c0, C, 1.0f, w);
-                load_params<T, SHIFT>(a.bias, a.wide, c0, C, 0.0f, b);
+                const int c0 = column(i);
+                uint4 raw = live(j) ? *slot_of(stage, j, 0, i) : make_uint4(0u, 0u, 0u, 0u);
+                if constexpr (F == Form::Joined) {
+                    if (live(j)) {
+                        const long long at = (row0 + j * step) * a.C;
+                        float2 r[V / 2];
+                        unpack<T>(raw, v[j][i]);
+                        unpack<T>(*slot_of(stage, j, 1, i), r);
+                        drop_piece(a.drop, gen, at + c0, v[j][i]);  // (pieces start at multiples of four elements of the whole tensor)
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[i][e] = fmaf(v[i][e] * rstd, w[e], b[e]);
-                if constexpr (F != Form::Integers) store_piece<T, SHIFT>(static_cast<T*>(a.y) + at, c0, C, pack<T>(v[i]));
+                        for (int e = 0; e < V / 2; ++e) v[j][i][e] = __fadd2_rn(r[e], v[j][i][e]);
+                        raw = pack<T>(v[j][i]);
+                        store_piece<T, SHIFT>(static_cast<T*>(a.h) + at, c0, a.C, raw);
+                    }
+                    if (!SHIFT && c0 >= a.C) raw = make_uint4(0u, 0u, 0u, 0u);
+                }
+                unpack<T>(SHIFT ? masked(raw, mask[i]) : raw, v[j][i]);
+            }
+        fetch(row0 + depth * R * step, stage);
+        stage = stage + 1 == depth ? 0 : stage + 1;
+        if constexpr (kParams) {
+            float s[R], mean[R];
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                float2 sum = both(0.0f);
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) sum = __fadd2_rn(sum, v[j][i][e]);
+                s[j] = sum.x + sum.y;
+            }
+            reduce.template sum<GROUP>(s, [&](float all) { return all * inv_C; });
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                mean[j] = s[j];
+                float2 sum = both(0.0f);
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i) {
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) v[j][i][e] = __fadd2_rn(v[j][i][e], both(-mean[j]));
+                    only_row<SHIFT>(column(i), a.C, v[j][i]);
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) sum = __ffma2_rn(v[j][i][e], v[j][i][e], sum);
+                }
+                s[j] = sum.x + sum.y;
+            }
+            reduce.template sum<GROUP>(s, [&](float all) { return 1.0f / sqrtf(all * inv_C + a.eps); });
+#pragma unroll
+            for (int j = 0; j < R; ++j)
+                if (lane == 0 && a.mean && live(j)) {
+                    a.mean[row0 + j * step] = mean[j];
+                    a.rstd[row0 + j * step] = s[j];
+                }
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int c0 = column(i);
+                if constexpr (!kKeep) {
+                    load_params<T, SHIFT>(a.weight, a.wide, c0, a.C, 1.0f, w[i]);
+                    load_params<T, SHIFT>(a.bias, a.wide, c0, a.C, 0.0f, b[i]);
+                }
+#pragma unroll
+                for (int j = 0; j < R; ++j) {
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) v[j][i][e] = __ffma2_rn(__fmul2_rn(v[j][i][e], both(s[j])), w[i][e], b[i][e]);
+                    if constexpr (F != Form::Integers)
+                        if (live(j)) store_piece<T, SHIFT>(static_cast<T*>(a.y) + (row0 + j * step) * a.C, c0, a.C, pack<T>(v[j][i]));
+                }
             }
         }
         if constexpr (F == Form::Integers || F == Form::Quantised) {
-            unsigned top = 0;
+            float top[R];
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i)
+            for (int j = 0; j < R; ++j) {
+                top[j] = 0.0f;
 #pragma unroll
-                for (int e = 0; e < V; ++e) top = max(top, magnitude(v[i][e]));
-            const float size = step_of(reduce.template largest<GROUP>(top)), inverse = 1.0f / size;
-            if (lane == 0 && live) a.scale[row] = size;
-            signed char* q = a.q + row * a.pitch_q;
+                for (int i = 0; i < ITEMS; ++i) {
+                    if constexpr (F == Form::Integers) only_row<SHIFT>(column(i), a.C, v[j][i]);  // (a bias of nothing may be there)
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) {
-                const int c0 = (lane + i * lanes) * V - shift;
-                unsigned word[V / 4];
+                    for (int e = 0; e < V / 2; ++e) top[j] = larger(top[j], v[j][i][e]);
+                }
+            }
+            reduce.template largest<GROUP>(top, [](float all) { return step_of(__float_as_uint(all)); });
 #pragma unroll
-                for (int e = 0; e < V; e += 4)
-                    word[e / 4] = (steps(v[i][e], inverse) & 255) | (steps(v[i][e + 1], inverse) & 255) << 8 |
-                                  (steps(v[i][e + 2], inverse) & 255) << 16 | static_cast<unsigned>(steps(v[i][e + 3], inverse)) << 24;
-                if (!SHIFT) {  // (the integers' rows start at multiples of 16 bytes then)
-                    if (c0 < C) {
-                        if constexpr (V == 8) *reinterpret_cast<uint2*>(q + c0) = make_uint2(word[0], word[1]);
-                        else *reinterpret_cast<unsigned*>(q + c0) = word[0];
-                    }
-                } else {
+            for (int j = 0; j < R; ++j) {
+                const float size = top[j], inverse = 1.0f / size;
+                if (lane == 0 && live(j)) a.scale[row0 + j * step] = size;
+                signed char* q = a.q + (live(j) ? row0 + j * step : 0) * a.pitch_q;
 #pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        if (in_row<SHIFT>(c0, e, C)) q[c0 + e] = static_cast<signed char>(word[e / 4] >> 8 * (e % 4));
+                for (int i = 0; i < ITEMS; ++i) {
+                    unsigned word[V / 4];
+#pragma unroll
+                    for (int e = 0; e < V / 4; ++e) word[e] = steps4(v[j][i][2 * e], v[j][i][2 * e + 1], inverse);
+                    store_integers<V, SHIFT>(q, column(i), live(j) ? a.C : 0, word, GROUP ? lane : threadIdx.x & 31, lanes);
                 }
             }
         }
@@ -135,34 +218,43 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : kMostThreads) norm_reg
 
 template <class T, Form F, int ITEMS, bool GROUP, bool SHIFT>
 int launch(const NormArgs& a, const RowPlan& p, const DeviceCtx* ctx, cudaStream_t st) {
-    static std::atomic<int> resident[64][33];  // blocks per SM by warps
+    constexpr auto kernel = norm_registers_kernel<T, F, ITEMS, GROUP, SHIFT>;
+    static OncePerDevice once;
+    const int most_smem = ctx->max_smem_optin - 2560;
+    int r = once([&] { return allow_smem(kernel, most_smem); });
+    if (r != kOk) return r;
+    // as many blocks as registers allow, with what they may have of shared memory
+    static std::atomic<int> resident[64][33];
     std::atomic<int>& known = resident[ctx->device][p.threads / 32];
     int per_sm = known.load(std::memory_order_acquire);
     if (per_sm == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, norm_registers_kernel<T, F, ITEMS, GROUP, SHIFT>, p.threads, 0) !=
-                cudaSuccess || per_sm < 1) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, p.threads, 0) != cudaSuccess || per_sm < 1) {
             cudaGetLastError();
             per_sm = 1;
         }
         known.store(per_sm, std::memory_order_release);
     }
-    const long long most = static_cast<long long>(per_sm) * ctx->sm_count, blocks = (a.rows + p.rows_per_block() - 1) / p.rows_per_block();
-    return launch_after(norm_registers_kernel<T, F, ITEMS, GROUP, SHIFT>, static_cast<unsigned>(blocks < most ? blocks : most), p.threads,
-                        0, st, a, p.lanes);
-}
-template <class T, Form F, int ITEMS>
-int launch(const NormArgs& a, const RowPlan& p, const DeviceCtx* ctx, cudaStream_t st) {
-    if (p.group) return p.shift ? launch<T, F, ITEMS, true, true>(a, p, ctx, st) : launch<T, F, ITEMS, true, false>(a, p, ctx, st);
-    return p.shift ? launch<T, F, ITEMS, false, true>(a, p, ctx, st) : launch<T, F, ITEMS, false, false>(a, p, ctx, st);
+    constexpr int R = rows_at_once(F, ITEMS * kPiece<T>, GROUP);
+    const long long row_bytes = static_cast<long long>(R) * kStreams<F> * ITEMS * p.threads * 16;
+    int depth = ring_depth(row_bytes, most_smem / per_sm - 1024);
+    while (depth < 2 && per_sm > 1) depth = ring_depth(row_bytes, most_smem / --per_sm - 1024);
+    if (depth < 1) depth = 1;  // (a row of 16384 in 32 bits and its residual: 128 KB)
+    const long long needed = (a.rows + p.rows_per_block() - 1) / p.rows_per_block();
+    long long blocks = static_cast<long long>(per_sm) * ctx->sm_count;
+    if (p.shift && !p.group) blocks = blocks / 8 * 8;
+    if (needed < blocks) blocks = needed;  // (a block has one row at most, then, and it does not matter how far they are apart)
+    const long long turns = (needed + R * blocks - 1) / (R * blocks);
+    if (turns < depth) depth = static_cast<int>(turns);
+    return launch_after(kernel, static_cast<unsigned>(blocks), p.threads, depth * row_bytes, st, a, p.lanes, depth);
 }
 template <class T, Form F>
 int launch(const NormArgs& a, const RowPlan& p, const DeviceCtx* ctx, cudaStream_t st) {
-    switch (p.items) {
-        case 1: return launch<T, F, 1>(a, p, ctx, st);
-        case 2: return launch<T, F, 2>(a, p, ctx, st);
-        case 4: return launch<T, F, 4>(a, p, ctx, st);
-        default: return launch<T, F, kMostItems<T>>(a, p, ctx, st);
-    }
+    constexpr int k8 = 8 / kPiece<T>, k16 = 16 / kPiece<T>, k32 = 32 / kPiece<T>;
+    constexpr int kBlock = F == Form::Joined || sizeof(T) == 4 ? k8 : k16;  // (as plan_elements has it)
+    if (p.group && p.items == k8) return p.shift ? launch<T, F, k8, true, true>(a, p, ctx, st) : launch<T, F, k8, true, false>(a, p, ctx, st);
+    if (p.group) return p.shift ? launch<T, F, k16, true, true>(a, p, ctx, st) : launch<T, F, k16, true, false>(a, p, ctx, st);
+    if (p.items == kBlock) return p.shift ? launch<T, F, kBlock, false, true>(a, p, ctx, st) : launch<T, F, kBlock, false, false>(a, p, ctx, st);
+    return p.shift ? launch<T, F, k32, false, true>(a, p, ctx, st) : launch<T, F, k32, false, false>(a, p, ctx, st);
 }
 
 }  // namespace
@@ -174,12 +266,12 @@ bool norm_in_registers(Form form, const NormArgs& a, int type, const DeviceCtx* 
     if (form == Form::Joined) match = match && rows_match(size, a.C, a.pitch_residual, aligned);
     bool shift = rows_shift(size, a.C) || !on16(a.weight) || !on16(a.bias);
     if (form == Form::Integers || form == Form::Quantised) {
-        // nothing has to match x but the integers, which are stored one by one where they do not
+        // nothing has to match x but the integers, which are put together where they do not
         match = (reinterpret_cast<uintptr_t>(a.x) & (size - 1)) == 0;
         shift = shift || !on16(a.x) || a.pitch * size % 16 != 0 || !on16(a.q) || a.pitch_q % 16 != 0;
     }
     RowPlan p;
-    if (!match || !plan_rows(a.C, 16 / size, shift, 2 * size, kMostThreads, 1, &p)) return false;
+    if (!match || !plan_elements(a.C, size, shift, form == Form::Joined, &p)) return false;
     *status = with_type(type, [&](auto t) {
         using T = decltype(t);
         switch (form) {
