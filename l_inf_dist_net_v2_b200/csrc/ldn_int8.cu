@@ -85,6 +85,7 @@ extern "C" LDN_API int ldn_int8_linear(const signed char* q, long long pitch_q, 
     if (r != kOk) return r;
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const ProductArgs a = {q, pitch_q, scale, w, pitch_w, w_scale, bias, M, N, K, activation, out};
+    if (product_is_single(a)) return launch_product_single(a, nullptr, 0, type, type, ctx, st);
     const Operands o = operands_of(a);
     Scratch scratch;
     if ((r = scratch.take(st, o.bytes_q + o.bytes_w)) != kOk) return r;
@@ -104,6 +105,7 @@ extern "C" LDN_API int ldn_int8_linear_float(const void* x, long long pitch, int
     const long long pitch_q = padded16(K);
     const size_t bytes_q = pad256(static_cast<size_t>(M) * pitch_q), bytes_scale = pad256(sizeof(float) * static_cast<size_t>(M));
     ProductArgs a = {nullptr, pitch_q, nullptr, w, pitch_w, w_scale, bias, M, N, K, activation, out};
+    if (product_is_single(a)) return launch_product_single(a, x, pitch, x_type, type, ctx, st);
     const Operands o = operands_of(a);
     Scratch scratch;
     if ((r = scratch.take(st, bytes_q + bytes_scale + o.bytes_w)) != kOk) return r;

@@ -20,6 +20,10 @@ struct ProductArgs {
 // (called, not inlined: sixteen copies of it in a loop over a thread's sums came from memory every time and cost more than the
 // products)
 static __device__ __noinline__ float tanh_called(float v) { return tanhf(v); }
+__device__ __forceinline__ float product_value(int sum, float scale, float w_scale, float bias, int activation) {
+    const float v = fmaf(__fmul_rn(static_cast<float>(sum), scale), w_scale, bias);
+    return activation == LDN_RELU ? (v < 0.0f ? 0.0f : v) : activation == LDN_TANH ? tanh_called(v) : v;
+}
 // What follows the sums of one output for N tokens, two at a time and without a branch per value (values in flight hide each
 // other's latency); bias: 0 where there is none
 template <int N>
@@ -44,5 +48,10 @@ __device__ __forceinline__ void product_values(const int (&sum)[N], const float 
 
 // Both operands' rows start at multiples of 16 bytes
 int launch_product_tiles(const ProductArgs& a, int type, int* status, const DeviceCtx* ctx, cudaStream_t st);
+
+// One to four tokens, the weight's rows at multiples of 16 bytes; x: rows of x_type to be quantised, or null (the product's integers)
+bool product_is_single(const ProductArgs& a);
+int launch_product_single(const ProductArgs& a, const void* x, long long pitch, int x_type, int out_type, const DeviceCtx* ctx,
+                          cudaStream_t st);
 
 }  // namespace ldn
