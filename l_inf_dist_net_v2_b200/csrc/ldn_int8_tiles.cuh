@@ -139,6 +139,12 @@ __host__ __device__ constexpr uint32_t product_kind(int rows, int columns) {
     return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(columns >> 3) << 17) | (static_cast<uint32_t>(rows >> 4) << 24);
 }
 
+// Results leave the L2 cache first: the operands are read again
+template <class T>
+__device__ __forceinline__ void store_once(T* p, T v) {
+    if constexpr (sizeof(T) == 4) __stcs(p, v);
+    else __stcs(reinterpret_cast<unsigned short*>(p), *reinterpret_cast<const unsigned short*>(&v));
+}
 // What follows the sums: a thread has one output of 16 tokens at a time, the first of them at `to`, `columns` of them there; the
 // tokens' scales lie in shared memory.
 template <class T>
@@ -155,11 +161,11 @@ __device__ __forceinline__ void store16(const ProductArgs& a, const int (&sum)[1
     const unsigned row = static_cast<unsigned>(a.N) * sizeof(T);  // (N is below 2^25 here, so that 15 rows are below 2^31)
     if (there && columns >= 16) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) *reinterpret_cast<T*>(p + j * row) = from_float<T>(v[j]);
+        for (int j = 0; j < 16; ++j) store_once(reinterpret_cast<T*>(p + j * row), from_float<T>(v[j]));
     } else if (there) {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-            if (j < columns) *reinterpret_cast<T*>(p + j * row) = from_float<T>(v[j]);
+            if (j < columns) store_once(reinterpret_cast<T*>(p + j * row), from_float<T>(v[j]));
     }
 }
 

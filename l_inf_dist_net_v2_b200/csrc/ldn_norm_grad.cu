@@ -52,34 +52,43 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPi
         bytes[i] = piece_bytes<T>(column(i), a.C);
         if constexpr (kKeep) load_params<T, SHIFT>(a.weight, a.wide, column(i), a.C, 1.0f, w[i]);
     }
+    // this thread's rows, and where their pieces are: those to be fetched, and those to be made
+    const int c0 = column(0), apart = lanes * V;
+    int to_fetch = mine < a.rows ? static_cast<int>((a.rows - mine + step - 1) / step) : 0, to_make = to_fetch;
+    Walk<const T> from_x(a.x, a.pitch, mine, step, c0), from_y(a.grad_y, a.C, mine, step, c0), from_h(a.grad_h, a.C, mine, step, c0);
+    Walk<T> to_x(a.grad_x, a.C, mine, step, c0), to_h(a.grad_residual, a.C, mine, step, c0);
+    long long row0 = mine, index = mine * a.C + c0;
     uint4* own = ring + threadIdx.x;
     auto slot_of = [&](int stage, int j, int stream, int i) { return own + (((stage * R + j) * S + stream) * ITEMS + i) * blockDim.x; };
-    auto fetch = [&](long long row, int stage) {
+    auto fetch = [&](int stage) {
 #pragma unroll
-        for (int j = 0; j < R; ++j, row += step)
-            if (row < a.rows) {
-                const T *x = static_cast<const T*>(a.x) + row * a.pitch, *g = static_cast<const T*>(a.grad_y) + row * a.C;
+        for (int j = 0; j < R; ++j)
+            if (j < to_fetch) {
 #pragma unroll
                 for (int i = 0; i < ITEMS; ++i) {
-                    copy_piece<T, SHIFT>(slot_of(stage, j, 0, i), x, column(i), bytes[i], row == 0);
-                    copy_piece<T, SHIFT>(slot_of(stage, j, 1, i), g, column(i), bytes[i], row == 0);
+                    copy_piece<T, SHIFT>(slot_of(stage, j, 0, i), from_x.of(j, i * apart), column(i), bytes[i], a.x);
+                    copy_piece<T, SHIFT>(slot_of(stage, j, 1, i), from_y.of(j, i * apart), column(i), bytes[i], a.grad_y);
                     if constexpr (JOINED)
-                        if (a.grad_h)
-                            copy_piece<T, SHIFT>(slot_of(stage, j, 2, i), static_cast<const T*>(a.grad_h) + row * a.C, column(i), bytes[i], row == 0);
+                        if (a.grad_h) copy_piece<T, SHIFT>(slot_of(stage, j, 2, i), from_h.of(j, i * apart), column(i), bytes[i], a.grad_h);
                 }
             }
         copies_commit();
+        to_fetch -= R;
+        from_x.on(R);
+        from_y.on(R);
+        if (JOINED) from_h.on(R);
     };
     for (int d = 0; d < depth * R * S; ++d)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
             if (!bytes[i]) own[(d * ITEMS + i) * blockDim.x] = make_uint4(0u, 0u, 0u, 0u);
-    for (int d = 0; d < depth; ++d) fetch(mine + d * R * step, d);
+    for (int d = 0; d < depth; ++d) fetch(d);
     int stage = 0;
-    // (a warp's groups take part in its shuffles whether they have a row or not)
-    for (long long first = static_cast<long long>(blockIdx.x) * per_block; first < a.rows; first += R * step) {
-        const long long row0 = GROUP ? first + threadIdx.x / lanes : first;
-        auto live = [&](int j) { return row0 + j * step < a.rows; };
+    // (a warp's groups take part in its shuffles whether they have a row or not: as many turns as the block's first has)
+    const long long block_first = static_cast<long long>(blockIdx.x) * per_block;
+    const int turns = block_first < a.rows ? static_cast<int>((a.rows - block_first + R * step - 1) / (R * step)) : 0;
+    for (int turn = 0; turn < turns; ++turn) {
+        auto live = [&](int j) { return j < to_make; };
         float mean[R], rstd[R], s[2 * R];
 #pragma unroll
         for (int j = 0; j < R; ++j) {
@@ -118,15 +127,14 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPi
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             if (!live(j)) continue;
-            const long long at = (row0 + j * step) * a.C;
             const float m1 = s[2 * j], m2 = s[2 * j + 1] * rstd[j];
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
-                const int c0 = column(i);
+                const int c = column(i);
                 float2 vx[V / 2], vg[V / 2];
                 unpack<T>(piece_of(j, 0, i), vx);
                 unpack<T>(piece_of(j, 1, i), vg);
-                if constexpr (!kKeep) load_params<T, SHIFT>(a.weight, a.wide, c0, a.C, 1.0f, w[i]);
+                if constexpr (!kKeep) load_params<T, SHIFT>(a.weight, a.wide, c, a.C, 1.0f, w[i]);
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e) {
                     const float2 p = __ffma2_rn(vg[e], w[i][e], both(-m1));
@@ -139,14 +147,21 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPi
 #pragma unroll
                         for (int e = 0; e < V / 2; ++e) vg[e] = __fadd2_rn(vg[e], vh[e]);
                     }
-                    if (a.grad_residual) store_piece<T, SHIFT>(static_cast<T*>(a.grad_residual) + at, c0, a.C, pack<T>(vg));
-                    if (a.grad_x) drop_piece(a.drop, gen, at + c0, vg);  // (pieces start at multiples of four elements of the tensor)
+                    if (a.grad_residual) store_piece<T, SHIFT>(to_h.of(j, i * apart), c, a.C, pack<T>(vg));
+                    if (a.grad_x) drop_piece(a.drop, gen, index + j * step * a.C + i * apart, vg);  // (pieces start at multiples of four)
                 }
-                if (a.grad_x) store_piece<T, SHIFT>(static_cast<T*>(a.grad_x) + at, c0, a.C, pack<T>(vg));
+                if (a.grad_x) store_piece<T, SHIFT>(to_x.of(j, i * apart), c, a.C, pack<T>(vg));
             }
         }
-        fetch(row0 + depth * R * step, stage);
+        fetch(stage);
         stage = stage + 1 == depth ? 0 : stage + 1;
+        to_make -= R;
+        row0 += R * step;
+        to_x.on(R);
+        if (JOINED) {
+            to_h.on(R);
+            index += R * step * a.C;
+        }
     }
     if (!a.parts) return;
     float* part = a.parts + static_cast<long long>(blockIdx.x) * 2 * a.C;

@@ -15,7 +15,7 @@ namespace {
 
 // Rows that a block takes at a time
 __host__ __device__ constexpr int rows_at_once(Form f, int elements, bool group) {
-    return group || elements > 16 ? 1 : elements > 8 || f == Form::Joined ? 2 : 4;
+    return group || elements > 16 || f == Form::Quantised ? 1 : elements > 8 || f == Form::Joined ? 2 : 4;
 }
 template <Form F>
 constexpr int kStreams = F == Form::Joined ? 2 : 1;
@@ -23,16 +23,16 @@ constexpr int kStreams = F == Form::Joined ? 2 : 1;
 // The integers of a piece, whose columns start at c0: words of four where memory allows, as pieces that are cut do not start at
 // multiples of four bytes of the integers' row: the last `ahead` bytes of a word come from the next lane's piece.
 template <int V, bool SHIFT>
-__device__ __forceinline__ void store_integers(signed char* q, int c0, int C, const unsigned (&word)[V / 4], int lane_in_warp, int lanes) {
+__device__ __forceinline__ void store_integers(signed char* to, int c0, int C, const unsigned (&word)[V / 4], int lane_in_warp, int lanes) {
     if (!SHIFT) {  // (rows start at multiples of 16 bytes then)
         if (c0 < C) {
-            if constexpr (V == 8) *reinterpret_cast<uint2*>(q + c0) = make_uint2(word[0], word[1]);
-            else *reinterpret_cast<unsigned*>(q + c0) = word[0];
+            if constexpr (V == 8) *reinterpret_cast<uint2*>(to) = make_uint2(word[0], word[1]);
+            else *reinterpret_cast<unsigned*>(to) = word[0];
         }
         return;
     }
     const unsigned next = __shfl_down_sync(0xffffffffu, word[0], 1);
-    const int ahead = (4 - static_cast<int>((reinterpret_cast<uintptr_t>(q) + c0) & 3u)) & 3;
+    const int ahead = (4 - static_cast<int>(reinterpret_cast<uintptr_t>(to) & 3u)) & 3;
     const bool last = lane_in_warp == (lanes < 32 ? lanes : 32) - 1, begins = lane_in_warp == 0;
     if (c0 >= 0 && c0 + V + 4 <= C && !last) {
         unsigned w[V / 4 + 1];
@@ -40,21 +40,21 @@ __device__ __forceinline__ void store_integers(signed char* q, int c0, int C, co
         for (int i = 0; i < V / 4; ++i) w[i] = word[i];
         w[V / 4] = next;
 #pragma unroll
-        for (int i = 0; i < V / 4; ++i) *reinterpret_cast<unsigned*>(q + c0 + ahead + 4 * i) = __funnelshift_r(w[i], w[i + 1], 8 * ahead);
+        for (int i = 0; i < V / 4; ++i) *reinterpret_cast<unsigned*>(to + ahead + 4 * i) = __funnelshift_r(w[i], w[i + 1], 8 * ahead);
         if (!begins && c0 >= V) return;  // (its first bytes are the lane's in front)
 #pragma unroll
         for (int e = 0; e < 3; ++e)
-            if (e < ahead) q[c0 + e] = static_cast<signed char>(word[0] >> 8 * e);
+            if (e < ahead) to[e] = static_cast<signed char>(word[0] >> 8 * e);
     } else {
         // (those that the lane in front has stored are stored again: the same bytes)
 #pragma unroll
         for (int e = 0; e < V; ++e)
-            if (static_cast<unsigned>(c0 + e) < static_cast<unsigned>(C)) q[c0 + e] = static_cast<signed char>(word[e / 4] >> 8 * (e % 4));
+            if (static_cast<unsigned>(c0 + e) < static_cast<unsigned>(C)) to[e] = static_cast<signed char>(word[e / 4] >> 8 * (e % 4));
     }
 }
 
 template <class T, Form F, int ITEMS, bool GROUP, bool SHIFT>
-__global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPiece<T>), !GROUP && ITEMS * kPiece<T> == 16 ? 2 : 1)
+__global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPiece<T>), !GROUP && ITEMS * kPiece<T> == 16 ? (F == Form::Quantised ? 4 : 2) : 1)
 norm_registers_kernel(NormArgs a, int lanes, int depth) {
     stream_order_begin();
     constexpr int V = kPiece<T>, S = kStreams<F>, R = rows_at_once(F, ITEMS * V, GROUP);
@@ -84,58 +84,66 @@ norm_registers_kernel(NormArgs a, int lanes, int depth) {
             load_params<T, SHIFT>(a.bias, a.wide, column(i), a.C, 0.0f, b[i]);
         }
     }
+    // this thread's rows, and where their pieces are: those to be fetched, and those to be made
+    const int c0 = column(0), apart = lanes * V;
+    int to_fetch = mine < a.rows ? static_cast<int>((a.rows - mine + step - 1) / step) : 0, to_make = to_fetch;
+    Walk<const T> from_x(a.x, a.pitch, mine, step, c0), from_onto(a.residual, a.pitch_residual, mine, step, c0);
+    Walk<T> to_h(a.h, a.C, mine, step, c0), to_y(a.y, a.C, mine, step, c0);
+    Walk<signed char> to_q(a.q, a.pitch_q, mine, step, c0);
+    long long row0 = mine, index = mine * a.C + c0;
     uint4* own = ring + threadIdx.x;
     auto slot_of = [&](int stage, int j, int stream, int i) { return own + (((stage * R + j) * S + stream) * ITEMS + i) * blockDim.x; };
-    auto fetch = [&](long long row, int stage) {
+    auto fetch = [&](int stage) {
 #pragma unroll
-        for (int j = 0; j < R; ++j, row += step)
-            if (row < a.rows) {
+        for (int j = 0; j < R; ++j)
+            if (j < to_fetch) {
 #pragma unroll
                 for (int i = 0; i < ITEMS; ++i) {
-                    copy_piece<T, SHIFT>(slot_of(stage, j, 0, i), static_cast<const T*>(a.x) + row * a.pitch, column(i), bytes[i],
-                                         row * a.pitch < V);
+                    copy_piece<T, SHIFT>(slot_of(stage, j, 0, i), from_x.of(j, i * apart), column(i), bytes[i], a.x);
                     if constexpr (S == 2)
-                        copy_piece<T, SHIFT>(slot_of(stage, j, 1, i), static_cast<const T*>(a.residual) + row * a.pitch_residual, column(i),
-                                             bytes[i], row == 0);
+                        copy_piece<T, SHIFT>(slot_of(stage, j, 1, i), from_onto.of(j, i * apart), column(i), bytes[i], a.residual);
                 }
             }
         copies_commit();
+        to_fetch -= R;
+        from_x.on(R);
+        if (S == 2) from_onto.on(R);
     };
     for (int d = 0; d < depth * R * S; ++d)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
             if (!bytes[i]) own[(d * ITEMS + i) * blockDim.x] = make_uint4(0u, 0u, 0u, 0u);
-    for (int d = 0; d < depth; ++d) fetch(mine + d * R * step, d);
+    for (int d = 0; d < depth; ++d) fetch(d);
     int stage = 0;
-    // (a warp's groups take part in its shuffles whether they have a row or not)
-    for (long long first = static_cast<long long>(blockIdx.x) * per_block; first < a.rows; first += R * step) {
-        const long long row0 = GROUP ? first + threadIdx.x / lanes : first;
-        auto live = [&](int j) { return row0 + j * step < a.rows; };
+    // (a warp's groups take part in its shuffles whether they have a row or not: as many turns as the block's first has)
+    const long long block_first = static_cast<long long>(blockIdx.x) * per_block;
+    const int turns = block_first < a.rows ? static_cast<int>((a.rows - block_first + R * step - 1) / (R * step)) : 0;
+    for (int turn = 0; turn < turns; ++turn) {
+        auto live = [&](int j) { return j < to_make; };
         copies_wait(depth);
         float2 v[R][ITEMS][V / 2];
 #pragma unroll
         for (int j = 0; j < R; ++j)
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
-                const int c0 = column(i);
+                const int c = column(i);
                 uint4 raw = live(j) ? *slot_of(stage, j, 0, i) : make_uint4(0u, 0u, 0u, 0u);
                 if constexpr (F == Form::Joined) {
                     if (live(j)) {
-                        const long long at = (row0 + j * step) * a.C;
                         float2 r[V / 2];
                         unpack<T>(raw, v[j][i]);
                         unpack<T>(*slot_of(stage, j, 1, i), r);
-                        drop_piece(a.drop, gen, at + c0, v[j][i]);  // (pieces start at multiples of four elements of the whole tensor)
+                        drop_piece(a.drop, gen, index + j * step * a.C + i * apart, v[j][i]);  // (pieces start at multiples of four elements)
 #pragma unroll
                         for (int e = 0; e < V / 2; ++e) v[j][i][e] = __fadd2_rn(r[e], v[j][i][e]);
                         raw = pack<T>(v[j][i]);
-                        store_piece<T, SHIFT>(static_cast<T*>(a.h) + at, c0, a.C, raw);
+                        store_piece<T, SHIFT>(to_h.of(j, i * apart), c, a.C, raw);
                     }
-                    if (!SHIFT && c0 >= a.C) raw = make_uint4(0u, 0u, 0u, 0u);
+                    if (!SHIFT && c >= a.C) raw = make_uint4(0u, 0u, 0u, 0u);
                 }
                 unpack<T>(SHIFT ? masked(raw, mask[i]) : raw, v[j][i]);
             }
-        fetch(row0 + depth * R * step, stage);
+        fetch(stage);
         stage = stage + 1 == depth ? 0 : stage + 1;
         if constexpr (kParams) {
             float s[R], mean[R];
@@ -172,17 +180,17 @@ norm_registers_kernel(NormArgs a, int lanes, int depth) {
                 }
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
-                const int c0 = column(i);
+                const int c = column(i);
                 if constexpr (!kKeep) {
-                    load_params<T, SHIFT>(a.weight, a.wide, c0, a.C, 1.0f, w[i]);
-                    load_params<T, SHIFT>(a.bias, a.wide, c0, a.C, 0.0f, b[i]);
+                    load_params<T, SHIFT>(a.weight, a.wide, c, a.C, 1.0f, w[i]);
+                    load_params<T, SHIFT>(a.bias, a.wide, c, a.C, 0.0f, b[i]);
                 }
 #pragma unroll
                 for (int j = 0; j < R; ++j) {
 #pragma unroll
                     for (int e = 0; e < V / 2; ++e) v[j][i][e] = __ffma2_rn(__fmul2_rn(v[j][i][e], both(s[j])), w[i][e], b[i][e]);
                     if constexpr (F != Form::Integers)
-                        if (live(j)) store_piece<T, SHIFT>(static_cast<T*>(a.y) + (row0 + j * step) * a.C, c0, a.C, pack<T>(v[j][i]));
+                        if (live(j)) store_piece<T, SHIFT>(to_y.of(j, i * apart), c, a.C, pack<T>(v[j][i]));
                 }
             }
         }
@@ -203,16 +211,24 @@ norm_registers_kernel(NormArgs a, int lanes, int depth) {
             for (int j = 0; j < R; ++j) {
                 const float size = top[j], inverse = 1.0f / size;
                 if (lane == 0 && live(j)) a.scale[row0 + j * step] = size;
-                signed char* q = a.q + (live(j) ? row0 + j * step : 0) * a.pitch_q;
 #pragma unroll
                 for (int i = 0; i < ITEMS; ++i) {
                     unsigned word[V / 4];
 #pragma unroll
                     for (int e = 0; e < V / 4; ++e) word[e] = steps4(v[j][i][2 * e], v[j][i][2 * e + 1], inverse);
-                    store_integers<V, SHIFT>(q, column(i), live(j) ? a.C : 0, word, GROUP ? lane : threadIdx.x & 31, lanes);
+                    store_integers<V, SHIFT>(to_q.of(j, i * apart), column(i), live(j) ? a.C : 0, word, GROUP ? lane : threadIdx.x & 31,
+                                             lanes);
                 }
             }
         }
+        to_make -= R;
+        row0 += R * step;
+        if constexpr (F == Form::Joined) {
+            to_h.on(R);
+            index += R * step * a.C;
+        }
+        if constexpr (F == Form::Plain || F == Form::Joined) to_y.on(R);
+        else to_q.on(R);
     }
 }
 

@@ -75,22 +75,23 @@ __device__ __forceinline__ int shift_of(const T* row) {
 }
 // A row's pieces on their way into shared memory: every thread copies its own and reads them back itself, so nothing waits for
 // another thread.  What is behind the row's end is not read (zeros come for it, and slots of pieces behind it are zeros from the
-// start); what is in front of the row's start is the end of the row before, and reads as it is, but for a row with no whole piece
-// in front of it (`first_row`), which comes element by element if it starts off 16 bytes.
+// start); what is in front of the row's start is the end of the row before, and reads as it is, but in front of the tensor, where a
+// piece comes element by element.
 template <class T>
 __device__ __forceinline__ int piece_bytes(int c0, int C) {
     const int left = (C - c0) * static_cast<int>(sizeof(T));
     return left < 0 ? 0 : left < 16 ? left : 16;
 }
+// from: the place of the piece's first element, of column c0; base: the tensor
 template <class T, bool SHIFT>
-__device__ __forceinline__ void copy_piece(uint4* slot, const T* row, int c0, int bytes, bool first_row) {
-    if (SHIFT && c0 < 0 && first_row) {
+__device__ __forceinline__ void copy_piece(uint4* slot, const T* from, int c0, int bytes, const void* base) {
+    if (SHIFT && c0 < 0 && reinterpret_cast<uintptr_t>(from) < reinterpret_cast<uintptr_t>(base)) {
         alignas(16) T v[kPiece<T>];
 #pragma unroll
-        for (int e = 0; e < kPiece<T>; ++e) v[e] = c0 + e >= 0 && e * static_cast<int>(sizeof(T)) < bytes ? row[c0 + e] : from_float<T>(0.0f);
+        for (int e = 0; e < kPiece<T>; ++e) v[e] = c0 + e >= 0 && e * static_cast<int>(sizeof(T)) < bytes ? from[e] : from_float<T>(0.0f);
         *slot = *reinterpret_cast<const uint4*>(v);
     } else if (bytes) {
-        copy_async<16>(slot, row + c0, SHIFT ? bytes : 16);
+        copy_async<16>(slot, from, SHIFT ? bytes : 16);
     }
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -146,20 +147,29 @@ __device__ __forceinline__ uint4 mask_of(int c0, int C) {
 }
 __device__ __forceinline__ uint4 masked(uint4 v, uint4 m) { return make_uint4(v.x & m.x, v.y & m.y, v.z & m.z, v.w & m.w); }
 template <class T, bool SHIFT>
-__device__ __forceinline__ void store_piece(T* row, int c0, int C, uint4 raw) {
+__device__ __forceinline__ void store_piece(T* to, int c0, int C, uint4 raw) {
     if (!SHIFT || (c0 >= 0 && c0 + kPiece<T> <= C)) {
-        if (!SHIFT && c0 >= C) return;
-        *reinterpret_cast<uint4*>(row + c0) = raw;
+        if (SHIFT || c0 < C) *reinterpret_cast<uint4*>(to) = raw;
         return;
     }
     const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
     for (int e = 0; e < kPiece<T>; ++e)
         if (static_cast<unsigned>(c0 + e) < static_cast<unsigned>(C)) {
-            if constexpr (sizeof(T) == 4) reinterpret_cast<unsigned*>(row)[c0 + e] = w[e];
-            else reinterpret_cast<unsigned short*>(row)[c0 + e] = static_cast<unsigned short>(w[e / 2] >> 16 * (e % 2));
+            if constexpr (sizeof(T) == 4) reinterpret_cast<unsigned*>(to)[e] = w[e];
+            else reinterpret_cast<unsigned short*>(to)[e] = static_cast<unsigned short>(w[e / 2] >> 16 * (e % 2));
         }
 }
+// Places of a thread's first piece in the rows that it has in turn
+template <class T>
+struct Walk {
+    T* at;
+    long long step;
+    __device__ __forceinline__ Walk(const void* base, long long pitch, long long row, long long step_rows, int c0)
+        : at(static_cast<T*>(const_cast<void*>(base)) + row * pitch + c0), step(step_rows * pitch) {}
+    __device__ __forceinline__ T* of(int j, int offset) const { return at + j * step + offset; }
+    __device__ __forceinline__ void on(int rows) { at += rows * step; }
+};
 // Parameters of a piece's columns (`none` outside the row, and where there is no parameter)
 template <class T, bool SHIFT>
 __device__ __forceinline__ void load_params(const void* p, bool wide, int c0, int C, float none, float2 (&v)[kPiece<T> / 2]) {
