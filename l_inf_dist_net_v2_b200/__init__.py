@@ -9,8 +9,8 @@ from .modules import NormDistBase, NormDist, NormDistConv, MeanShift, apply_if_n
 
 from .bound_modules import BoundSequential, BoundTanh, BoundReLU, BoundLinear, BoundFinalLinear  # noqa: F401
 from .head import (layer_norm, dropout, dropout_add_layer_norm, quantize_rows, layer_norm_quantized, int8_linear,  # noqa: F401
-                   LayerNorm, Dropout, Int8Linear)
-from .models import MLPModel, HybridModel, check_inf_and_eval, set_p_norm  # noqa: F401
+                   LayerNorm, Dropout, Int8Linear, ResidualHead, QuantizedHead)
+from .models import MLPModel, HybridModel, ResidualModel, check_inf_and_eval, set_p_norm  # noqa: F401
 from .attack import AttackPGD  # noqa: F401
 from . import losses  # noqa: F401
 

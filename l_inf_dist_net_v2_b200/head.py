@@ -13,7 +13,7 @@ import torch.nn as nn
 from . import norm_dist_cuda as _C
 
 __all__ = ["layer_norm", "dropout", "dropout_add_layer_norm", "quantize_rows", "layer_norm_quantized", "int8_linear", "LayerNorm",
-           "Dropout", "Int8Linear"]
+           "Dropout", "Int8Linear", "ResidualHead", "QuantizedHead"]
 
 _ACTIVATIONS = {"none": 0, "relu": 1, "tanh": 2}
 
@@ -157,3 +157,52 @@ class Int8Linear(nn.Module):
 
     def extra_repr(self):
         return f"{self.weight.size(1)}, {self.weight.size(0)}, bias={self.bias is not None}, activation={self.activation}"
+
+
+class ResidualHead(nn.Module):
+    """A pre-norm residual feed-forward head: every block adds dropout(down(relu(up(norm(h))))) to the stream h, and the classes are a
+    linear map of the last norm.  Between the products of neighbouring blocks there is one kernel each way: dropout, residual and the
+    next block's norm.  It has no interval bounds, so what it answers is not certified."""
+
+    def __init__(self, width, hidden, num_classes=10, blocks=2, dropout=0.1, eps=1e-5, seed=None):
+        super().__init__()
+        self.up = nn.ModuleList(nn.Linear(width, hidden) for _ in range(blocks))
+        self.down = nn.ModuleList(nn.Linear(hidden, width) for _ in range(blocks))
+        self.norm = nn.ModuleList(LayerNorm(width, eps) for _ in range(blocks + 1))
+        self.drop = nn.ModuleList(Dropout(dropout, None if seed is None else seed + i) for i in range(blocks))
+        self.final = nn.Linear(width, num_classes)
+
+    def forward(self, h):
+        y = self.norm[0](h)
+        for up, down, norm, drop in zip(self.up, self.down, self.norm[1:], self.drop):
+            p, (seed, offset) = (drop.p, drop.draw()) if self.training else (0.0, (0, 0))
+            y, h = dropout_add_layer_norm(down(torch.relu(up(y))), h, norm.weight, norm.bias, p, seed, offset, norm.eps)
+        return self.final(y)
+
+    def quantized(self):
+        """The head as it answers in 8-bit integers, from the weights as they are now."""
+        return QuantizedHead(self)
+
+
+class QuantizedHead(nn.Module):
+    """A residual head whose products are in 8-bit integers: the norms' rows leave as integers, hidden rows are quantised in the product
+    that takes them.  It answers only; the stream has the type that it comes in."""
+
+    def __init__(self, head):
+        super().__init__()
+        self.eps = head.norm[0].eps
+        self.up = nn.ModuleList(Int8Linear.from_linear(m, "relu") for m in head.up)
+        self.down = nn.ModuleList(Int8Linear.from_linear(m) for m in head.down)
+        self.final = Int8Linear.from_linear(head.final)
+        for i, m in enumerate(head.norm):
+            self.register_buffer(f"norm_weight{i}", m.weight.detach().clone())
+            self.register_buffer(f"norm_bias{i}", m.bias.detach().clone())
+
+    def _normed(self, i, h):
+        return layer_norm_quantized(h, getattr(self, f"norm_weight{i}"), getattr(self, f"norm_bias{i}"), self.eps)
+
+    @torch.no_grad()
+    def forward(self, h):
+        for i, (up, down) in enumerate(zip(self.up, self.down)):
+            h = h + down(up(self._normed(i, h), out_dtype=h.dtype))
+        return self.final(self._normed(len(self.up), h), out_dtype=h.dtype)

@@ -18,9 +18,10 @@ import torch.nn as nn
 
 from . import norm_dist_cuda as _C
 from .bound_modules import BoundFinalLinear, BoundLinear, BoundSequential, BoundTanh
+from .head import ResidualHead
 from .modules import NormDist, NormDistBase
 
-__all__ = ["MLPModel", "HybridModel", "check_inf_and_eval", "set_p_norm"]
+__all__ = ["MLPModel", "HybridModel", "ResidualModel", "check_inf_and_eval", "set_p_norm"]
 
 
 def check_inf_and_eval(model):
@@ -100,3 +101,33 @@ class HybridModel(nn.Module):
         if targets is not None and (lower is None or upper is None):
             lower, upper = dist - eps, dist + eps
         return self.fc_final(*self.fc_linear((dist, lower, upper)), targets=targets)
+
+
+class ResidualModel(nn.Module):
+    """depth - 2 distance layers (all with mean shift, no bias) followed by a residual feed-forward head (head.py); not in the
+    reference.  The distance layers are 1-Lipschitz, the head is not bounded: model(x) -> logits, without a worst case.
+
+    `quantize()` makes it answer with the head's products in 8-bit integers (in eval mode, without gradients) until `train()`."""
+
+    def __init__(self, depth, width, input_dim, hidden=512, num_classes=10, blocks=2, dropout=0.1, std=1.0, identity_val=None,
+                 seed=None):
+        super().__init__()
+        pixels = input_dim[0] * input_dim[1] * input_dim[2]
+        self.fc_dist = _dist_stack([pixels] + [width] * (depth - 2), False, std, identity_val)
+        self.head = ResidualHead(width, hidden, num_classes, blocks, dropout, seed=seed)
+        self._answer = []  # the quantised head, if there is one (in a list: it is no part of what is trained or saved)
+
+    def quantize(self):
+        self.eval()
+        self._answer = [self.head.quantized()]
+        return self
+
+    def train(self, mode=True):
+        self._answer = []
+        return super().train(mode)
+
+    def forward(self, x):
+        features, _, _ = self.fc_dist(_flat_triple(x, 0, None, None, False))
+        if self._answer and not torch.is_grad_enabled():
+            return self._answer[0](features)
+        return self.head(features)

@@ -498,3 +498,87 @@ def test_layers_train_and_answer():
     again = ldn.Int8Linear(torch.zeros(20, 96, device="cuda"), torch.zeros(20, device="cuda"))
     again.load_state_dict(small.state_dict())
     assert torch.equal(again(n), small(n))
+
+
+# ---- the head as it is used -----------------------------------------------------------------------------------------------------------
+def _model(**kwargs):
+    torch.manual_seed(0)
+    model = ldn.ResidualModel(4, 96, [1, 8, 8], hidden=128, blocks=3, seed=11, **kwargs).cuda()
+    ldn.set_p_norm(model, float("inf"))
+    return model
+
+
+def test_a_head_is_its_formula():
+    model = _model(dropout=0.2)
+    head, features = model.head, _rows(50, 96, F32, 1).requires_grad_()
+    got = head(features)
+
+    def plain(h):
+        h = h.double()
+        y = oracle.norm(h, head.norm[0].weight, head.norm[0].bias, 1e-5)[0]
+        for i in range(3):
+            u = torch.relu(y @ head.up[i].weight.double().t() + head.up[i].bias.double()) @ head.down[i].weight.double().t() + head.down[i].bias.double()
+            h = h + torch.where(oracle.keep((50, 96), 0.2, 11 + i, 0).cuda(), u / 0.8, 0.0)
+            y = oracle.norm(h, head.norm[i + 1].weight, head.norm[i + 1].bias, 1e-5)[0]
+        return y @ head.final.weight.double().t() + head.final.bias.double()
+    want = plain(features)
+    # four products of up to 128 terms, three blocks: some hundred roundings of numbers of the stream's size
+    assert (got - want).abs().max() <= 1000 * oracle.EPS32 * want.abs().max()
+    v = torch.randn(50, 10, **_gen(2))
+    params = [p for p in head.parameters()]
+    for a, b in zip(torch.autograd.grad(got, [features] + params, v), torch.autograd.grad((want * v).sum(), [features] + params)):
+        assert (a - b).abs().max() <= 4000 * oracle.EPS32 * b.abs().max()
+
+
+def test_a_model_learns_and_answers():
+    model = _model()
+    x = torch.rand(64, 1, 8, 8, **_gen(1))
+    targets = torch.arange(64, device="cuda") % 10
+    from l_inf_dist_net_v2_b200.optim import FusedAdam
+    optimizer = FusedAdam(model.parameters(), lr=1e-3)
+    losses = []
+    for _ in range(40):
+        loss = torch.nn.functional.cross_entropy(model(x), targets)
+        optimizer.zero_grad()
+        loss.backward()
+        optimizer.step()
+        losses.append(loss.item())
+    assert losses[-1] < 0.5 * losses[0]
+    with torch.no_grad():
+        want = model.eval()(x)
+        assert torch.equal(model(x), want)  # no dropout
+        got = model.quantize()(x)
+        assert (got - want).abs().max() <= 0.1 * want.abs().max() and (got.argmax(1) == want.argmax(1)).float().mean() >= 0.9
+        assert torch.equal(model(x[:1]), got[:1]) and torch.equal(model(x[:30]), got[:30])  # whatever the kernel for the batch
+    assert not torch.equal(model.train()(x), want)
+    again = _model()
+    again.load_state_dict(model.state_dict())
+    with torch.no_grad():
+        assert torch.equal(again.eval()(x), model.eval()(x))
+
+
+def test_a_training_step_in_a_graph_draws_again():
+    """Masks of a replay follow the words on the device, gradients those of the same replay."""
+    x, r = (_rows(20, 64, F32, k).requires_grad_() for k in (1, 2))
+    w, b = (t.requires_grad_() for t in _params(64, F32, 3))
+    g = torch.randn(20, 64, **_gen(4))
+    state = torch.tensor([5, 0], device="cuda")
+
+    def step():
+        y, h = ldn.dropout_add_layer_norm(x, r, w, b, 0.5, state)
+        grads = torch.autograd.grad((y, h), (x, r), (g, g))
+        state[1] += 1
+        return h, grads[0]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        h, gx = step()
+    for offset in (1, 2, 3):
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = oracle.keep((20, 64), 0.5, 5, offset).cuda()
+        assert torch.equal(h, r + oracle.dropped(x, kept, 0.5)) and not gx[~kept].any()
