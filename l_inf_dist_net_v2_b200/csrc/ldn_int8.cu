@@ -114,5 +114,6 @@ extern "C" LDN_API int ldn_int8_linear_float(const void* x, long long pitch, int
     if ((r = launch_quantize(x, pitch, M, K, x_type, q, pitch_q, scale, st)) != kOk) return r;
     a.q = q;
     a.scale = scale;
+    a.w_early = !o.copy_w;
     return launch_product(a, type, o, scratch.base + bytes_q + bytes_scale, scratch.status, ctx, st);
 }

@@ -14,6 +14,8 @@ struct ProductArgs {
     long long M;
     int N, K, activation;
     void* out;  // [M][N]
+    bool w_early = false;  // the weight may be read before the kernel in front is done: that is this call's own quantising, which lets
+                           // this one begin only when all in front of it is
 };
 
 #ifdef __CUDACC__

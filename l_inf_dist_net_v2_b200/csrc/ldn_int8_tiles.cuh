@@ -169,6 +169,20 @@ __device__ __forceinline__ void store16(const ProductArgs& a, const int (&sum)[1
     }
 }
 
+// Place in a ring of N stages, and the parity of its turn: counted, as one thread issues a stage's work and a division of the count is
+// longer than that (10000 tokens, 5120 -> 5120: pairs' products 145 us with the counts divided, 190 with the tile's, too)
+template <int N>
+struct RingPlace {
+    int stage = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++stage == N) {
+            stage = 0;
+            parity ^= 1;
+        }
+    }
+};
+
 // ---- tiles of 128 outputs x TOKENS, the terms split over a cluster ----------------------------------------------------------------
 // For up to some hundred tokens the weight's bytes are what takes the time, and there are fewer tiles than SMs: up to eight CTAs of
 // a cluster have a share of the terms each, and add their integer sums up in shared memory, in which no order shows.
@@ -212,6 +226,15 @@ product_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         tma_prefetch_desc(&map_w);
         tma_prefetch_desc(&map_q);
     }
+    const int early = a.w_early ? (k_count < kStages ? k_count : kStages) : 0;
+    auto load_weight = [&](int i, int slot) {
+        mbar_expect_tx(&B->full[slot], kBytes);
+        load_tile(stage + slot * kBytes, &map_w, &B->full[slot], (k_first + i) * kTerms, n0);
+    };
+    __syncwarp();
+    if (warp == 0 && elected())
+        for (int i = 0; i < early; ++i) load_weight(i, i);
+    __syncwarp();
     stream_order_begin();  // (tensor memory is asked for behind it: whoever is in front has given theirs back)
     if (warp == 1) tensor_alloc<1>(&B->tensor, kColumns);
     tensor_fence_before();
@@ -225,15 +248,14 @@ product_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     if (warp == 0) {
         if (elected()) {
             int i = 0;
-            for (; i < k_count; ++i) {
-                const int s = i % kStages;
-                if (i >= kStages && !mbar_wait_bounded(&B->empty[s], (i / kStages - 1) & 1)) {
+            RingPlace<kStages> at;
+            for (; i < k_count; ++i, at.next()) {
+                if (i >= kStages && !mbar_wait_bounded(&B->empty[at.stage], at.parity ^ 1)) {
                     give_up();
                     break;
                 }
-                mbar_expect_tx(&B->full[s], kBytes);
-                load_tile(stage + s * kBytes, &map_w, &B->full[s], (k_first + i) * kTerms, n0);
-                load_tile(stage + s * kBytes + kLaneBytes, &map_q, &B->full[s], (k_first + i) * kTerms, static_cast<int>(m0));
+                if (i >= early) load_weight(i, at.stage);
+                load_tile(stage + at.stage * kBytes + kLaneBytes, &map_q, &B->full[at.stage], (k_first + i) * kTerms, static_cast<int>(m0));
             }
             for (int j = i < kStages ? 0 : i - kStages; j < i; ++j)  // (no copy is in flight when the block ends)
                 if (!mbar_wait_bounded(&B->full[j % kStages], (j / kStages) & 1)) give_up();
@@ -241,16 +263,17 @@ product_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     } else if (warp == 1) {
         if (elected()) {
             bool fine = true;
-            for (int i = 0; i < k_count; ++i) {
-                const int s = i % kStages;
-                fine = mbar_wait_bounded(&B->full[s], (i / kStages) & 1);
+            RingPlace<kStages> at;
+            const uint64_t w0 = operand(stage);
+            for (int i = 0; i < k_count; ++i, at.next()) {
+                fine = mbar_wait_bounded(&B->full[at.stage], at.parity);
                 if (!fine) break;
                 tensor_fence_after();
-                const uint64_t w = operand(stage + s * kBytes), q = operand(stage + s * kBytes + kLaneBytes);
+                const uint64_t w = w0 + at.stage * (kBytes >> 4), q = w + (kLaneBytes >> 4);
 #pragma unroll
                 for (int k = 0; k < kTerms / 32; ++k)
                     multiply<1>(tensor, w + 2 * k, q + 2 * k, product_kind(kLanes, TOKENS), i > 0 || k > 0);
-                arrive_when_done<1>(&B->empty[s]);
+                arrive_when_done<1>(&B->empty[at.stage]);
             }
             arrive_when_done<1>(&B->done);
             if (!fine) give_up();
@@ -407,19 +430,19 @@ product_pairs_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         if (elected()) {
             long long i = 0;
             bool fine = true;
+            RingPlace<kPairStages> at;
             for (int tile = pair; tile < tiles && fine; tile += pairs) {
                 const int n = (tile % tiles_n) * 2 * kLanes + rank * kLanes, m = (tile / tiles_n) * kPairTokens + rank * kLanes;
-                for (int k = 0; k < kt; ++k, ++i) {
-                    const int s = static_cast<int>(i % kPairStages);
-                    if (i >= kPairStages && !mbar_wait_bounded(&B->empty[s], (i / kPairStages - 1) & 1)) {
+                for (int k = 0; k < kt; ++k, ++i, at.next()) {
+                    if (i >= kPairStages && !mbar_wait_bounded(&B->empty[at.stage], at.parity ^ 1)) {
                         fine = false;
                         give_up();
                         break;
                     }
-                    const uint32_t full = in_cta(&B->full[s], 0);
-                    if (rank == 0) mbar_expect_tx(&B->full[s], 2 * kPairBytes);
-                    load_tile_of_pair(stage + s * kPairBytes, &map_w, full, k * kTerms, n);
-                    load_tile_of_pair(stage + s * kPairBytes + kLaneBytes, &map_q, full, k * kTerms, m);
+                    const uint32_t full = in_cta(&B->full[at.stage], 0);
+                    if (rank == 0) mbar_expect_tx(&B->full[at.stage], 2 * kPairBytes);
+                    load_tile_of_pair(stage + at.stage * kPairBytes, &map_w, full, k * kTerms, n);
+                    load_tile_of_pair(stage + at.stage * kPairBytes + kLaneBytes, &map_q, full, k * kTerms, m);
                 }
             }
             // (nothing is in flight towards this CTA when it ends: neither its copies nor the pair's arrivals)
@@ -432,26 +455,26 @@ product_pairs_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         }
     } else if (warp == 1) {
         if (rank == 0 && elected()) {
-            long long i = 0;
             bool fine = true;
             int t = 0;
+            RingPlace<kPairStages> at;
+            const uint64_t w0 = operand(stage);
             for (int tile = pair; tile < tiles && fine; tile += pairs, ++t) {
                 if (t >= 2 && !wait_bounded_cluster(&B->taken[t & 1], (t / 2 - 1) & 1)) {
                     fine = false;
                     break;
                 }
                 tensor_fence_after();
-                for (int k = 0; k < kt; ++k, ++i) {
-                    const int s = static_cast<int>(i % kPairStages);
-                    fine = mbar_wait_bounded(&B->full[s], (i / kPairStages) & 1);
+                for (int k = 0; k < kt; ++k, at.next()) {
+                    fine = mbar_wait_bounded(&B->full[at.stage], at.parity);
                     if (!fine) break;
                     tensor_fence_after();
-                    const uint64_t w = operand(stage + s * kPairBytes), q = operand(stage + s * kPairBytes + kLaneBytes);
+                    const uint64_t w = w0 + at.stage * (kPairBytes >> 4), q = w + (kLaneBytes >> 4);
 #pragma unroll
                     for (int u = 0; u < kTerms / 32; ++u)
                         multiply<2>(tensor + (t & 1) * kPairTokens, w + 2 * u, q + 2 * u, product_kind(2 * kLanes, kPairTokens),
                                     k > 0 || u > 0);
-                    arrive_when_done<2>(&B->empty[s]);
+                    arrive_when_done<2>(&B->empty[at.stage]);
                 }
                 if (fine) arrive_when_done<2>(&B->sums[t & 1]);
             }

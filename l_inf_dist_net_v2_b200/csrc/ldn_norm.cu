@@ -15,7 +15,8 @@ constexpr int kRowThreads = 256;
 // Any length, alignment and pitch: a block per row, one element per thread and step; the row is read again for every pass.
 template <class T, Form F>
 __global__ void __launch_bounds__(kRowThreads) norm_rows_kernel(NormArgs a) {
-    stream_order_begin();
+    stream_order_wait();  // (quantised rows: what comes behind may read what was there before this kernel)
+    stream_order_release();
     __shared__ float slots[kRowThreads / 32];
     Generator gen;
     if constexpr (F == Form::Joined) gen = generator_of(a.drop);

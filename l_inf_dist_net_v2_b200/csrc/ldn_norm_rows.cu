@@ -56,7 +56,12 @@ __device__ __forceinline__ void store_integers(signed char* to, int c0, int C, c
 template <class T, Form F, int ITEMS, bool GROUP, bool SHIFT>
 __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPiece<T>), !GROUP && ITEMS * kPiece<T> == 16 ? (F == Form::Quantised ? 4 : 2) : 1)
 norm_registers_kernel(NormArgs a, int lanes, int depth) {
-    stream_order_begin();
+    if constexpr (F == Form::Quantised) {  // (what comes behind may read what was there before this kernel)
+        stream_order_wait();
+        stream_order_release();
+    } else {
+        stream_order_begin();
+    }
     constexpr int V = kPiece<T>, S = kStreams<F>, R = rows_at_once(F, ITEMS * V, GROUP);
     constexpr bool kParams = F != Form::Quantised, kKeep = kParams && ITEMS * V <= 16;
     __shared__ float slots[2 * RowSum::kSlots];
