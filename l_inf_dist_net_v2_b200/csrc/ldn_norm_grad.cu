@@ -27,9 +27,10 @@ template <class T, bool JOINED, int ITEMS, bool GROUP, bool SHIFT>
 __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPiece<T>), !GROUP && ITEMS * kPiece<T> == 16 ? 2 : 1) norm_grad_registers_kernel(NormGradArgs a, int lanes, int depth) {
     stream_order_begin();
     constexpr int V = kPiece<T>, S = kStreams<JOINED>, R = rows_at_once(JOINED, ITEMS * V, GROUP);
+    constexpr bool kStatsCome = !GROUP && sizeof(T) == 2;
     constexpr bool kKeep = ITEMS * V <= 16;  // the columns' weights stay in registers, too
     __shared__ float slots[2 * RowSum::kSlots];
-    extern __shared__ uint4 ring[];  // [depth][row][stream][item][thread]; at the end, groups: [warp][2][C] floats
+    extern __shared__ uint4 ring[];  // [depth][row][stream][item][thread], then [warp][depth][row][2] floats; at the end, groups: [warp][2][C] floats
     RowSum reduce{lanes, slots, 0};
     Generator gen;
     if constexpr (JOINED) gen = generator_of(a.drop);
@@ -60,7 +61,14 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPi
     long long row0 = mine, index = mine * a.C + c0;
     uint4* own = ring + threadIdx.x;
     auto slot_of = [&](int stage, int j, int stream, int i) { return own + (((stage * R + j) * S + stream) * ITEMS + i) * blockDim.x; };
+    float* stats = reinterpret_cast<float*>(ring + static_cast<size_t>(depth) * R * S * ITEMS * blockDim.x) + (threadIdx.x >> 5) * depth * 2 * R;
+    const float* from_stat = ((threadIdx.x & 1) ? a.rstd : a.mean) + mine + (threadIdx.x & 31) / 2 * step;
     auto fetch = [&](int stage) {
+        if (kStatsCome) {
+            const int k = threadIdx.x & 31;  // mean and 1 / deviation of row k / 2
+            if (k < 2 * R && k / 2 < to_fetch) copy_async<4>(stats + stage * 2 * R + k, from_stat, 4);
+            from_stat += R * step;
+        }
 #pragma unroll
         for (int j = 0; j < R; ++j)
             if (j < to_fetch) {
@@ -83,6 +91,18 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPi
         for (int i = 0; i < ITEMS; ++i)
             if (!bytes[i]) own[(d * ITEMS + i) * blockDim.x] = make_uint4(0u, 0u, 0u, 0u);
     for (int d = 0; d < depth; ++d) fetch(d);
+    // The statistics of the next turn's rows: loaded when they were wanted, they were what 16-bit rows waited for most (16384 x 5120:
+    // 119 us, 108 so).  Blocks of such have them come with the rows, a warp's first lanes for the warp; groups have registers for them;
+    // 32-bit blocks, with more bytes to wait for, load them at once (8192 x 5120: 92 us, 97 the other way).
+    float next_mean[R], next_rstd[R];
+    auto fetch_stats = [&](long long row, int rows) {
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            next_mean[j] = j < rows ? a.mean[row + j * step] : 0.0f;
+            next_rstd[j] = j < rows ? a.rstd[row + j * step] : 0.0f;
+        }
+    };
+    if (GROUP) fetch_stats(row0, to_make);
     int stage = 0;
     // (a warp's groups take part in its shuffles whether they have a row or not: as many turns as the block's first has)
     const long long block_first = static_cast<long long>(blockIdx.x) * per_block;
@@ -90,12 +110,30 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPi
     for (int turn = 0; turn < turns; ++turn) {
         auto live = [&](int j) { return j < to_make; };
         float mean[R], rstd[R], s[2 * R];
+        if constexpr (!GROUP && !kStatsCome) {
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            mean[j] = live(j) ? a.mean[row0 + j * step] : 0.0f;
-            rstd[j] = live(j) ? a.rstd[row0 + j * step] : 0.0f;
+            for (int j = 0; j < R; ++j) {
+                mean[j] = live(j) ? a.mean[row0 + j * step] : 0.0f;
+                rstd[j] = live(j) ? a.rstd[row0 + j * step] : 0.0f;
+            }
         }
         copies_wait(depth);
+        if constexpr (GROUP) {
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                mean[j] = next_mean[j];
+                rstd[j] = next_rstd[j];
+            }
+            fetch_stats(row0 + R * step, to_make - R);
+        } else if constexpr (kStatsCome) {
+            __syncwarp();  // (the lane that copied them has waited)
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                mean[j] = live(j) ? stats[stage * 2 * R + 2 * j] : 0.0f;
+                rstd[j] = live(j) ? stats[stage * 2 * R + 2 * j + 1] : 0.0f;
+            }
+            __syncwarp();
+        }
         // (outside the row the gradient is 0, and x a number; where there is no row, all is 0)
         auto piece_of = [&](int j, int stream, int i) {
             uint4 raw = live(j) ? *slot_of(stage, j, stream, i) : make_uint4(0u, 0u, 0u, 0u);
@@ -222,7 +260,7 @@ bool plan_of(bool joined, const NormGradArgs& a, int type, const DeviceCtx* ctx,
         !plan_elements(a.C, size, shift, joined, &p))
         return false;
     const int elements = p.items * (16 / size), R = rows_at_once(joined, elements, p.group);
-    const long long row_bytes = static_cast<long long>(R) * (joined ? 3 : 2) * p.items * p.threads * 16, most_smem = ctx->max_smem_optin - 2560;
+    const long long row_bytes = static_cast<long long>(R) * (joined ? 3 : 2) * p.items * p.threads * 16, most_smem = ctx->max_smem_optin - 4096;
     // blocks per SM: up to 102 registers per thread, 128 with 32 elements, and rows under way behind those that are summed
     int per_sm = 65536 / (p.threads * (elements <= 16 ? 102 : 128));
     if (per_sm > 4) per_sm = 4;
@@ -237,7 +275,7 @@ bool plan_of(bool joined, const NormGradArgs& a, int type, const DeviceCtx* ctx,
     const long long turns = (needed + R * blocks - 1) / (R * blocks);
     if (turns < s->depth) s->depth = static_cast<int>(turns);
     s->blocks = static_cast<int>(blocks);
-    s->smem = static_cast<size_t>(s->depth) * row_bytes;
+    s->smem = static_cast<size_t>(s->depth) * (row_bytes + (p.threads / 32) * R * 2 * sizeof(float));
     const size_t columns = p.group ? static_cast<size_t>(kGroupThreads / 32) * 2 * a.C * sizeof(float) : 0;
     if (s->smem < columns) s->smem = columns;
     return true;
