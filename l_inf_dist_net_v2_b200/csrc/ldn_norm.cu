@@ -133,8 +133,9 @@ __global__ void __launch_bounds__(kColumns * kColumnLanes) norm_grad_columns_ker
     }
 }
 
-// The parts in order: a thread has a column of one of the two sums and every 32nd part, eight of them under way.
-constexpr int kFoldLanes = 32;
+// The parts in order: a thread has a column of one of the two sums and every 16th part, ten of them under way.  Blocks are small
+// enough for all of them to be on the device at once (of 1024 threads, the last ones of 5120 columns came in a second wave: 9 us).
+constexpr int kFoldLanes = 16, kFoldAhead = 10;
 template <class T>
 __global__ void __launch_bounds__(kColumns * kFoldLanes) norm_grad_fold_kernel(const float* parts, int count, int C, bool wide,
                                                                                void* grad_weight, void* grad_bias) {
@@ -144,22 +145,25 @@ __global__ void __launch_bounds__(kColumns * kFoldLanes) norm_grad_fold_kernel(c
     const float* from = parts + static_cast<long long>(blockIdx.y) * C + c;
     float s = 0.0f;
     if (c < C)
-        for (int i = part; i < count; i += 8 * kFoldLanes) {
-            float v[8];
+        for (int i = part; i < count; i += kFoldAhead * kFoldLanes) {
+            float v[kFoldAhead];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
+            for (int u = 0; u < kFoldAhead; ++u) {
                 const int k = i + u * kFoldLanes;
                 v[u] = k < count ? from[2LL * k * C] : 0.0f;
             }
 #pragma unroll
-            for (int u = 0; u < 8; ++u) s += v[u];
+            for (int u = 0; u < kFoldAhead; ++u) s += v[u];
         }
     sums[part][lane] = s;
     __syncthreads();
-    // a warp adds up a column's sums
-    s = warp_sum(sums[lane][part]);
+    // a warp adds up two columns' sums, half of it each
+    const int column = 2 * part + lane / kFoldLanes;
+    s = sums[lane % kFoldLanes][column];
+#pragma unroll
+    for (int d = kFoldLanes / 2; d > 0; d /= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
     void* to = blockIdx.y == 0 ? grad_weight : grad_bias;
-    if (lane == 0 && blockIdx.x * kColumns + part < C && to) set_param<T>(to, wide, blockIdx.x * kColumns + part, s);
+    if (lane % kFoldLanes == 0 && blockIdx.x * kColumns + column < C && to) set_param<T>(to, wide, blockIdx.x * kColumns + column, s);
 }
 
 bool params_fit(int type, int param_type, const void* weight, const void* bias) {

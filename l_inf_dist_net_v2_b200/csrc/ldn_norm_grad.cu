@@ -206,13 +206,23 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPi
     if constexpr (!GROUP) {
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            const int c0 = (lane + i * lanes) * V - shift;
+            const int c = column(i);
+            if constexpr (!SHIFT) {
+                if (c >= a.C) continue;
 #pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (static_cast<unsigned>(c0 + e) < static_cast<unsigned>(a.C)) {
-                    part[c0 + e] = at_of(sum_w[i], e);
-                    part[a.C + c0 + e] = at_of(sum_b[i], e);
+                for (int e = 0; e < V / 2; e += 2) {
+                    *reinterpret_cast<float4*>(part + c + 2 * e) = make_float4(sum_w[i][e].x, sum_w[i][e].y, sum_w[i][e + 1].x, sum_w[i][e + 1].y);
+                    *reinterpret_cast<float4*>(part + a.C + c + 2 * e) =
+                        make_float4(sum_b[i][e].x, sum_b[i][e].y, sum_b[i][e + 1].x, sum_b[i][e + 1].y);
                 }
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (static_cast<unsigned>(c + e) < static_cast<unsigned>(a.C)) {
+                        part[c + e] = at_of(sum_w[i], e);
+                        part[a.C + c + e] = at_of(sum_b[i], e);
+                    }
+            }
         }
     } else {
         // a warp's groups add to its columns in turn, then the warps' are added up
