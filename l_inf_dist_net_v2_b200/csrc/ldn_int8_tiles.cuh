@@ -487,6 +487,7 @@ product_pairs_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         const int quarter = warp & 3, turn = (warp - 2) >> 2;
         T* out = static_cast<T*>(a.out);
         int t = 0;
+        bool lost = false;  // the products of a tile did not come in time: this warp stores nothing more, but meets the others
         for (int tile = pair; tile < tiles; tile += pairs, ++t) {
             const int n = (tile % tiles_n) * 2 * kLanes + rank * kLanes + quarter * 32 + lane;
             const long long m0 = static_cast<long long>(tile / tiles_n) * kPairTokens;
@@ -499,11 +500,14 @@ product_pairs_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             static_assert(kPairTokens == 32 * kStoreWarps, "a thread each");
             token_scale[threadIdx.x - 64] = m0 + threadIdx.x - 64 < a.M ? a.scale[m0 + threadIdx.x - 64] : 0.0f;
             asm volatile("bar.sync 1, %0;" ::"n"(32 * kStoreWarps) : "memory");  // (a tile later all have read the one before)
-            if (!mbar_wait_bounded(&B->sums[t & 1], (t / 2) & 1)) {
+            // (one answer for the whole warp, whose loads and stores are common; and no warp leaves the loop, as the barrier above
+            // counts all of them in every turn)
+            if (lost) continue;
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&B->sums[t & 1], (t / 2) & 1))) {
                 give_up();
-                break;
+                lost = true;
+                continue;
             }
-            __syncwarp();
             tensor_fence_after();
             const int columns = a.M - m0 < kPairTokens ? static_cast<int>(a.M - m0) : kPairTokens;
             T* to = out + (m0 + 16 * turn) * a.N + n;
