@@ -161,7 +161,7 @@ __device__ __forceinline__ void store16(const ProductArgs& a, const int (&sum)[1
     }
     product_values(sum, scale, w_scale, bias, a.activation, v);
     char* p = reinterpret_cast<char*>(to);
-    const unsigned row = static_cast<unsigned>(a.N) * sizeof(T);  // (N is below 2^25 here, so that 15 rows are below 2^31)
+    const size_t row = static_cast<size_t>(a.N) * sizeof(T);  // (15 rows of 72 million outputs are more than 32 bits count)
     if (there && columns >= 16) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) store_once(reinterpret_cast<T*>(p + j * row), from_float<T>(v[j]));
