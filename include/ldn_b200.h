@@ -330,7 +330,8 @@ LDN_API int ldn_bound_inf_dist_forward_nograd_shifted(const float* inputL, const
 /* ---- a head behind the distance layers: layer norm, dropout, the product in 8-bit integers ------------------------- */
 /* None of these has a counterpart in the reference.  Activations are rows of C elements of one `type`; a pitch is the distance
  * of two rows in elements, and rows that the library writes without a pitch are contiguous.  Pointers need the alignment of
- * their elements only (16-byte aligned rows are faster). */
+ * their elements only (16-byte aligned rows are faster).  Rows of the norms and of integers, and outputs of the product, are at most
+ * 2^31 - 1 - 2^22. */
 #define LDN_F32 0
 #define LDN_F16 1
 #define LDN_BF16 2

@@ -53,7 +53,10 @@ void parameter(const MaybeTensor& t, const Tensor& x, const char* name) {
     TORCH_CHECK((t->scalar_type() == at::kFloat || t->scalar_type() == x.scalar_type()) && t->device() == x.device(), name,
                 " must be float32 or of the type of x, on its device");
 }
+constexpr int64_t kMostColumns = std::numeric_limits<int>::max() - (1 << 22);
+void row_fits(const Tensor& x) { TORCH_CHECK(x.size(-1) <= kMostColumns, "rows have at most ", kMostColumns, " elements, not ", x.size(-1)); }
 void parameters(const MaybeTensor& weight, const MaybeTensor& bias, const Tensor& x, double eps) {
+    row_fits(x);
     parameter(weight, x, "weight");
     parameter(bias, x, "bias");
     TORCH_CHECK(!weight.has_value() || !bias.has_value() || weight->scalar_type() == bias->scalar_type(),
@@ -318,6 +321,7 @@ void answers_only(bool grad, const char* what) { TORCH_CHECK(!grad, what, " has 
 std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
     unobserved("quantize_rows");
     activations(x, "x");
+    row_fits(x);
     answers_only(wants_grad({&x}), "quantize_rows");
     const c10::cuda::CUDAGuard guard(x.device());
     const Rows rows = rows_of(x);
@@ -357,7 +361,7 @@ Tensor int8_linear(const Tensor& x, const MaybeTensor& x_scale, const Tensor& we
     else activations(x, "x");
     bytes(weight, "weight");
     TORCH_CHECK(weight.dim() == 2 && weight.size(1) == x.size(-1), "weight must be (outputs, ", x.size(-1), "), not ", weight.sizes());
-    TORCH_CHECK(weight.size(0) >= 1 && weight.size(0) <= std::numeric_limits<int>::max(), "weight has no outputs");
+    TORCH_CHECK(weight.size(0) >= 1 && weight.size(0) <= kMostColumns, "weight must have 1 to ", kMostColumns, " outputs");
     TORCH_CHECK(weight.size(1) <= 131071, "sums of ", weight.size(1), " products do not fit 32 bits: at most 131071 do");
     TORCH_CHECK(weight.device() == x.device(), "weight must be on the device of x");
     for (const Tensor* t : {&weight_scale, at_of(bias), at_of(x_scale)})

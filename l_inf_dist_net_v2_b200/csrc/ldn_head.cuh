@@ -13,6 +13,9 @@
 namespace ldn {
 
 inline bool known_type(int type) { return type == LDN_F32 || type == LDN_F16 || type == LDN_BF16; }
+// Columns of a row and outputs of a product, at most: a column plus a grid's or a tile's size is still an int
+constexpr int kMostColumns = 0x7fffffff - (1 << 22);
+inline bool row_fits(int C) { return C > 0 && C <= kMostColumns; }
 inline int size_of(int type) { return type == LDN_F32 ? 4 : 2; }
 
 // Calls f(T()) with the element type that `type` names; `type` is known.

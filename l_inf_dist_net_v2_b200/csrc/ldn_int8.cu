@@ -57,7 +57,7 @@ int launch_product(ProductArgs a, int type, const Operands& o, char* scratch, in
 }
 
 bool product_fits(long long M, int N, int K, int activation, int type, long long pitch_w) {
-    return M >= 0 && N > 0 && K > 0 && K <= kMostTerms && activation >= LDN_NO_ACTIVATION && activation <= LDN_TANH &&
+    return M >= 0 && row_fits(N) && K > 0 && K <= kMostTerms && activation >= LDN_NO_ACTIVATION && activation <= LDN_TANH &&
            known_type(type) && pitch_w >= K;
 }
 
@@ -68,7 +68,7 @@ using namespace ldn;
 
 extern "C" LDN_API int ldn_quantize_rows(const void* x, long long pitch, long long rows, int C, int type, signed char* q,
                                          long long pitch_q, float* scale, ldn_stream_t stream) {
-    if (rows < 0 || C <= 0 || !known_type(type) || pitch_q < C) return kBadArgument;
+    if (rows < 0 || !row_fits(C) || !known_type(type) || pitch_q < C) return kBadArgument;
     if (rows == 0) return kOk;
     if (!x || !q || !scale) return kBadArgument;
     return launch_quantize(x, pitch, rows, C, type, q, pitch_q, scale, reinterpret_cast<cudaStream_t>(stream));

@@ -242,7 +242,7 @@ using namespace ldn;
 extern "C" LDN_API int ldn_layer_norm(const void* x, long long pitch, long long rows, int C, int type, const void* weight,
                                       const void* bias, int param_type, float eps, void* y, float* mean, float* rstd,
                                       ldn_stream_t stream) {
-    if (rows < 0 || C <= 0 || !known_type(type) || !params_fit(type, param_type, weight, bias) || !(eps >= 0.0f) || !mean != !rstd)
+    if (rows < 0 || !row_fits(C) || !known_type(type) || !params_fit(type, param_type, weight, bias) || !(eps >= 0.0f) || !mean != !rstd)
         return kBadArgument;
     if (rows == 0) return kOk;
     if (!x || !y) return kBadArgument;
@@ -256,7 +256,7 @@ extern "C" LDN_API int ldn_layer_norm(const void* x, long long pitch, long long 
 extern "C" LDN_API int ldn_layer_norm_backward(const void* grad_y, const void* x, long long pitch, long long rows, int C, int type,
                                                const float* mean, const float* rstd, const void* weight, int param_type,
                                                void* grad_x, void* grad_weight, void* grad_bias, ldn_stream_t stream) {
-    if (rows < 0 || C <= 0 || !known_type(type) || !known_type(param_type) || !params_fit(type, param_type, weight, grad_weight))
+    if (rows < 0 || !row_fits(C) || !known_type(type) || !known_type(param_type) || !params_fit(type, param_type, weight, grad_weight))
         return kBadArgument;
     if (rows > 0 && (!grad_y || !x || !mean || !rstd)) return kBadArgument;
     NormGradArgs a = {};
@@ -272,7 +272,7 @@ extern "C" LDN_API int ldn_dropout_add_layer_norm(const void* x, long long pitch
                                                   unsigned long long offset, const unsigned long long* state, void* h, void* y,
                                                   float* mean, float* rstd, ldn_stream_t stream) {
     NormArgs a = {};
-    if (rows < 0 || C <= 0 || !known_type(type) || !params_fit(type, param_type, weight, bias) || !(eps >= 0.0f) ||
+    if (rows < 0 || !row_fits(C) || !known_type(type) || !params_fit(type, param_type, weight, bias) || !(eps >= 0.0f) ||
         !mean != !rstd || !make_dropout(p, seed, offset, state, &a.drop))
         return kBadArgument;
     if (rows == 0) return kOk;
@@ -290,7 +290,7 @@ extern "C" LDN_API int ldn_dropout_add_layer_norm_backward(const void* grad_y, c
                                                            void* grad_x, void* grad_residual, void* grad_weight, void* grad_bias,
                                                            ldn_stream_t stream) {
     NormGradArgs a = {};
-    if (rows < 0 || C <= 0 || !known_type(type) || !known_type(param_type) || !params_fit(type, param_type, weight, grad_weight) ||
+    if (rows < 0 || !row_fits(C) || !known_type(type) || !known_type(param_type) || !params_fit(type, param_type, weight, grad_weight) ||
         !make_dropout(p, seed, offset, state, &a.drop))
         return kBadArgument;
     if (rows > 0 && (!grad_y || !h || !mean || !rstd)) return kBadArgument;
@@ -303,7 +303,7 @@ extern "C" LDN_API int ldn_dropout_add_layer_norm_backward(const void* grad_y, c
 extern "C" LDN_API int ldn_layer_norm_quantized(const void* x, long long pitch, long long rows, int C, int type, const void* weight,
                                                 const void* bias, int param_type, float eps, signed char* q, long long pitch_q,
                                                 float* scale, ldn_stream_t stream) {
-    if (rows < 0 || C <= 0 || !known_type(type) || !params_fit(type, param_type, weight, bias) || !(eps >= 0.0f) || pitch_q < C)
+    if (rows < 0 || !row_fits(C) || !known_type(type) || !params_fit(type, param_type, weight, bias) || !(eps >= 0.0f) || pitch_q < C)
         return kBadArgument;
     if (rows == 0) return kOk;
     if (!x || !q || !scale) return kBadArgument;
