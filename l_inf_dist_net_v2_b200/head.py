@@ -91,8 +91,12 @@ class LayerNorm(nn.Module):
         self.weight = nn.Parameter(torch.ones(features)) if affine else None
         self.bias = nn.Parameter(torch.zeros(features)) if affine else None
 
-    def forward(self, x):
-        return layer_norm(x, self.weight, self.bias, self.eps)
+    def forward(self, x, residual=None, p=0.0, seed=0, offset=0):
+        """The norm of x; with a residual (y, h) of `dropout_add_layer_norm`.  (Either is a call of the layer that has the parameters,
+        as hooks on layers have to see: the data-parallel wrapper updates a layer in front of its call.)"""
+        if residual is None:
+            return layer_norm(x, self.weight, self.bias, self.eps)
+        return dropout_add_layer_norm(x, residual, self.weight, self.bias, p, seed, offset, self.eps)
 
     def extra_repr(self):
         return f"{self.features}, eps={self.eps}, affine={self.weight is not None}"
@@ -176,7 +180,7 @@ class ResidualHead(nn.Module):
         y = self.norm[0](h)
         for up, down, norm, drop in zip(self.up, self.down, self.norm[1:], self.drop):
             p, (seed, offset) = (drop.p, drop.draw()) if self.training else (0.0, (0, 0))
-            y, h = dropout_add_layer_norm(down(torch.relu(up(y))), h, norm.weight, norm.bias, p, seed, offset, norm.eps)
+            y, h = norm(down(torch.relu(up(y))), h, p, seed, offset)
         return self.final(y)
 
     def quantized(self):

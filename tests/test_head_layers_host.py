@@ -1,13 +1,97 @@
 """The head's layers as a program uses them (data-parallel training, recomputation, ranks), with torch operations in place of the
 kernels, and sizes that the library refuses."""
+import copy
 import ctypes
+import os
+import socket
 
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
+import l_inf_dist_net_v2_b200 as ldn
+from head_stand_in import RowOperators
+from l_inf_dist_net_v2_b200 import head as head_module
 from l_inf_dist_net_v2_b200._lib import lib
+from l_inf_dist_net_v2_b200.parallel import OverlappedDataParallel, allreduce_mean_
 
 BAD = 1
+
+
+@pytest.fixture
+def on_the_host(monkeypatch):
+    monkeypatch.setattr(head_module, "_native", lambda: RowOperators)
+
+
+def _head(**kwargs):
+    torch.manual_seed(0)
+    return ldn.ResidualHead(12, 20, num_classes=5, blocks=2, seed=7, **{"dropout": 0.25, **kwargs})
+
+
+# ---- the data-parallel wrapper ----------------------------------------------------------------------------------------------------
+def _train_both_ways(rank):
+    """Four steps: with the wrapper, whose updates wait for a layer's next forward, and in the plain order."""
+    a = _head()
+    b = copy.deepcopy(a)
+    make = lambda params: torch.optim.Adam(params, lr=0.02)  # noqa: E731
+    wrapper, plain = OverlappedDataParallel(a, make), make(list(b.parameters()))
+    start = [p.detach().clone() for p in a.parameters()]
+    gen = torch.Generator().manual_seed(rank)
+    for _ in range(4):
+        x, t = torch.randn(8, 12, generator=gen), torch.randint(0, 5, (8,), generator=gen)
+        logits = a(x)
+        torch.nn.functional.cross_entropy(logits, t).backward()
+        wrapper.step()
+        plain.zero_grad(set_to_none=True)
+        want = b(x)
+        torch.nn.functional.cross_entropy(want, t).backward()
+        if dist.is_initialized():
+            allreduce_mean_([p.grad for p in b.parameters()])
+        plain.step()
+        if not torch.allclose(logits, want, rtol=0, atol=1e-6):
+            return False
+    wrapper.finish()
+    return all(torch.allclose(p, q, rtol=0, atol=1e-6) and not torch.equal(p, s) and p.grad is None
+               for p, q, s in zip(a.parameters(), b.parameters(), start))
+
+
+def test_the_data_parallel_wrapper_updates_every_layer(on_the_host):
+    assert _train_both_ways(0)
+
+
+def _free_port():
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        return s.getsockname()[1]
+
+
+def _ranks(rank, world, port, out_dir, what):
+    os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
+    head_module._native = lambda: RowOperators
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        with open(os.path.join(out_dir, str(rank)), "w") as f:
+            f.write(str(what(rank)))
+    finally:
+        dist.destroy_process_group()
+
+
+def _on_two_ranks(tmp_path, what):
+    mp.spawn(_ranks, args=(2, _free_port(), str(tmp_path), what), nprocs=2, join=True)
+    return [(tmp_path / str(r)).read_text() for r in range(2)]
+
+
+def test_the_data_parallel_wrapper_updates_every_layer_on_two_ranks(tmp_path):
+    assert _on_two_ranks(tmp_path, _train_both_ways) == ["True", "True"]
+
+
+def test_hooks_of_every_norm_run(on_the_host):
+    head, seen = _head(), []
+    for i, norm in enumerate(head.norm):
+        norm.register_forward_hook(lambda *_, i=i: seen.append(i))
+    head(torch.randn(3, 12))
+    assert seen == [0, 1, 2]
 
 
 # ---- sizes whose sums with a tile's or a grid's would pass 32 bits (none of these calls may launch anything) -----------------------------
