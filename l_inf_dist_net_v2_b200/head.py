@@ -104,20 +104,40 @@ class LayerNorm(nn.Module):
 
 class Dropout(nn.Module):
     """Dropout with a seed of its own (from torch's generator where none is given) and the number of calls so far as the offset, so
-    that every call draws another mask; both are in the state_dict.  In eval mode the identity."""
+    that every call draws another mask; both are in the state_dict.  In eval mode the identity.
+
+    A call that torch.utils.checkpoint makes again in a backward pass draws the mask that it drew before: every call takes a number
+    from torch's generator on the host, which the recomputation finds in the state that it had, and by it the layer knows its last
+    4096 calls."""
+
+    REMEMBERED = 4096
 
     def __init__(self, p=0.1, seed=None):
         super().__init__()
         if not 0 <= p <= 1:
             raise ValueError("p must be a probability")
         self.p = p
-        self.seed = int(torch.randint(1 << 62, ())) if seed is None else seed
+        self.seed = self._number() if seed is None else seed
         self.calls = 0
+        self._offsets = {}  # of the last calls, by their numbers
+
+    @staticmethod
+    def _number():
+        return int(torch.randint(1 << 62, (), device="cpu"))
 
     def draw(self):
         """(seed, offset) of a call."""
+        number = self._number()
+        if torch._C._current_graph_task_id() != -1:  # (in a backward pass)
+            if number not in self._offsets:
+                raise RuntimeError("dropout in a backward pass does not find the call that it repeats: recomputation has to keep the "
+                                   "generator's state (preserve_rng_state=True) and to come within the layer's next 4096 calls")
+            return self.seed, self._offsets[number]
+        offset = self._offsets[number] = self.calls
         self.calls += 1
-        return self.seed, self.calls - 1
+        if len(self._offsets) > self.REMEMBERED:
+            del self._offsets[next(iter(self._offsets))]
+        return self.seed, offset
 
     def get_extra_state(self):
         return dict(seed=self.seed, calls=self.calls)

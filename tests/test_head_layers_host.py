@@ -9,6 +9,7 @@ import pytest
 import torch
 import torch.distributed as dist
 import torch.multiprocessing as mp
+from torch.utils.checkpoint import checkpoint
 
 import l_inf_dist_net_v2_b200 as ldn
 from head_stand_in import RowOperators
@@ -92,6 +93,47 @@ def test_hooks_of_every_norm_run(on_the_host):
         norm.register_forward_hook(lambda *_, i=i: seen.append(i))
     head(torch.randn(3, 12))
     assert seen == [0, 1, 2]
+
+
+# ---- recomputation ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_recomputed_head_has_the_gradients_of_its_masks(on_the_host, reentrant):
+    a = _head(dropout=0.5)
+    b = copy.deepcopy(a)
+    xs = [torch.randn(6, 12, requires_grad=True) for _ in range(3)]
+    # three calls before the first backward pass, and another one behind it
+    outs = [checkpoint(a, x, use_reentrant=reentrant) for x in xs]
+    wants = [b(x) for x in xs]
+    for out, want in reversed(list(zip(outs, wants))):
+        assert torch.equal(out, want)
+        out.square().sum().backward()
+        want.square().sum().backward()
+    assert all(torch.equal(p.grad, q.grad) for p, q in zip(a.parameters(), b.parameters()))
+    assert torch.equal(a(xs[0]), b(xs[0])) and [d.calls for d in a.drop] == [d.calls for d in b.drop] == [4, 4]
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_one_layer_in_several_recomputed_parts(on_the_host, reentrant):
+    drop = ldn.Dropout(0.5, seed=3)
+    plain = copy.deepcopy(drop)
+    x = torch.randn(5, 8, requires_grad=True)
+    other = x.detach().clone().requires_grad_()
+    y, want = x, other
+    for _ in range(3):
+        y = checkpoint(lambda v: drop(v * 2), y, use_reentrant=reentrant)
+        want = plain(want * 2)
+    g = torch.randn(5, 8)
+    y.backward(g)
+    want.backward(g)
+    assert torch.equal(y, want) and torch.equal(x.grad, other.grad)
+
+
+def test_recomputation_without_the_generators_state_is_refused(on_the_host):
+    drop = ldn.Dropout(0.5, seed=3)
+    x = torch.randn(5, 8, requires_grad=True)
+    y = checkpoint(lambda v: drop(v).square(), x, use_reentrant=False, preserve_rng_state=False)
+    with pytest.raises(RuntimeError, match="preserve_rng_state"):
+        y.sum().backward()
 
 
 # ---- sizes whose sums with a tile's or a grid's would pass 32 bits (none of these calls may launch anything) -----------------------------
