@@ -129,6 +129,25 @@ void once(const variable_list& grads, const char* what) {
                     " cannot be differentiated again");
 }
 
+// A gradient that is one once only: it goes on as a function of `of`, so that whoever differentiates it again, wherever the
+// differentiation comes from, is told that there is no such derivative (without it, it would pass for a constant).
+struct OnceFn : public torch::autograd::Function<OnceFn> {
+    static Tensor forward(AutogradContext* ctx, Tensor grad, Tensor of, std::string what) {
+        ctx->saved_data["what"] = what;
+        return grad.detach();
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list) {
+        TORCH_CHECK(false, "the gradient of ", ctx->saved_data["what"].toStringRef(), " cannot be differentiated again");
+        return {};
+    }
+};
+Tensor once_of(const Tensor& grad, std::initializer_list<const Tensor*> depends_on, const char* what) {
+    if (grad.defined() && at::GradMode::is_enabled())
+        for (const Tensor* t : depends_on)
+            if (t->defined() && t->requires_grad()) return OnceFn::apply(grad, *t, std::string(what));
+    return grad;
+}
+
 // ---- layer norm ---------------------------------------------------------------------------------------------------------------
 void norm_forward(const Rows& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps, Tensor& y, float* stats) {
     check(ldn_layer_norm(x.t.data_ptr(), x.pitch, x.rows, x.C, type_of(x.t), ptr(weight), ptr(bias), param_type(weight, bias),
@@ -167,7 +186,7 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
                                       floats(stats) + rows.rows, w.defined() ? w.data_ptr() : nullptr, params, ptr(gx), ptr(gw),
                                       ptr(gb), stream()),
               "layer_norm_backward");
-        return {gx, gw, gb, Tensor()};
+        return {once_of(gx, {&x, &w}, "layer_norm"), once_of(gw, {&x}, "layer_norm"), gb, Tensor()};
     }
 };
 
@@ -256,6 +275,7 @@ struct DropoutAddNormFn : public torch::autograd::Function<DropoutAddNormFn> {
         d.keep(ctx);
         ctx->saved_data["param_type"] = param_type(weight, bias);
         ctx->saved_data["bias"] = bias.has_value();
+        ctx->saved_data["rows"] = x.requires_grad() || residual.requires_grad();
         ctx->save_for_backward({h, w.has_value() ? *w : Tensor(), stats});
         return {y, h};
     }
@@ -282,7 +302,9 @@ struct DropoutAddNormFn : public torch::autograd::Function<DropoutAddNormFn> {
                                                   params, d.p, d.seed64(), d.offset64(), d.words(), ptr(gx), ptr(gr), ptr(gw),
                                                   ptr(gb), stream()),
               "dropout_add_layer_norm_backward");
-        return {gx, gr, gw, gb, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        const char* what = "dropout_add_layer_norm";
+        if (ctx->saved_data["rows"].toBool()) gw = once_of(gw, {&h}, what);  // (h has a gradient if the weight alone has one, too)
+        return {once_of(gx, {&h, &w}, what), once_of(gr, {&h, &w}, what), gw, gb, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 

@@ -22,6 +22,54 @@ def _model(**kwargs):
     return model
 
 
+# ---- differentiated again ---------------------------------------------------------------------------------------------------------
+def _norm_case():
+    f = _gen(1)
+    x, r = (torch.randn(6, 40, **f).requires_grad_() for _ in range(2))
+    w, b = (torch.randn(40, **f).requires_grad_() for _ in range(2))
+    return x, r, w, b
+
+
+def _again(tensor):
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        tensor.square().sum().backward()
+
+
+def test_a_norm_differentiated_twice_says_so():
+    x, _, w, b = _norm_case()
+    v = torch.randn(6, 40, **_gen(2))
+    plain = torch.autograd.grad((ldn.layer_norm(x, w, b) * v).sum(), (x, w, b))
+    for weight in (w, w.detach(), None):
+        y = ldn.layer_norm(x, weight, b)
+        gx, = torch.autograd.grad((y * v).sum(), x, create_graph=True)
+        assert gx.requires_grad
+        _again(gx)
+    gx, gw, gb = torch.autograd.grad((ldn.layer_norm(x, w, b) * v).sum(), (x, w, b), create_graph=True)
+    assert all(torch.equal(s, t) for s, t in zip((gx, gw, gb), plain))
+    _again(gw)
+    # through what is in front of the norm
+    z = ldn.layer_norm(x * 2, w, b)
+    gx, = torch.autograd.grad(z.sum(), x, create_graph=True)
+    _again(gx)
+    # a gradient that depends on nothing that is differentiated is one
+    gw, = torch.autograd.grad((ldn.layer_norm(x.detach(), w, b) * v).sum(), w, create_graph=True)
+    assert not gw.requires_grad and torch.equal(gw, plain[1])
+
+
+def test_the_joined_norm_differentiated_twice_says_so():
+    x, r, w, b = _norm_case()
+    v = torch.randn(6, 40, **_gen(2))
+    for leaves, wanted in [((x, r, w, b), x), ((x, r, w, b), r), ((x, r, w, b), w), ((x.detach(), r, w.detach(), b), r)]:
+        y, h = ldn.dropout_add_layer_norm(*leaves, 0.3, 5)
+        plain, = torch.autograd.grad((y * v).sum(), wanted, retain_graph=True)
+        g, = torch.autograd.grad((y * v).sum(), wanted, create_graph=True)
+        assert torch.equal(g, plain)
+        _again(g)
+    y, _ = ldn.dropout_add_layer_norm(x.detach(), r.detach(), w, b, 0.3, 5)
+    gw, = torch.autograd.grad((y * v).sum(), w, create_graph=True)
+    assert not gw.requires_grad
+
+
 # ---- recomputed ---------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("reentrant", [False, True])
 def test_a_recomputed_head_has_the_gradients_of_its_masks(reentrant):
