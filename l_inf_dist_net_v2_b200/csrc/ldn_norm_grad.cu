@@ -151,12 +151,12 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPi
                 if constexpr (!kKeep) load_params<T, SHIFT>(a.weight, a.wide, column(i), a.C, 1.0f, w[i]);
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e) {
-                    const float2 z = __fmul2_rn(__fadd2_rn(vx[e], both(-mean[j])), both(rstd[j]));
-                    sum_w[i][e] = __ffma2_rn(vg[e], z, sum_w[i][e]);
+                    // (no z here: outside the row the gradient is 0 and x - mean a number, but (0 - mean) rstd may be infinite)
+                    const float2 u = __fmul2_rn(vg[e], __fadd2_rn(vx[e], both(-mean[j])));
+                    sum_w[i][e] = __ffma2_rn(u, both(rstd[j]), sum_w[i][e]);
                     sum_b[i][e] = __fadd2_rn(sum_b[i][e], vg[e]);
-                    const float2 p = __fmul2_rn(vg[e], w[i][e]);
-                    s0 = __fadd2_rn(s0, p);
-                    s1 = __ffma2_rn(p, z, s1);
+                    s0 = __ffma2_rn(vg[e], w[i][e], s0);
+                    s1 = __ffma2_rn(u, w[i][e], s1);
                 }
             }
             s[2 * j] = s0.x + s0.y;
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPi
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             if (!live(j)) continue;
-            const float m1 = s[2 * j], m2 = s[2 * j + 1] * rstd[j];
+            const float m1 = s[2 * j], m2 = s[2 * j + 1] * rstd[j] * rstd[j];
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
                 const int c = column(i);
