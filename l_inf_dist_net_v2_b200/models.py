@@ -107,7 +107,8 @@ class ResidualModel(nn.Module):
     """depth - 2 distance layers (all with mean shift, no bias) followed by a residual feed-forward head (head.py); not in the
     reference.  The distance layers are 1-Lipschitz, the head is not bounded: model(x) -> logits, without a worst case.
 
-    `quantize()` makes it answer with the head's products in 8-bit integers (in eval mode, without gradients) until `train()`."""
+    `quantize()` puts it into eval mode and makes it answer with the head's products in 8-bit integers, without gradients, until
+    `train()`."""
 
     def __init__(self, depth, width, input_dim, hidden=512, num_classes=10, blocks=2, dropout=0.1, std=1.0, identity_val=None,
                  seed=None):
@@ -123,11 +124,11 @@ class ResidualModel(nn.Module):
         return self
 
     def train(self, mode=True):
-        self._answer = []
+        if mode:
+            self._answer = []
         return super().train(mode)
 
     def forward(self, x):
-        features, _, _ = self.fc_dist(_flat_triple(x, 0, None, None, False))
-        if self._answer and not torch.is_grad_enabled():
-            return self._answer[0](features)
-        return self.head(features)
+        with torch.set_grad_enabled(torch.is_grad_enabled() and not self._answer):
+            features, _, _ = self.fc_dist(_flat_triple(x, 0, None, None, False))
+        return self._answer[0](features) if self._answer else self.head(features)

@@ -22,6 +22,10 @@ def _model(**kwargs):
     return model
 
 
+def _images(n=40, seed=1):
+    return torch.rand(n, 1, 8, 8, **_gen(seed))
+
+
 # ---- differentiated again ---------------------------------------------------------------------------------------------------------
 def _norm_case():
     f = _gen(1)
@@ -84,3 +88,26 @@ def test_a_recomputed_head_has_the_gradients_of_its_masks(reentrant):
         want.square().sum().backward()
         assert torch.equal(x.grad, g)
     assert all(torch.equal(p.grad, q.grad) for p, q in zip(a.parameters(), b.parameters()))
+
+
+# ---- answering -------------------------------------------------------------------------------------------------------------------------
+def _fresh(model, x):
+    """What the model's weights of now answer in integers."""
+    with torch.no_grad():
+        features, _, _ = model.fc_dist((x.flatten(1), None, None))
+        return model.head.quantized()(features)
+
+
+def test_integers_last_until_train():
+    model, x = _model(), _images()
+    want = _fresh(model.eval(), x)
+    model.quantize()
+    for answers in (model, model.eval(), model.train(False), copy.deepcopy(model)):
+        with torch.no_grad():
+            assert torch.equal(answers(x), want)
+        y = answers(x)  # integers without torch.no_grad(), too, and no gradient
+        assert torch.equal(y, want) and not y.requires_grad
+    model.train()
+    assert model(x).requires_grad
+    with torch.no_grad():
+        assert not torch.equal(model.eval()(x), want)
