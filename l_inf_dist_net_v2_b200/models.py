@@ -17,6 +17,7 @@ import torch
 import torch.nn as nn
 
 from . import norm_dist_cuda as _C
+from . import optim
 from .bound_modules import BoundFinalLinear, BoundLinear, BoundSequential, BoundTanh
 from .head import ResidualHead
 from .modules import NormDist, NormDistBase
@@ -103,12 +104,28 @@ class HybridModel(nn.Module):
         return self.fc_final(*self.fc_linear((dist, lower, upper)), targets=targets)
 
 
+class _Contents:
+    """Modules and parameters below a module as they are now: torch counts the changes of each tensor, and the optimisers of this package,
+    whose kernels it does not see, count their steps."""
+
+    def __init__(self, module):
+        self.places = [(d, name, v) for m in module.modules() for d in (m._modules, m._parameters) for name, v in d.items()]
+        self.versions = [(p, p._version, p.data_ptr()) for p in module.parameters()]
+        self.steps = optim.steps_taken()
+
+    def changed(self):
+        return (self.steps != optim.steps_taken() or any(p._version != n or p.data_ptr() != at for p, n, at in self.versions)
+                or any(d.get(name) is not v for d, name, v in self.places))
+
+
 class ResidualModel(nn.Module):
     """depth - 2 distance layers (all with mean shift, no bias) followed by a residual feed-forward head (head.py); not in the
     reference.  The distance layers are 1-Lipschitz, the head is not bounded: model(x) -> logits, without a worst case.
 
     `quantize()` puts it into eval mode and makes it answer with the head's products in 8-bit integers, without gradients, until
-    `train()`."""
+    `train()`.  They are made again when the head is moved or loaded, parts of it are replaced, or its parameters are changed by torch's
+    operations or an optimiser.  What a replayed graph writes, or a write to a parameter's `.data`, is not seen: call `quantize()`
+    again then."""
 
     def __init__(self, depth, width, input_dim, hidden=512, num_classes=10, blocks=2, dropout=0.1, std=1.0, identity_val=None,
                  seed=None):
@@ -116,19 +133,29 @@ class ResidualModel(nn.Module):
         pixels = input_dim[0] * input_dim[1] * input_dim[2]
         self.fc_dist = _dist_stack([pixels] + [width] * (depth - 2), False, std, identity_val)
         self.head = ResidualHead(width, hidden, num_classes, blocks, dropout, seed=seed)
-        self._answer = []  # the quantised head, if there is one (in a list: it is no part of what is trained or saved)
+        self._integers = False
+        self._answer = []  # the quantised head and what it was made of (in a list: it is no part of what is trained or saved)
 
     def quantize(self):
         self.eval()
-        self._answer = [self.head.quantized()]
+        self._integers = True
+        self._answer = [self.head.quantized(), _Contents(self.head)]
         return self
 
     def train(self, mode=True):
         if mode:
-            self._answer = []
+            self._integers, self._answer = False, []
         return super().train(mode)
 
+    def _apply(self, fn, recurse=True):
+        self._answer = []
+        return super()._apply(fn, recurse)
+
     def forward(self, x):
-        with torch.set_grad_enabled(torch.is_grad_enabled() and not self._answer):
+        with torch.set_grad_enabled(torch.is_grad_enabled() and not self._integers):
             features, _, _ = self.fc_dist(_flat_triple(x, 0, None, None, False))
-        return self._answer[0](features) if self._answer else self.head(features)
+        if not self._integers:
+            return self.head(features)
+        if not self._answer or self._answer[1].changed():
+            self._answer = [self.head.quantized(), _Contents(self.head)]
+        return self._answer[0](features)

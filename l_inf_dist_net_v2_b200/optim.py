@@ -24,6 +24,19 @@ def _check_tensor(t, what):
         raise RuntimeError(f"{what} must be a contiguous float32 CUDA tensor")
 
 
+_steps = 0
+
+
+def steps_taken():
+    """Steps of all optimisers of this module so far (their kernels' writes do not show in a tensor's version)."""
+    return _steps
+
+
+def _count_step():
+    global _steps
+    _steps += 1
+
+
 class _Fused(torch.optim.Optimizer):
     def _select(self, group, params):
         chosen = []
@@ -76,6 +89,7 @@ class FusedAdam(_Fused):
 
     @torch.no_grad()
     def step(self, params=None):
+        _count_step()
         for group in self.param_groups:
             if group.get("capturable"):
                 self._step_capturable(group, params)
@@ -110,6 +124,7 @@ class FusedSGD(_Fused):
 
     @torch.no_grad()
     def step(self, params=None):
+        _count_step()
         for group in self.param_groups:
             fresh, warm = [], []
             for q, g in self._select(group, params):

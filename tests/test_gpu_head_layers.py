@@ -7,6 +7,7 @@ import torch
 from torch.utils.checkpoint import checkpoint
 
 import l_inf_dist_net_v2_b200 as ldn
+from l_inf_dist_net_v2_b200.optim import FusedAdam, FusedSGD
 
 pytestmark = pytest.mark.gpu
 
@@ -111,3 +112,28 @@ def test_integers_last_until_train():
     assert model(x).requires_grad
     with torch.no_grad():
         assert not torch.equal(model.eval()(x), want)
+
+
+@pytest.mark.parametrize("change", ["load", "adam", "sgd", "torch", "copy", "part", "to", "half and back"])
+def test_integers_are_those_of_the_weights(change):
+    model, x = _model(), _images()
+    torch.nn.functional.cross_entropy(model(x), torch.arange(40, device="cuda") % 10).backward()
+    before = model.quantize()(x)
+    if change == "load":
+        torch.manual_seed(5)
+        model.load_state_dict(ldn.ResidualModel(4, 96, [1, 8, 8], hidden=120, blocks=3).cuda().state_dict())
+    elif change in ("adam", "sgd", "torch"):
+        make = dict(adam=FusedAdam, sgd=FusedSGD, torch=torch.optim.SGD)[change]
+        make(model.head.parameters(), lr=0.05).step()
+    elif change == "copy":
+        with torch.no_grad():
+            model.head.final.weight.mul_(2)
+    elif change == "part":
+        model.head.up[1] = torch.nn.Linear(96, 120, device="cuda")
+    elif change == "to":
+        model.cpu()
+        model.cuda()
+    else:
+        model.head.half().float()
+    after = model(x)
+    assert torch.equal(after, _fresh(model, x)) and torch.equal(after, before) == (change == "to")
