@@ -8,6 +8,7 @@ current stream.  There is no other path: arguments that do not fit raise Runtime
 function transforms, torch.compile and the tracer, which would not see the kernels.
 """
 import torch
+import torch.distributed as dist
 import torch.nn as nn
 
 from . import norm_dist_cuda as _C
@@ -104,7 +105,8 @@ class LayerNorm(nn.Module):
 
 class Dropout(nn.Module):
     """Dropout with a seed of its own (from torch's generator where none is given) and the number of calls so far as the offset, so
-    that every call draws another mask; both are in the state_dict.  In eval mode the identity.
+    that every call draws another mask; both are in the state_dict.  In a process group the ranks' offsets are 2^40 apart, so that ranks
+    with one seed, as after loading one checkpoint, draw masks of their own.  In eval mode the identity.
 
     A call that torch.utils.checkpoint makes again in a backward pass draws the mask that it drew before: every call takes a number
     from torch's generator on the host, which the recomputation finds in the state that it had, and by it the layer knows its last
@@ -133,7 +135,8 @@ class Dropout(nn.Module):
                 raise RuntimeError("dropout in a backward pass does not find the call that it repeats: recomputation has to keep the "
                                    "generator's state (preserve_rng_state=True) and to come within the layer's next 4096 calls")
             return self.seed, self._offsets[number]
-        offset = self._offsets[number] = self.calls
+        rank = dist.get_rank() if dist.is_available() and dist.is_initialized() else 0
+        offset = self._offsets[number] = self.calls + (rank << 40)
         self.calls += 1
         if len(self._offsets) > self.REMEMBERED:
             del self._offsets[next(iter(self._offsets))]

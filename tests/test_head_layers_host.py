@@ -136,6 +136,21 @@ def test_recomputation_without_the_generators_state_is_refused(on_the_host):
         y.sum().backward()
 
 
+# ---- masks of ranks -------------------------------------------------------------------------------------------------------------------
+def _draws(rank):
+    drop = ldn.Dropout(0.5, seed=1 + rank)
+    drop.draw()
+    drop.load_state_dict({"_extra_state": dict(seed=5, calls=3)})  # (one checkpoint for all ranks)
+    return [drop.draw() for _ in range(2)]
+
+
+def test_ranks_with_one_seed_draw_masks_of_their_own(tmp_path):
+    first, second = (eval(s) for s in _on_two_ranks(tmp_path, _draws))
+    assert first == [(5, 3), (5, 4)]
+    assert [seed for seed, _ in second] == [5, 5] and not {o for _, o in first} & {o for _, o in second}
+    assert all(0 <= o < 1 << 64 for _, o in second)
+
+
 # ---- sizes whose sums with a tile's or a grid's would pass 32 bits (none of these calls may launch anything) -----------------------------
 MOST = (1 << 31) - 1
 
