@@ -189,7 +189,10 @@ class Int8Linear(nn.Module):
 class ResidualHead(nn.Module):
     """A pre-norm residual feed-forward head: every block adds dropout(down(relu(up(norm(h))))) to the stream h, and the classes are a
     linear map of the last norm.  Between the products of neighbouring blocks there is one kernel each way: dropout, residual and the
-    next block's norm.  It has no interval bounds, so what it answers is not certified."""
+    next block's norm.  It has no interval bounds, so what it answers is not certified.
+
+    The stream has the type of the head's weights (features of distance layers have 32 bits, a head may have 16), under torch.autocast
+    too, where the products may give another."""
 
     def __init__(self, width, hidden, num_classes=10, blocks=2, dropout=0.1, eps=1e-5, seed=None):
         super().__init__()
@@ -200,10 +203,11 @@ class ResidualHead(nn.Module):
         self.final = nn.Linear(width, num_classes)
 
     def forward(self, h):
+        h = h.to(self.final.weight.dtype)
         y = self.norm[0](h)
         for up, down, norm, drop in zip(self.up, self.down, self.norm[1:], self.drop):
             p, (seed, offset) = (drop.p, drop.draw()) if self.training else (0.0, (0, 0))
-            y, h = norm(down(torch.relu(up(y))), h, p, seed, offset)
+            y, h = norm(down(torch.relu(up(y))).to(h.dtype), h, p, seed, offset)
         return self.final(y)
 
     def quantized(self):
@@ -222,8 +226,9 @@ class QuantizedHead(nn.Module):
         self.down = nn.ModuleList(Int8Linear.from_linear(m) for m in head.down)
         self.final = Int8Linear.from_linear(head.final)
         for i, m in enumerate(head.norm):
-            self.register_buffer(f"norm_weight{i}", m.weight.detach().clone())
-            self.register_buffer(f"norm_bias{i}", m.bias.detach().clone())
+            # (in 32 bits, which go with rows of any type)
+            self.register_buffer(f"norm_weight{i}", m.weight.detach().float().clone())
+            self.register_buffer(f"norm_bias{i}", m.bias.detach().float().clone())
 
     def _normed(self, i, h):
         return layer_norm_quantized(h, getattr(self, f"norm_weight{i}"), getattr(self, f"norm_bias{i}"), self.eps)

@@ -11,6 +11,8 @@ from l_inf_dist_net_v2_b200.optim import FusedAdam, FusedSGD
 
 pytestmark = pytest.mark.gpu
 
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
 
 def _gen(seed):
     return dict(device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed))
@@ -89,6 +91,39 @@ def test_a_recomputed_head_has_the_gradients_of_its_masks(reentrant):
         want.square().sum().backward()
         assert torch.equal(x.grad, g)
     assert all(torch.equal(p.grad, q.grad) for p, q in zip(a.parameters(), b.parameters()))
+
+
+# ---- mixed precision -----------------------------------------------------------------------------------------------------------------
+# seven products whose operands and results are rounded to eight bits (2^-9 each), and as many times the stream and the norms in 16
+# bits: of the largest logit
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_a_model_under_autocast(dtype):
+    model, x = _model(dropout=0.2), _images()
+    plain = copy.deepcopy(model)
+    want = plain(x)
+    with torch.autocast("cuda", dtype=dtype):
+        got = model(x)
+        loss = torch.nn.functional.cross_entropy(got, torch.arange(40, device="cuda") % 10)
+    assert got.dtype == dtype and (got - want).abs().max() <= 7 * 3 * 2.0 ** -9 * want.abs().max()
+    loss.backward()
+    assert all(p.grad is not None and p.grad.dtype == F32 and p.grad.isfinite().all() for p in model.head.parameters())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_a_head_in_16_bits_behind_distance_layers(dtype):
+    model, x = _model(dropout=0.2), _images()
+    want = copy.deepcopy(model)(x)
+    model.head.to(dtype)
+    got = model(x)
+    assert got.dtype == dtype and (got - want).abs().max() <= 7 * 6 * 2.0 ** -9 * want.abs().max()
+    torch.nn.functional.cross_entropy(got.float(), torch.arange(40, device="cuda") % 10).backward()
+    assert all(p.grad is not None and p.grad.dtype == dtype and p.grad.isfinite().all() for p in model.head.parameters())
+    whole = copy.deepcopy(model).eval()  # (with the running means of the step above)
+    whole.head.float()
+    with torch.no_grad():
+        want = whole(x)
+    answer = model.quantize()(x)
+    assert (answer - want).abs().max() <= 0.1 * want.abs().max()
 
 
 # ---- answering -------------------------------------------------------------------------------------------------------------------------
