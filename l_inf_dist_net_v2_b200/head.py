@@ -40,6 +40,11 @@ def _signed(v):
     return v - (1 << 64) if v >= 1 << 63 else v
 
 
+def _padded(terms):
+    """The distance of rows of integers that start at multiples of 16 bytes."""
+    return (terms + 15) // 16 * 16
+
+
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension; gradients of x, weight and bias."""
     return _native().layer_norm(x, weight, bias, eps)
@@ -159,7 +164,8 @@ class Dropout(nn.Module):
 
 
 class Int8Linear(nn.Module):
-    """A linear layer that answers in 8-bit integers: weight (outputs, terms) with a scale per output, rows quantised as they come."""
+    """A linear layer that answers in 8-bit integers: weight (outputs, terms) with a scale per output, rows quantised as they come.
+    Wherever it is moved its rows start at multiples of 16 bytes, and scales and bias have 32 bits."""
 
     def __init__(self, weight, bias=None, activation="none"):
         super().__init__()
@@ -171,6 +177,17 @@ class Int8Linear(nn.Module):
         self.register_buffer("weight_scale", scale)
         self.register_buffer("bias", None if bias is None else bias.detach().float().clone())
         self.activation = activation
+
+    def _apply(self, fn, recurse=True):
+        before = {name: getattr(self, name) for name in ("weight_scale", "bias")}
+        super()._apply(fn, recurse)
+        for name, t in before.items():
+            if t is not None:
+                setattr(self, name, t.to(getattr(self, name).device))
+        rows, terms = self.weight.shape
+        if self.weight.stride() != (_padded(terms), 1):  # (a copy of rows that are apart leaves them side by side)
+            self.weight = self.weight.new_zeros(rows, _padded(terms))[:, :terms].copy_(self.weight)
+        return self
 
     @classmethod
     def from_linear(cls, linear, activation="none"):

@@ -172,3 +172,15 @@ def test_integers_are_those_of_the_weights(change):
         model.head.half().float()
     after = model(x)
     assert torch.equal(after, _fresh(model, x)) and torch.equal(after, before) == (change == "to")
+
+
+# ---- an integer layer that is moved -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("terms", [96, 100])
+def test_an_integer_layer_that_is_moved(terms):
+    layer = ldn.Int8Linear(torch.randn(30, terms, **_gen(1)), torch.randn(30, **_gen(2)), "relu")
+    x = torch.randn(9, terms, **_gen(3))
+    want = layer(x)
+    for moved in (copy.deepcopy(layer), copy.deepcopy(layer).cpu().cuda(), copy.deepcopy(layer).half(), copy.deepcopy(layer).cpu().bfloat16().cuda(),
+                  torch.nn.Sequential(copy.deepcopy(layer)).cpu().cuda()[0]):
+        assert moved.weight.stride() == layer.weight.stride() and moved.weight_scale.dtype == moved.bias.dtype == F32
+        assert torch.equal(moved(x), want) and moved.state_dict().keys() == layer.state_dict().keys()
