@@ -1,6 +1,7 @@
 """The head's layers and models in the ways that a program uses them: differentiated again, recomputed, in mixed precision, moved,
 answering in integers while their weights change, from several threads."""
 import copy
+import threading
 
 import pytest
 import torch
@@ -184,3 +185,37 @@ def test_an_integer_layer_that_is_moved(terms):
                   torch.nn.Sequential(copy.deepcopy(layer)).cpu().cuda()[0]):
         assert moved.weight.stride() == layer.weight.stride() and moved.weight_scale.dtype == moved.bias.dtype == F32
         assert torch.equal(moved(x), want) and moved.state_dict().keys() == layer.state_dict().keys()
+
+
+# ---- threads ---------------------------------------------------------------------------------------------------------------------------------
+def test_several_threads():
+    weight = ldn.quantize_rows(torch.randn(130, 500, **_gen(1)))
+
+    def work(k):
+        x, r = (torch.randn(40 + 90 * k, 500, **_gen(10 * k + i)).requires_grad_() for i in (2, 3))
+        w, b = (torch.randn(500, **_gen(10 * k + i)).requires_grad_() for i in (4, 5))
+        y, h = ldn.dropout_add_layer_norm(x, r, w, b, 0.2, k)
+        d = ldn.dropout(ldn.layer_norm(h, w, b), 0.1, k, 1)
+        grads = torch.autograd.grad((y, d), (x, r, w, b), (x.detach(), r.detach()))
+        with torch.no_grad():
+            return (y, h, d) + grads + (ldn.int8_linear(x, weight), ldn.int8_linear(ldn.layer_norm_quantized(x, w, b), weight))
+    wants = [work(k) for k in range(4)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def repeat(k):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(25):
+                    if not all(torch.equal(s, t) for s, t in zip(work(k), wants[k])):
+                        wrong.append(k)
+            stream.synchronize()
+        except Exception as e:  # (a thread's own end says nothing to the test)
+            wrong.append(e)
+    threads = [threading.Thread(target=repeat, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
