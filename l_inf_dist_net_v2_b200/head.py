@@ -163,7 +163,18 @@ class Dropout(nn.Module):
         return f"p={self.p}"
 
 
-class Int8Linear(nn.Module):
+class _Answers(nn.Module):
+    """A module whose buffers of floating point have 32 bits wherever it is moved: the kernels take no other."""
+
+    def _apply(self, fn, recurse=True):
+        before = {name: t for name, t in self._buffers.items() if t is not None and t.is_floating_point()}
+        super()._apply(fn, recurse)
+        for name, t in before.items():
+            self._buffers[name] = t.to(self._buffers[name].device)
+        return self
+
+
+class Int8Linear(_Answers):
     """A linear layer that answers in 8-bit integers: weight (outputs, terms) with a scale per output, rows quantised as they come.
     Wherever it is moved its rows start at multiples of 16 bytes, and scales and bias have 32 bits."""
 
@@ -179,11 +190,7 @@ class Int8Linear(nn.Module):
         self.activation = activation
 
     def _apply(self, fn, recurse=True):
-        before = {name: getattr(self, name) for name in ("weight_scale", "bias")}
         super()._apply(fn, recurse)
-        for name, t in before.items():
-            if t is not None:
-                setattr(self, name, t.to(getattr(self, name).device))
         rows, terms = self.weight.shape
         if self.weight.stride() != (_padded(terms), 1):  # (a copy of rows that are apart leaves them side by side)
             self.weight = self.weight.new_zeros(rows, _padded(terms))[:, :terms].copy_(self.weight)
@@ -232,7 +239,7 @@ class ResidualHead(nn.Module):
         return QuantizedHead(self)
 
 
-class QuantizedHead(nn.Module):
+class QuantizedHead(_Answers):
     """A residual head whose products are in 8-bit integers: the norms' rows leave as integers, hidden rows are quantised in the product
     that takes them.  It answers only; the stream has the type that it comes in."""
 

@@ -187,6 +187,16 @@ def test_an_integer_layer_that_is_moved(terms):
         assert torch.equal(moved(x), want) and moved.state_dict().keys() == layer.state_dict().keys()
 
 
+@pytest.mark.parametrize("move", [lambda m: m.half(), lambda m: m.cpu().cuda(), lambda m: m.to(torch.bfloat16), lambda m: m.double()])
+def test_an_integer_head_that_is_moved(move):
+    head = _model().head.quantized()
+    h = torch.randn(20, 96, **_gen(1))
+    want = head(h)
+    moved = move(copy.deepcopy(head))
+    assert torch.equal(moved(h), want) and moved(h.half()).dtype == F16
+    assert all(b.dtype in (F32, torch.int8) for b in moved.buffers())
+
+
 # ---- threads ---------------------------------------------------------------------------------------------------------------------------------
 def test_several_threads():
     weight = ldn.quantize_rows(torch.randn(130, 500, **_gen(1)))
