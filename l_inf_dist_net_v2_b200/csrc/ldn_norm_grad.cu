@@ -4,8 +4,9 @@
 // A block takes every gridDim-th row, so its threads' columns stay (rows that start anywhere in 16 bytes: the grid is a multiple of
 // eight, and rows that far apart start alike).  Rows are under way into shared memory while others are summed, as in the forward
 // pass, and are read there twice: in front of the sums and behind them.  Bound by memory: x, the incoming and the outgoing gradients
-// once; joined, also by the words of the dropout.  16384 x 5120 bf16: 95 us, 5.3 TB/s (50000 rows: 255 us, 6.0 TB/s; joined 597, 4.3;
-// 16383 x 4097, cut rows: 134, 3.0).
+// once; joined, also by the latency of the dropout's words.  16384 x 5120 bf16: 97 us, 5.2 TB/s (50000 rows: 265 us, 5.8 TB/s; joined
+// 589, 4.3; 16383 x 4097, cut rows: 132, 3.0; 8192 x 5120 f32: 91, 5.5).  Rows beyond 5120 take the parameters again for every row, one
+// row at a time: 8192 x 8192 bf16 132 us, 3.0 TB/s.
 #include "ldn_norm.cuh"
 #include "ldn_rows.cuh"
 
@@ -151,12 +152,22 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPi
                 if constexpr (!kKeep) load_params<T, SHIFT>(a.weight, a.wide, column(i), a.C, 1.0f, w[i]);
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e) {
-                    // (no z here: outside the row the gradient is 0 and x - mean a number, but (0 - mean) rstd may be infinite)
-                    const float2 u = __fmul2_rn(vg[e], __fadd2_rn(vx[e], both(-mean[j])));
-                    sum_w[i][e] = __ffma2_rn(u, both(rstd[j]), sum_w[i][e]);
+                    // (what is summed is a (x - mean), with rstd behind the sum: outside the row the gradient is 0 and x - mean a
+                    // number, but (0 - mean) rstd may be infinite.  Two orders of the products, for their registers: 50000 x 4096
+                    // bf16 208 and 226 us, joined 507 and 505, cut rows of 4097 in f16 410 and 370)
+                    const float2 d = __fadd2_rn(vx[e], both(-mean[j]));
                     sum_b[i][e] = __fadd2_rn(sum_b[i][e], vg[e]);
-                    s0 = __ffma2_rn(vg[e], w[i][e], s0);
-                    s1 = __ffma2_rn(u, w[i][e], s1);
+                    if constexpr (!SHIFT && !JOINED) {
+                        const float2 p = __fmul2_rn(vg[e], w[i][e]);
+                        s0 = __fadd2_rn(s0, p);
+                        s1 = __ffma2_rn(p, d, s1);
+                        sum_w[i][e] = __ffma2_rn(vg[e], __fmul2_rn(d, both(rstd[j])), sum_w[i][e]);
+                    } else {
+                        const float2 u = __fmul2_rn(vg[e], d);
+                        sum_w[i][e] = __ffma2_rn(u, both(rstd[j]), sum_w[i][e]);
+                        s0 = __ffma2_rn(vg[e], w[i][e], s0);
+                        s1 = __ffma2_rn(u, w[i][e], s1);
+                    }
                 }
             }
             s[2 * j] = s0.x + s0.y;
