@@ -1,8 +1,9 @@
 // Dropout with a counter-based generator: out = [residual +] (x / (1 - p) where its word says so, else 0).  No mask is stored;
 // the backward pass is the same kernel on the gradient with the same seed and offset.
 //
-// Bound by the integer pipe in 16 bits, by memory in 32: 50000 x 5120 bf16 takes 260 us (3.9 TB/s), with a residual 305 (5.0);
-// 8192 x 5120 f32 61 us (5.5 TB/s).
+// Bound by the latency of the generator's ten dependent rounds in 16 bits (the integer pipe is 58 % busy; its words alone take 50 of
+// the 90 us of 16384 x 5120, memory 51), by memory in 32: 50000 x 5120 bf16 takes 258 us (4.0 TB/s), with a residual 304 (5.1);
+// 8192 x 5120 f32 61 us (5.5 TB/s).  Any other pitch or alignment: 16384 x 5120 bf16 with a pitch of 5121 170 us.
 #include "ldn_rows.cuh"
 
 namespace ldn {

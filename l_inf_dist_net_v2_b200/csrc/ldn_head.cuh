@@ -102,8 +102,8 @@ __device__ __forceinline__ void set_param(void* p, bool wide, long long i, float
 // from a 64-bit key and a 128-bit counter, here the seed and (block, offset).  Element i takes word i % 4 of block i / 4, so the
 // mask is a function of seed, offset and the element's place alone: the backward pass makes it again, whatever its launch.
 //
-// An integer product of two words takes the integer pipe for two clocks a warp, as an exclusive or does, and both are what bounds
-// 16-bit dropout (16384 x 5120 bf16: 51 us of memory, 58 of these).  So what does not depend on the block is made once: the round
+// An integer product of two words takes the integer pipe for two clocks a warp, as an exclusive or does (84 million words take 50 us
+// at best; 16-bit dropout takes 90, memory 51).  So what does not depend on the block is made once: the round
 // keys, and of the first two rounds all but one product each, as the block's high word is 0 for the first 2^34 elements.
 struct Generator {
     unsigned key[20], c2, c3;

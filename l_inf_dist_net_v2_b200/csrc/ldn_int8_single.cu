@@ -3,7 +3,7 @@
 // weight of up to 1024 terms are dealt out to its warps (whole rows would leave a third of them idle at 35 outputs per SM), four
 // products per instruction and token, and their sums meet in shared memory as integers, in which no order shows.
 //
-// 5120 -> 5120 in bf16, weight in L2, us, one launch / quantising and tiles on the tensor cores: one token 7.3 / 9.8, two 9.0 / 9.9,
+// 5120 -> 5120 in bf16, from memory 14.3 us between events (the first load waits for the kernel in front); weight in L2, us, one launch / quantising and tiles on the tensor cores: one token 7.3 / 9.8, two 9.0 / 9.9,
 // four 12.3 / 10.2 (4 x 1000 x 3000: 5.8 / 8); as whole rows with scalar loads one token took 9.2.
 #include "ldn_int8.cuh"
 

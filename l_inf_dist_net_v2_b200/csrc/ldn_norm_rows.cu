@@ -4,9 +4,10 @@
 // Bound by memory: what a call cannot do without is x and y once (joined: x, the residual, h and y).  So a block always has rows
 // under way, into shared memory without registers, and takes several rows at a time, whose sums share their barriers: with one row
 // that was loaded when the one before was done, a 16384 x 5120 bf16 norm took 104 us at 49 % of the copy rate, with rows under
-// way 65 at 78 % (50000 rows: 189 us at 83 %; 16383 x 4097, cut rows: 77 us at 53 %).  A thread keeps its columns' weight and bias from row to row (a block takes every gridDim-th row; where rows
-// start anywhere in 16 bytes the grid is a multiple of eight, and rows that far apart start alike).  Rows of 8192 to 16384 have no
-// registers for that and read them again.
+// way 65 to 68 at 76 % (50000 rows: 190 us at 83 %; 16383 x 4097, cut rows: 76 us at 54 %; as integers 131 us at 23 %).  A thread keeps
+// its columns' weight and bias from row to row (a block takes every gridDim-th row; where rows start anywhere in 16 bytes the grid is
+// a multiple of eight, and rows that far apart start alike).  Rows of 5121 to 16384 have no registers for that and read them again
+// (8192 x 8192 bf16: 84 us at 49 %; 13104 x 5121, cut rows: 203 at 20 %).
 #include "ldn_norm.cuh"
 #include "ldn_rows.cuh"
 
