@@ -126,7 +126,7 @@ class Dropout(nn.Module):
         self.p = p
         self.seed = self._number() if seed is None else seed
         self.calls = 0
-        self._offsets = {}  # of the last calls, by their numbers
+        self._offsets = {}  # of the last calls, by their numbers, and whether a backward pass has repeated them
 
     @staticmethod
     def _number():
@@ -135,13 +135,19 @@ class Dropout(nn.Module):
     def draw(self):
         """(seed, offset) of a call."""
         number = self._number()
+        known, repeated = self._offsets.pop(number, (None, True))
         if torch._C._current_graph_task_id() != -1:  # (in a backward pass)
-            if number not in self._offsets:
+            if known is None:
                 raise RuntimeError("dropout in a backward pass does not find the call that it repeats: recomputation has to keep the "
-                                   "generator's state (preserve_rng_state=True) and to come within the layer's next 4096 calls")
-            return self.seed, self._offsets[number]
+                                   "generator's state (preserve_rng_state=True), to come within the layer's next 4096 calls, and to "
+                                   "find no two calls of the layer with the generator in the same state")
+            self._offsets[number] = (known, True)
+            return self.seed, known
         rank = dist.get_rank() if dist.is_available() and dist.is_initialized() else 0
-        offset = self._offsets[number] = self.calls + (rank << 40)
+        offset = self.calls + (rank << 40)
+        # (a program that seeds the generator anew for every step has the number again: the call before has been repeated, or it is
+        # not known which of the two would be)
+        self._offsets[number] = (offset if repeated else None, False)
         self.calls += 1
         if len(self._offsets) > self.REMEMBERED:
             del self._offsets[next(iter(self._offsets))]

@@ -136,6 +136,23 @@ def test_recomputation_without_the_generators_state_is_refused(on_the_host):
         y.sum().backward()
 
 
+def test_calls_that_recomputation_cannot_tell_apart_are_refused(on_the_host):
+    drop = ldn.Dropout(0.5, seed=3)
+    plain = copy.deepcopy(drop)
+    x = torch.randn(5, 8, requires_grad=True)
+
+    def seeded():
+        torch.manual_seed(1)
+        return checkpoint(lambda v: drop(v).square(), x, use_reentrant=False).sum()
+    for _ in range(3):  # a generator seeded anew for every step
+        got, = torch.autograd.grad(seeded(), x)
+        assert torch.equal(got, torch.autograd.grad(plain(x).square().sum(), x)[0])
+    first, second = seeded(), seeded()
+    for y in (first, second):
+        with pytest.raises(RuntimeError, match="same state"):
+            torch.autograd.grad(y, x)
+
+
 # ---- masks of ranks -------------------------------------------------------------------------------------------------------------------
 def _draws(rank):
     drop = ldn.Dropout(0.5, seed=1 + rank)
