@@ -138,8 +138,8 @@ class ResidualModel(nn.Module):
 
     def quantize(self):
         self.eval()
-        self._integers = True
         self._answer = [self.head.quantized(), _Contents(self.head)]
+        self._integers = True
         return self
 
     def train(self, mode=True):

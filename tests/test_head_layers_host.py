@@ -153,6 +153,13 @@ def test_calls_that_recomputation_cannot_tell_apart_are_refused(on_the_host):
             torch.autograd.grad(y, x)
 
 
+def test_a_model_that_cannot_be_quantized_stays_as_it_is():
+    model = ldn.ResidualModel(4, 12, [1, 2, 2], hidden=20)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        model.quantize()
+    assert not model._integers and not model._answer
+
+
 # ---- masks of ranks -------------------------------------------------------------------------------------------------------------------
 def _draws(rank):
     drop = ldn.Dropout(0.5, seed=1 + rank)
