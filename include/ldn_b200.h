@@ -414,6 +414,31 @@ LDN_API int ldn_int8_linear_float(const void* x, long long pitch, int x_type, co
                                   const float* w_scale, const float* bias, long long M, int N, int K, int activation, void* out,
                                   int type, ldn_stream_t stream);
 
+/*
+ * The gated projection of a block, y = act(g) u with g = x w_gate' + b_gate and u = x w_up' + b_up: rows of K elements, weights of H rows
+ * of K, all of `type`; biases (either may be NULL) have H elements of param_type: LDN_F32, or `type`.  activation: LDN_RELU,
+ * LDN_SILU (g / (1 + e^-g)), LDN_GELU (g times the normal distribution's function) or LDN_SIGMOID.  g and u receive both projections
+ * for the backward pass, [rows][pitch_saved] at multiples of 32 bytes, pitch_saved a multiple of 16 not below H, or are both NULL.
+ * Sums have 32 bits.  float32 operands are multiplied as three bfloat16 numbers each (24 bits); infinities then give not-a-numbers.
+ */
+#define LDN_SILU 3
+#define LDN_GELU 4
+#define LDN_SIGMOID 5
+LDN_API int ldn_gated_linear(const void* x, long long pitch, long long rows, int K, int H, int type, const void* w_gate,
+                             long long pitch_gate, const void* w_up, long long pitch_up, const void* b_gate, const void* b_up,
+                             int param_type, int activation, void* y, void* g, void* u, long long pitch_saved, ldn_stream_t stream);
+
+/*
+ * Gradients of ldn_gated_linear: with dg = grad_y u act'(g) and du = grad_y act(g) (rounded to `type` in products),
+ *   grad_x = dg w_gate + du w_up,  grad_w_gate = dg' x,  grad_w_up = du' x,  grad_b_gate and grad_b_up the column sums of dg and du.
+ * grad_y and the results are contiguous; grad_x, both of the weights' gradients, and either of the biases' may be NULL.  Sums are taken
+ * in a fixed order (no atomics).  rows == 0 sets the weights' and biases' to zero.
+ */
+LDN_API int ldn_gated_linear_backward(const void* grad_y, const void* x, long long pitch, long long rows, int K, int H, int type,
+                                      const void* w_gate, long long pitch_gate, const void* w_up, long long pitch_up, const void* g,
+                                      const void* u, long long pitch_saved, int activation, void* grad_x, void* grad_w_gate,
+                                      void* grad_w_up, void* grad_b_gate, void* grad_b_up, int param_type, ldn_stream_t stream);
+
 /* ---- allocation-free variant ------------------------------------------------------------------ */
 
 /*

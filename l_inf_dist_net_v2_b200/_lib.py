@@ -61,6 +61,8 @@ SIGNATURES = {
     "ldn_layer_norm_quantized": [_p, _l, _l, _i, _i, _p, _p, _i, _f, _p, _l, _p, _s],
     "ldn_int8_linear": [_p, _l, _p, _p, _l, _p, _p, _l, _i, _i, _i, _p, _i, _s],
     "ldn_int8_linear_float": [_p, _l, _i, _p, _l, _p, _p, _l, _i, _i, _i, _p, _i, _s],
+    "ldn_gated_linear": [_p, _l, _l, _i, _i, _i, _p, _l, _p, _l, _p, _p, _i, _i, _p, _p, _p, _l, _s],
+    "ldn_gated_linear_backward": [_p, _p, _l, _l, _i, _i, _i, _p, _l, _p, _l, _p, _p, _l, _i, _p, _p, _p, _p, _p, _i, _s],
     "ldn_check_status": [_s],
     "ldn_noalloc_check_status": [_s],
     "ldn_release_scratch": [],

@@ -424,6 +424,105 @@ Tensor int8_linear(const Tensor& x, const MaybeTensor& x_scale, const Tensor& we
     return out;
 }
 
+// ---- the gated projection -------------------------------------------------------------------------------------------------------
+struct Gated {
+    Rows x, w_gate, w_up;
+    MaybeTensor b_gate, b_up;
+    int activation;
+};
+// (the same in both passes)
+Gated gated_of(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const MaybeTensor& b_gate, const MaybeTensor& b_up,
+               int64_t activation) {
+    return {rows_of(x), rows_of(w_gate), rows_of(w_up), whole(b_gate), whole(b_up), static_cast<int>(activation)};
+}
+long long weight_pitch(const Rows& w) { return w.rows == 1 ? (w.C + 7) / 8 * 8 : w.pitch; }
+
+Tensor gated_forward(const Tensor& x, const Gated& a, Tensor* kept) {
+    std::vector<int64_t> shape = x.sizes().vec();
+    const int64_t H = a.w_gate.rows, pitch = (H + 15) / 16 * 16;
+    shape.back() = H;
+    Tensor y = at::empty(shape, x.options());
+    if (kept) *kept = at::empty({2, a.x.rows, pitch}, x.options());
+    char* g = kept ? static_cast<char*>(kept->data_ptr()) : nullptr;
+    check(ldn_gated_linear(a.x.t.data_ptr(), a.x.pitch, a.x.rows, a.x.C, static_cast<int>(H), type_of(x), a.w_gate.t.data_ptr(),
+                           weight_pitch(a.w_gate), a.w_up.t.data_ptr(), weight_pitch(a.w_up), ptr(a.b_gate), ptr(a.b_up),
+                           param_type(a.b_gate, a.b_up), a.activation, y.data_ptr(), g, g ? g + a.x.rows * pitch * x.element_size() : nullptr,
+                           pitch, stream()),
+          "gated_linear");
+    return y;
+}
+
+struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
+    static Tensor forward(AutogradContext* ctx, Tensor x, Tensor w_gate, Tensor w_up, MaybeTensor b_gate, MaybeTensor b_up,
+                          int64_t activation) {
+        const c10::cuda::CUDAGuard guard(x.device());
+        Tensor kept;
+        Tensor y = gated_forward(x, gated_of(x, w_gate, w_up, b_gate, b_up, activation), &kept);
+        ctx->saved_data["activation"] = activation;
+        ctx->saved_data["biases"] = (b_gate.has_value() ? 1 : 0) + (b_up.has_value() ? 2 : 0);
+        ctx->saved_data["param_type"] = param_type(b_gate, b_up);
+        ctx->save_for_backward({x, w_gate, w_up, kept});
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once(grads, "gated_linear");
+        variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w_gate = saved[1], &w_up = saved[2], &kept = saved[3];
+        const c10::cuda::CUDAGuard guard(x.device());
+        const Gated a = gated_of(x, w_gate, w_up, c10::nullopt, c10::nullopt, ctx->saved_data["activation"].toInt());
+        const Tensor dy = grads[0].contiguous();
+        const int params = static_cast<int>(ctx->saved_data["param_type"].toInt());
+        const int64_t biases = ctx->saved_data["biases"].toInt(), H = a.w_gate.rows;
+        const auto as_param = x.options().dtype(params == LDN_F32 ? at::kFloat : x.scalar_type());
+        Tensor gx, gwg, gwu, gbg, gbu;
+        if (ctx->needs_input_grad(0)) gx = at::empty(x.sizes(), x.options(), at::MemoryFormat::Contiguous);
+        const bool for_gate = ctx->needs_input_grad(1), for_up = ctx->needs_input_grad(2);
+        if (for_gate || for_up) {  // (one launch has both)
+            gwg = at::empty({H, a.x.C}, x.options());
+            gwu = at::empty({H, a.x.C}, x.options());
+        }
+        int edge = 3;  // (absent biases have none)
+        if ((biases & 1) && ctx->needs_input_grad(edge++)) gbg = at::empty({H}, as_param);
+        if ((biases & 2) && ctx->needs_input_grad(edge++)) gbu = at::empty({H}, as_param);
+        const char* g = static_cast<const char*>(kept.data_ptr());
+        check(ldn_gated_linear_backward(dy.data_ptr(), a.x.t.data_ptr(), a.x.pitch, a.x.rows, a.x.C, static_cast<int>(H), type_of(x),
+                                        a.w_gate.t.data_ptr(), weight_pitch(a.w_gate), a.w_up.t.data_ptr(), weight_pitch(a.w_up), g,
+                                        g + a.x.rows * kept.size(2) * x.element_size(), kept.size(2), a.activation, ptr(gx), ptr(gwg),
+                                        ptr(gwu), ptr(gbg), ptr(gbu), params, stream()),
+              "gated_linear_backward");
+        const char* what = "gated_linear";
+        return {once_of(gx, {&x, &w_gate, &w_up}, what), for_gate ? once_of(gwg, {&x, &w_gate, &w_up}, what) : Tensor(),
+                for_up ? once_of(gwu, {&x, &w_gate, &w_up}, what) : Tensor(), once_of(gbg, {&x, &w_gate, &w_up}, what),
+                once_of(gbu, {&x, &w_gate, &w_up}, what), Tensor()};
+    }
+};
+
+Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const MaybeTensor& b_gate, const MaybeTensor& b_up,
+                    int64_t activation) {
+    unobserved("gated_linear");
+    activations(x, "x");
+    row_fits(x);
+    TORCH_CHECK(x.numel() / x.size(-1) <= kMostColumns, "at most ", kMostColumns, " rows at a time, not ", x.numel() / x.size(-1));
+    for (const Tensor* w : {&w_gate, &w_up}) {
+        plain(*w, "weight");
+        TORCH_CHECK(w->scalar_type() == x.scalar_type() && w->device() == x.device(), "weights must have the type and device of x");
+        TORCH_CHECK(w->dim() == 2 && w->size(1) == x.size(-1) && w->size(0) >= 1 && w->size(0) <= kMostColumns, "weights must be (outputs, ",
+                    x.size(-1), "), not ", w->sizes());
+        TORCH_CHECK(w->sizes() == w_gate.sizes(), "the weights must have one shape");
+    }
+    for (const MaybeTensor* b : {&b_gate, &b_up})
+        if (b->has_value()) {
+            plain(**b, "bias");
+            TORCH_CHECK((*b)->dim() == 1 && (*b)->size(0) == w_gate.size(0), "a bias must have one value per output");
+            TORCH_CHECK(((*b)->scalar_type() == at::kFloat || (*b)->scalar_type() == x.scalar_type()) && (*b)->device() == x.device(),
+                        "biases must be float32 or of the type of x, on its device");
+        }
+    TORCH_CHECK(!b_gate.has_value() || !b_up.has_value() || b_gate->scalar_type() == b_up->scalar_type(), "the biases must have one type");
+    if (wants_grad({&x, &w_gate, &w_up, at_of(b_gate), at_of(b_up)})) return GatedLinearFn::apply(x, w_gate, w_up, b_gate, b_up, activation);
+    const c10::cuda::CUDAGuard guard(x.device());
+    return gated_forward(x, gated_of(x, w_gate, w_up, b_gate, b_up, activation), nullptr);
+}
+
 }  // namespace
 
 void register_head(pybind11::module& m) {
@@ -433,4 +532,5 @@ void register_head(pybind11::module& m) {
     m.def("quantize_rows", &quantize_rows);
     m.def("layer_norm_quantized", &layer_norm_quantized);
     m.def("int8_linear", &int8_linear);
+    m.def("gated_linear", &gated_linear);
 }

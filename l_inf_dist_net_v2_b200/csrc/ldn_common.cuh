@@ -256,6 +256,10 @@ int make_tensor_map(CUtensorMap* map, const float* base, const unsigned long lon
 // Tiled 2-D tensor map over rows of bytes that start at multiples of 16 bytes: boxes of 128 bytes x box_rows, 128-byte swizzle.
 int make_byte_map(CUtensorMap* map, const void* base, unsigned long long columns, unsigned long long rows, unsigned long long pitch,
                   unsigned box_rows);
+// Tiled 3-D tensor map over images of rows of 16-bit elements that start at multiples of 16 bytes (pitch and the images' distance in
+// elements): boxes of 64 x box_rows x 1, 128-byte swizzle.
+int make_image_map(CUtensorMap* map, const void* base, unsigned long long columns, unsigned long long rows, unsigned long long images,
+                   unsigned long long pitch, unsigned long long apart, unsigned box_rows);
 
 // optional CUDA-event pair around the most recent tile-kernel launch (ldn_diag.cu); no-ops unless enabled
 void timing_before(cudaStream_t st);

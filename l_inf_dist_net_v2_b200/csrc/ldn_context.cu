@@ -224,4 +224,16 @@ int make_byte_map(CUtensorMap* map, const void* base, unsigned long long columns
     return r == CUDA_SUCCESS ? kOk : kTensorMap;
 }
 
+int make_image_map(CUtensorMap* map, const void* base, unsigned long long columns, unsigned long long rows, unsigned long long images,
+                   unsigned long long pitch, unsigned long long apart, unsigned box_rows) {
+    const int found = find_encode();
+    if (found != kOk) return found;
+    cuuint64_t gdim[3] = {columns, rows, images}, gstr[2] = {pitch * 2, apart * 2};
+    cuuint32_t bdim[3] = {64, box_rows, 1}, estr[3] = {1, 1, 1};
+    CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), gdim, gstr, bdim, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? kOk : kTensorMap;
+}
+
 }  // namespace ldn

@@ -1,0 +1,115 @@
+// The gated projection of a handful of rows: the weights are read once and the products are made where they arrive.
+//
+// Bound by memory: 2 H K elements of the weights.  A block has some outputs, and its threads share their terms in pieces of 16 bytes, so
+// that every output's two weight rows are under way at once in whole lines; the rows themselves come from the first-level cache.
+#include "ldn_gated.cuh"
+
+namespace ldn {
+namespace {
+
+constexpr int kFewThreads = 128;
+constexpr int kFewRows = 8;
+
+// A piece of eight elements, `there` of them in the row
+template <class T>
+__device__ __forceinline__ void piece(const T* p, bool whole, int there, float (&v)[8]) {
+    if (whole) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            const uint4 raw = *reinterpret_cast<const uint4*>(p);
+            const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = to_float(e[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < there ? to_float(p[j]) : 0.0f;
+    }
+}
+
+template <class T, int ROWS, int OUTPUTS>
+__global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_constant__ GatedArgs a, bool aligned) {
+    stream_order_begin();
+    __shared__ float sums[kFewThreads / 32][2 * OUTPUTS][ROWS];
+    const int h0 = blockIdx.x * OUTPUTS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float acc[2 * OUTPUTS][ROWS] = {};
+    const T* w[2 * OUTPUTS];
+#pragma unroll
+    for (int o = 0; o < OUTPUTS; ++o) {
+        const long long h = h0 + o < a.H ? h0 + o : a.H - 1;
+        w[2 * o] = static_cast<const T*>(a.w_gate) + h * a.pitch_gate;
+        w[2 * o + 1] = static_cast<const T*>(a.w_up) + h * a.pitch_up;
+    }
+#pragma unroll 2
+    for (int c = threadIdx.x * 8; c < a.K; c += kFewThreads * 8) {
+        const bool whole = aligned && c + 8 <= a.K;
+        float wv[2 * OUTPUTS][8];
+#pragma unroll
+        for (int o = 0; o < 2 * OUTPUTS; ++o) piece(w[o] + c, whole, a.K - c, wv[o]);
+#pragma unroll
+        for (int t = 0; t < ROWS; ++t) {
+            float xv[8];
+            const long long row = t < a.T ? t : a.T - 1;
+            piece(static_cast<const T*>(a.x) + row * a.pitch_x + c, whole, a.K - c, xv);
+#pragma unroll
+            for (int o = 0; o < 2 * OUTPUTS; ++o)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[o][t] = fmaf(wv[o][j], xv[j], acc[o][t]);
+        }
+    }
+#pragma unroll
+    for (int o = 0; o < 2 * OUTPUTS; ++o)
+#pragma unroll
+        for (int t = 0; t < ROWS; ++t) {
+            const float s = warp_sum(acc[o][t]);
+            if (lane == 0) sums[warp][o][t] = s;
+        }
+    __syncthreads();
+    if (threadIdx.x < OUTPUTS * ROWS) {
+        const int o = threadIdx.x / ROWS, t = threadIdx.x % ROWS, h = h0 + o;
+        if (h < a.H && t < a.T) {
+            float g[1] = {0.0f}, u = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kFewThreads / 32; ++i) {
+                g[0] += sums[i][2 * o][t];
+                u += sums[i][2 * o + 1][t];
+            }
+            if (a.b_gate) g[0] += param_at<T>(a.b_gate, a.wide, h);
+            if (a.b_up) u += param_at<T>(a.b_up, a.wide, h);
+            if (a.g) {
+                static_cast<T*>(a.g)[t * a.pitch_saved + h] = from_float<T>(g[0]);
+                static_cast<T*>(a.u)[t * a.pitch_saved + h] = from_float<T>(u);
+            }
+            activate(g, a.activation);
+            static_cast<T*>(a.y)[static_cast<long long>(t) * a.H + h] = from_float<T>(g[0] * u);
+        }
+    }
+}
+
+template <class T, int ROWS>
+int launch(const GatedArgs& a, bool aligned, cudaStream_t st) {
+    constexpr int kOutputs = ROWS >= 4 ? 2 : 1;
+    return launch_after(gated_few_kernel<T, ROWS, kOutputs>, (a.H + kOutputs - 1) / kOutputs, kFewThreads, 0, st, a, aligned);
+}
+bool at_16(const void* p, long long pitch, long long rows, int size) {
+    return ((reinterpret_cast<uintptr_t>(p) | (rows > 1 ? static_cast<uintptr_t>(pitch) * size : 0)) & 15u) == 0;
+}
+
+}  // namespace
+
+bool gated_is_few(const GatedArgs& a, int type) { return a.T <= kFewRows; }
+
+int launch_gated_few(const GatedArgs& a, int type, const DeviceCtx* ctx, cudaStream_t st) {
+    const int size = size_of(type);
+    const bool aligned = at_16(a.x, a.pitch_x, a.T, size) && at_16(a.w_gate, a.pitch_gate, a.H, size) && at_16(a.w_up, a.pitch_up, a.H, size);
+    return with_type(type, [&](auto t) {
+        using T = decltype(t);
+        return a.T == 1 ? launch<T, 1>(a, aligned, st) : a.T == 2 ? launch<T, 2>(a, aligned, st)
+             : a.T <= 4 ? launch<T, 4>(a, aligned, st) : launch<T, 8>(a, aligned, st);
+    });
+}
+
+}  // namespace ldn

@@ -13,10 +13,11 @@ import torch.nn as nn
 
 from . import norm_dist_cuda as _C
 
-__all__ = ["layer_norm", "dropout", "dropout_add_layer_norm", "quantize_rows", "layer_norm_quantized", "int8_linear", "LayerNorm",
+__all__ = ["layer_norm", "dropout", "dropout_add_layer_norm", "quantize_rows", "layer_norm_quantized", "int8_linear", "gated_linear", "LayerNorm",
            "Dropout", "Int8Linear", "ResidualHead", "QuantizedHead"]
 
 _ACTIVATIONS = {"none": 0, "relu": 1, "tanh": 2}
+_GATES = {"relu": 1, "silu": 3, "gelu": 4, "sigmoid": 5}
 
 
 def _native():
@@ -87,6 +88,18 @@ def int8_linear(x, weight, bias=None, activation="none", out_dtype=None):
         raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, not {activation!r}")
     x, x_scale = (x, None) if isinstance(x, torch.Tensor) else x
     return _native().int8_linear(x, x_scale, weight[0], weight[1], bias, _ACTIVATIONS[activation], out_dtype)
+
+
+def gated_linear(x, weight_gate, weight_up, bias_gate=None, bias_up=None, activation="silu"):
+    """act(x @ weight_gate.T + bias_gate) * (x @ weight_up.T + bias_up): both projections, the activation and the product in one kernel,
+    with the gradients of all five.  activation: "silu", "gelu" (of the normal distribution's function), "sigmoid" or "relu".
+
+    Weights are (outputs, terms) of the type of x, biases of that type or float32; sums have 32 bits.  Both projections are kept in the type
+    of x for the backward pass.  Rows of 16-bit tensors that start at multiples of 16 bytes are read where they lie, others are copied
+    first; float32 is multiplied on the tensor cores as three bfloat16 numbers (24 bits), where an infinity gives not-a-numbers."""
+    if activation not in _GATES:
+        raise ValueError(f"activation must be one of {sorted(_GATES)}, not {activation!r}")
+    return _native().gated_linear(x, weight_gate, weight_up, bias_gate, bias_up, _GATES[activation])
 
 
 class LayerNorm(nn.Module):
