@@ -426,7 +426,7 @@ LDN_API int ldn_int8_linear_float(const void* x, long long pitch, int x_type, co
 #define LDN_SIGMOID 5
 LDN_API int ldn_gated_linear(const void* x, long long pitch, long long rows, int K, int H, int type, const void* w_gate,
                              long long pitch_gate, const void* w_up, long long pitch_up, const void* b_gate, const void* b_up,
-                             int param_type, int activation, void* y, void* g, void* u, long long pitch_saved, ldn_stream_t stream);
+                             int param_type, int activation, void* y, float* g, float* u, long long pitch_saved, ldn_stream_t stream);
 
 /*
  * Gradients of ldn_gated_linear: with dg = grad_y u act'(g) and du = grad_y act(g) (rounded to `type` in products),
@@ -435,9 +435,58 @@ LDN_API int ldn_gated_linear(const void* x, long long pitch, long long rows, int
  * in a fixed order (no atomics).  rows == 0 sets the weights' and biases' to zero.
  */
 LDN_API int ldn_gated_linear_backward(const void* grad_y, const void* x, long long pitch, long long rows, int K, int H, int type,
-                                      const void* w_gate, long long pitch_gate, const void* w_up, long long pitch_up, const void* g,
-                                      const void* u, long long pitch_saved, int activation, void* grad_x, void* grad_w_gate,
+                                      const void* w_gate, long long pitch_gate, const void* w_up, long long pitch_up, const float* g,
+                                      const float* u, long long pitch_saved, int activation, void* grad_x, void* grad_w_gate,
                                       void* grad_w_up, void* grad_b_gate, void* grad_b_up, int param_type, ldn_stream_t stream);
+
+/*
+ * A block's result joined to the residual stream between two norms: with norm(v) = (v - mean) / sqrt(mean((v - mean)^2) + eps),
+ *   h = residual + gate * scale * (norm(x) * post_weight + post_bias), rounded to the rows' type,   y = norm(h) * weight + bias.
+ * gate_kind: LDN_GATE_NONE (1), LDN_GATE_ROW (a number per row, contiguous) or LDN_GATE_ALL (a number per element, rows pitch_gate apart), of
+ * the rows' type.  scale and the norms' parameters (any may be NULL) have C elements of param_type: LDN_F32, or the rows' type.
+ * stats: 4 x rows floats for the backward pass, or NULL.  y and h are contiguous.
+ */
+#define LDN_GATE_NONE 0
+#define LDN_GATE_ROW 1
+#define LDN_GATE_ALL 2
+LDN_API int ldn_sandwich_norm(const void* x, long long pitch, const void* residual, long long pitch_residual, const void* gate,
+                              long long pitch_gate, int gate_kind, long long rows, int C, int type, const void* scale,
+                              const void* post_weight, const void* post_bias, const void* weight, const void* bias, int param_type,
+                              float eps, void* h, void* y, float* stats, ldn_stream_t stream);
+
+/*
+ * Gradients of ldn_sandwich_norm from those of y and h (contiguous; one may be NULL).  All results but grad_gate of a row's gate are
+ * contiguous rows or columns of the arguments' types; any may be NULL.  Column sums are taken in a fixed order (no atomics).  rows == 0
+ * sets the parameters' gradients to zero.
+ */
+LDN_API int ldn_sandwich_norm_backward(const void* grad_y, const void* grad_h, const void* x, long long pitch, const void* h,
+                                       const void* gate, long long pitch_gate, int gate_kind, long long rows, int C, int type,
+                                       const void* scale, const void* post_weight, const void* post_bias, const void* weight,
+                                       int param_type, const float* stats, void* grad_x, void* grad_residual, void* grad_gate,
+                                       void* grad_scale, void* grad_post_weight, void* grad_post_bias, void* grad_weight,
+                                       void* grad_bias, ldn_stream_t stream);
+
+/*
+ * Distillation of rows of V logits from a teacher's top logits: per row, with p = softmax(values / tau) over the row's k entries (those
+ * with an index below 0 are absent) and q = softmax(x / tau) over all classes,
+ *   losses[row] = part * tau^2 * sum p (log p - log q) + mix * (log sum e^x - x[target]).
+ * Rows without entries (or with nothing but minus infinity in them) have no first term, rows with a target below 0, and all where
+ * targets is NULL, no second.  An index or target of V or more makes a row's loss and gradient not-a-numbers.  1 <= k <= 1024; the same
+ * index may come several times.  value_type: type of the values.  stats: 5 x rows floats for the backward pass, or NULL.
+ * loss: receives loss_scale * the sum of the losses, in a fixed order, or NULL.
+ */
+LDN_API int ldn_distillation(const void* x, long long pitch, long long rows, int V, int type, const void* values, int value_type,
+                             const long long* indices, int k, const long long* targets, float tau, float part, float mix,
+                             float* losses, float* stats, float loss_scale, float* loss, ldn_stream_t stream);
+
+/*
+ * grad[row] = u (part * tau * (q - p) + mix * (softmax(x) - [target])), u = up_scale * up[row], or up_scale * up[0] where up_per_row is 0;
+ * contiguous, of the type of x.
+ */
+LDN_API int ldn_distillation_backward(const void* x, long long pitch, long long rows, int V, int type, const void* values,
+                                      int value_type, const long long* indices, int k, const long long* targets, float tau,
+                                      float part, float mix, const float* stats, const float* up, int up_per_row, float up_scale,
+                                      void* grad, ldn_stream_t stream);
 
 /* ---- allocation-free variant ------------------------------------------------------------------ */
 

@@ -63,6 +63,10 @@ SIGNATURES = {
     "ldn_int8_linear_float": [_p, _l, _i, _p, _l, _p, _p, _l, _i, _i, _i, _p, _i, _s],
     "ldn_gated_linear": [_p, _l, _l, _i, _i, _i, _p, _l, _p, _l, _p, _p, _i, _i, _p, _p, _p, _l, _s],
     "ldn_gated_linear_backward": [_p, _p, _l, _l, _i, _i, _i, _p, _l, _p, _l, _p, _p, _l, _i, _p, _p, _p, _p, _p, _i, _s],
+    "ldn_sandwich_norm": [_p, _l, _p, _l, _p, _l, _i, _l, _i, _i] + [_p] * 5 + [_i, _f, _p, _p, _p, _s],
+    "ldn_sandwich_norm_backward": [_p, _p, _p, _l, _p, _p, _l, _i, _l, _i, _i] + [_p] * 4 + [_i] + [_p] * 9 + [_s],
+    "ldn_distillation": [_p, _l, _l, _i, _i, _p, _i, _p, _i, _p, _f, _f, _f, _p, _p, _f, _p, _s],
+    "ldn_distillation_backward": [_p, _l, _l, _i, _i, _p, _i, _p, _i, _p, _f, _f, _f, _p, _p, _i, _f, _p, _s],
     "ldn_check_status": [_s],
     "ldn_noalloc_check_status": [_s],
     "ldn_release_scratch": [],

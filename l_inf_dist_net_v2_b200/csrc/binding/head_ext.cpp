@@ -442,11 +442,11 @@ Tensor gated_forward(const Tensor& x, const Gated& a, Tensor* kept) {
     const int64_t H = a.w_gate.rows, pitch = (H + 15) / 16 * 16;
     shape.back() = H;
     Tensor y = at::empty(shape, x.options());
-    if (kept) *kept = at::empty({2, a.x.rows, pitch}, x.options());
-    char* g = kept ? static_cast<char*>(kept->data_ptr()) : nullptr;
+    if (kept) *kept = at::empty({2, a.x.rows, pitch}, x.options().dtype(at::kFloat));
+    float* g = kept ? floats(*kept) : nullptr;
     check(ldn_gated_linear(a.x.t.data_ptr(), a.x.pitch, a.x.rows, a.x.C, static_cast<int>(H), type_of(x), a.w_gate.t.data_ptr(),
                            weight_pitch(a.w_gate), a.w_up.t.data_ptr(), weight_pitch(a.w_up), ptr(a.b_gate), ptr(a.b_up),
-                           param_type(a.b_gate, a.b_up), a.activation, y.data_ptr(), g, g ? g + a.x.rows * pitch * x.element_size() : nullptr,
+                           param_type(a.b_gate, a.b_up), a.activation, y.data_ptr(), g, g ? g + a.x.rows * pitch : nullptr,
                            pitch, stream()),
           "gated_linear");
     return y;
@@ -484,10 +484,10 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
         int edge = 3;  // (absent biases have none)
         if ((biases & 1) && ctx->needs_input_grad(edge++)) gbg = at::empty({H}, as_param);
         if ((biases & 2) && ctx->needs_input_grad(edge++)) gbu = at::empty({H}, as_param);
-        const char* g = static_cast<const char*>(kept.data_ptr());
+        const float* g = floats(kept);
         check(ldn_gated_linear_backward(dy.data_ptr(), a.x.t.data_ptr(), a.x.pitch, a.x.rows, a.x.C, static_cast<int>(H), type_of(x),
                                         a.w_gate.t.data_ptr(), weight_pitch(a.w_gate), a.w_up.t.data_ptr(), weight_pitch(a.w_up), g,
-                                        g + a.x.rows * kept.size(2) * x.element_size(), kept.size(2), a.activation, ptr(gx), ptr(gwg),
+                                        g + a.x.rows * kept.size(2), kept.size(2), a.activation, ptr(gx), ptr(gwg),
                                         ptr(gwu), ptr(gbg), ptr(gbu), params, stream()),
               "gated_linear_backward");
         const char* what = "gated_linear";
@@ -523,6 +523,203 @@ Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, c
     return gated_forward(x, gated_of(x, w_gate, w_up, b_gate, b_up, activation), nullptr);
 }
 
+// ---- the residual stream between two norms ----------------------------------------------------------------------------------------
+struct SandwichParams {
+    MaybeTensor scale, post_weight, post_bias, weight, bias;
+    int type;
+};
+int gate_kind(const MaybeTensor& gate, const Tensor& x) {
+    return !gate.has_value() ? LDN_GATE_NONE : gate->size(-1) == x.size(-1) ? LDN_GATE_ALL : LDN_GATE_ROW;
+}
+// A gate as the library takes it: rows where they lie, or one contiguous number per row
+Rows gate_rows(const MaybeTensor& gate, int kind) {
+    if (kind == LDN_GATE_NONE) return Rows{Tensor(), 0, 0, 0};
+    if (kind == LDN_GATE_ALL) return rows_of(*gate);
+    const Tensor g = gate->contiguous();
+    return Rows{g, 1, g.numel(), 1};
+}
+void sandwich_forward(const Tensor& x, const Tensor& residual, const MaybeTensor& gate, const SandwichParams& p, double eps, Tensor& h,
+                      Tensor& y, float* stats) {
+    const int kind = gate_kind(gate, x);
+    const Rows rows = rows_of(x), onto = rows_of(residual), g = gate_rows(gate, kind);
+    check(ldn_sandwich_norm(rows.t.data_ptr(), rows.pitch, onto.t.data_ptr(), onto.pitch, kind ? g.t.data_ptr() : nullptr, g.pitch, kind, rows.rows,
+                            rows.C, type_of(x), ptr(p.scale), ptr(p.post_weight), ptr(p.post_bias), ptr(p.weight), ptr(p.bias), p.type,
+                            static_cast<float>(eps), h.data_ptr(), y.data_ptr(), stats, stream()),
+          "sandwich_norm");
+}
+Tensor or_none(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
+MaybeTensor or_null(const Tensor& t) { return t.defined() ? MaybeTensor(t) : c10::nullopt; }
+
+struct SandwichFn : public torch::autograd::Function<SandwichFn> {
+    static variable_list forward(AutogradContext* ctx, Tensor x, Tensor residual, MaybeTensor gate, MaybeTensor scale, MaybeTensor post_weight,
+                                 MaybeTensor post_bias, MaybeTensor weight, MaybeTensor bias, int64_t type, double eps) {
+        const c10::cuda::CUDAGuard guard(x.device());
+        const SandwichParams p = {whole(scale), whole(post_weight), whole(post_bias), whole(weight), whole(bias), static_cast<int>(type)};
+        Tensor y = at::empty(x.sizes(), x.options(), at::MemoryFormat::Contiguous), h = at::empty_like(y);
+        Tensor stats = at::empty({4, x.numel() / x.size(-1)}, x.options().dtype(at::kFloat));
+        sandwich_forward(x, residual, gate, p, eps, h, y, floats(stats));
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["type"] = type;
+        ctx->saved_data["bias"] = bias.has_value();
+        ctx->saved_data["rows"] = x.requires_grad() || residual.requires_grad();
+        ctx->save_for_backward({x, h, or_none(gate), or_none(p.scale), or_none(p.post_weight), or_none(p.post_bias), or_none(p.weight), stats});
+        return {y, h};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        if (!grads[0].defined() && !grads[1].defined()) return variable_list(10);
+        once(grads, "sandwich_norm");
+        variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &h = saved[1], &gate = saved[2], &scale = saved[3], &post_weight = saved[4], &post_bias = saved[5],
+                     &weight = saved[6], &stats = saved[7];
+        const c10::cuda::CUDAGuard guard(x.device());
+        const Tensor gy = grads[0].defined() ? grads[0].contiguous() : Tensor(), gh = grads[1].defined() ? grads[1].contiguous() : Tensor();
+        const int type = static_cast<int>(ctx->saved_data["type"].toInt()), kind = gate_kind(or_null(gate), x);
+        const Rows rows = rows_of(x), g = gate_rows(or_null(gate), kind);
+        const auto as_param = x.options().dtype(type == LDN_F32 ? at::kFloat : x.scalar_type());
+        Tensor gx, gr, gg, gs, gpw, gpb, gw, gb;
+        int edge = 0;  // (absent tensors have none)
+        if (ctx->needs_input_grad(edge++)) gx = at::empty(x.sizes(), x.options(), at::MemoryFormat::Contiguous);
+        if (ctx->needs_input_grad(edge++)) gr = at::empty(x.sizes(), x.options(), at::MemoryFormat::Contiguous);
+        if (kind && ctx->needs_input_grad(edge++)) gg = at::empty(gate.sizes(), x.options(), at::MemoryFormat::Contiguous);
+        auto column = [&](bool there, Tensor& t) {
+            if (there && ctx->needs_input_grad(edge++)) t = at::empty({rows.C}, as_param);
+        };
+        column(scale.defined(), gs);
+        column(post_weight.defined(), gpw);
+        column(post_bias.defined(), gpb);
+        column(weight.defined(), gw);
+        column(ctx->saved_data["bias"].toBool(), gb);
+        const SandwichParams p = {or_null(scale), or_null(post_weight), or_null(post_bias), or_null(weight), c10::nullopt, type};
+        check(ldn_sandwich_norm_backward(ptr(gy), ptr(gh), rows.t.data_ptr(), rows.pitch, h.data_ptr(), kind ? g.t.data_ptr() : nullptr, g.pitch, kind,
+                                         rows.rows, rows.C, type_of(x), ptr(p.scale), ptr(p.post_weight), ptr(p.post_bias), ptr(p.weight), type,
+                                         floats(stats), ptr(gx), ptr(gr), ptr(gg), ptr(gs), ptr(gpw), ptr(gpb), ptr(gw), ptr(gb), stream()),
+              "sandwich_norm_backward");
+        const char* what = "sandwich_norm";
+        const bool by_rows = ctx->saved_data["rows"].toBool();
+        for (Tensor* t : {&gx, &gr, &gg, &gs, &gpw, &gpb, &gw})
+            *t = by_rows ? once_of(*t, {&h, &gate, &scale, &post_weight, &post_bias, &weight}, what)
+                         : once_of(*t, {&gate, &scale, &post_weight, &post_bias, &weight}, what);
+        return {gx, gr, gg, gs, gpw, gpb, gw, gb, Tensor(), Tensor()};
+    }
+};
+
+std::tuple<Tensor, Tensor> sandwich_norm(const Tensor& x, const Tensor& residual, const MaybeTensor& gate, const MaybeTensor& scale,
+                                         const MaybeTensor& post_weight, const MaybeTensor& post_bias, const MaybeTensor& weight,
+                                         const MaybeTensor& bias, double eps) {
+    unobserved("sandwich_norm");
+    activations(x, "x");
+    same_rows(residual, x, "residual");
+    row_fits(x);
+    int64_t type = LDN_F32;
+    const Tensor* first = nullptr;
+    const std::pair<const MaybeTensor*, const char*> params[] = {{&scale, "scale"}, {&post_weight, "post_weight"}, {&post_bias, "post_bias"},
+                                                                 {&weight, "weight"}, {&bias, "bias"}};
+    for (const auto& [t, name] : params) {
+        parameter(*t, x, name);
+        if (!t->has_value()) continue;
+        TORCH_CHECK(!first || first->scalar_type() == (*t)->scalar_type(), "scale and the norms' parameters must have one type");
+        first = &**t;
+        type = type_of(**t);
+    }
+    if (gate.has_value()) {
+        activations(*gate, "gate");
+        TORCH_CHECK(gate->scalar_type() == x.scalar_type() && gate->device() == x.device(), "gate must have the type and device of x");
+        TORCH_CHECK(gate->dim() == x.dim() && gate->sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1) &&
+                        (gate->size(-1) == 1 || gate->size(-1) == x.size(-1)),
+                    "gate must have the shape of x, or one number per row, not ", gate->sizes());
+    }
+    TORCH_CHECK(eps >= 0.0, "eps must not be negative");
+    if (wants_grad({&x, &residual, at_of(gate), at_of(scale), at_of(post_weight), at_of(post_bias), at_of(weight), at_of(bias)})) {
+        variable_list out = SandwichFn::apply(x, residual, gate, scale, post_weight, post_bias, weight, bias, type, eps);
+        return std::make_tuple(out[0], out[1]);
+    }
+    const c10::cuda::CUDAGuard guard(x.device());
+    Tensor y = at::empty(x.sizes(), x.options(), at::MemoryFormat::Contiguous), h = at::empty_like(y);
+    const SandwichParams p = {whole(scale), whole(post_weight), whole(post_bias), whole(weight), whole(bias), static_cast<int>(type)};
+    sandwich_forward(x, residual, gate, p, eps, h, y, nullptr);
+    return std::make_tuple(y, h);
+}
+
+// ---- distillation -------------------------------------------------------------------------------------------------------------------
+enum class Reduction { Mean, Sum, None };
+struct Distil {
+    Rows x;
+    Tensor values, indices, targets;  // contiguous; targets may be undefined
+    float tau, part, mix;
+    const long long* target_ptr() const { return targets.defined() ? reinterpret_cast<const long long*>(targets.data_ptr<int64_t>()) : nullptr; }
+    const long long* index_ptr() const { return reinterpret_cast<const long long*>(indices.data_ptr<int64_t>()); }
+    float of_all(Reduction r) const { return r == Reduction::Mean ? 1.0f / static_cast<float>(x.rows) : 1.0f; }
+};
+Distil distil_of(const Tensor& x, const Tensor& values, const Tensor& indices, const MaybeTensor& targets, double tau, double mix) {
+    return {rows_of(x), values.contiguous(), indices.contiguous(), targets.has_value() ? targets->contiguous() : Tensor(), static_cast<float>(tau),
+            static_cast<float>(1.0 - mix), static_cast<float>(mix)};
+}
+Tensor distil_forward(const Tensor& x, const Distil& a, Reduction reduction, float* stats) {
+    Tensor losses = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    Tensor loss = reduction == Reduction::None ? losses : at::empty({}, losses.options());
+    check(ldn_distillation(a.x.t.data_ptr(), a.x.pitch, a.x.rows, a.x.C, type_of(x), a.values.data_ptr(), type_of(a.values), a.index_ptr(),
+                           static_cast<int>(a.values.size(-1)), a.target_ptr(), a.tau, a.part, a.mix, floats(losses), stats, a.of_all(reduction),
+                           reduction == Reduction::None ? nullptr : floats(loss), stream()),
+          "distillation_loss");
+    return loss;
+}
+struct DistilFn : public torch::autograd::Function<DistilFn> {
+    static Tensor forward(AutogradContext* ctx, Tensor x, Tensor values, Tensor indices, MaybeTensor targets, double tau, double mix,
+                          int64_t reduction) {
+        const c10::cuda::CUDAGuard guard(x.device());
+        const Distil a = distil_of(x, values, indices, targets, tau, mix);
+        Tensor stats = at::empty({5, a.x.rows}, x.options().dtype(at::kFloat));
+        Tensor loss = distil_forward(x, a, static_cast<Reduction>(reduction), floats(stats));
+        ctx->saved_data["tau"] = tau;
+        ctx->saved_data["mix"] = mix;
+        ctx->saved_data["reduction"] = reduction;
+        ctx->save_for_backward({x, a.values, a.indices, a.targets, stats});
+        return loss;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once(grads, "distillation_loss");
+        variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &stats = saved[4];
+        const c10::cuda::CUDAGuard guard(x.device());
+        const Distil a = distil_of(x, saved[1], saved[2], or_null(saved[3]), ctx->saved_data["tau"].toDouble(), ctx->saved_data["mix"].toDouble());
+        const Reduction reduction = static_cast<Reduction>(ctx->saved_data["reduction"].toInt());
+        const Tensor up = grads[0].contiguous();
+        Tensor gx = at::empty(x.sizes(), x.options(), at::MemoryFormat::Contiguous);
+        check(ldn_distillation_backward(a.x.t.data_ptr(), a.x.pitch, a.x.rows, a.x.C, type_of(x), a.values.data_ptr(), type_of(a.values), a.index_ptr(),
+                                        static_cast<int>(a.values.size(-1)), a.target_ptr(), a.tau, a.part, a.mix, floats(stats), floats(up),
+                                        reduction == Reduction::None, a.of_all(reduction), gx.data_ptr(), stream()),
+              "distillation_loss_backward");
+        return {once_of(gx, {&x}, "distillation_loss"), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor distillation_loss(const Tensor& x, const Tensor& values, const Tensor& indices, const MaybeTensor& targets, double tau, double mix,
+                         int64_t reduction) {
+    unobserved("distillation_loss");
+    activations(x, "logits");
+    row_fits(x);
+    activations(values, "teacher_values");
+    plain(indices, "teacher_indices");
+    TORCH_CHECK(x.numel() / x.size(-1) <= kMostColumns, "at most ", kMostColumns, " rows at a time, not ", x.numel() / x.size(-1));
+    TORCH_CHECK(indices.scalar_type() == at::kLong, "teacher_indices must be int64, not ", indices.scalar_type());
+    TORCH_CHECK(values.dim() == x.dim() && values.sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1) && values.size(-1) <= 1024 &&
+                    indices.sizes() == values.sizes(),
+                "the teacher must have 1 to 1024 values and as many indices per row of the logits, not ", values.sizes(), " and ", indices.sizes());
+    TORCH_CHECK(values.device() == x.device() && indices.device() == x.device(), "the teacher must be on the device of the logits");
+    if (targets.has_value()) {
+        plain(*targets, "targets");
+        TORCH_CHECK(targets->scalar_type() == at::kLong && targets->device() == x.device() && targets->sizes() == x.sizes().slice(0, x.dim() - 1),
+                    "targets must be one int64 per row, on the device of the logits");
+    }
+    TORCH_CHECK(tau > 0.0 && tau <= std::numeric_limits<float>::max() && static_cast<float>(tau) >= std::numeric_limits<float>::min(),
+                "temperature must be a positive number, not ", tau);
+    TORCH_CHECK(mix >= 0.0 && mix <= 1.0, "mix must be a share, not ", mix);
+    TORCH_CHECK(!wants_grad({&values}), "distillation_loss has no gradient for the teacher: detach it");
+    if (wants_grad({&x})) return DistilFn::apply(x, values, indices, targets, tau, mix, reduction);
+    const c10::cuda::CUDAGuard guard(x.device());
+    return distil_forward(x, distil_of(x, values, indices, targets, tau, mix), static_cast<Reduction>(reduction), nullptr);
+}
+
 }  // namespace
 
 void register_head(pybind11::module& m) {
@@ -533,4 +730,6 @@ void register_head(pybind11::module& m) {
     m.def("layer_norm_quantized", &layer_norm_quantized);
     m.def("int8_linear", &int8_linear);
     m.def("gated_linear", &gated_linear);
+    m.def("sandwich_norm", &sandwich_norm);
+    m.def("distillation_loss", &distillation_loss);
 }

@@ -1,9 +1,10 @@
 // The gated projection, forward and backward: operands as the tensor cores' loads want them, the gradients of the two projections, and
 // the entry points.
 //
-// The backward pass needs both projections again.  They are kept in the rows' type (16 bits: rounded, 2^-9 of each, as the rows that came
-// in are; making them again would cost a third of a training step's products).  Bound by memory: dy, both projections, both gradients
-// once.
+// The backward pass needs both projections again.  They are kept in 32 bits: rounded to bfloat16 they took the weights' gradients from
+// 2.4e-3 to 3.1e-3 of 64 bits (1.7e-3 is their own rounding), and making them again would cost a third of a training step's products.
+// What enters the products as dg and du has the rows' type: the tensor cores multiply no other at that rate.  Bound by memory: dy, both
+// projections, both gradients once.
 #include "ldn_gated.cuh"
 
 namespace ldn {
@@ -138,7 +139,7 @@ struct Operands {
 // ---- gradients of the projections --------------------------------------------------------------------------------------------------
 struct GradArgs {
     const void* grad_y;  // [T][H]
-    const void *g, *u;   // [T][pitch_saved]
+    const float *g, *u;  // [T][pitch_saved]
     long long pitch_saved, T;
     int H, activation;
     unsigned short* to;  // [side][part][T][pitch_to]
@@ -179,8 +180,8 @@ __global__ void __launch_bounds__(kGradLanes * kGradRows) gated_grad_kernel(cons
         for (long long row = static_cast<long long>(blockIdx.y) * kGradRows + part; row < a.T; row += static_cast<long long>(gridDim.y) * kGradRows) {
             float dy[8], g[8], u[8], dg[8], du[8];
             load8(static_cast<const T*>(a.grad_y) + row * a.H + c, whole, there, dy);
-            load8(static_cast<const T*>(a.g) + row * a.pitch_saved + c, there >= 8, there, g);
-            load8(static_cast<const T*>(a.u) + row * a.pitch_saved + c, there >= 8, there, u);
+            load8(a.g + row * a.pitch_saved + c, there >= 8, there, g);
+            load8(a.u + row * a.pitch_saved + c, there >= 8, there, u);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float2 f = activation_and_slope(g[j], a.activation);
@@ -258,7 +259,7 @@ using namespace ldn;
 
 extern "C" LDN_API int ldn_gated_linear(const void* x, long long pitch, long long rows, int K, int H, int type, const void* w_gate,
                                         long long pitch_gate, const void* w_up, long long pitch_up, const void* b_gate, const void* b_up,
-                                        int param_type, int activation, void* y, void* g, void* u, long long pitch_saved,
+                                        int param_type, int activation, void* y, float* g, float* u, long long pitch_saved,
                                         ldn_stream_t stream) {
     if (!gated_fits(rows, K, H, type, param_type, b_gate, b_up, activation, pitch_gate, pitch_up) || !g != !u) return kBadArgument;
     if (g && (pitch_saved < H || pitch_saved % 16 || !on32(g) || !on32(u))) return kBadArgument;
@@ -290,8 +291,8 @@ extern "C" LDN_API int ldn_gated_linear(const void* x, long long pitch, long lon
 }
 
 extern "C" LDN_API int ldn_gated_linear_backward(const void* grad_y, const void* x, long long pitch, long long rows, int K, int H, int type,
-                                                 const void* w_gate, long long pitch_gate, const void* w_up, long long pitch_up, const void* g,
-                                                 const void* u, long long pitch_saved, int activation, void* grad_x, void* grad_w_gate,
+                                                 const void* w_gate, long long pitch_gate, const void* w_up, long long pitch_up, const float* g,
+                                                 const float* u, long long pitch_saved, int activation, void* grad_x, void* grad_w_gate,
                                                  void* grad_w_up, void* grad_b_gate, void* grad_b_up, int param_type, ldn_stream_t stream) {
     if (!gated_fits(rows, K, H, type, param_type, grad_b_gate, grad_b_up, activation, pitch_gate, pitch_up) || !grad_w_gate != !grad_w_up ||
         pitch_saved < H || pitch_saved % 16)

@@ -17,8 +17,8 @@ struct GatedArgs {
     long long T;
     int K, H, activation;
     void* y;              // [T][H]
-    void *g, *u;          // [T][pitch_saved], kept for the backward pass; may be null
-    long long pitch_saved;  // a multiple of 16 elements, as the addresses are of 32 bytes
+    float *g, *u;           // [T][pitch_saved], kept for the backward pass; may be null
+    long long pitch_saved;  // a multiple of 16, as the addresses are of 32 bytes
 };
 
 inline bool gated_activation(int a) { return a == LDN_RELU || a == LDN_SILU || a == LDN_GELU || a == LDN_SIGMOID; }

@@ -80,8 +80,8 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_con
             if (a.b_gate) g[0] += param_at<T>(a.b_gate, a.wide, h);
             if (a.b_up) u += param_at<T>(a.b_up, a.wide, h);
             if (a.g) {
-                static_cast<T*>(a.g)[t * a.pitch_saved + h] = from_float<T>(g[0]);
-                static_cast<T*>(a.u)[t * a.pitch_saved + h] = from_float<T>(u);
+                a.g[t * a.pitch_saved + h] = g[0];
+                a.u[t * a.pitch_saved + h] = u;
             }
             activate(g, a.activation);
             static_cast<T*>(a.y)[static_cast<long long>(t) * a.H + h] = from_float<T>(g[0] * u);

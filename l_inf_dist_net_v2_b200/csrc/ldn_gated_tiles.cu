@@ -45,7 +45,7 @@ void plan(GatedForm form, long long M, int N, int terms, int type, const DeviceC
     a->side_units = steps_over(a->side_steps, unit_steps);
     a->units = a->side_units * (form == GatedForm::GradRows ? 2 : 1);
     const long long least = parted ? 1 : 4, shares = (static_cast<long long>(a->tiles) * a->units + least - 1) / least;
-    const int resident = resident_pairs(ctx);
+    const int held = resident_pairs(ctx), resident = held < kMostPairs ? held : kMostPairs;
     a->pairs = static_cast<int>(shares < resident ? shares : resident);
     const int rest = a->tiles % a->pairs;
     a->whole = a->tiles;
@@ -72,7 +72,8 @@ int launch(const TileArgs& a, const CUtensorMap& map_a, const CUtensorMap& map_b
     if (r != kOk) return r;
     r = launch_after_in_clusters(kernel, 2, static_cast<unsigned>(2 * a.pairs), kProductThreads, kTileSmem, st, map_a, map_b0, map_b1, a);
     if (r != kOk || a.whole == a.tiles) return r;
-    return launch_after(gated_parts_kernel<T, F>, dim3(a.tiles - a.whole, kSide / kFixRows), kFixThreads, 0, st, a);
+    const unsigned rows = a.M < kSide ? static_cast<unsigned>((a.M + kFixRows - 1) / kFixRows) : kSide / kFixRows;
+    return launch_after(gated_parts_kernel<T, F>, dim3(a.tiles - a.whole, rows), kFixRows * kFixRuns<F>, 0, st, a);
 }
 
 }  // namespace

@@ -143,6 +143,9 @@ __device__ __forceinline__ void store_run(T* to, const float (&v)[N], int column
                 store_32_bytes(to + i, w);
             }
         }
+    } else if (sizeof(T) == 4 && columns >= N && (at & 15u) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(to + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     } else if (sizeof(T) == 2 && columns >= N && (at & 3u) == 0) {
 #pragma unroll
         for (int i = 0; i < N; i += 2) reinterpret_cast<uint32_t*>(to)[i / 2] = two_of<T>(v[i], v[i + 1]);
@@ -167,8 +170,8 @@ __device__ __forceinline__ void finish(const TileArgs& a, int which, long long m
             for (int j = 0; j < N; ++j) v1[j] += j < columns ? param_at<T>(a.b_up, a.wide, n + j) : 0.0f;
         }
         if (a.out1) {  // (rows of these are a whole number of runs)
-            store_run<T, N>(static_cast<T*>(a.out1) + m * a.pitch_saved + n, v0, N);
-            store_run<T, N>(static_cast<T*>(a.out2) + m * a.pitch_saved + n, v1, N);
+            store_run<float, N>(static_cast<float*>(a.out1) + m * a.pitch_saved + n, v0, N);
+            store_run<float, N>(static_cast<float*>(a.out2) + m * a.pitch_saved + n, v1, N);
         }
         activate(v0, a.activation);
 #pragma unroll
@@ -408,43 +411,64 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     }
 }
 
-// The parts of a tile that several pairs share, added up in the order of their terms; a block has 16 rows of a tile, a thread four columns.
-constexpr int kFixRows = 16, kFixThreads = 256;
+// The parts of a tile that several pairs share, added up in the order of their terms; a block has four rows of a tile, a thread four columns.
+// Which pairs have a part is found by a thread each, and four parts are under way at a time (found and loaded one after the other, 15 parts
+// of 64 rows took 29 us).
+constexpr int kFixRows = 4, kMostPairs = 128;
+template <GatedForm F>
+constexpr int kFixRuns = F == GatedForm::Forward ? 32 : 64;  // of four columns
 template <class T, GatedForm F>
-__global__ void __launch_bounds__(kFixThreads) gated_parts_kernel(const __grid_constant__ TileArgs a) {
+__global__ void __launch_bounds__(kFixRows * kFixRuns<F>) gated_parts_kernel(const __grid_constant__ TileArgs a) {
     stream_order_begin();
     constexpr bool kGated = F == GatedForm::Forward;
-    constexpr int kRuns = kGated ? 32 : 64;  // of four columns
+    __shared__ int slots[kMostPairs], first, last, alone;
     const int i = blockIdx.x, all_m = F == GatedForm::GradWeights ? 2 * a.tiles_m : a.tiles_m;
     const long long begin = static_cast<long long>(i) * a.units, end = begin + a.units;
-    const long long all = static_cast<long long>(a.tiles - a.whole) * a.units;
-    int first = static_cast<int>(begin * a.pairs / all);
-    while (first > 0 && range_begin(a, first) > begin) --first;
-    while (range_begin(a, first + 1) <= begin) ++first;
-    if (range_begin(a, first) <= begin && range_begin(a, first + 1) >= end) return;  // (one pair has all of it, and has stored it)
+    if (threadIdx.x == 0) {
+        first = kMostPairs;
+        last = alone = 0;
+    }
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < a.pairs) {
+        const int q = threadIdx.x;
+        const long long b = range_begin(a, q), e = range_begin(a, q + 1);
+        const bool there = b < e && b < end && e > begin;
+        slots[q] = there ? 2 * q + (b < begin) : -1;
+        if (there) {
+            atomicMin(&first, q);
+            atomicMax(&last, q);
+            if (b <= begin && e >= end) alone = 1;
+        }
+    }
+    __syncthreads();
+    if (alone) return;  // (one pair has all of the tile, and has stored it)
     const Place p = place_of(a, a.whole + i, all_m);
     const int which = F == GatedForm::GradWeights && p.m >= a.tiles_m;
-    const long long m0 = static_cast<long long>(which ? p.m - a.tiles_m : p.m) * kSide + blockIdx.y * kFixRows;
-    for (int item = threadIdx.x; item < kFixRows * kRuns; item += kFixThreads) {
-        const int row = item / kRuns, run = item % kRuns;
-        const int n = kGated ? p.n * 128 + 4 * run : p.n * kSide + 4 * run;
-        if (m0 + row >= a.M || n >= a.N) continue;
-        const float* from = a.partials + (static_cast<size_t>(blockIdx.y) * kFixRows + row) * kSide + 4 * run;
-        float v0[4] = {}, v1[4] = {};
-        for (int q = first; q < a.pairs; ++q) {
-            const long long b = range_begin(a, q);
-            if (b >= end) break;
-            if (b == range_begin(a, q + 1)) continue;
-            const float* f = from + static_cast<size_t>(2 * q + (b < begin)) * kSide * kSide;
-            const float4 s = *reinterpret_cast<const float4*>(f);
-            v0[0] += s.x; v0[1] += s.y; v0[2] += s.z; v0[3] += s.w;
-            if constexpr (kGated) {
-                const float4 t = *reinterpret_cast<const float4*>(f + 128);
-                v1[0] += t.x; v1[1] += t.y; v1[2] += t.z; v1[3] += t.w;
+    const int row = blockIdx.y * kFixRows + threadIdx.x / kFixRuns<F>, run = threadIdx.x % kFixRuns<F>;
+    const long long m = static_cast<long long>(which ? p.m - a.tiles_m : p.m) * kSide + row;
+    const int n = kGated ? p.n * 128 + 4 * run : p.n * kSide + 4 * run;
+    if (m >= a.M || n >= a.N) return;
+    const float* from = a.partials + static_cast<size_t>(row) * kSide + 4 * run;
+    float v0[4] = {}, v1[4] = {};
+    for (int q0 = first; q0 <= last; q0 += 4) {
+        float4 s[4], t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int slot = q0 + j <= last ? slots[q0 + j] : -1;
+            s[j] = t[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (slot >= 0) {
+                const float* f = from + static_cast<size_t>(slot) * kSide * kSide;
+                s[j] = *reinterpret_cast<const float4*>(f);
+                if constexpr (kGated) t[j] = *reinterpret_cast<const float4*>(f + 128);
             }
         }
-        finish<T, F, 4>(a, which, m0 + row, n, v0, v1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v0[0] += s[j].x; v0[1] += s[j].y; v0[2] += s[j].z; v0[3] += s[j].w;
+            if constexpr (kGated) { v1[0] += t[j].x; v1[1] += t[j].y; v1[2] += t[j].z; v1[3] += t[j].w; }
+        }
     }
+    finish<T, F, 4>(a, which, m, n, v0, v1);
 }
 
 }  // namespace

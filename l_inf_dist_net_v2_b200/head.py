@@ -13,7 +13,8 @@ import torch.nn as nn
 
 from . import norm_dist_cuda as _C
 
-__all__ = ["layer_norm", "dropout", "dropout_add_layer_norm", "quantize_rows", "layer_norm_quantized", "int8_linear", "gated_linear", "LayerNorm",
+__all__ = ["layer_norm", "dropout", "dropout_add_layer_norm", "quantize_rows", "layer_norm_quantized", "int8_linear", "gated_linear", "sandwich_norm",
+           "LayerNorm",
            "Dropout", "Int8Linear", "ResidualHead", "QuantizedHead"]
 
 _ACTIVATIONS = {"none": 0, "relu": 1, "tanh": 2}
@@ -94,12 +95,22 @@ def gated_linear(x, weight_gate, weight_up, bias_gate=None, bias_up=None, activa
     """act(x @ weight_gate.T + bias_gate) * (x @ weight_up.T + bias_up): both projections, the activation and the product in one kernel,
     with the gradients of all five.  activation: "silu", "gelu" (of the normal distribution's function), "sigmoid" or "relu".
 
-    Weights are (outputs, terms) of the type of x, biases of that type or float32; sums have 32 bits.  Both projections are kept in the type
-    of x for the backward pass.  Rows of 16-bit tensors that start at multiples of 16 bytes are read where they lie, others are copied
+    Weights are (outputs, terms) of the type of x, biases of that type or float32; sums have 32 bits.  Both projections are kept in 32 bits
+    for the backward pass.  Rows of 16-bit tensors that start at multiples of 16 bytes are read where they lie, others are copied
     first; float32 is multiplied on the tensor cores as three bfloat16 numbers (24 bits), where an infinity gives not-a-numbers."""
     if activation not in _GATES:
         raise ValueError(f"activation must be one of {sorted(_GATES)}, not {activation!r}")
     return _native().gated_linear(x, weight_gate, weight_up, bias_gate, bias_up, _GATES[activation])
+
+
+def sandwich_norm(x, residual, weight=None, bias=None, post_weight=None, post_bias=None, scale=None, gate=None, eps=1e-5):
+    """(y, h): h = residual + gate * scale * layer_norm(x, post_weight, post_bias), in the type of x, and y = layer_norm(h, weight, bias):
+    the norm behind a block, its gate and residual scale, and the next block's norm in one kernel each way, with the gradients of
+    all of them.
+
+    `gate` has the shape of x, or one number per row (a last dimension of 1), in the type of x; `scale` and the norms' parameters have one
+    value per column, all of one type: float32 or that of x."""
+    return _native().sandwich_norm(x, residual, gate, scale, post_weight, post_bias, weight, bias, eps)
 
 
 class LayerNorm(nn.Module):

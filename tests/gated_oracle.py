@@ -55,8 +55,8 @@ def backward(dy, x, wg, wu, f, name, dtype):
     unit = 0.0 if dtype == torch.float32 else UNIT[dtype]
     dy, x, wg, wu = dy.double().flatten(0, -2), x.double().flatten(0, -2), wg.double(), wu.double()
     a, s = act(f["g"], name)
-    # both projections are kept in the rows' type, and their gradients enter the products in it
-    off_g, off_u = f["off_g"] + (unit + EPS32) * f["g"].abs(), f["off_u"] + (unit + EPS32) * f["u"].abs()
+    # (their gradients enter the products in the rows' type)
+    off_g, off_u = f["off_g"] + EPS32 * f["g"].abs(), f["off_u"] + EPS32 * f["u"].abs()
     dg, du = dy * f["u"] * s, dy * a
     off_s = CURVE[name] * off_g + (16 + 4 * f["g"].abs()) * EPS32
     if name == "relu":  # (on the other side of zero)

@@ -1,0 +1,108 @@
+"""Distillation from a teacher's top logits on a B200 against the formulas in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import distil_oracle as oracle
+import head_oracle
+import l_inf_dist_net_v2_b200 as ldn
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+TYPES = [F32, F16, BF16]
+
+
+def made(rows, V, k, dtype, teacher=None, ragged=False, masked=False, layout="plain", seed=0):
+    f = dict(device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed + V))
+    x = 2 * torch.randn(rows, V, **f) + 3 * torch.randn(rows, 1, **f)
+    t = 0.5 * x + torch.randn(rows, V, **f)
+    if masked:
+        gone = torch.rand(rows, V, **f) < 0.2
+        gone[:, :k] = False
+        x.masked_fill_(gone, -math.inf)
+        t.masked_fill_(gone, -math.inf)
+    values, indices = t.topk(k, 1)
+    targets = indices[:, -1].clone()
+    if ragged:
+        indices = torch.where(torch.rand(rows, k, **f) < torch.rand(rows, 1, **f), indices, -1)
+        indices[0] = -1
+        targets[1::3] = -1
+    x = x.to(dtype)
+    if layout == "slice":
+        x = torch.nn.functional.pad(x, (0, 3))[:, :V]
+    if layout == "shifted":
+        flat = torch.empty(rows * V + 1, device="cuda", dtype=dtype)
+        flat[1:] = x.reshape(-1)
+        x = flat[1:].view(rows, V)
+    return x, values.to(teacher or dtype), indices, targets, torch.randn(rows, **f)
+
+
+def check(x, values, indices, targets, up, tau, mix):
+    leaf = x.detach().requires_grad_()
+    losses = ldn.distillation_loss(leaf, values, indices, targets, tau, mix, "none")
+    want, bound, dx, off = oracle.loss_and_gradient(x, values, indices, targets, tau, mix, up)
+    assert losses.dtype == torch.float32 and losses.shape == x.shape[:-1]
+    assert head_oracle.near(losses.detach(), want, bound)
+    got, = torch.autograd.grad(losses, leaf, up)
+    assert got.dtype == x.dtype and got.shape == x.shape
+    assert head_oracle.near(got, dx, off)
+    with torch.no_grad():
+        assert torch.equal(ldn.distillation_loss(x, values, indices, targets, tau, mix, "none"), losses)
+    for reduction, by in (("sum", 1.0), ("mean", 1.0 / x.size(0))):
+        leaf = x.detach().requires_grad_()
+        loss = ldn.distillation_loss(leaf, values, indices, targets, tau, mix, reduction)
+        # (a chain of rows / 4096 + 24 additions)
+        near = (bound.sum() + (x.size(0) / 4096 + 28) * head_oracle.EPS32 * want.abs().sum()) * by
+        assert loss.dim() == 0 and head_oracle.near(loss.detach(), want.sum() * by, near)
+        same, = torch.autograd.grad(loss, leaf, torch.full_like(loss, 3.0))
+        _, _, dx1, off1 = oracle.loss_and_gradient(x, values, indices, targets, tau, mix, torch.full_like(up, 3.0 * by))
+        assert head_oracle.near(same, dx1, off1)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows, V, k", [(1, 1, 1), (5, 2, 2), (33, 10, 3), (9, 33, 33), (7, 1000, 20), (3, 2048, 64), (3, 2049, 64), (2, 4097, 1),
+                                        (5, 40001, 100), (1, 131072, 1000), (300, 8192, 7), (2, 16384, 3), (3000, 17, 2)])
+def test_sizes(rows, V, k, dtype):
+    for tau, mix in ((1.0, 0.0), (2.0, 0.3), (1.0, 0.4), (4.0, 1.0)):
+        check(*made(rows, V, k, dtype), tau, mix)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("V", [10, 1001, 5003])
+def test_lists_of_different_lengths_masks_and_layouts(V, dtype):
+    for layout in ("plain", "slice", "shifted"):
+        check(*made(13, V, 5, dtype, ragged=True, masked=True, layout=layout), 2.0, 0.3)
+        check(*made(13, V, 5, dtype, teacher=F32, ragged=True, layout=layout), 0.5, 0.0)
+
+
+@pytest.mark.parametrize("V", [10, 1001, 5003])
+def test_one_class_several_times_and_in_any_order(V):
+    for dtype in TYPES:
+        x, values, indices, targets, up = made(6, V, 5, dtype)
+        indices[:, 3] = indices[:, 0]
+        indices[1] = indices[1, 0]
+        targets[2] = indices[2, 3]
+        check(x, values.flip(1), indices, targets, up, 2.0, 0.3)
+
+
+@pytest.mark.parametrize("V", [12, 3000])
+def test_rows_that_say_nothing_and_rows_that_are_wrong(V):
+    x, values, indices, targets, up = made(8, V, 4, F32)
+    x[0] = -math.inf            # no choice, no list, no label
+    indices[0], targets[0] = -1, -1
+    values[1] = -math.inf       # a list of nothing but minus infinity
+    targets[1] = -1
+    indices[2, 1] = V           # beyond the classes
+    targets[3] = V
+    x[4, 5] = math.nan
+    x[5, 5] = math.inf
+    values[6, 0] = math.nan
+    x[7, indices[7, 0]] = -math.inf  # what the teacher prefers is no choice
+    leaf = x.detach().requires_grad_()
+    losses = ldn.distillation_loss(leaf, values, indices, targets, 2.0, 0.3, "none")
+    dx, = torch.autograd.grad(losses.sum(), leaf)
+    assert torch.equal(losses[:2].detach(), torch.zeros(2, device="cuda")) and torch.equal(dx[:2], torch.zeros_like(dx[:2]))
+    assert losses[2:7].isnan().all() and dx[2:6].isnan().all() and dx[6, indices[6]].isnan().all()
+    assert losses[7] == math.inf and dx[7].isfinite().all()
