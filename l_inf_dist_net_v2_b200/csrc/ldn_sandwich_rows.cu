@@ -16,7 +16,8 @@ template <Gate G>
 constexpr int kForwardStreams = G == Gate::All ? 3 : 2;
 template <Gate G>
 constexpr int kBackwardStreams = G == Gate::All ? 5 : 4;
-__host__ __device__ constexpr int rows_at_once(int elements, bool group) { return group || elements > 8 ? 1 : 2; }
+// Rows that a block takes at a time
+__host__ __device__ constexpr int rows_forward(int elements, bool group) { return group || elements > 16 ? 1 : 2; }
 
 // scale weight and scale bias of a piece's columns (1 and 0 outside the row)
 template <class T, bool SHIFT>
@@ -36,7 +37,7 @@ template <class T, Gate G, int ITEMS, bool GROUP, bool SHIFT>
 __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPiece<T>), 1)
 sandwich_registers_kernel(const __grid_constant__ SandwichArgs a, int lanes, int depth) {
     stream_order_begin();
-    constexpr int V = kPiece<T>, S = kForwardStreams<G>, R = rows_at_once(ITEMS * V, GROUP);
+    constexpr int V = kPiece<T>, S = kForwardStreams<G>, R = rows_forward(ITEMS * V, GROUP);
     constexpr bool kKeep = ITEMS * V <= 16;
     __shared__ float slots[2 * RowSum::kSlots];
     extern __shared__ uint4 ring[];  // [depth][row][stream][item][thread]
@@ -209,10 +210,10 @@ template <class T, Gate G, int ITEMS, bool GROUP, bool SHIFT>
 __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPiece<T>), 1)
 sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int lanes, int depth) {
     stream_order_begin();
-    constexpr int V = kPiece<T>, S = kBackwardStreams<G>, R = rows_at_once(ITEMS * V, GROUP);
+    constexpr int V = kPiece<T>, S = kBackwardStreams<G>, R = 1;
     constexpr int K = G == Gate::Row ? 4 : 2;  // sums of a row in the second round (a power of two)
     __shared__ float slots[2 * RowSum::kSlots];
-    extern __shared__ uint4 ring[];  // [depth][row][stream][item][thread]; at the end, groups: [warp][4][C] floats
+    extern __shared__ uint4 ring[];  // [depth][row][stream][item][thread], then blocks: [3][item][V / 4][thread]; at the end, groups: [warp][4][C] floats
     RowSum reduce{lanes, slots, 0};
     const int lane = GROUP ? threadIdx.x & (lanes - 1) : threadIdx.x;
     const int per_block = GROUP ? kGroupThreads / lanes : 1;
@@ -221,7 +222,35 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
     const float inv_C = 1.0f / a.C;
     const int shift = SHIFT ? shift_of(static_cast<const T*>(a.x) + (mine < a.rows ? mine : 0) * a.pitch) : 0;
     auto column = [&](int i) { return (lane + i * lanes) * V - shift; };
-    float2 w1[ITEMS][V / 2], b1[ITEMS][V / 2], w2[ITEMS][V / 2];
+    // a group's columns' parameters stay in registers, a block's in shared memory, where each thread puts and finds its own (as registers, the
+    // kernel spilled: 16384 x 5120 bf16 415 us)
+    float2 kept[GROUP ? 3 : 1][ITEMS][V / 2];
+    uint4* params = ring + static_cast<size_t>(depth) * R * S * ITEMS * blockDim.x + threadIdx.x;
+    auto set_param_piece = [&](int k, int i, const float2 (&v)[V / 2]) {
+#pragma unroll
+        for (int e = 0; e < V / 2; e += 2) {
+            if constexpr (GROUP) {
+                kept[k][i][e] = v[e];
+                kept[k][i][e + 1] = v[e + 1];
+            } else {
+                params[((k * ITEMS + i) * (V / 4) + e / 2) * blockDim.x] =
+                    make_uint4(__float_as_uint(v[e].x), __float_as_uint(v[e].y), __float_as_uint(v[e + 1].x), __float_as_uint(v[e + 1].y));
+            }
+        }
+    };
+    auto param_piece = [&](int k, int i, float2 (&v)[V / 2]) {
+#pragma unroll
+        for (int e = 0; e < V / 2; e += 2) {
+            if constexpr (GROUP) {
+                v[e] = kept[k][i][e];
+                v[e + 1] = kept[k][i][e + 1];
+            } else {
+                const uint4 raw = params[((k * ITEMS + i) * (V / 4) + e / 2) * blockDim.x];
+                v[e] = make_float2(__uint_as_float(raw.x), __uint_as_float(raw.y));
+                v[e + 1] = make_float2(__uint_as_float(raw.z), __uint_as_float(raw.w));
+            }
+        }
+    };
     float2 sums[4][ITEMS][V / 2];  // dy z2, dy, d gate z1, d gate
     uint4 mask[ITEMS];
     int bytes[ITEMS];
@@ -233,8 +262,12 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
             for (int e = 0; e < V / 2; ++e) sums[k][i][e] = both(0.0f);
         mask[i] = mask_of<T, SHIFT>(column(i), a.C);
         bytes[i] = piece_bytes<T>(column(i), a.C);
-        load_scaled<T, SHIFT>(a.p, column(i), a.C, w1[i], b1[i]);
-        load_params<T, SHIFT>(a.p.weight, a.p.wide, column(i), a.C, 1.0f, w2[i]);
+        float2 w[V / 2], b[V / 2];
+        load_scaled<T, SHIFT>(a.p, column(i), a.C, w, b);
+        set_param_piece(0, i, w);
+        set_param_piece(1, i, b);
+        load_params<T, SHIFT>(a.p.weight, a.p.wide, column(i), a.C, 1.0f, w);
+        set_param_piece(2, i, w);
     }
     const int c0 = column(0), apart = lanes * V;
     int to_fetch = mine < a.rows ? static_cast<int>((a.rows - mine + step - 1) / step) : 0, to_make = to_fetch;
@@ -310,17 +343,18 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
             float2 s0 = both(0.0f), s1 = both(0.0f);
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
-                float2 h[V / 2], dy[V / 2];
+                float2 h[V / 2], dy[V / 2], w2[V / 2];
                 piece_of(j, 1, i, h);
                 piece_of(j, 2, i, dy);
+                param_piece(2, i, w2);
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e) {
                     // (rstd behind the sum: outside the row the gradient is 0 and h - mean a number, but (0 - mean) rstd may be infinite)
                     const float2 u = __fmul2_rn(dy[e], __fadd2_rn(h[e], both(-mean2[j])));
                     sums[0][i][e] = __ffma2_rn(u, both(rstd2[j]), sums[0][i][e]);
                     sums[1][i][e] = __fadd2_rn(sums[1][i][e], dy[e]);
-                    s0 = __ffma2_rn(dy[e], w2[i][e], s0);
-                    s1 = __ffma2_rn(u, w2[i][e], s1);
+                    s0 = __ffma2_rn(dy[e], w2[e], s0);
+                    s1 = __ffma2_rn(u, w2[e], s1);
                 }
             }
             s[2 * j] = s0.x + s0.y;
@@ -335,21 +369,26 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
                 const int c = column(i);
-                float2 d[V / 2], h[V / 2], dh[V / 2], x[V / 2], n[V / 2];
+                float2 d[V / 2], h[V / 2], x[V / 2], n[V / 2], w[V / 2];
                 piece_of(j, 1, i, h);
                 piece_of(j, 2, i, d);
-                piece_of(j, 3, i, dh);
+                param_piece(2, i, w);
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e)
+                    d[e] = __ffma2_rn(__fadd2_rn(h[e], both(-mean2[j])), both(-m2), __ffma2_rn(d[e], w[e], both(-m1)));
+                piece_of(j, 3, i, h);
                 piece_of(j, 0, i, x);
+                param_piece(0, i, w);
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e) {
-                    const float2 p = __ffma2_rn(d[e], w2[i][e], both(-m1));
-                    d[e] = __ffma2_rn(__ffma2_rn(__fadd2_rn(h[e], both(-mean2[j])), both(-m2), p), both(rstd2[j]), dh[e]);
+                    d[e] = __ffma2_rn(d[e], both(rstd2[j]), h[e]);
                     x[e] = __fadd2_rn(x[e], both(-mean1[j]));  // (rstd behind the sums, as above)
                 }
                 if (live(j) && a.grad_residual) store_piece<T, SHIFT>(to_onto.of(j, i * apart), c, a.C, pack<T>(d));
                 if constexpr (G != Gate::None) {
+                    param_piece(1, i, n);
 #pragma unroll
-                    for (int e = 0; e < V / 2; ++e) n[e] = __fmul2_rn(d[e], __ffma2_rn(__fmul2_rn(x[e], both(rstd1[j])), w1[i][e], b1[i][e]));
+                    for (int e = 0; e < V / 2; ++e) n[e] = __fmul2_rn(d[e], __ffma2_rn(__fmul2_rn(x[e], both(rstd1[j])), w[e], n[e]));
                 }
                 if constexpr (G == Gate::All) {
                     if (live(j) && a.grad_gate) store_piece<T, SHIFT>(to_gate.of(j, i * apart), c, a.C, pack<T>(n));
@@ -374,9 +413,9 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
                     const float2 u = __fmul2_rn(d[e], x[e]);
                     sums[2][i][e] = __ffma2_rn(u, both(rstd1[j]), sums[2][i][e]);
                     sums[3][i][e] = __fadd2_rn(sums[3][i][e], d[e]);
-                    by[j][i][e] = __fmul2_rn(d[e], w1[i][e]);
+                    by[j][i][e] = __fmul2_rn(d[e], w[e]);
                     t0 = __fadd2_rn(t0, by[j][i][e]);
-                    t1 = __ffma2_rn(u, w1[i][e], t1);
+                    t1 = __ffma2_rn(u, w[e], t1);
                 }
             }
             t[K * j] = t0.x + t0.y;
@@ -471,28 +510,32 @@ struct RowShape {
     int blocks, depth;
     size_t smem;
 };
-RowShape shape_of(const RowPlan& p, long long rows, int R, int streams, int per_sm, const DeviceCtx* ctx) {
-    RowShape s = {p, 0, 0, 0};
+// extra: bytes of a block beside its rows
+bool shape_of(const RowPlan& p, long long rows, int R, int streams, long long extra, int per_sm, const DeviceCtx* ctx, RowShape* s) {
     const long long row_bytes = static_cast<long long>(R) * streams * p.items * p.threads * 16, most_smem = ctx->max_smem_optin - 4096;
-    s.depth = ring_depth(row_bytes, most_smem / per_sm - 1024);
-    while (s.depth < 2 && per_sm > 1) s.depth = ring_depth(row_bytes, most_smem / --per_sm - 1024);
+    s->p = p;
+    s->depth = ring_depth(row_bytes, most_smem / per_sm - 1024 - extra);
+    while (s->depth < 2 && per_sm > 1) s->depth = ring_depth(row_bytes, most_smem / --per_sm - 1024 - extra);
+    if (s->depth < 1) return false;
     const long long needed = (rows + p.rows_per_block() - 1) / p.rows_per_block();
     long long blocks = static_cast<long long>(per_sm) * ctx->sm_count;
     if (p.shift && !p.group) blocks = blocks / 8 * 8;
     if (needed < blocks) blocks = needed;  // (a block has one row at most, then, and it does not matter how far they are apart)
     const long long turns = (needed + R * blocks - 1) / (R * blocks);
-    if (turns < s.depth) s.depth = static_cast<int>(turns);
-    s.blocks = static_cast<int>(blocks);
-    s.smem = static_cast<size_t>(s.depth) * row_bytes;
-    return s;
+    if (turns < s->depth) s->depth = static_cast<int>(turns);
+    s->blocks = static_cast<int>(blocks);
+    s->smem = static_cast<size_t>(s->depth * row_bytes + extra);
+    return true;
 }
+// Calls f with a variant's numbers.  Blocks' rows: 16 elements per thread of 16 bits (the instructions around an element count: 16384 x 5120
+// with 8 took 203 and 415 us), 8 of 32; 32 where that does not reach.
 template <class T, class F>
 int with_items(const RowPlan& p, F f) {
-    constexpr int k8 = 8 / kPiece<T>, k16 = 16 / kPiece<T>, k32 = 32 / kPiece<T>;
+    constexpr int k8 = 8 / kPiece<T>, k16 = 16 / kPiece<T>, k32 = 32 / kPiece<T>, kBlock = sizeof(T) == 4 ? k8 : k16;
     using std::integral_constant;
     auto go = [&](auto items, auto group) { return p.shift ? f(items, group, std::true_type()) : f(items, group, std::false_type()); };
     if (p.group) return p.items == k8 ? go(integral_constant<int, k8>(), std::true_type()) : go(integral_constant<int, k16>(), std::true_type());
-    return p.items == k8 ? go(integral_constant<int, k8>(), std::false_type()) : go(integral_constant<int, k32>(), std::false_type());
+    return p.items == kBlock ? go(integral_constant<int, kBlock>(), std::false_type()) : go(integral_constant<int, k32>(), std::false_type());
 }
 template <class F>
 int with_gate(Gate gate, F f) {
@@ -502,6 +545,24 @@ int with_gate(Gate gate, F f) {
         default: return f(std::integral_constant<Gate, Gate::All>());
     }
 }
+// Blocks of a kernel that an SM's registers hold, and the kernel's right to shared memory
+template <auto KERNEL>
+int resident_blocks(int threads, const DeviceCtx* ctx, int* per_sm) {
+    static OncePerDevice once;
+    const int r = once([&] { return allow_smem(KERNEL, ctx->max_smem_optin - 2560); });
+    if (r != kOk) return r;
+    static std::atomic<int> resident[64][33];
+    std::atomic<int>& known = resident[ctx->device][threads / 32];
+    *per_sm = known.load(std::memory_order_acquire);
+    if (*per_sm == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(per_sm, KERNEL, threads, 0) != cudaSuccess || *per_sm < 1) {
+            cudaGetLastError();
+            *per_sm = 1;
+        }
+        known.store(*per_sm, std::memory_order_release);
+    }
+    return kOk;
+}
 
 bool plan_forward(Gate gate, const SandwichArgs& a, int type, RowPlan* p) {
     const int size = size_of(type);
@@ -510,25 +571,48 @@ bool plan_forward(Gate gate, const SandwichArgs& a, int type, RowPlan* p) {
                        (gate != Gate::All || rows_match(size, a.C, a.pitch_gate, aligned));
     const bool shift = rows_shift(size, a.C) || !on16(a.p.scale) || !on16(a.p.post_weight) || !on16(a.p.post_bias) || !on16(a.p.weight) ||
                        !on16(a.p.bias);
-    return match && plan_elements(a.C, size, shift, true, p);
+    return match && plan_elements(a.C, size, shift, false, p);
 }
-bool plan_backward(Gate gate, const SandwichGradArgs& a, int type, const DeviceCtx* ctx, RowShape* s) {
+bool plan_backward(Gate gate, const SandwichGradArgs& a, int type, RowPlan* p) {
     const int size = size_of(type);
     const bool aligned = on16(a.x) && on16(a.h) && on16(a.grad_y) && on16(a.grad_h) && on16(a.grad_x) && on16(a.grad_residual) &&
                          (gate != Gate::All || (on16(a.gate) && on16(a.grad_gate)));
     const bool match = rows_match(size, a.C, a.pitch, aligned) && (gate != Gate::All || rows_match(size, a.C, a.pitch_gate, aligned));
     const bool shift = rows_shift(size, a.C) || !on16(a.p.scale) || !on16(a.p.post_weight) || !on16(a.p.post_bias) || !on16(a.p.weight);
+    // (the column sums of 32 elements do not fit the registers)
+    return match && plan_elements(a.C, size, shift, false, p) && p->items * (16 / size) <= 16;
+}
+// The backward kernel for these rows, with its shape: f(kernel, shape); kBadArgument where there is none
+template <class F>
+int with_backward(Gate gate, const SandwichGradArgs& a, int type, const DeviceCtx* ctx, F f) {
     RowPlan p;
-    if (!match || !plan_elements(a.C, size, shift, true, &p)) return false;
-    const int elements = p.items * (16 / size), R = rows_at_once(elements, p.group), streams = gate == Gate::All ? 5 : 4;
-    if (elements > 16) return false;  // (the column sums of 32 elements do not fit the registers)
-    int per_sm = 65536 / (p.threads * (p.group ? 168 : 102));
-    if (per_sm < 1) per_sm = 1;
-    *s = shape_of(p, a.rows, R, streams, per_sm, ctx);
-    if (s->depth < 1) return false;
-    const size_t columns = p.group ? static_cast<size_t>(kGroupThreads / 32) * 4 * a.C * sizeof(float) : 0;
-    if (s->smem < columns) s->smem = columns;
-    return true;
+    if (!plan_backward(gate, a, type, &p)) return kBadArgument;
+    return with_type(type, [&](auto t) {
+        using T = decltype(t);
+        return with_gate(gate, [&](auto g) {
+            return with_items<T>(p, [&](auto items, auto group, auto shift) {
+                constexpr Gate G = decltype(g)::value;
+                constexpr int kItems = decltype(items)::value;
+                constexpr bool kGroup = decltype(group)::value;
+                if constexpr (kItems * kPiece<T> > 16) {
+                    return static_cast<int>(kBadArgument);
+                } else {
+                    constexpr auto kernel = sandwich_grad_registers_kernel<T, G, kItems, kGroup, decltype(shift)::value>;
+                    int per_sm;
+                    const int r = resident_blocks<kernel>(p.threads, ctx, &per_sm);
+                    if (r != kOk) return r;
+                    RowShape s;
+                    const long long params = kGroup ? 0 : 3LL * kItems * (kPiece<T> / 4) * p.threads * 16;
+                    if (!shape_of(p, a.rows, 1, kBackwardStreams<G>, params, per_sm, ctx, &s)) return static_cast<int>(kBadArgument);
+                    if constexpr (kGroup) {
+                        const size_t columns = static_cast<size_t>(kGroupThreads / 32) * 4 * a.C * sizeof(float);
+                        if (s.smem < columns) s.smem = columns;
+                    }
+                    return f(kernel, s);
+                }
+            });
+        });
+    });
 }
 
 }  // namespace
@@ -536,64 +620,38 @@ bool plan_backward(Gate gate, const SandwichGradArgs& a, int type, const DeviceC
 bool sandwich_in_registers(Gate gate, const SandwichArgs& a, int type, const DeviceCtx* ctx, cudaStream_t st, int* status) {
     RowPlan p;
     if (!plan_forward(gate, a, type, &p)) return false;
-    const int streams = gate == Gate::All ? 3 : 2, elements = p.items * (16 / size_of(type));
-    if (static_cast<long long>(streams) * p.items * p.threads * 16 > ctx->max_smem_optin - 4096) return false;
-    *status = with_type(type, [&](auto t) {
+    bool fits = true;
+    const int r = with_type(type, [&](auto t) {
         using T = decltype(t);
         return with_gate(gate, [&](auto g) {
             return with_items<T>(p, [&](auto items, auto group, auto shift) {
-                constexpr auto kernel = sandwich_registers_kernel<T, decltype(g)::value, decltype(items)::value, decltype(group)::value, decltype(shift)::value>;
-                static OncePerDevice once;
-                const int r = once([&] { return allow_smem(kernel, ctx->max_smem_optin - 2560); });
+                constexpr Gate G = decltype(g)::value;
+                constexpr int kItems = decltype(items)::value;
+                constexpr bool kGroup = decltype(group)::value;
+                constexpr auto kernel = sandwich_registers_kernel<T, G, kItems, kGroup, decltype(shift)::value>;
+                int per_sm;
+                const int r = resident_blocks<kernel>(p.threads, ctx, &per_sm);
                 if (r != kOk) return r;
-                static std::atomic<int> resident[64][33];
-                std::atomic<int>& known = resident[ctx->device][p.threads / 32];
-                int per_sm = known.load(std::memory_order_acquire);
-                if (per_sm == 0) {
-                    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, p.threads, 0) != cudaSuccess || per_sm < 1) {
-                        cudaGetLastError();
-                        per_sm = 1;
-                    }
-                    known.store(per_sm, std::memory_order_release);
-                }
-                RowShape s = shape_of(p, a.rows, rows_at_once(elements, p.group), streams, per_sm, ctx);
-                if (s.depth < 1) {  // (a row of 16384 in 32 bits, its residual and its gate: 192 KB)
-                    s.depth = 1;
-                    s.smem = static_cast<size_t>(streams) * p.items * p.threads * 16;
-                }
-                return launch_after(kernel, s.blocks, p.threads, s.smem, st, a, p.lanes, s.depth);
+                RowShape s;
+                fits = shape_of(p, a.rows, rows_forward(kItems * kPiece<T>, kGroup), kForwardStreams<G>, 0, per_sm, ctx, &s);
+                return fits ? launch_after(kernel, s.blocks, p.threads, s.smem, st, a, p.lanes, s.depth) : static_cast<int>(kOk);
             });
         });
     });
-    return true;
+    if (fits) *status = r;
+    return fits;
 }
 
 bool sandwich_grad_in_registers(Gate gate, const SandwichGradArgs& a, int type, const DeviceCtx* ctx, int* blocks) {
-    RowShape s;
-    if (!plan_backward(gate, a, type, ctx, &s)) return false;
-    *blocks = s.blocks;
-    return true;
+    return with_backward(gate, a, type, ctx, [&](auto, const RowShape& s) {
+        *blocks = s.blocks;
+        return static_cast<int>(kOk);
+    }) == kOk;
 }
 
 int launch_sandwich_grad_in_registers(Gate gate, const SandwichGradArgs& a, int type, const DeviceCtx* ctx, cudaStream_t st) {
-    RowShape s;
-    if (!plan_backward(gate, a, type, ctx, &s)) return kBadArgument;
-    return with_type(type, [&](auto t) {
-        using T = decltype(t);
-        return with_gate(gate, [&](auto g) {
-            return with_items<T>(s.p, [&](auto items, auto group, auto shift) {
-                if constexpr (decltype(items)::value * kPiece<T> > 16) {
-                    return static_cast<int>(kBadArgument);
-                } else {
-                    constexpr auto kernel =
-                        sandwich_grad_registers_kernel<T, decltype(g)::value, decltype(items)::value, decltype(group)::value, decltype(shift)::value>;
-                    static OncePerDevice once;
-                    const int r = once([&] { return allow_smem(kernel, ctx->max_smem_optin - 2560); });
-                    if (r != kOk) return r;
-                    return launch_after(kernel, s.blocks, s.p.threads, s.smem, st, a, s.p.lanes, s.depth);
-                }
-            });
-        });
+    return with_backward(gate, a, type, ctx, [&](auto kernel, const RowShape& s) {
+        return launch_after(kernel, s.blocks, s.p.threads, s.smem, st, a, s.p.lanes, s.depth);
     });
 }
 
