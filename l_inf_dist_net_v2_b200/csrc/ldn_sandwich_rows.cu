@@ -33,15 +33,110 @@ __device__ __forceinline__ void load_scaled(const SandwichParams& p, int c0, int
     }
 }
 
+// Numbers of the rows that a block takes next (statistics, a gate per row), in shared memory, some hundred rows at a time: fetched a turn ahead
+// into registers, they were what the warps waited for (16384 x 5120 bf16 backward: 351 us with them, 277 without any).
+constexpr int kNumberRows = 256;
+template <int N>
+struct RowNumbers {
+    float (*slots)[kNumberRows];
+    int per_turn, turns;  // rows of a turn, turns of a batch
+    __device__ __forceinline__ RowNumbers(float (*s)[kNumberRows], int rows_of_turn) : slots(s), per_turn(rows_of_turn), turns(kNumberRows / rows_of_turn) {}
+    // load(k, row): number k of a row; row_of(i): the i-th row from this turn on, or rows and more where there is none
+    template <class RowOf, class Load>
+    __device__ __forceinline__ void at_turn(int turn, long long rows, RowOf row_of, Load load) {
+        if (turn % turns) return;
+        __syncthreads();
+        for (int i = threadIdx.x; i < N * kNumberRows; i += blockDim.x) {
+            const int k = i / kNumberRows, at = i % kNumberRows;
+            const long long row = at < turns * per_turn ? row_of(at) : rows;
+            slots[k][at] = row < rows ? load(k, row) : 0.0f;
+        }
+        __syncthreads();
+    }
+    // index: of a row in its turn
+    __device__ __forceinline__ float of(int k, int turn, int index) const { return slots[k][turn % turns * per_turn + index]; }
+};
+
+// Sums over a block of rows held together, as RowSum has them, with the warps' sums read by all of a block's threads as whole pieces and
+// added up by each (half the way of a second round of shuffles: the sums are what a block's warps wait for).  Sums over a
+// group's lanes are RowSum's.
+template <bool GROUP>
+struct SumOf {
+    int lanes;
+    float* slots;  // [2][kSlots], zeros at first
+    int turn;
+    static constexpr int kSlots = 20 * 8;  // (warps of a block) x K, a multiple of four numbers
+    __device__ __forceinline__ void begin() {
+        if constexpr (!GROUP)
+            for (int i = threadIdx.x; i < 2 * kSlots; i += blockDim.x) slots[i] = 0.0f;
+        __syncthreads();
+    }
+    template <int K, class End>
+    __device__ __forceinline__ void operator()(float (&v)[K], End end) {
+        if constexpr (GROUP) {
+            RowSum{lanes, nullptr, 0}.over_group(v, [](float a, float b) { return a + b; }, end);
+        } else {
+            const int lane = threadIdx.x & 31;
+            constexpr int kShare = 32 / K;  // lanes that end with the same number
+            int half = 16;
+#pragma unroll
+            for (int n = K; n > 1; n /= 2, half /= 2) {
+                const bool upper = lane & half;
+#pragma unroll
+                for (int i = 0; i < n / 2; ++i) {
+                    const float send = upper ? v[i] : v[i + n / 2], keep = upper ? v[i + n / 2] : v[i];
+                    v[i] = keep + __shfl_xor_sync(0xffffffffu, send, half);
+                }
+            }
+#pragma unroll
+            for (int d = kShare / 2; d > 0; d /= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], d);
+            float* s = slots + turn * kSlots;
+            turn ^= 1;
+            if (lane % kShare == 0) s[(threadIdx.x >> 5) * K + lane / kShare] = v[0];
+            __syncthreads();
+            const int pieces = (static_cast<int>(blockDim.x >> 5) * K + 3) / 4;
+            const float4* from = reinterpret_cast<const float4*>(s);
+            if constexpr (K == 8) {
+                float4 a = from[0], b = from[1];
+                for (int i = 2; i < pieces; i += 2) {
+                    const float4 c = from[i], d = from[i + 1];
+                    a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
+                    b.x += d.x; b.y += d.y; b.z += d.z; b.w += d.w;
+                }
+                v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+                v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+            } else {
+                float4 a = from[0];
+#pragma unroll 5
+                for (int i = 1; i < pieces; ++i) {
+                    const float4 c = from[i];
+                    a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
+                }
+                if constexpr (K == 4) {
+                    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+                } else if constexpr (K == 2) {
+                    v[0] = a.x + a.z;
+                    v[1] = a.y + a.w;
+                } else {
+                    v[0] = (a.x + a.y) + (a.z + a.w);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < K; ++i) v[i] = end(v[i]);
+        }
+    }
+};
+
 template <class T, Gate G, int ITEMS, bool GROUP, bool SHIFT>
 __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPiece<T>), 1)
 sandwich_registers_kernel(const __grid_constant__ SandwichArgs a, int lanes, int depth) {
     stream_order_begin();
     constexpr int V = kPiece<T>, S = kForwardStreams<G>, R = rows_forward(ITEMS * V, GROUP);
     constexpr bool kKeep = ITEMS * V <= 16;
-    __shared__ float slots[2 * RowSum::kSlots];
+    __shared__ alignas(16) float slots[2 * SumOf<GROUP>::kSlots];
     extern __shared__ uint4 ring[];  // [depth][row][stream][item][thread]
-    RowSum reduce{lanes, slots, 0};
+    SumOf<GROUP> reduce{lanes, slots, 0};
+    reduce.begin();
     const int lane = GROUP ? threadIdx.x & (lanes - 1) : threadIdx.x;
     const int per_block = GROUP ? kGroupThreads / lanes : 1;
     const long long step = static_cast<long long>(gridDim.x) * per_block;
@@ -94,33 +189,34 @@ sandwich_registers_kernel(const __grid_constant__ SandwichArgs a, int lanes, int
         for (int i = 0; i < ITEMS; ++i)
             if (!bytes[i]) own[(d * ITEMS + i) * blockDim.x] = make_uint4(0u, 0u, 0u, 0u);
     for (int d = 0; d < depth; ++d) fetch(d);
-    // a row's gate comes a turn ahead
-    float next_gate[R];
-    auto fetch_gates = [&](long long row, int rows) {
-#pragma unroll
-        for (int j = 0; j < R; ++j) next_gate[j] = G == Gate::Row && j < rows ? to_float(static_cast<const T*>(a.gate)[row + j * step]) : 1.0f;
-    };
-    fetch_gates(row0, to_make);
+    __shared__ float numbers[1][G == Gate::Row ? kNumberRows : 1];
     int stage = 0;
     // (a warp's groups take part in its shuffles whether they have a row or not: as many turns as the block's first has)
     const long long block_first = static_cast<long long>(blockIdx.x) * per_block;
     const int turns = block_first < a.rows ? static_cast<int>((a.rows - block_first + R * step - 1) / (R * step)) : 0;
+    auto row_of = [&](int turn, int i) { return block_first + (static_cast<long long>(turn) * R + i / per_block) * step + i % per_block; };
     for (int turn = 0; turn < turns; ++turn) {
         auto live = [&](int j) { return j < to_make; };
+        float gate[R];
+        if constexpr (G == Gate::Row) {
+            RowNumbers<1> gates(numbers, R * per_block);
+            gates.at_turn(turn, a.rows, [&](int i) { return row_of(turn, i); },
+                          [&](int, long long row) { return to_float(static_cast<const T*>(a.gate)[row]); });
+#pragma unroll
+            for (int j = 0; j < R; ++j) gate[j] = gates.of(0, turn, j * per_block + (GROUP ? threadIdx.x / lanes : 0));
+        }
         copies_wait(depth);
         float2 v[R][ITEMS][V / 2];
-        float s[R], gate[R], mean[R];
+        float s[R], mean[R];
         auto piece_of = [&](int j, int stream, int i) { return live(j) ? *slot_of(stage, j, stream, i) : make_uint4(0u, 0u, 0u, 0u); };
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            gate[j] = next_gate[j];
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
                 const uint4 raw = piece_of(j, 0, i);
                 unpack<T>(SHIFT ? masked(raw, mask[i]) : raw, v[j][i]);
             }
         }
-        fetch_gates(row0 + R * step, to_make - R);
         // mean and deviation of what the registers hold: v becomes v - mean, s 1 / deviation
         auto statistics = [&](float* to) {
 #pragma unroll
@@ -132,7 +228,7 @@ sandwich_registers_kernel(const __grid_constant__ SandwichArgs a, int lanes, int
                     for (int e = 0; e < V / 2; ++e) sum = __fadd2_rn(sum, v[j][i][e]);
                 s[j] = sum.x + sum.y;
             }
-            reduce.template sum<GROUP>(s, [&](float all) { return all * inv_C; });
+            reduce(s, [&](float all) { return all * inv_C; });
 #pragma unroll
             for (int j = 0; j < R; ++j) {
                 mean[j] = s[j];
@@ -147,7 +243,7 @@ sandwich_registers_kernel(const __grid_constant__ SandwichArgs a, int lanes, int
                 }
                 s[j] = sum.x + sum.y;
             }
-            reduce.template sum<GROUP>(s, [&](float all) { return 1.0f / sqrtf(all * inv_C + a.eps); });
+            reduce(s, [&](float all) { return 1.0f / sqrtf(all * inv_C + a.eps); });
             if (lane == 0 && a.stats)
 #pragma unroll
                 for (int j = 0; j < R; ++j)
@@ -212,9 +308,10 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
     stream_order_begin();
     constexpr int V = kPiece<T>, S = kBackwardStreams<G>, R = 1;
     constexpr int K = G == Gate::Row ? 4 : 2;  // sums of a row in the second round (a power of two)
-    __shared__ float slots[2 * RowSum::kSlots];
+    __shared__ alignas(16) float slots[2 * SumOf<GROUP>::kSlots];
     extern __shared__ uint4 ring[];  // [depth][row][stream][item][thread], then blocks: [3][item][V / 4][thread]; at the end, groups: [warp][4][C] floats
-    RowSum reduce{lanes, slots, 0};
+    SumOf<GROUP> reduce{lanes, slots, 0};
+    reduce.begin();
     const int lane = GROUP ? threadIdx.x & (lanes - 1) : threadIdx.x;
     const int per_block = GROUP ? kGroupThreads / lanes : 1;
     const long long step = static_cast<long long>(gridDim.x) * per_block;
@@ -305,34 +402,29 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
         for (int i = 0; i < ITEMS; ++i)
             if (!bytes[i] || (!a.grad_y && d % S == 2) || (!a.grad_h && d % S == 3)) own[(d * ITEMS + i) * blockDim.x] = make_uint4(0u, 0u, 0u, 0u);
     for (int d = 0; d < depth; ++d) fetch(d);
-    // a row's statistics and gate come a turn ahead
     constexpr int kNumbers = G == Gate::Row ? 5 : 4;
-    float next[R][kNumbers];
-    auto fetch_numbers = [&](long long row, int rows) {
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) next[j][k] = j < rows ? a.stats[k * a.rows + row + j * step] : 0.0f;
-            if constexpr (G == Gate::Row) next[j][4] = j < rows ? to_float(static_cast<const T*>(a.gate)[row + j * step]) : 0.0f;
-        }
-    };
-    fetch_numbers(row0, to_make);
+    __shared__ float numbers[kNumbers][kNumberRows];
     int stage = 0;
     const long long block_first = static_cast<long long>(blockIdx.x) * per_block;
     const int turns = block_first < a.rows ? static_cast<int>((a.rows - block_first + R * step - 1) / (R * step)) : 0;
+    auto row_of = [&](int turn, int i) { return block_first + (static_cast<long long>(turn) * R + i / per_block) * step + i % per_block; };
     for (int turn = 0; turn < turns; ++turn) {
         auto live = [&](int j) { return j < to_make; };
         float mean1[R], rstd1[R], mean2[R], rstd2[R], gate[R], s[2 * R], t[K * R];
+        RowNumbers<kNumbers> of_rows(numbers, R * per_block);
+        of_rows.at_turn(turn, a.rows, [&](int i) { return row_of(turn, i); }, [&](int k, long long row) {
+            return k < 4 ? a.stats[k * a.rows + row] : to_float(static_cast<const T*>(a.gate)[row]);
+        });
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            mean1[j] = next[j][0];
-            rstd1[j] = next[j][1];
-            mean2[j] = next[j][2];
-            rstd2[j] = next[j][3];
-            gate[j] = G == Gate::Row ? next[j][kNumbers - 1] : 1.0f;
+            const int index = j * per_block + (GROUP ? threadIdx.x / lanes : 0);
+            mean1[j] = of_rows.of(0, turn, index);
+            rstd1[j] = of_rows.of(1, turn, index);
+            mean2[j] = of_rows.of(2, turn, index);
+            rstd2[j] = of_rows.of(3, turn, index);
+            gate[j] = G == Gate::Row ? of_rows.of(kNumbers - 1, turn, index) : 1.0f;
         }
         copies_wait(depth);
-        fetch_numbers(row0 + R * step, to_make - R);
         // (outside the row all is 0)
         auto piece_of = [&](int j, int stream, int i, float2 (&v)[V / 2]) {
             const uint4 raw = live(j) ? *slot_of(stage, j, stream, i) : make_uint4(0u, 0u, 0u, 0u);
@@ -360,7 +452,7 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
             s[2 * j] = s0.x + s0.y;
             s[2 * j + 1] = s1.x + s1.y;
         }
-        reduce.template sum<GROUP>(s, [&](float all) { return all * inv_C; });
+        reduce(s, [&](float all) { return all * inv_C; });
         float2 by[R][ITEMS][V / 2];  // what goes into the first norm's gradient
 #pragma unroll
         for (int j = 0; j < R; ++j) {
@@ -425,7 +517,7 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
                 t[K * j + 3] = 0.0f;
             }
         }
-        reduce.template sum<GROUP>(t, [&](float all) { return all; });
+        reduce(t, [&](float all) { return all; });
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             if (!live(j)) continue;
@@ -510,12 +602,18 @@ struct RowShape {
     int blocks, depth;
     size_t smem;
 };
+// (sums' slots and rows' numbers)
+constexpr int kStaticBytes = (2 * SumOf<false>::kSlots + 5 * kNumberRows) * sizeof(float) + 256;
 // extra: bytes of a block beside its rows
 bool shape_of(const RowPlan& p, long long rows, int R, int streams, long long extra, int per_sm, const DeviceCtx* ctx, RowShape* s) {
-    const long long row_bytes = static_cast<long long>(R) * streams * p.items * p.threads * 16, most_smem = ctx->max_smem_optin - 4096;
+    const long long row_bytes = static_cast<long long>(R) * streams * p.items * p.threads * 16;
+    auto room = [&] { return ctx->max_smem_optin / per_sm - 1024 - kStaticBytes - extra; };
     s->p = p;
-    s->depth = ring_depth(row_bytes, most_smem / per_sm - 1024 - extra);
-    while (s->depth < 2 && per_sm > 1) s->depth = ring_depth(row_bytes, most_smem / --per_sm - 1024 - extra);
+    s->depth = ring_depth(row_bytes, room());
+    while (s->depth < 2 && per_sm > 1) {
+        --per_sm;
+        s->depth = ring_depth(row_bytes, room());
+    }
     if (s->depth < 1) return false;
     const long long needed = (rows + p.rows_per_block() - 1) / p.rows_per_block();
     long long blocks = static_cast<long long>(per_sm) * ctx->sm_count;
@@ -549,7 +647,7 @@ int with_gate(Gate gate, F f) {
 template <auto KERNEL>
 int resident_blocks(int threads, const DeviceCtx* ctx, int* per_sm) {
     static OncePerDevice once;
-    const int r = once([&] { return allow_smem(KERNEL, ctx->max_smem_optin - 2560); });
+    const int r = once([&] { return allow_smem(KERNEL, ctx->max_smem_optin - kStaticBytes); });
     if (r != kOk) return r;
     static std::atomic<int> resident[64][33];
     std::atomic<int>& known = resident[ctx->device][threads / 32];
