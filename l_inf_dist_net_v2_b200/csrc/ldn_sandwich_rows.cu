@@ -16,8 +16,11 @@ template <Gate G>
 constexpr int kForwardStreams = G == Gate::All ? 3 : 2;
 template <Gate G>
 constexpr int kBackwardStreams = G == Gate::All ? 5 : 4;
-// Rows that a block takes at a time
-__host__ __device__ constexpr int rows_forward(int elements, bool group) { return group || elements > 16 ? 1 : 2; }
+// Rows that a block, or each of its groups, takes at a time forward; backward one (524288 x 96 bf16 with a gate per row, 1 / 2 / 4 rows of a
+// group: 172 / 145 / 131 us, backward 236 / 306; 1000000 x 17, cut rows: 107 / 111 / 141; 200000 x 40 f32: 45 / 43 / 49)
+__host__ __device__ constexpr int rows_forward(int elements, int size, bool group, bool shift) {
+    return group ? (elements <= 8 && size == 2 && !shift ? 4 : 2) : elements > 16 ? 1 : 2;
+}
 
 // scale weight and scale bias of a piece's columns (1 and 0 outside the row)
 template <class T, bool SHIFT>
@@ -35,19 +38,19 @@ __device__ __forceinline__ void load_scaled(const SandwichParams& p, int c0, int
 
 // Numbers of the rows that a block takes next (statistics, a gate per row), in shared memory, some hundred rows at a time: fetched a turn ahead
 // into registers, they were what the warps waited for (16384 x 5120 bf16 backward: 351 us with them, 277 without any).
-constexpr int kNumberRows = 256;
-template <int N>
+constexpr int kNumberRows = 256;  // (times the rows that a group takes at a time: a turn's rows are there at least)
+template <int N, int ROWS>
 struct RowNumbers {
-    float (*slots)[kNumberRows];
+    float (*slots)[ROWS];
     int per_turn, turns;  // rows of a turn, turns of a batch
-    __device__ __forceinline__ RowNumbers(float (*s)[kNumberRows], int rows_of_turn) : slots(s), per_turn(rows_of_turn), turns(kNumberRows / rows_of_turn) {}
+    __device__ __forceinline__ RowNumbers(float (*s)[ROWS], int rows_of_turn) : slots(s), per_turn(rows_of_turn), turns(ROWS / rows_of_turn) {}
     // load(k, row): number k of a row; row_of(i): the i-th row from this turn on, or rows and more where there is none
     template <class RowOf, class Load>
     __device__ __forceinline__ void at_turn(int turn, long long rows, RowOf row_of, Load load) {
         if (turn % turns) return;
         __syncthreads();
-        for (int i = threadIdx.x; i < N * kNumberRows; i += blockDim.x) {
-            const int k = i / kNumberRows, at = i % kNumberRows;
+        for (int i = threadIdx.x; i < N * ROWS; i += blockDim.x) {
+            const int k = i / ROWS, at = i % ROWS;
             const long long row = at < turns * per_turn ? row_of(at) : rows;
             slots[k][at] = row < rows ? load(k, row) : 0.0f;
         }
@@ -131,7 +134,7 @@ template <class T, Gate G, int ITEMS, bool GROUP, bool SHIFT>
 __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPiece<T>), 1)
 sandwich_registers_kernel(const __grid_constant__ SandwichArgs a, int lanes, int depth) {
     stream_order_begin();
-    constexpr int V = kPiece<T>, S = kForwardStreams<G>, R = rows_forward(ITEMS * V, GROUP);
+    constexpr int V = kPiece<T>, S = kForwardStreams<G>, R = rows_forward(ITEMS * V, sizeof(T), GROUP, SHIFT);
     constexpr bool kKeep = ITEMS * V <= 16;
     __shared__ alignas(16) float slots[2 * SumOf<GROUP>::kSlots];
     extern __shared__ uint4 ring[];  // [depth][row][stream][item][thread]
@@ -189,7 +192,7 @@ sandwich_registers_kernel(const __grid_constant__ SandwichArgs a, int lanes, int
         for (int i = 0; i < ITEMS; ++i)
             if (!bytes[i]) own[(d * ITEMS + i) * blockDim.x] = make_uint4(0u, 0u, 0u, 0u);
     for (int d = 0; d < depth; ++d) fetch(d);
-    __shared__ float numbers[1][G == Gate::Row ? kNumberRows : 1];
+    __shared__ float numbers[1][G == Gate::Row ? R * kNumberRows : 1];
     int stage = 0;
     // (a warp's groups take part in its shuffles whether they have a row or not: as many turns as the block's first has)
     const long long block_first = static_cast<long long>(blockIdx.x) * per_block;
@@ -199,7 +202,7 @@ sandwich_registers_kernel(const __grid_constant__ SandwichArgs a, int lanes, int
         auto live = [&](int j) { return j < to_make; };
         float gate[R];
         if constexpr (G == Gate::Row) {
-            RowNumbers<1> gates(numbers, R * per_block);
+            RowNumbers<1, R * kNumberRows> gates(numbers, R * per_block);
             gates.at_turn(turn, a.rows, [&](int i) { return row_of(turn, i); },
                           [&](int, long long row) { return to_float(static_cast<const T*>(a.gate)[row]); });
 #pragma unroll
@@ -307,6 +310,7 @@ __global__ void __launch_bounds__(GROUP ? kGroupThreads : threads_of(ITEMS * kPi
 sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int lanes, int depth) {
     stream_order_begin();
     constexpr int V = kPiece<T>, S = kBackwardStreams<G>, R = 1;
+    constexpr bool kSums = ITEMS * V <= 16;  // (rows of 32 elements per thread leave their column sums to a kernel of its own)
     constexpr int K = G == Gate::Row ? 4 : 2;  // sums of a row in the second round (a power of two)
     __shared__ alignas(16) float slots[2 * SumOf<GROUP>::kSlots];
     extern __shared__ uint4 ring[];  // [depth][row][stream][item][thread], then blocks: [3][item][V / 4][thread]; at the end, groups: [warp][4][C] floats
@@ -321,7 +325,7 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
     auto column = [&](int i) { return (lane + i * lanes) * V - shift; };
     // a group's columns' parameters stay in registers, a block's in shared memory, where each thread puts and finds its own (as registers, the
     // kernel spilled: 16384 x 5120 bf16 415 us)
-    float2 kept[GROUP ? 3 : 1][ITEMS][V / 2];
+    float2 kept[GROUP ? 3 : 1][GROUP ? ITEMS : 1][V / 2];
     uint4* params = ring + static_cast<size_t>(depth) * R * S * ITEMS * blockDim.x + threadIdx.x;
     auto set_param_piece = [&](int k, int i, const float2 (&v)[V / 2]) {
 #pragma unroll
@@ -335,36 +339,46 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
             }
         }
     };
-    auto param_piece = [&](int k, int i, float2 (&v)[V / 2]) {
+    auto param_piece = [&](int k, int i, int first, float2 (&v)[V / 2]) {
+        if constexpr (!kSums) {
+            float2 other[V / 2];
+            if (k == 2) load_params<T, SHIFT>(a.p.weight, a.p.wide, first, a.C, 1.0f, v);
+            else if (k == 1) load_scaled<T, SHIFT>(a.p, first, a.C, other, v);
+            else load_scaled<T, SHIFT>(a.p, first, a.C, v, other);
+        } else {
 #pragma unroll
-        for (int e = 0; e < V / 2; e += 2) {
-            if constexpr (GROUP) {
-                v[e] = kept[k][i][e];
-                v[e + 1] = kept[k][i][e + 1];
-            } else {
-                const uint4 raw = params[((k * ITEMS + i) * (V / 4) + e / 2) * blockDim.x];
-                v[e] = make_float2(__uint_as_float(raw.x), __uint_as_float(raw.y));
-                v[e + 1] = make_float2(__uint_as_float(raw.z), __uint_as_float(raw.w));
+            for (int e = 0; e < V / 2; e += 2) {
+                if constexpr (GROUP) {
+                    v[e] = kept[k][i][e];
+                    v[e + 1] = kept[k][i][e + 1];
+                } else {
+                    const uint4 raw = params[((k * ITEMS + i) * (V / 4) + e / 2) * blockDim.x];
+                    v[e] = make_float2(__uint_as_float(raw.x), __uint_as_float(raw.y));
+                    v[e + 1] = make_float2(__uint_as_float(raw.z), __uint_as_float(raw.w));
+                }
             }
         }
     };
-    float2 sums[4][ITEMS][V / 2];  // dy z2, dy, d gate z1, d gate
+    float2 sums[4][kSums ? ITEMS : 1][V / 2];  // dy z2, dy, d gate z1, d gate
     uint4 mask[ITEMS];
     int bytes[ITEMS];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
+        if constexpr (kSums)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int e = 0; e < V / 2; ++e) sums[k][i][e] = both(0.0f);
+                for (int e = 0; e < V / 2; ++e) sums[k][i][e] = both(0.0f);
         mask[i] = mask_of<T, SHIFT>(column(i), a.C);
         bytes[i] = piece_bytes<T>(column(i), a.C);
-        float2 w[V / 2], b[V / 2];
-        load_scaled<T, SHIFT>(a.p, column(i), a.C, w, b);
-        set_param_piece(0, i, w);
-        set_param_piece(1, i, b);
-        load_params<T, SHIFT>(a.p.weight, a.p.wide, column(i), a.C, 1.0f, w);
-        set_param_piece(2, i, w);
+        if constexpr (kSums) {
+            float2 w[V / 2], b[V / 2];
+            load_scaled<T, SHIFT>(a.p, column(i), a.C, w, b);
+            set_param_piece(0, i, w);
+            set_param_piece(1, i, b);
+            load_params<T, SHIFT>(a.p.weight, a.p.wide, column(i), a.C, 1.0f, w);
+            set_param_piece(2, i, w);
+        }
     }
     const int c0 = column(0), apart = lanes * V;
     int to_fetch = mine < a.rows ? static_cast<int>((a.rows - mine + step - 1) / step) : 0, to_make = to_fetch;
@@ -411,7 +425,7 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
     for (int turn = 0; turn < turns; ++turn) {
         auto live = [&](int j) { return j < to_make; };
         float mean1[R], rstd1[R], mean2[R], rstd2[R], gate[R], s[2 * R], t[K * R];
-        RowNumbers<kNumbers> of_rows(numbers, R * per_block);
+        RowNumbers<kNumbers, R * kNumberRows> of_rows(numbers, R * per_block);
         of_rows.at_turn(turn, a.rows, [&](int i) { return row_of(turn, i); }, [&](int k, long long row) {
             return k < 4 ? a.stats[k * a.rows + row] : to_float(static_cast<const T*>(a.gate)[row]);
         });
@@ -438,13 +452,15 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
                 float2 h[V / 2], dy[V / 2], w2[V / 2];
                 piece_of(j, 1, i, h);
                 piece_of(j, 2, i, dy);
-                param_piece(2, i, w2);
+                param_piece(2, i, column(i), w2);
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e) {
                     // (rstd behind the sum: outside the row the gradient is 0 and h - mean a number, but (0 - mean) rstd may be infinite)
                     const float2 u = __fmul2_rn(dy[e], __fadd2_rn(h[e], both(-mean2[j])));
-                    sums[0][i][e] = __ffma2_rn(u, both(rstd2[j]), sums[0][i][e]);
-                    sums[1][i][e] = __fadd2_rn(sums[1][i][e], dy[e]);
+                    if constexpr (kSums) {
+                        sums[0][i][e] = __ffma2_rn(u, both(rstd2[j]), sums[0][i][e]);
+                        sums[1][i][e] = __fadd2_rn(sums[1][i][e], dy[e]);
+                    }
                     s0 = __ffma2_rn(dy[e], w2[e], s0);
                     s1 = __ffma2_rn(u, w2[e], s1);
                 }
@@ -458,19 +474,24 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
         for (int j = 0; j < R; ++j) {
             float2 t0 = both(0.0f), t1 = both(0.0f), tg = both(0.0f);
             const float m1 = s[2 * j], m2 = s[2 * j + 1] * rstd2[j] * rstd2[j];
+            if constexpr (!kSums)
+                if (threadIdx.x == 0 && live(j) && a.row_sums) {
+                    a.row_sums[row0 + j * step] = m1;
+                    a.row_sums[a.rows + row0 + j * step] = s[2 * j + 1] * rstd2[j];
+                }
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
                 const int c = column(i);
                 float2 d[V / 2], h[V / 2], x[V / 2], n[V / 2], w[V / 2];
                 piece_of(j, 1, i, h);
                 piece_of(j, 2, i, d);
-                param_piece(2, i, w);
+                param_piece(2, i, c, w);
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e)
                     d[e] = __ffma2_rn(__fadd2_rn(h[e], both(-mean2[j])), both(-m2), __ffma2_rn(d[e], w[e], both(-m1)));
                 piece_of(j, 3, i, h);
                 piece_of(j, 0, i, x);
-                param_piece(0, i, w);
+                param_piece(0, i, c, w);
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e) {
                     d[e] = __ffma2_rn(d[e], both(rstd2[j]), h[e]);
@@ -478,7 +499,7 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
                 }
                 if (live(j) && a.grad_residual) store_piece<T, SHIFT>(to_onto.of(j, i * apart), c, a.C, pack<T>(d));
                 if constexpr (G != Gate::None) {
-                    param_piece(1, i, n);
+                    param_piece(1, i, c, n);
 #pragma unroll
                     for (int e = 0; e < V / 2; ++e) n[e] = __fmul2_rn(d[e], __ffma2_rn(__fmul2_rn(x[e], both(rstd1[j])), w[e], n[e]));
                 }
@@ -503,8 +524,10 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e) {
                     const float2 u = __fmul2_rn(d[e], x[e]);
-                    sums[2][i][e] = __ffma2_rn(u, both(rstd1[j]), sums[2][i][e]);
-                    sums[3][i][e] = __fadd2_rn(sums[3][i][e], d[e]);
+                    if constexpr (kSums) {
+                        sums[2][i][e] = __ffma2_rn(u, both(rstd1[j]), sums[2][i][e]);
+                        sums[3][i][e] = __fadd2_rn(sums[3][i][e], d[e]);
+                    }
                     by[j][i][e] = __fmul2_rn(d[e], w[e]);
                     t0 = __fadd2_rn(t0, by[j][i][e]);
                     t1 = __ffma2_rn(u, w[e], t1);
@@ -545,6 +568,7 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
         to_onto.on(R);
         to_gate.on(R);
     }
+    if constexpr (!kSums) return;
     if (!a.parts) return;
     float* part = a.parts + static_cast<long long>(blockIdx.x) * 4 * a.C;
     if constexpr (!GROUP) {
@@ -558,11 +582,11 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
 #pragma unroll
                     for (int e = 0; e < V / 2; e += 2)
                         *reinterpret_cast<float4*>(part + k * a.C + c + 2 * e) =
-                            make_float4(sums[k][i][e].x, sums[k][i][e].y, sums[k][i][e + 1].x, sums[k][i][e + 1].y);
+                            make_float4(sums[k][kSums ? i : 0][e].x, sums[k][kSums ? i : 0][e].y, sums[k][kSums ? i : 0][e + 1].x, sums[k][kSums ? i : 0][e + 1].y);
                 } else {
 #pragma unroll
                     for (int e = 0; e < V; ++e)
-                        if (static_cast<unsigned>(c + e) < static_cast<unsigned>(a.C)) part[k * a.C + c + e] = at_of(sums[k][i], e);
+                        if (static_cast<unsigned>(c + e) < static_cast<unsigned>(a.C)) part[k * a.C + c + e] = at_of(sums[k][kSums ? i : 0], e);
                 }
             }
         }
@@ -582,7 +606,7 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
                         const int c = column(i) + e;
                         if (static_cast<unsigned>(c) < static_cast<unsigned>(a.C))
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) own[k * a.C + c] = at_of(sums[k][i], e) + (q ? own[k * a.C + c] : 0.0f);
+                            for (int k = 0; k < 4; ++k) own[k * a.C + c] = at_of(sums[k][kSums ? i : 0], e) + (q ? own[k * a.C + c] : 0.0f);
                     }
             __syncwarp();
         }
@@ -677,8 +701,7 @@ bool plan_backward(Gate gate, const SandwichGradArgs& a, int type, RowPlan* p) {
                          (gate != Gate::All || (on16(a.gate) && on16(a.grad_gate)));
     const bool match = rows_match(size, a.C, a.pitch, aligned) && (gate != Gate::All || rows_match(size, a.C, a.pitch_gate, aligned));
     const bool shift = rows_shift(size, a.C) || !on16(a.p.scale) || !on16(a.p.post_weight) || !on16(a.p.post_bias) || !on16(a.p.weight);
-    // (the column sums of 32 elements do not fit the registers)
-    return match && plan_elements(a.C, size, shift, false, p) && p->items * (16 / size) <= 16;
+    return match && plan_elements(a.C, size, shift, false, p);
 }
 // The backward kernel for these rows, with its shape: f(kernel, shape); kBadArgument where there is none
 template <class F>
@@ -692,22 +715,18 @@ int with_backward(Gate gate, const SandwichGradArgs& a, int type, const DeviceCt
                 constexpr Gate G = decltype(g)::value;
                 constexpr int kItems = decltype(items)::value;
                 constexpr bool kGroup = decltype(group)::value;
-                if constexpr (kItems * kPiece<T> > 16) {
-                    return static_cast<int>(kBadArgument);
-                } else {
-                    constexpr auto kernel = sandwich_grad_registers_kernel<T, G, kItems, kGroup, decltype(shift)::value>;
-                    int per_sm;
-                    const int r = resident_blocks<kernel>(p.threads, ctx, &per_sm);
-                    if (r != kOk) return r;
-                    RowShape s;
-                    const long long params = kGroup ? 0 : 3LL * kItems * (kPiece<T> / 4) * p.threads * 16;
-                    if (!shape_of(p, a.rows, 1, kBackwardStreams<G>, params, per_sm, ctx, &s)) return static_cast<int>(kBadArgument);
-                    if constexpr (kGroup) {
-                        const size_t columns = static_cast<size_t>(kGroupThreads / 32) * 4 * a.C * sizeof(float);
-                        if (s.smem < columns) s.smem = columns;
-                    }
-                    return f(kernel, s);
+                constexpr auto kernel = sandwich_grad_registers_kernel<T, G, kItems, kGroup, decltype(shift)::value>;
+                int per_sm;
+                const int r = resident_blocks<kernel>(p.threads, ctx, &per_sm);
+                if (r != kOk) return r;
+                RowShape s;
+                const long long params = kGroup || kItems * kPiece<T> > 16 ? 0 : 3LL * kItems * (kPiece<T> / 4) * p.threads * 16;
+                if (!shape_of(p, a.rows, 1, kBackwardStreams<G>, params, per_sm, ctx, &s)) return static_cast<int>(kBadArgument);
+                if constexpr (kGroup) {
+                    const size_t columns = static_cast<size_t>(kGroupThreads / 32) * 4 * a.C * sizeof(float);
+                    if (s.smem < columns) s.smem = columns;
                 }
+                return f(kernel, s, kItems * kPiece<T> <= 16);
             });
         });
     });
@@ -731,7 +750,7 @@ bool sandwich_in_registers(Gate gate, const SandwichArgs& a, int type, const Dev
                 const int r = resident_blocks<kernel>(p.threads, ctx, &per_sm);
                 if (r != kOk) return r;
                 RowShape s;
-                fits = shape_of(p, a.rows, rows_forward(kItems * kPiece<T>, kGroup), kForwardStreams<G>, 0, per_sm, ctx, &s);
+                fits = shape_of(p, a.rows, rows_forward(kItems * kPiece<T>, sizeof(T), kGroup, decltype(shift)::value), kForwardStreams<G>, 0, per_sm, ctx, &s);
                 return fits ? launch_after(kernel, s.blocks, p.threads, s.smem, st, a, p.lanes, s.depth) : static_cast<int>(kOk);
             });
         });
@@ -740,17 +759,25 @@ bool sandwich_in_registers(Gate gate, const SandwichArgs& a, int type, const Dev
     return fits;
 }
 
-bool sandwich_grad_in_registers(Gate gate, const SandwichGradArgs& a, int type, const DeviceCtx* ctx, int* blocks) {
-    return with_backward(gate, a, type, ctx, [&](auto, const RowShape& s) {
+int sandwich_grad_in_registers(Gate gate, const SandwichGradArgs& a, int type, const DeviceCtx* ctx, bool sums, int* blocks) {
+    int on_chip = kNothing;
+    with_backward(gate, a, type, ctx, [&](auto, const RowShape& s, bool with_sums) {
         *blocks = s.blocks;
+        on_chip = with_sums || !sums ? kRowsAndSums : kRows;
         return static_cast<int>(kOk);
-    }) == kOk;
+    });
+    return on_chip;
 }
 
 int launch_sandwich_grad_in_registers(Gate gate, const SandwichGradArgs& a, int type, const DeviceCtx* ctx, cudaStream_t st) {
-    return with_backward(gate, a, type, ctx, [&](auto kernel, const RowShape& s) {
+    return with_backward(gate, a, type, ctx, [&](auto kernel, const RowShape& s, bool) {
         return launch_after(kernel, s.blocks, s.p.threads, s.smem, st, a, s.p.lanes, s.depth);
     });
+}
+
+bool sandwich_runs(Gate gate, const SandwichGradArgs& a, int type) {
+    RowPlan p;
+    return plan_backward(gate, a, type, &p) && !rows_shift(size_of(type), a.C);
 }
 
 }  // namespace ldn
