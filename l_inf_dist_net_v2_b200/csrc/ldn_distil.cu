@@ -79,37 +79,52 @@ struct Pieces {
     __device__ __forceinline__ int first(int j) const { return j * N - shift; }
     __device__ __forceinline__ bool whole(int j) const { return first(j) >= 0 && first(j) + N <= V; }
     __device__ __forceinline__ uint4 load(int j) const { return *reinterpret_cast<const uint4*>(row + first(j)); }
-    static __device__ __forceinline__ void unpack(uint4 raw, float (&v)[N]) {
-        const T* e = reinterpret_cast<const T*>(&raw);
+    static __device__ __forceinline__ void unpack(uint4 raw, float2* v) {
+        const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = to_float(e[i]);
+        for (int i = 0; i < N / 2; ++i) {
+            if constexpr (sizeof(T) == 4) v[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+            else if constexpr (std::is_same_v<T, __half>) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            else v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+        }
     }
     // a piece at either end, `none` outside the row
-    __device__ __forceinline__ void edge(int j, float none, float (&v)[N]) const {
+    __device__ __forceinline__ void edge(int j, float none, float2* v) const {
+        auto at = [&](int c) { return static_cast<unsigned>(c) < static_cast<unsigned>(V) ? to_float(row[c]) : none; };
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = first(j) + i;
-            v[i] = static_cast<unsigned>(c) < static_cast<unsigned>(V) ? to_float(row[c]) : none;
-        }
+        for (int i = 0; i < N / 2; ++i) v[i] = make_float2(at(first(j) + 2 * i), at(first(j) + 2 * i + 1));
     }
 };
 
+// 2 N values, two at a time
 template <int N>
-__device__ __forceinline__ void add_values(Sums& a, const float (&v)[N], float c, float c1, bool second) {
-    float top = v[0];
+__device__ __forceinline__ void add_values(Sums& a, const float2 (&v)[N], float c, float c1, bool second) {
+    float top = largest_of(v[0].x, v[0].y);
 #pragma unroll
-    for (int i = 1; i < N; ++i) top = largest_of(top, v[i]);
+    for (int i = 1; i < N; ++i) asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(top) : "f"(top), "f"(v[i].x), "f"(v[i].y));
     if (!(top <= a.m)) {
         a.s *= exp2_fast((a.m - top) * c);
         a.s1 *= exp2_fast((a.m - top) * c1);
         a.m = top;
     }
     if (a.m == minus_infinity()) return;
+    const float2 m = make_float2(-a.m, -a.m), by = make_float2(c, c);
+    float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < N; ++i) a.s += exp2_fast((v[i] - a.m) * c);
+    for (int i = 0; i < N; ++i) {
+        const float2 d = __fmul2_rn(__fadd2_rn(v[i], m), by);
+        sum = __fadd2_rn(sum, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
+    }
+    a.s += sum.x + sum.y;
     if (second) {
+        const float2 by1 = make_float2(c1, c1);
+        sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) a.s1 += exp2_fast((v[i] - a.m) * c1);
+        for (int i = 0; i < N; ++i) {
+            const float2 d = __fmul2_rn(__fadd2_rn(v[i], m), by1);
+            sum = __fadd2_rn(sum, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
+        }
+        a.s1 += sum.x + sum.y;
     }
 }
 
@@ -119,112 +134,178 @@ __device__ __forceinline__ float value_at(const DistilArgs& a, long long i) {
                                    : __bfloat162float(static_cast<const __nv_bfloat16*>(a.values)[i]);
 }
 
-// What a warp makes of a row's sums: its loss, and what the backward pass needs
-template <class T>
-__device__ __forceinline__ void finish_row(const DistilArgs& a, long long row, const Sums& sums) {
-    const int lane = threadIdx.x & 31;
+// Sums, and the largest, over the LANES threads that share a row: lanes of a warp (a power of two), or a block with a
+// number per warp at `slots`
+template <int LANES, class Op>
+__device__ __forceinline__ float over_row(float v, Op op, float* slots) {
+#pragma unroll
+    for (int d = (LANES < 32 ? LANES : 32) / 2; d > 0; d >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, d));
+    if constexpr (LANES > 32) {
+        if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = slots[0];
+#pragma unroll
+        for (int w = 1; w < LANES / 32; ++w) v = op(v, slots[w]);
+    }
+    return v;
+}
+struct Plus {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+struct Largest {
+    __device__ __forceinline__ float operator()(float a, float b) const { return largest_of(a, b); }
+};
+
+// What of a row's loss does not wait for its sums: with t = value / tau - top, p = e^t / sum, and the largest of the list's logits as reference,
+// terms = sum p (t - log sum - (x - reference) / tau)
+struct List {
+    float top, inv_sum, terms, reference, target;
+    bool some, label, bad;
+};
+template <class T, int LANES>
+__device__ __forceinline__ List read_list(const DistilArgs& a, long long row, float* slots) {
+    constexpr int kWarps = LANES > 32 ? LANES / 32 : 0;  // (a block's rounds have slots of their own)
+    const int lane = threadIdx.x & (LANES - 1);
     const T* x = static_cast<const T*>(a.x) + row * a.pitch;
-    const long long* indices = a.indices + row * a.k;
+    const long long *indices = a.indices + row * a.k, target = a.targets ? a.targets[row] : -1;
     const float inv_tau = 1.0f / a.tau;
-    bool bad = false;
-    float top = minus_infinity();
-    for (int j = lane; j < a.k; j += 32) {
+    // (a lane's first entry stays in registers: lists are short)
+    const bool mine = lane < a.k;
+    const long long i0 = mine ? indices[lane] : -1;
+    const float v0 = mine ? value_at(a, row * a.k + lane) * inv_tau : 0.0f;
+    const bool fine0 = i0 >= 0 && i0 < a.V;
+    const float x0 = fine0 ? to_float(x[i0]) : minus_infinity();
+    List l;
+    l.target = target >= 0 && target < a.V ? to_float(x[target]) : 0.0f;
+    l.label = target >= 0;
+    float bad = (mine && i0 >= a.V) || target >= a.V ? 1.0f : 0.0f, top = i0 >= 0 ? v0 : minus_infinity(), reference = x0;
+    for (int j = lane + LANES; j < a.k; j += LANES) {
         const long long i = indices[j];
-        bad = bad || i >= a.V;
+        if (i >= a.V) bad = 1.0f;
         if (i >= 0) top = largest_of(top, value_at(a, row * a.k + j) * inv_tau);
+        if (i >= 0 && i < a.V) reference = largest_of(reference, to_float(x[i]));
     }
-    for (int d = 16; d > 0; d >>= 1) top = largest_of(top, __shfl_xor_sync(0xffffffffu, top, d));
-    bad = __any_sync(0xffffffffu, bad);
-    float sum = 0.0f;
-    const bool some = top != minus_infinity();  // (a list of nothing but minus infinity says nothing)
-    if (some)
-        for (int j = lane; j < a.k; j += 32)
+    l.bad = over_row<LANES>(bad, Largest(), slots) != 0.0f;
+    l.top = top = over_row<LANES>(top, Largest(), slots + kWarps);
+    l.reference = reference = over_row<LANES>(reference, Largest(), slots + 2 * kWarps);
+    l.some = top != minus_infinity();  // (a list of nothing but minus infinity says nothing)
+    float sum = l.some && i0 >= 0 ? expf(v0 - top) : 0.0f;
+    if (l.some)
+        for (int j = lane + LANES; j < a.k; j += LANES)
             if (indices[j] >= 0) sum += expf(value_at(a, row * a.k + j) * inv_tau - top);
-    sum = warp_sum(sum);
-    const float log_s = logf(sums.s), log_sum = logf(sum), inv_sum = 1.0f / sum;
+    sum = over_row<LANES>(sum, Plus(), slots + 3 * kWarps);
+    l.inv_sum = 1.0f / sum;
+    const float log_sum = logf(sum);
+    auto term = [&](float v, float at) {
+        const float t = v - top, p = expf(t) * l.inv_sum;
+        return p != 0.0f ? p * ((t - log_sum) - (at - reference) * inv_tau) : 0.0f;
+    };
+    float terms = 0.0f;
+    if (l.some && !l.bad) {
+        if (fine0) terms = term(v0, x0);
+        for (int j = lane + LANES; j < a.k; j += LANES)
+            if (indices[j] >= 0) terms += term(value_at(a, row * a.k + j) * inv_tau, to_float(x[indices[j]]));
+    }
+    l.terms = over_row<LANES>(terms, Plus(), slots + 4 * kWarps);
+    return l;
+}
+// The rest, by one lane: the loss, and what the backward pass needs
+__device__ __forceinline__ void finish_row(const DistilArgs& a, long long row, const List& l, const Sums& sums) {
+    const float s1 = a.tau == 1.0f ? sums.s : sums.s1;
     float loss = 0.0f;
-    if (some && !bad) {
-        for (int j = lane; j < a.k; j += 32) {
-            const long long i = indices[j];
-            if (i < 0) continue;
-            const float t = value_at(a, row * a.k + j) * inv_tau - top, p = expf(t) * inv_sum;
-            // log p - log q, each relative to its largest
-            if (p != 0.0f) loss += p * ((t - log_sum) - ((to_float(x[i]) - sums.m) * inv_tau - log_s));
-        }
-        loss = warp_sum(loss) * (a.part * a.tau * a.tau);
-    }
-    float s1 = sums.s1;
-    if (a.tau == 1.0f) s1 = sums.s;
-    if (a.targets) {
-        const long long target = a.targets[row];
-        bad = bad || target >= a.V;
-        if (target >= 0 && !bad) loss += a.mix * (logf(s1) - (to_float(x[target]) - sums.m));
-    }
-    if (lane == 0) {
-        a.losses[row] = bad ? not_a_number() : loss;
-        if (a.stats) {
-            a.stats[row] = sums.m;
-            a.stats[a.rows + row] = bad ? not_a_number() : 1.0f / sums.s;
-            a.stats[2 * a.rows + row] = bad ? not_a_number() : 1.0f / s1;
-            a.stats[3 * a.rows + row] = top;
-            a.stats[4 * a.rows + row] = bad ? not_a_number() : some ? inv_sum : 0.0f;
-        }
+    // (a preferred class that is no choice: infinity, whatever the others are)
+    if (l.some) loss = a.part * a.tau * a.tau * (l.reference == minus_infinity() ? -minus_infinity() : l.terms - ((l.reference - sums.m) / a.tau - logf(sums.s)));
+    if (l.label) loss += a.mix * (logf(s1) - (l.target - sums.m));
+    a.losses[row] = l.bad ? not_a_number() : loss;
+    if (a.stats) {
+        a.stats[row] = sums.m;
+        a.stats[a.rows + row] = l.bad ? not_a_number() : 1.0f / sums.s;
+        a.stats[2 * a.rows + row] = l.bad ? not_a_number() : 1.0f / s1;
+        a.stats[3 * a.rows + row] = l.top;
+        a.stats[4 * a.rows + row] = l.bad ? not_a_number() : l.some ? l.inv_sum : 0.0f;
     }
 }
 
-// A row of up to kShort classes: a warp.  Longer ones: a block, or the blocks of a cluster, each with a range of the pieces.
-constexpr int kShort = 2048, kAhead = 4;
-template <class T>
-__device__ __forceinline__ void read_pieces(const Pieces<T>& p, int first, int last, int thread, int threads, const DistilArgs& a, float c,
-                                            float c1, bool second, Sums& sums) {
-    constexpr int N = Pieces<T>::N;
-    int j = first + thread;
-    for (; j + (kAhead - 1) * threads < last; j += kAhead * threads) {
-        uint4 raw[kAhead];
-        const bool whole = p.whole(j) && p.whole(j + (kAhead - 1) * threads);  // (and so are those between)
-        if (whole) {
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) raw[u] = p.load(j + u * threads);
-            float v[kAhead * N];
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) Pieces<T>::unpack(raw[u], reinterpret_cast<float(&)[N]>(v[u * N]));
-            add_values(sums, v, c, c1, second);
-        } else {
-            for (int u = 0; u < kAhead; ++u) {
-                float v[N];
-                p.edge(j + u * threads, minus_infinity(), v);
-                add_values(sums, v, c, c1, second);
-            }
-        }
+// Short rows: some lanes of a warp (distil_lanes).  Longer ones: a block, or the blocks of a cluster, each with a range of the pieces.
+constexpr int kAhead = 4;
+constexpr int kShortEntries = 128;  // of a list, in the backward pass
+// The pieces from `first` to in front of `last`, by a thread of some.  Four are loaded while the four in front of them are worked on (without:
+// 8192 x 40001 bf16 178 us); those at a row's cut ends, element by element, come last.
+// meanwhile: what is done with the first four under way.
+template <class T, class F>
+__device__ __forceinline__ void read_pieces(const Pieces<T>& p, int first, int last, int thread, int threads, float c, float c1, bool second,
+                                            Sums& sums, F meanwhile) {
+    constexpr int H = Pieces<T>::N / 2;
+    if (first >= last) {
+        meanwhile();
+        return;
     }
-    for (; j < last; j += threads) {
-        float v[N];
-        if (p.whole(j)) Pieces<T>::unpack(p.load(j), v);
-        else p.edge(j, minus_infinity(), v);
+    const int begin = p.whole(first) ? first : first + 1, end = p.whole(last - 1) ? last : last - 1;
+    int j = begin + thread;
+    uint4 raw[kAhead];
+    auto load = [&] {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) raw[u] = p.load(j + u * threads);
+    };
+    bool more = j + (kAhead - 1) * threads < end;
+    if (more) load();
+    meanwhile();
+    while (more) {
+        float2 v[kAhead * H];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) Pieces<T>::unpack(raw[u], v + u * H);
+        j += kAhead * threads;
+        more = j + (kAhead - 1) * threads < end;
+        if (more) load();
+        add_values(sums, v, c, c1, second);
+    }
+    for (; j < end; j += threads) {
+        float2 v[H];
+        Pieces<T>::unpack(p.load(j), v);
+        add_values(sums, v, c, c1, second);
+    }
+    if (begin > first && thread == 0) {
+        float2 v[H];
+        p.edge(first, minus_infinity(), v);
+        add_values(sums, v, c, c1, second);
+    }
+    if (end < last && last - 1 >= begin && thread == 1) {
+        float2 v[H];
+        p.edge(last - 1, minus_infinity(), v);
         add_values(sums, v, c, c1, second);
     }
 }
 
-template <class T>
-__global__ void __launch_bounds__(kDistilThreads) distil_short_kernel(const __grid_constant__ DistilArgs a) {
+template <class T, int LANES>
+__global__ void __launch_bounds__(kDistilThreads, 3) distil_short_kernel(const __grid_constant__ DistilArgs a) {
     stream_order_begin();
+    constexpr int kRows = kDistilThreads / LANES;
     const float c = kLog2e / a.tau, c1 = kLog2e;
     const bool second = a.targets && a.tau != 1.0f;
-    for (long long row = static_cast<long long>(blockIdx.x) * kDistilWarps + (threadIdx.x >> 5); row < a.rows;
-         row += static_cast<long long>(gridDim.x) * kDistilWarps) {
+    const int lane = threadIdx.x & (LANES - 1);
+    for (long long row0 = static_cast<long long>(blockIdx.x) * kRows; row0 < a.rows; row0 += static_cast<long long>(gridDim.x) * kRows) {
+        const bool there = row0 + threadIdx.x / LANES < a.rows;  // (lanes without a row of their own go along with the last one)
+        const long long row = there ? row0 + threadIdx.x / LANES : a.rows - 1;
         const Pieces<T> p(static_cast<const T*>(a.x) + row * a.pitch, a.V);
         Sums sums = {minus_infinity(), 0.0f, 0.0f};
-        read_pieces(p, 0, p.count, threadIdx.x & 31, 32, a, c, c1, second, sums);
+        List list;
+        read_pieces(p, 0, p.count, lane, LANES, c, c1, second, sums, [&] {
+            __syncwarp();
+            list = read_list<T, LANES>(a, row, nullptr);
+        });
         __syncwarp();
-        sums.over_lanes(32, c, c1);
-        finish_row<T>(a, row, sums);
+        sums.over_lanes(LANES, c, c1);
+        if (lane == 0 && there) finish_row(a, row, list, sums);
     }
 }
 
+// (the first CTA's first warp makes the loss)
 template <class T>
-__global__ void __launch_bounds__(kDistilThreads) distil_long_kernel(const __grid_constant__ DistilArgs a) {
+__global__ void __launch_bounds__(kDistilThreads, 4) distil_long_kernel(const __grid_constant__ DistilArgs a) {
     stream_order_begin();
     __shared__ Sums of_warps[kDistilWarps], of_ranks[kMostRanks];
+    __shared__ float slots[5 * kDistilWarps];
+    __shared__ List list;
     const float c = kLog2e / a.tau, c1 = kLog2e;
     const bool second = a.targets && a.tau != 1.0f;
     const uint32_t rank = cluster_rank(), ranks = cluster_size();
@@ -234,14 +315,18 @@ __global__ void __launch_bounds__(kDistilThreads) distil_long_kernel(const __gri
     const Pieces<T> p(static_cast<const T*>(a.x) + row * a.pitch, a.V);
     Sums sums = {minus_infinity(), 0.0f, 0.0f};
     read_pieces(p, static_cast<int>(static_cast<long long>(p.count) * rank / ranks), static_cast<int>(static_cast<long long>(p.count) * (rank + 1) / ranks),
-                threadIdx.x, kDistilThreads, a, c, c1, second, sums);
+                threadIdx.x, kDistilThreads, c, c1, second, sums, [&] {
+                    if (rank != 0) return;
+                    const List l = read_list<T, kDistilThreads>(a, row, slots);
+                    if (threadIdx.x == 0) list = l;
+                });
     __syncwarp();
     sums.over_lanes(32, c, c1);
     if (lane == 0) of_warps[warp] = sums;
     __syncthreads();
     if (warp == 0) {
         sums = lane < kDistilWarps ? of_warps[lane] : Sums{minus_infinity(), 0.0f, 0.0f};
-        sums.over_lanes(32, c, c1);
+        sums.over_lanes(kDistilWarps, c, c1);
         if (ranks > 1 && lane == 0) {
             const uint32_t to = in_cta(&of_ranks[rank], 0);
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(sums.m) : "memory");
@@ -254,10 +339,10 @@ __global__ void __launch_bounds__(kDistilThreads) distil_long_kernel(const __gri
         cluster_barrier();
         if (rank == 0 && warp == 0) {
             sums = lane < static_cast<int>(ranks) ? of_ranks[lane] : Sums{minus_infinity(), 0.0f, 0.0f};
-            sums.over_lanes(32, c, c1);
+            sums.over_lanes(kMostRanks, c, c1);
         }
     }
-    if (rank == 0 && warp == 0) finish_row<T>(a, row, sums);
+    if (rank == 0 && threadIdx.x == 0) finish_row(a, row, list, sums);
 }
 
 // The rows' losses in a fixed order
@@ -288,8 +373,10 @@ struct RowGradient {
     }
 };
 
+// index, minus: room for a list and a label, in whole fours
+__host__ __device__ __forceinline__ int list_room(int k) { return (k + 4) / 4 * 4; }
 template <class T, int THREADS>
-__device__ __forceinline__ void gradient_of_row(const DistilArgs& a, long long row, int part, int parts, int thread, long long* index, float* minus) {
+__device__ __forceinline__ void gradient_of_row(const DistilArgs& a, long long row, int part, int parts, int thread, int* index, float* minus, bool there) {
     constexpr int N = Pieces<T>::N;
     const T* x = static_cast<const T*>(a.x) + row * a.pitch;
     T* to = static_cast<T*>(a.grad) + row * a.V;
@@ -312,32 +399,38 @@ __device__ __forceinline__ void gradient_of_row(const DistilArgs& a, long long r
         g.two = false;
     }
     const Pieces<T> p(x, a.V);
-    const int first = static_cast<int>(static_cast<long long>(p.count) * part / parts), last = static_cast<int>(static_cast<long long>(p.count) * (part + 1) / parts);
-    const int begin = p.first(first) > 0 ? p.first(first) : 0, end = p.first(last) < a.V ? p.first(last) : a.V;
+    const int first = static_cast<int>(static_cast<long long>(p.count) * part / parts);
+    int last_piece = static_cast<int>(static_cast<long long>(p.count) * (part + 1) / parts);
+    const int begin = p.first(first) > 0 ? p.first(first) : 0, end = !there ? 0 : p.first(last_piece) < a.V ? p.first(last_piece) : a.V;
     // the list, and the label behind it
-    for (int j = thread; j <= a.k; j += THREADS) {
-        const long long i = j < a.k ? a.indices[row * a.k + j] : target;
-        index[j] = i;
-        minus[j] = j == a.k ? by_label : i >= 0 && list ? by_list * (expf(value_at(a, row * a.k + j) * inv_tau - top) * inv_sum) : 0.0f;
+    const int room = list_room(a.k);
+    for (int j = thread; j < room; j += THREADS) {
+        const long long i = j < a.k ? a.indices[row * a.k + j] : j == a.k ? target : -1;
+        index[j] = i >= 0 && i < a.V ? static_cast<int>(i) : -1;
+        minus[j] = j == a.k ? by_label : j < a.k && i >= 0 && list ? by_list * (expf(value_at(a, row * a.k + j) * inv_tau - top) * inv_sum) : 0.0f;
     }
+    if (!there) last_piece = first;
     const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(to)) & 15u) == 0;
     constexpr int kRow = 2;
     if (same) {
-        for (int j0 = first + thread; j0 < last; j0 += kRow * THREADS) {
+        for (int j0 = first + thread; j0 < last_piece; j0 += kRow * THREADS) {
             uint4 raw[kRow];
 #pragma unroll
             for (int u = 0; u < kRow; ++u)
-                if (j0 + u * THREADS < last && p.whole(j0 + u * THREADS)) raw[u] = p.load(j0 + u * THREADS);
+                if (j0 + u * THREADS < last_piece && p.whole(j0 + u * THREADS)) raw[u] = p.load(j0 + u * THREADS);
 #pragma unroll
             for (int u = 0; u < kRow; ++u) {
                 const int j = j0 + u * THREADS;
-                if (j >= last) continue;
+                if (j >= last_piece) continue;
                 if (p.whole(j)) {
-                    float v[N];
+                    float2 v[N / 2];
                     Pieces<T>::unpack(raw[u], v);
                     T e[N];
 #pragma unroll
-                    for (int i = 0; i < N; ++i) e[i] = from_float<T>(g(v[i]));
+                    for (int i = 0; i < N / 2; ++i) {
+                        e[2 * i] = from_float<T>(g(v[i].x));
+                        e[2 * i + 1] = from_float<T>(g(v[i].y));
+                    }
                     *reinterpret_cast<uint4*>(to + p.first(j)) = *reinterpret_cast<const uint4*>(e);
                 } else {
                     for (int i = 0; i < N; ++i) {
@@ -350,47 +443,69 @@ __device__ __forceinline__ void gradient_of_row(const DistilArgs& a, long long r
     } else {
         for (int c = begin + thread; c < end; c += THREADS) to[c] = from_float<T>(g(to_float(x[c])));
     }
-    if constexpr (THREADS == 32) __syncwarp();
+    if constexpr (THREADS <= 32) __syncwarp();
     else __syncthreads();
     // the list's classes once more: the first entry of a class writes what all its entries take off
     for (int j = thread; j <= a.k; j += THREADS) {
-        const long long i = index[j];
+        const int i = index[j];
         if (i < begin || i >= end) continue;
         float off = 0.0f;
         bool own = true;
-        for (int o = 0; o <= a.k; ++o)
-            if (index[o] == i) {
-                own = own && o >= j;
-                off += minus[o];
-            }
+        for (int o = 0; o < room; o += 4) {
+            const int4 q = *reinterpret_cast<const int4*>(index + o);
+            if (q.x != i && q.y != i && q.z != i && q.w != i) continue;
+            own = own && !((o < j && q.x == i) || (o + 1 < j && q.y == i) || (o + 2 < j && q.z == i) || (o + 3 < j && q.w == i));
+            if (q.x == i) off += minus[o];
+            if (q.y == i) off += minus[o + 1];
+            if (q.z == i) off += minus[o + 2];
+            if (q.w == i) off += minus[o + 3];
+        }
         if (own) to[i] = from_float<T>(g(to_float(x[i])) - off);
     }
-    if constexpr (THREADS == 32) __syncwarp();
+    if constexpr (THREADS <= 32) __syncwarp();
 }
 
-template <class T>
+template <class T, int LANES>
 __global__ void __launch_bounds__(kDistilThreads) distil_grad_short_kernel(const __grid_constant__ DistilArgs a) {
     stream_order_begin();
-    extern __shared__ long long list[];  // [warp][k + 1], then as many floats
-    const int warp = threadIdx.x >> 5;
-    float* minus = reinterpret_cast<float*>(list + kDistilWarps * (a.k + 1));
-    for (long long row = static_cast<long long>(blockIdx.x) * kDistilWarps + warp; row < a.rows; row += static_cast<long long>(gridDim.x) * kDistilWarps)
-        gradient_of_row<T, 32>(a, row, 0, 1, threadIdx.x & 31, list + warp * (a.k + 1), minus + warp * (a.k + 1));
+    extern __shared__ int4 list[];  // [row of the block][room], then as many floats
+    constexpr int kRows = kDistilThreads / LANES;
+    const int mine = threadIdx.x / LANES, room = list_room(a.k);
+    int* index = reinterpret_cast<int*>(list);
+    float* minus = reinterpret_cast<float*>(index + kRows * room);
+    for (long long row0 = static_cast<long long>(blockIdx.x) * kRows; row0 < a.rows; row0 += static_cast<long long>(gridDim.x) * kRows) {
+        const bool there = row0 + mine < a.rows;
+        gradient_of_row<T, LANES>(a, there ? row0 + mine : a.rows - 1, 0, 1, threadIdx.x & (LANES - 1), index + mine * room, minus + mine * room, there);
+    }
 }
 template <class T>
 __global__ void __launch_bounds__(kDistilThreads) distil_grad_long_kernel(const __grid_constant__ DistilArgs a) {
     stream_order_begin();
-    extern __shared__ long long list[];
+    extern __shared__ int4 list[];
     const int parts = gridDim.y;
-    gradient_of_row<T, kDistilThreads>(a, blockIdx.x, blockIdx.y, parts, threadIdx.x, list, reinterpret_cast<float*>(list + a.k + 1));
+    int* index = reinterpret_cast<int*>(list);
+    gradient_of_row<T, kDistilThreads>(a, blockIdx.x, blockIdx.y, parts, threadIdx.x, index, reinterpret_cast<float*>(index + list_room(a.k)), true);
 }
 
 bool distil_fits(long long rows, int V, int type, int value_type, int k, float tau) {
     return rows >= 0 && rows <= kMostColumns && row_fits(V) && known_type(type) && known_type(value_type) && k >= 1 && k <= kMostEntries &&
            tau > 0.0f && tau <= 3.402823466e38f;
 }
-int short_blocks(long long rows, const DeviceCtx* ctx) {
-    const long long needed = (rows + kDistilWarps - 1) / kDistilWarps, most = 64LL * ctx->sm_count;
+// Lanes of a warp that share a row, 0: a block or more per row.  What bounds short rows is the way from a row's loads to its loss, so there are as
+// many at once as can be.
+int distil_lanes(long long rows, int V, const DeviceCtx* ctx) {
+    if (V <= 256) return 8;
+    if (V <= 1024) return 16;
+    return V <= 2048 || (V <= 8192 && rows >= 16LL * ctx->sm_count) ? 32 : 0;
+}
+template <class F>
+int with_lanes(int lanes, F f) {
+    using std::integral_constant;
+    return lanes == 8 ? f(integral_constant<int, 8>()) : lanes == 16 ? f(integral_constant<int, 16>()) : f(integral_constant<int, 32>());
+}
+int short_blocks(long long rows, int lanes, const DeviceCtx* ctx) {
+    const int of_block = kDistilThreads / lanes;
+    const long long needed = (rows + of_block - 1) / of_block, most = 64LL * ctx->sm_count;
     return static_cast<int>(needed < most ? needed : most);
 }
 
@@ -416,7 +531,10 @@ extern "C" LDN_API int ldn_distillation(const void* x, long long pitch, long lon
         a.losses = losses; a.stats = stats;
         r = with_type(type, [&](auto t) {
             using T = decltype(t);
-            if (V <= kShort) return launch_after(distil_short_kernel<T>, short_blocks(rows, ctx), kDistilThreads, 0, st, a);
+            if (const int lanes = distil_lanes(rows, V, ctx))
+                return with_lanes(lanes, [&](auto n) {
+                    return launch_after(distil_short_kernel<T, decltype(n)::value>, short_blocks(rows, lanes, ctx), kDistilThreads, 0, st, a);
+                });
             // as many CTAs per row as it takes to fill the device twice, each with 4096 classes at least
             int ranks = 1;
             while (ranks < kMostRanks && rows * ranks < 2LL * ctx->sm_count && V / (2 * ranks) >= 4096) ranks *= 2;
@@ -446,17 +564,15 @@ extern "C" LDN_API int ldn_distillation_backward(const void* x, long long pitch,
     a.up = up; a.up_step = up_per_row ? 1 : 0; a.up_scale = up_scale; a.grad = grad;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        const int entry = sizeof(long long) + sizeof(float);
-        if (V <= kShort) {
-            constexpr auto kernel = distil_grad_short_kernel<T>;
-            static OncePerDevice once;
-            const int s = once([] { return allow_smem(kernel, kDistilWarps * (kMostEntries + 1) * (sizeof(long long) + sizeof(float))); });
-            if (s != kOk) return s;
-            return launch_after(kernel, short_blocks(rows, ctx), kDistilThreads, static_cast<size_t>(kDistilWarps) * (k + 1) * entry, st, a);
-        }
+        const size_t of_row = static_cast<size_t>(list_room(k)) * 8;
+        const int lanes = k <= kShortEntries ? distil_lanes(rows, V, ctx) : 0;
+        if (lanes)
+            return with_lanes(lanes, [&](auto n) {
+                return launch_after(distil_grad_short_kernel<T, decltype(n)::value>, short_blocks(rows, lanes, ctx), kDistilThreads,
+                                    kDistilThreads / lanes * of_row, st, a);
+            });
         int parts = 1;
         while (parts < 64 && rows * parts < 4LL * ctx->sm_count && V / (2 * parts) >= 2048) parts *= 2;
-        return launch_after(distil_grad_long_kernel<T>, dim3(static_cast<unsigned>(rows), parts), kDistilThreads, static_cast<size_t>(k + 1) * entry,
-                            st, a);
+        return launch_after(distil_grad_long_kernel<T>, dim3(static_cast<unsigned>(rows), parts), kDistilThreads, of_row, st, a);
     });
 }
