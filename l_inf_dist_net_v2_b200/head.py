@@ -1,6 +1,6 @@
 """Operators and layers of a head behind the distance layers: layer norm, dropout whose mask is never stored, both joined on a
-residual stream, and the matrix product in 8-bit integers that the head answers with.  The reference has none of them (its head
-is linear, tanh, linear; core/modules/basic_modules.py:11-46).
+residual stream, and the matrix product in 8-bit integers that the head answers with; a gated projection, and the stream between
+two norms, for gated blocks.  The reference has none of them (its head is linear, tanh, linear; core/modules/basic_modules.py:11-46).
 
 Rows are the last dimension of a float32, float16 or bfloat16 CUDA tensor; a norm's weight and bias are float32 or of that type.
 Statistics, sums and gradients' sums have 32 bits whatever the type, and results are rounded once.  Launches go to PyTorch's
@@ -14,7 +14,7 @@ import torch.nn as nn
 from . import norm_dist_cuda as _C
 
 __all__ = ["layer_norm", "dropout", "dropout_add_layer_norm", "quantize_rows", "layer_norm_quantized", "int8_linear", "gated_linear", "sandwich_norm",
-           "LayerNorm",
+           "LayerNorm", "GatedLinear", "SandwichNorm", "GatedHead",
            "Dropout", "Int8Linear", "ResidualHead", "QuantizedHead"]
 
 _ACTIVATIONS = {"none": 0, "relu": 1, "tanh": 2}
@@ -193,6 +193,51 @@ class Dropout(nn.Module):
         return f"p={self.p}"
 
 
+class GatedLinear(nn.Module):
+    """act(gate(x)) * up(x) of two linear maps, as one kernel.  Under torch.autocast in its type, as torch's linear layers are."""
+
+    def __init__(self, features, outputs, activation="silu", bias=True):
+        super().__init__()
+        if activation not in _GATES:
+            raise ValueError(f"activation must be one of {sorted(_GATES)}, not {activation!r}")
+        self.activation = activation
+        for name in ("gate", "up"):
+            start = nn.Linear(features, outputs, bias=bias)
+            setattr(self, f"weight_{name}", start.weight)
+            self.register_parameter(f"bias_{name}", start.bias)
+
+    def forward(self, x):
+        gate, up = self.weight_gate, self.weight_up
+        if torch.is_autocast_enabled("cuda"):
+            dtype = torch.get_autocast_dtype("cuda")
+            x, gate, up = x.to(dtype), gate.to(dtype), up.to(dtype)
+        biases = [b if b is None or b.dtype == x.dtype else b.float() for b in (self.bias_gate, self.bias_up)]
+        return gated_linear(x, gate, up, *biases, activation=self.activation)
+
+    def extra_repr(self):
+        return f"{self.weight_gate.size(1)}, {self.weight_gate.size(0)}, activation={self.activation}, bias={self.bias_gate is not None}"
+
+
+class SandwichNorm(nn.Module):
+    """`sandwich_norm` with its parameters: the norm behind a block, the scale that its rows join the stream with, and the next block's norm."""
+
+    def __init__(self, features, scale=1.0, eps=1e-5):
+        super().__init__()
+        self.features = features
+        self.eps = eps
+        self.post_weight = nn.Parameter(torch.ones(features))
+        self.post_bias = nn.Parameter(torch.zeros(features))
+        self.scale = nn.Parameter(torch.full((features,), float(scale)))
+        self.weight = nn.Parameter(torch.ones(features))
+        self.bias = nn.Parameter(torch.zeros(features))
+
+    def forward(self, x, residual, gate=None):
+        return sandwich_norm(x, residual, self.weight, self.bias, self.post_weight, self.post_bias, self.scale, gate, self.eps)
+
+    def extra_repr(self):
+        return f"{self.features}, eps={self.eps}"
+
+
 class _Answers(nn.Module):
     """A module whose buffers of floating point have 32 bits wherever it is moved: the kernels take no other."""
 
@@ -267,6 +312,33 @@ class ResidualHead(nn.Module):
     def quantized(self):
         """The head as it answers in 8-bit integers, from the weights as they are now."""
         return QuantizedHead(self)
+
+
+class GatedHead(nn.Module):
+    """A residual head of gated blocks between two norms: with y the norm of the stream h, a block adds
+
+        gate(y) scale norm(dropout(down(act(g(y)) * u(y))))
+
+    to h, gate(y) = sigmoid of one number per row and scale one per column, small at first; the classes are a linear map of the last norm.
+    Each block is `gated_linear`, a product and `sandwich_norm`.  As a `ResidualHead` it has no interval bounds, and its stream has the
+    type of its weights, under torch.autocast too.  It answers in floating point."""
+
+    def __init__(self, width, hidden, num_classes=10, blocks=2, dropout=0.1, activation="silu", scale=0.1, eps=1e-5, seed=None):
+        super().__init__()
+        self.norm = LayerNorm(width, eps)
+        self.wide = nn.ModuleList(GatedLinear(width, hidden, activation) for _ in range(blocks))
+        self.down = nn.ModuleList(nn.Linear(hidden, width) for _ in range(blocks))
+        self.drop = nn.ModuleList(Dropout(dropout, None if seed is None else seed + i) for i in range(blocks))
+        self.gate = nn.ModuleList(nn.Linear(width, 1) for _ in range(blocks))
+        self.join = nn.ModuleList(SandwichNorm(width, scale, eps) for _ in range(blocks))
+        self.final = nn.Linear(width, num_classes)
+
+    def forward(self, h):
+        h = h.to(self.final.weight.dtype)
+        y = self.norm(h)
+        for wide, down, drop, gate, join in zip(self.wide, self.down, self.drop, self.gate, self.join):
+            y, h = join(drop(down(wide(y)).to(h.dtype)), h, torch.sigmoid(gate(y)).to(h.dtype))
+        return self.final(y)
 
 
 class QuantizedHead(_Answers):

@@ -19,7 +19,7 @@ import torch.nn as nn
 from . import norm_dist_cuda as _C
 from . import optim
 from .bound_modules import BoundFinalLinear, BoundLinear, BoundSequential, BoundTanh
-from .head import ResidualHead
+from .head import GatedHead, ResidualHead
 from .modules import NormDist, NormDistBase
 
 __all__ = ["MLPModel", "HybridModel", "ResidualModel", "check_inf_and_eval", "set_p_norm"]
@@ -125,18 +125,22 @@ class ResidualModel(nn.Module):
     `quantize()` puts it into eval mode and makes it answer with the head's products in 8-bit integers, without gradients, until
     `train()`.  They are made again when the head is moved or loaded, parts of it are replaced, or its parameters are changed by torch's
     operations or an optimiser.  What a replayed graph writes, or a write to a parameter's `.data`, is not seen: call `quantize()`
-    again then."""
+    again then.
+
+    `gated`: with a `GatedHead`, which answers in floating point only."""
 
     def __init__(self, depth, width, input_dim, hidden=512, num_classes=10, blocks=2, dropout=0.1, std=1.0, identity_val=None,
-                 seed=None):
+                 seed=None, gated=False):
         super().__init__()
         pixels = input_dim[0] * input_dim[1] * input_dim[2]
         self.fc_dist = _dist_stack([pixels] + [width] * (depth - 2), False, std, identity_val)
-        self.head = ResidualHead(width, hidden, num_classes, blocks, dropout, seed=seed)
+        self.head = (GatedHead if gated else ResidualHead)(width, hidden, num_classes, blocks, dropout, seed=seed)
         self._integers = False
         self._answer = []  # the quantised head and what it was made of (in a list: it is no part of what is trained or saved)
 
     def quantize(self):
+        if isinstance(self.head, GatedHead):
+            raise RuntimeError("a gated head answers in floating point: there are no integers of it")
         self.eval()
         self._answer = [self.head.quantized(), _Contents(self.head)]
         self._integers = True

@@ -21,3 +21,14 @@ class RowOperators:
     def dropout_add_layer_norm(cls, x, residual, weight, bias, p, seed, offset, state, eps):
         h = cls.dropout(x, p, seed, offset, state, residual)
         return cls.layer_norm(h, weight, bias, eps), h
+
+    @staticmethod
+    def gated_linear(x, w_gate, w_up, b_gate, b_up, activation):
+        act = {1: torch.relu, 3: torch.nn.functional.silu, 4: torch.nn.functional.gelu, 5: torch.sigmoid}[activation]
+        return act(torch.nn.functional.linear(x, w_gate, b_gate)) * torch.nn.functional.linear(x, w_up, b_up)
+
+    @classmethod
+    def sandwich_norm(cls, x, residual, gate, scale, post_weight, post_bias, weight, bias, eps):
+        by = (1.0 if gate is None else gate) * (1.0 if scale is None else scale)
+        h = residual + by * cls.layer_norm(x, post_weight, post_bias, eps)
+        return cls.layer_norm(h, weight, bias, eps), h

@@ -106,3 +106,82 @@ def test_rows_that_say_nothing_and_rows_that_are_wrong(V):
     assert torch.equal(losses[:2].detach(), torch.zeros(2, device="cuda")) and torch.equal(dx[:2], torch.zeros_like(dx[:2]))
     assert losses[2:7].isnan().all() and dx[2:6].isnan().all() and dx[6, indices[6]].isnan().all()
     assert losses[7] == math.inf and dx[7].isfinite().all()
+
+
+def test_shapes_and_no_rows():
+    x, values, indices, targets, up = made(12, 50, 4, F32)
+    want = ldn.distillation_loss(x, values, indices, targets, 2.0, 0.3, "none")
+    cube = ldn.distillation_loss(x.view(3, 4, 50), values.view(3, 4, 4), indices.view(3, 4, 4), targets.view(3, 4), 2.0, 0.3, "none")
+    assert torch.equal(cube, want.view(3, 4))
+    assert torch.equal(ldn.distillation_loss(x[0], values[0], indices[0], targets[0], 2.0, 0.3, "none"), want[0])
+    turned = ldn.distillation_loss(x.t().contiguous().t(), values.t().contiguous().t(), indices.t().contiguous().t(), targets, 2.0, 0.3, "none")
+    assert torch.equal(turned, want)
+    for dtype in TYPES:
+        leaf = x[:0].to(dtype).requires_grad_()
+        losses = ldn.distillation_loss(leaf, values[:0], indices[:0], reduction="none")
+        assert losses.shape == (0,) and torch.autograd.grad(losses, leaf, losses.detach())[0].shape == (0, 50)
+        assert ldn.distillation_loss(leaf, values[:0], indices[:0], reduction="sum") == 0
+
+
+def test_a_teacher_of_all_classes_is_the_plain_loss():
+    """With every class in the list it is the Kullback-Leibler divergence, and with mix = 1 the cross-entropy, of torch in 64 bits."""
+    x, values, indices, targets, up = made(20, 60, 60, F32)
+    q = torch.log_softmax(x.double() / 3, 1)
+    p = torch.zeros_like(q).scatter_(1, indices, torch.softmax(values.double() / 3, 1))
+    want = torch.nn.functional.kl_div(q, p, reduction="batchmean") * 9
+    assert abs(ldn.distillation_loss(x, values, indices, temperature=3.0) - want) <= 1e-5 * want
+    want = torch.nn.functional.cross_entropy(x.double(), targets)
+    assert abs(ldn.distillation_loss(x, values, indices, targets, 3.0, 1.0) - want) <= 1e-5 * want
+
+
+def test_gradient_against_differences():
+    x, values, indices, targets, up = made(5, 40, 6, F32, ragged=True)
+    leaf = x.requires_grad_()
+    for tau, mix in ((1.0, 0.0), (2.0, 0.4)):
+        g, = torch.autograd.grad(ldn.distillation_loss(leaf, values, indices, targets, tau, mix, "none"), leaf, up)
+        step = torch.randn_like(x)
+        a, b = ((oracle.loss_and_gradient(x.detach().double() + s * 2 ** -10 * step, values, indices, targets, tau, mix, up)[0] * up.double()).sum()
+                for s in (1, -1))
+        assert abs((a - b) / 2 ** -9 - (g.double() * step).sum()) <= 2.0 ** -16 * (up.abs().sum() + (g * step).abs().sum())
+
+
+def test_differentiated_twice_says_so():
+    x, values, indices, targets, up = made(5, 40, 6, F32)
+    leaf = x.requires_grad_()
+    g, = torch.autograd.grad(ldn.distillation_loss(leaf, values, indices), leaf, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        g.square().sum().backward()
+
+
+def test_offsets_beyond_32_bits():
+    rows, V = 20000, 131072
+    x = torch.empty(rows, V, device="cuda", dtype=BF16).normal_()
+    values, indices = x[:, :5].clone(), torch.randint(V, (rows, 5), device="cuda")
+    targets, up = indices[:, 0].clone(), torch.zeros(rows, device="cuda")
+    up[-3:] = 1.0
+    leaf = x.requires_grad_()
+    losses = ldn.distillation_loss(leaf, values, indices, targets, 2.0, 0.3, "none")
+    dx, = torch.autograd.grad(losses, leaf, up)
+    want, bound, grad, off = oracle.loss_and_gradient(x.detach()[-3:], values[-3:], indices[-3:], targets[-3:], 2.0, 0.3, up[-3:])
+    assert head_oracle.near(losses.detach()[-3:], want, bound) and head_oracle.near(dx[-3:], grad, off) and not dx[:-3].any()
+
+
+def test_refusals():
+    x, values, indices, targets, _ = made(4, 9, 3, F32)
+    loss = ldn.distillation_loss
+    refused = [
+        lambda: loss(x.double(), values, indices), lambda: loss(x, values.double(), indices), lambda: loss(x, values, indices.int()),
+        lambda: loss(x, values[:3], indices[:3]), lambda: loss(x, values, indices[:, :2]), lambda: loss(x, values[:, :0], indices[:, :0]),
+        lambda: loss(x, values.cpu(), indices), lambda: loss(x, values, indices, targets[:3], mix=0.5), lambda: loss(x, values, indices, targets.int(), mix=0.5),
+        lambda: loss(x, values, indices, targets.float(), mix=0.5), lambda: loss(x, values, indices, temperature=0.0),
+        lambda: loss(x, values, indices, temperature=-1.0), lambda: loss(x, values, indices, temperature=math.inf),
+        lambda: loss(x, values, indices, temperature=math.nan), lambda: loss(x, values, indices, targets, mix=1.5),
+        lambda: loss(x, values, indices, targets, mix=-0.5), lambda: loss(x, values.requires_grad_(), indices), lambda: loss(x[:, :0], values, indices),
+        lambda: loss(x, torch.zeros(4, 1025, device="cuda"), torch.zeros(4, 1025, device="cuda", dtype=torch.int64)),
+        lambda: torch.vmap(lambda a: loss(a, values.detach(), indices))(x[None]),
+    ]
+    before = ldn._lib.lib.ldn_kernel_launches()
+    for attempt in refused:
+        with pytest.raises(RuntimeError):
+            attempt()
+    assert ldn._lib.lib.ldn_kernel_launches() == before

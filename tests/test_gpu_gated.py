@@ -41,3 +41,161 @@ def check(x, wg, wu, bg, bu, dy, name):
                                      (300, 1000, 520), (20, 5119, 513), (600, 2048, 1100), (1000, 10, 10), (1, 5120, 1025), (33, 1, 1)])
 def test_sizes(T, K, H, dtype):
     check(*made(T, K, H, dtype), "silu")
+
+
+@pytest.mark.parametrize("name", ["gelu", "sigmoid", "relu"])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("T, K, H", [(2, 64, 40), (70, 200, 150), (300, 136, 264)])
+def test_activations(T, K, H, dtype, name):
+    check(*made(T, K, H, dtype), name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("biases", [(False, False), (True, False), (False, True)])
+def test_biases_of_32_bits_and_absent_ones(dtype, biases):
+    for T in (3, 90):
+        check(*made(T, 96, 72, dtype, params=torch.float32, biases=biases), "silu")
+        check(*made(T, 96, 72, dtype, biases=biases), "gelu")
+
+
+def laid_out(t, layout):
+    if layout == "slice":
+        return torch.nn.functional.pad(t, (0, 5))[:, :t.size(1)]
+    if layout == "wide":
+        return torch.nn.functional.pad(t, (0, 16))[:, :t.size(1)]
+    if layout == "shifted":
+        flat = torch.empty(t.numel() + 1, device="cuda", dtype=t.dtype)
+        flat[1:] = t.reshape(-1)
+        return flat[1:].view(t.shape)
+    if layout == "transposed":
+        return t.t().contiguous().t()
+    return t[:, None].expand(-1, 2, -1)[:, 0]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("layout", ["slice", "wide", "shifted", "transposed", "one of two"])
+@pytest.mark.parametrize("T", [2, 70])
+def test_layouts(T, layout, dtype):
+    x, wg, wu, bg, bu, dy = made(T, 104, 50, dtype)
+    check(laid_out(x, layout), wg, wu, bg, bu, dy, "silu")
+    check(x, laid_out(wg, layout), wu, bg, bu, laid_out(dy, layout), "silu")
+    check(x, wg, laid_out(wu, layout), bg, bu, dy, "silu")
+
+
+def test_shapes():
+    x, wg, wu, bg, bu, dy = made(12, 40, 24, torch.float32)
+    want = ldn.gated_linear(x, wg, wu, bg, bu)
+    assert torch.equal(ldn.gated_linear(x.view(3, 4, 40), wg, wu, bg, bu), want.view(3, 4, 24))
+    assert torch.equal(ldn.gated_linear(x[0], wg, wu, bg, bu), ldn.gated_linear(x[:1], wg, wu, bg, bu)[0])
+    one = torch.randn(1, 40, device="cuda")[:, ::1].expand(9, 40)
+    assert torch.equal(ldn.gated_linear(one, wg, wu), ldn.gated_linear(one.contiguous(), wg, wu))
+    for dtype in TYPES:
+        leaves = [t.to(dtype).requires_grad_() for t in (x[:0], wg, wu, bg, bu)]
+        y = ldn.gated_linear(*leaves)
+        grads = torch.autograd.grad(y, leaves, torch.empty_like(y))
+        assert y.shape == (0, 24) and grads[0].shape == (0, 40) and not any(g.any() for g in grads[1:])
+
+
+@pytest.mark.parametrize("T", [3, 200])
+def test_gradients_that_are_asked_for_one_by_one(T):
+    for dtype in TYPES:
+        x, wg, wu, bg, bu, dy = made(T, 64, 48, dtype)
+        leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+        whole = torch.autograd.grad(ldn.gated_linear(*leaves), leaves, dy)
+        for i, t in enumerate(leaves):
+            alone = [s if s is t else s.detach() for s in leaves]
+            assert torch.equal(torch.autograd.grad(ldn.gated_linear(*alone), t, dy)[0], whole[i])
+
+
+def test_gradient_against_differences():
+    x, wg, wu, bg, bu, dy = made(6, 24, 16, torch.float32)
+    for name in ("silu", "gelu", "sigmoid", "relu"):
+        leaves = [t.detach().requires_grad_() for t in (x, wg, wu, bg, bu)]
+        grads = torch.autograd.grad(ldn.gated_linear(*leaves, activation=name), leaves, dy)
+        for i, g in enumerate(grads):
+            step = torch.randn_like(g)
+            at = [[t.detach() + (s * 2 ** -9 * step if k == i else 0) for k, t in enumerate(leaves)] for s in (1, -1)]
+            up, down = [(oracle.forward(*a, name, torch.float32)["y"] * dy.double()).sum() for a in at]
+            if name == "relu" and i in (0, 1, 3):  # (steps over a border count as far as the line on either side of it)
+                continue
+            # (third derivatives of the functions are 1 at most: 2^-18 of the size of the gradients)
+            assert abs((up - down) / 2 ** -8 - (g.double() * step).sum()) <= 2.0 ** -14 * (g.double().abs() * step.abs()).sum()
+
+
+def test_differentiated_twice_says_so():
+    x, wg, wu, bg, bu, dy = made(20, 24, 16, torch.float32)
+    leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    for wanted in leaves:
+        g, = torch.autograd.grad((ldn.gated_linear(*leaves) * dy).sum(), wanted, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            g.square().sum().backward()
+
+
+@pytest.mark.parametrize("T", [3, 150])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_rows_that_are_not_finite_stay_by_themselves(T, dtype):
+    x, wg, wu, bg, bu, dy = made(T, 72, 40, dtype)
+    want = ldn.gated_linear(x, wg, wu, bg, bu)
+    bad = x.clone()
+    bad[1, 5] = float("nan")
+    bad[0, 3] = float("inf")
+    got = ldn.gated_linear(bad, wg, wu, bg, bu)
+    assert got[1].isnan().all() and torch.equal(got[2:], want[2:])
+    if T > 8:
+        assert not got[0].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_operands_of_all_sizes(dtype):
+    """Numbers that need each image of a 32-bit operand, from the smallest to the largest."""
+    x, wg, wu, bg, bu, dy = made(40, 136, 72, dtype)
+    f = dict(device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    small, large = (-60, 60) if dtype != torch.float16 else (-6, 4)
+    scale = torch.pow(2.0, torch.randint(small, large, (40, 1), **f).float())
+    x = (x.float() * scale).to(dtype)
+    want = oracle.forward(x, wg, wu, None, None, "sigmoid", dtype)
+    got = ldn.gated_linear(x, wg, wu, activation="sigmoid")
+    assert head_oracle.near(got, want["y"], want["off_y"])
+    if dtype == torch.float32:  # (the largest numbers are rounded towards zero in their first image)
+        one = torch.full((20, 8), torch.finfo(dtype).max, device="cuda")
+        eye = torch.eye(8, device="cuda")
+        assert torch.equal(ldn.gated_linear(one, eye, eye * 0.5, activation="sigmoid"), one * 0.5)
+
+
+def test_it_repeats_itself():
+    for dtype in TYPES:
+        case = made(700, 520, 264, dtype)
+        leaves = [t.requires_grad_() for t in case[:5]]
+        runs = [(lambda y: (y.detach(),) + torch.autograd.grad(y, leaves, case[5]))(ldn.gated_linear(*leaves)) for _ in range(3)]
+        assert all(torch.equal(s, t) for r in runs[1:] for s, t in zip(runs[0], r))
+
+
+def test_offsets_beyond_32_bits():
+    T, K, H = 70001, 16, 32768
+    x, wg, wu, bg, bu, _ = made(T, K, H, torch.bfloat16)
+    leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    y = ldn.gated_linear(*leaves)
+    dy = torch.zeros_like(y)
+    dy[-3:] = torch.randn(3, H, device="cuda").bfloat16()
+    f = oracle.forward(x[-3:], wg, wu, bg, bu, "silu", torch.bfloat16)
+    assert head_oracle.near(y[-3:].detach(), f["y"], f["off_y"])
+    gx, gw = torch.autograd.grad(y, (x, wg), dy)
+    exact = oracle.backward(dy[-3:], x[-3:], wg, wu, f, "silu", torch.bfloat16)
+    assert head_oracle.near(gx[-3:], *exact["x"]) and not gx[:-3].any() and head_oracle.near(gw, *exact["w_gate"])
+
+
+def test_refusals():
+    x, wg, wu, bg, bu, _ = made(4, 8, 6, torch.float32)
+    refused = [
+        lambda: ldn.gated_linear(x.double(), wg, wu), lambda: ldn.gated_linear(x, wg.half(), wu.half()), lambda: ldn.gated_linear(x, wg, wu[:5]),
+        lambda: ldn.gated_linear(x[:, :7], wg, wu), lambda: ldn.gated_linear(x, wg[0], wu[0]), lambda: ldn.gated_linear(x, wg.cpu(), wu),
+        lambda: ldn.gated_linear(x, wg, wu, bg[:5]), lambda: ldn.gated_linear(x, wg, wu, bg.half()), lambda: ldn.gated_linear(x, wg, wu, bg.double()),
+        lambda: ldn.gated_linear(x.half(), wg.half(), wu.half(), bg.half(), bu), lambda: ldn.gated_linear(x, wg[:0], wu[:0]),
+        lambda: ldn.gated_linear(x[:, :0], wg[:, :0], wu[:, :0]), lambda: ldn.gated_linear(x[0, 0], wg, wu),
+        lambda: torch.vmap(lambda t: ldn.gated_linear(t, wg, wu))(x[None]),
+    ]
+    before = ldn._lib.lib.ldn_kernel_launches()
+    for call in refused:
+        with pytest.raises(RuntimeError):
+            call()
+    assert ldn._lib.lib.ldn_kernel_launches() == before

@@ -92,3 +92,125 @@ def test_absent_parameters(C, absent):
 def test_one_gradient_comes(C, use):
     for dtype in (F32, BF16):
         check(*made(33, C, dtype, "all", F32), use=use)
+
+
+def test_shapes_strides_and_no_rows():
+    t, dy, dh = made(12, 40, F32, "row")
+    y, h = call(t)
+    cube = {k: v.view(3, 4, -1) if k in ("x", "residual", "gate") else v for k, v in t.items()}
+    for got, want in zip(call(cube), (y, h)):
+        assert torch.equal(got, want.view(3, 4, 40))
+    turned = {k: v.t().contiguous().t() if k in ("x", "residual", "gate") else v for k, v in t.items()}
+    for got, want in zip(call(turned), (y, h)):
+        assert torch.equal(got, want)
+    for dtype in TYPES:
+        for gate in ("none", "row", "all"):
+            t, _, _ = made(3, 40, dtype, gate)
+            t = {k: v if v is None else (v[:0] if k in ("x", "residual", "gate") else v).detach().requires_grad_() for k, v in t.items()}
+            wanted = [v for v in t.values() if v is not None]
+            y, h = call(t)
+            grads = torch.autograd.grad((y, h), wanted, (torch.empty_like(y), torch.empty_like(h)))
+            assert y.shape == h.shape == (0, 40) and not any(g.any() for g in grads)
+
+
+@pytest.mark.parametrize("C", [40, 1024])
+def test_gradients_that_are_asked_for_one_by_one(C):
+    for gate in ("row", "all"):
+        t, dy, dh = made(30, C, BF16, gate, F32)
+        t = {k: v.requires_grad_() for k, v in t.items()}
+        whole = torch.autograd.grad(call(t), list(t.values()), (dy, dh))
+        for name, g in zip(t, whole):
+            alone = {k: v if k == name else v.detach() for k, v in t.items()}
+            if name in ("w", "b"):
+                got, = torch.autograd.grad(call(alone)[0], alone[name], dy)
+            else:
+                got, = torch.autograd.grad(call(alone), alone[name], (dy, dh))
+            assert torch.equal(got, g), name
+
+
+def test_gradient_against_differences():
+    for gate in ("none", "row", "all"):
+        t, dy, dh = made(5, 24, F32, gate)
+        leaves = {k: v.double().requires_grad_() for k, v in t.items() if v is not None}
+        grads = dict(zip(leaves, torch.autograd.grad(call({k: v.float() if v is not None else None for k, v in {**t, **leaves}.items()}),
+                                                      list(leaves.values()), (dy, dh))))
+
+        def value(at):
+            h, _ = oracle.forward(*[at.get(k) for k in ("x", "residual", "gate", "scale", "pw", "pb")], 1e-5)
+            y = head_oracle.norm(h, at.get("w"), at.get("b"), 1e-5)[0]
+            return (y * dy.double()).sum() + (h * dh.double()).sum()
+        for name, g in grads.items():
+            step = torch.randn_like(leaves[name])
+            up, down = (value({k: v.detach() + (s * 2 ** -10 * step if k == name else 0) for k, v in leaves.items()}) for s in (1, -1))
+            size = sum((v.abs() * torch.ones_like(v)).sum() for v in (g.abs() * step.abs(),)) + dy.double().abs().sum()
+            assert abs((up - down) / 2 ** -9 - (g * step).sum()) <= 2.0 ** -14 * size, name
+
+
+def test_differentiated_twice_says_so():
+    t, dy, dh = made(6, 40, F32, "row")
+    t = {k: v.requires_grad_() for k, v in t.items()}
+    for name in ("x", "residual", "gate", "scale", "pw", "w"):
+        y, _ = call(t)
+        g, = torch.autograd.grad((y * dy).sum(), t[name], create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            g.square().sum().backward()
+
+
+@pytest.mark.parametrize("C", [8, 96, 1001, 4096, 6001])
+def test_rows_that_are_constant_large_or_not_finite(C):
+    t, dy, dh = made(9, C, F32, "row", layout="plain")
+    t["x"][0] = 3.0             # (nothing but the first norm's bias joins the stream)
+    t["x"][1] *= 1e15
+    t["residual"][2] += 1e6
+    t["x"][3, 0] = float("nan")
+    t["residual"][4, C // 2] = float("inf")
+    t["gate"][5] = 0.0
+    t = {k: v.requires_grad_() for k, v in t.items()}
+    y, h = call(t)
+    held = {k: v.detach() for k, v in t.items()}
+    want, bound = oracle.forward(*[held[k] for k in ("x", "residual", "gate", "scale", "pw", "pb")], 1e-5)
+    good = [0, 1, 2, 5, 6, 7, 8]
+    assert head_oracle.near(h.detach()[good], want[good], bound[good])
+    assert torch.equal(h[5], held["residual"][5]) and y[[3, 4]].isnan().any(1).all() and y[good].isfinite().all()
+    gx, gr = torch.autograd.grad((y, h), (t["x"], t["residual"]), (dy, dh))
+    assert gx[good].isfinite().all() and gr[good].isfinite().all() and not gx[5].any()
+
+
+def test_offsets_beyond_32_bits():
+    rows, C = 300000, 8000
+    f = dict(device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    t = {k: torch.empty(rows, C, device="cuda", dtype=BF16).normal_(generator=f["generator"]) for k in ("x", "residual")}
+    t["gate"] = torch.rand(rows, 1, **f).to(BF16)
+    t.update({k: torch.randn(C, **f) for k in ("scale", "pw", "pb", "w", "b")})
+    t = {k: v.requires_grad_() for k, v in t.items()}
+    dy, dh = torch.zeros(2, rows, C, device="cuda", dtype=BF16)
+    dy[-5:], dh[-5:] = torch.randn(2, 5, C, **f)
+    y, h = call(t)
+    grads = dict(zip(t, torch.autograd.grad((y, h), list(t.values()), (dy, dh))))
+    few = {k: (v[-5:] if v.size(0) == rows else v).detach().requires_grad_() for k, v in t.items()}
+    y5, h5 = call(few)
+    want = dict(zip(few, torch.autograd.grad((y5, h5), list(few.values()), (dy[-5:], dh[-5:]))))
+    assert torch.equal(y[-5:], y5) and torch.equal(h[-5:], h5)
+    for name, g in grads.items():
+        if g.size(0) == rows:
+            assert torch.equal(g[-5:], want[name])
+        else:
+            assert torch.allclose(g, want[name], rtol=1e-5, atol=1e-5 * want[name].abs().max().item())
+
+
+def test_refusals():
+    t, _, _ = made(4, 8, F32, "row")
+    x, r, g, w = t["x"], t["residual"], t["gate"], t["w"]
+    refused = [
+        lambda: ldn.sandwich_norm(x.double(), r), lambda: ldn.sandwich_norm(x, r[:3]), lambda: ldn.sandwich_norm(x, r.half()),
+        lambda: ldn.sandwich_norm(x, r, w[:7]), lambda: ldn.sandwich_norm(x, r, w.half()), lambda: ldn.sandwich_norm(x, r, w.cpu()),
+        lambda: ldn.sandwich_norm(x.half(), r.half(), w.half(), post_weight=w), lambda: ldn.sandwich_norm(x, r, gate=g[:, 0]),
+        lambda: ldn.sandwich_norm(x, r, gate=g.half()), lambda: ldn.sandwich_norm(x, r, gate=torch.ones(4, 3, device="cuda")),
+        lambda: ldn.sandwich_norm(x, r, eps=-1.0), lambda: ldn.sandwich_norm(x[:, :0], r[:, :0]), lambda: ldn.sandwich_norm(x, r, scale=w[None]),
+        lambda: torch.vmap(lambda a: ldn.sandwich_norm(a, a)[0])(x[None]),
+    ]
+    before = ldn._lib.lib.ldn_kernel_launches()
+    for attempt in refused:
+        with pytest.raises(RuntimeError):
+            attempt()
+    assert ldn._lib.lib.ldn_kernel_launches() == before
