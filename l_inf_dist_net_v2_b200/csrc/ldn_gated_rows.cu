@@ -30,6 +30,19 @@ __device__ __forceinline__ void piece(const T* p, bool whole, int there, float (
     }
 }
 
+// (weights are read once: they leave the first-level cache to the rows)
+__device__ __forceinline__ uint4 load_once(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+template <class T>
+__device__ __forceinline__ void unpack8(const uint4 (&raw)[sizeof(T) / 2], float (&v)[8]) {
+    const T* e = reinterpret_cast<const T*>(raw);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_float(e[j]);
+}
+
 template <class T, int ROWS, int OUTPUTS>
 __global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_constant__ GatedArgs a, bool aligned) {
     stream_order_begin();
@@ -43,12 +56,7 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_con
         w[2 * o] = static_cast<const T*>(a.w_gate) + h * a.pitch_gate;
         w[2 * o + 1] = static_cast<const T*>(a.w_up) + h * a.pitch_up;
     }
-#pragma unroll 2
-    for (int c = threadIdx.x * 8; c < a.K; c += kFewThreads * 8) {
-        const bool whole = aligned && c + 8 <= a.K;
-        float wv[2 * OUTPUTS][8];
-#pragma unroll
-        for (int o = 0; o < 2 * OUTPUTS; ++o) piece(w[o] + c, whole, a.K - c, wv[o]);
+    auto add = [&](const float (&wv)[2 * OUTPUTS][8], int c, bool whole) {
 #pragma unroll
         for (int t = 0; t < ROWS; ++t) {
             float xv[8];
@@ -59,6 +67,35 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_con
 #pragma unroll
                 for (int j = 0; j < 8; ++j) acc[o][t] = fmaf(wv[o][j], xv[j], acc[o][t]);
         }
+    };
+    // Whole pieces, kAhead of each weight row under way at a time (two at a time, and through the cache: 26.6 us for 1, 5120 -> 5120 bf16)
+    constexpr int kStep = kFewThreads * 8, kAhead = sizeof(T) * OUTPUTS >= 8 ? 2 : 4, kWords = sizeof(T) / 2;
+    const int whole_end = aligned ? a.K / 8 * 8 : 0;
+    int c = threadIdx.x * 8;
+    for (; c < whole_end; c += kAhead * kStep) {
+        uint4 raw[kAhead][2 * OUTPUTS][kWords];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (c + u * kStep < whole_end)
+#pragma unroll
+                for (int o = 0; o < 2 * OUTPUTS; ++o)
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i) raw[u][o][i] = load_once(reinterpret_cast<const uint4*>(w[o] + c + u * kStep) + i);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (c + u * kStep < whole_end) {
+                float wv[2 * OUTPUTS][8];
+#pragma unroll
+                for (int o = 0; o < 2 * OUTPUTS; ++o) unpack8<T>(raw[u][o], wv[o]);
+                add(wv, c + u * kStep, true);
+            }
+    }
+    // what is left of a row, or all of it where rows are not aligned
+    for (c = whole_end + threadIdx.x * 8; c < a.K; c += kStep) {
+        float wv[2 * OUTPUTS][8];
+#pragma unroll
+        for (int o = 0; o < 2 * OUTPUTS; ++o) piece(w[o] + c, false, a.K - c, wv[o]);
+        add(wv, c, false);
     }
 #pragma unroll
     for (int o = 0; o < 2 * OUTPUTS; ++o)

@@ -32,7 +32,7 @@ int resident_pairs(const DeviceCtx* ctx) {
 int steps_over(long long n, int size) { return static_cast<int>((n + size - 1) / size); }
 
 // The tiles behind the last whole round are shared out in equal ranges where that saves more than storing and adding up the parts costs
-// (both in clocks: a step takes 260, a pair stores and another kernel reads 1 KB per row of a part at 4000 bytes per clock).
+// (both in clocks: a step takes 512, a pair stores and another kernel reads 1 KB per row of a part at 4000 bytes per clock).
 void plan(GatedForm form, long long M, int N, int terms, int type, const DeviceCtx* ctx, TileArgs* a) {
     const bool parted = type == LDN_F32;
     const int unit_steps = parted ? kUnitSteps<float> : 1;
@@ -50,7 +50,7 @@ void plan(GatedForm form, long long M, int N, int terms, int type, const DeviceC
     const int rest = a->tiles % a->pairs;
     a->whole = a->tiles;
     if (rest) {
-        const double tile = static_cast<double>(a->units) * unit_steps * (parted ? 6 : 1) * 260.0;
+        const double tile = static_cast<double>(a->units) * unit_steps * (parted ? 6 : 1) * 512.0;
         const double rows = M < kSide ? static_cast<double>(M) : kSide;
         if (tile * (1.0 - static_cast<double>(rest) / a->pairs) > 5000.0 + (a->pairs + rest) * rows * 2048.0 / 4000.0) a->whole = a->tiles - rest;
         else if (a->tiles < a->pairs) a->pairs = a->tiles;
