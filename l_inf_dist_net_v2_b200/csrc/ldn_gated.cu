@@ -300,7 +300,7 @@ extern "C" LDN_API int ldn_gated_linear(const void* x, long long pitch, long lon
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const GatedArgs a = {x, pitch, w_gate, w_up, pitch_gate, pitch_up, b_gate, b_up, param_type == LDN_F32, rows, K, H, activation, y, g, u,
                          pitch_saved};
-    if (gated_is_few(a, type)) return launch_gated_few(a, type, ctx, st);
+    if (gated_is_few(a, type)) return launch_gated_few(a, type, st);
     Operands o{type};
     o.add(x, pitch, rows, K);
     o.add(w_gate, pitch_gate, H, K);

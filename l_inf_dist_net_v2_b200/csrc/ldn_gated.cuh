@@ -25,7 +25,7 @@ inline bool gated_activation(int a) { return a == LDN_RELU || a == LDN_SILU || a
 
 // A handful of rows, without tensor cores (ldn_gated_rows.cu)
 bool gated_is_few(const GatedArgs& a, int type);
-int launch_gated_few(const GatedArgs& a, int type, const DeviceCtx* ctx, cudaStream_t st);
+int launch_gated_few(const GatedArgs& a, int type, cudaStream_t st);
 
 // ---- products on the tensor cores (ldn_gated_tiles.cu) --------------------------------------------------------------------------
 // An operand as the tensor cores' loads want it: [image][row][pitch] of 16 bits, rows at multiples of 16 bytes.  32-bit operands are three

@@ -8,7 +8,6 @@ namespace ldn {
 namespace {
 
 constexpr int kFewThreads = 128;
-constexpr int kFewRows = 8;
 
 // A piece of eight elements, `there` of them in the row
 template <class T>
@@ -126,26 +125,38 @@ __global__ void __launch_bounds__(kFewThreads) gated_few_kernel(const __grid_con
     }
 }
 
+// (a block's outputs, 1 / 2: 1 row 5120 -> 5120 bf16 21.5 / 20.2 us; 128 threads, 64: 21.0, 256: 23.2 with one output each)
+constexpr int kOutputs = 2;
 template <class T, int ROWS>
 int launch(const GatedArgs& a, bool aligned, cudaStream_t st) {
-    constexpr int kOutputs = ROWS >= 4 ? 2 : 1;
     return launch_after(gated_few_kernel<T, ROWS, kOutputs>, (a.H + kOutputs - 1) / kOutputs, kFewThreads, 0, st, a, aligned);
 }
 bool at_16(const void* p, long long pitch, long long rows, int size) {
     return ((reinterpret_cast<uintptr_t>(p) | (rows > 1 ? static_cast<uintptr_t>(pitch) * size : 0)) & 15u) == 0;
 }
+bool all_at_16(const GatedArgs& a, int size) {
+    return at_16(a.x, a.pitch_x, a.T, size) && at_16(a.w_gate, a.pitch_gate, a.H, size) && at_16(a.w_up, a.pitch_up, a.H, size);
+}
 
 }  // namespace
 
-bool gated_is_few(const GatedArgs& a, int type) { return a.T <= kFewRows; }
+// Where the tensor cores take longer.  5120 -> 5120, us, here / there: bf16 1 row 20 / 29, 2 rows 22 / 29, 4 rows 33 / 29; one row of 5119, whose
+// weights would be copied, 37; float32, whose weights would be written as three images, 8 rows 69 / 182.
+bool gated_is_few(const GatedArgs& a, int type) {
+    return a.T <= (type == LDN_F32 ? 16 : all_at_16(a, size_of(type)) ? 2 : 4);
+}
 
-int launch_gated_few(const GatedArgs& a, int type, const DeviceCtx* ctx, cudaStream_t st) {
-    const int size = size_of(type);
-    const bool aligned = at_16(a.x, a.pitch_x, a.T, size) && at_16(a.w_gate, a.pitch_gate, a.H, size) && at_16(a.w_up, a.pitch_up, a.H, size);
+int launch_gated_few(const GatedArgs& a, int type, cudaStream_t st) {
+    const bool aligned = all_at_16(a, size_of(type));
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        return a.T == 1 ? launch<T, 1>(a, aligned, st) : a.T == 2 ? launch<T, 2>(a, aligned, st)
-             : a.T <= 4 ? launch<T, 4>(a, aligned, st) : launch<T, 8>(a, aligned, st);
+        if (a.T <= 1) return launch<T, 1>(a, aligned, st);
+        if (a.T <= 2) return launch<T, 2>(a, aligned, st);
+        if constexpr (sizeof(T) == 4) {
+            if (a.T > 8) return launch<T, 16>(a, aligned, st);
+            if (a.T > 4) return launch<T, 8>(a, aligned, st);
+        }
+        return launch<T, 4>(a, aligned, st);
     });
 }
 
