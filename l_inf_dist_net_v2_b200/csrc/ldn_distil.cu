@@ -97,8 +97,19 @@ struct Pieces {
 };
 
 // 2 N values, two at a time
+// How a row's sums are made: at both temperatures where it has a label and tau is not 1; `squares`: where tau is 2 or 4, e^d is
+// e^(d / tau) squared once or twice (32-bit products beside powers of two, of which an SM makes 16 per clock: with a second
+// one, 8192 x 40001 bf16 took 215 us, with one 152)
+struct Way {
+    float c, c1;
+    bool second;
+    int squares;
+    __device__ __forceinline__ explicit Way(const DistilArgs& a)
+        : c(kLog2e / a.tau), c1(kLog2e), second(a.targets && a.tau != 1.0f), squares(a.tau == 2.0f ? 1 : a.tau == 4.0f ? 2 : 0) {}
+};
 template <int N>
-__device__ __forceinline__ void add_values(Sums& a, const float2 (&v)[N], float c, float c1, bool second) {
+__device__ __forceinline__ void add_values(Sums& a, const float2 (&v)[N], const Way& way) {
+    const float c = way.c, c1 = way.c1;
     float top = largest_of(v[0].x, v[0].y);
 #pragma unroll
     for (int i = 1; i < N; ++i) asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(top) : "f"(top), "f"(v[i].x), "f"(v[i].y));
@@ -110,13 +121,27 @@ __device__ __forceinline__ void add_values(Sums& a, const float2 (&v)[N], float 
     if (a.m == minus_infinity()) return;
     const float2 m = make_float2(-a.m, -a.m), by = make_float2(c, c);
     float2 sum = make_float2(0.0f, 0.0f);
+    if (way.second && way.squares) {
+        float2 sum1 = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float2 d = __fmul2_rn(__fadd2_rn(v[i], m), by), e = make_float2(exp2_fast(d.x), exp2_fast(d.y));
+            float2 q = __fmul2_rn(e, e);
+            if (way.squares == 2) q = __fmul2_rn(q, q);
+            sum = __fadd2_rn(sum, e);
+            sum1 = __fadd2_rn(sum1, q);
+        }
+        a.s += sum.x + sum.y;
+        a.s1 += sum1.x + sum1.y;
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const float2 d = __fmul2_rn(__fadd2_rn(v[i], m), by);
         sum = __fadd2_rn(sum, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
     }
     a.s += sum.x + sum.y;
-    if (second) {
+    if (way.second) {
         const float2 by1 = make_float2(c1, c1);
         sum = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -165,21 +190,36 @@ struct List {
 template <class T, int LANES>
 __device__ __forceinline__ List read_list(const DistilArgs& a, long long row, float* slots) {
     constexpr int kWarps = LANES > 32 ? LANES / 32 : 0;  // (a block's rounds have slots of their own)
+    constexpr int kHeld = LANES > 32 ? 1 : 4;            // a lane's first entries: asked for together, and kept
     const int lane = threadIdx.x & (LANES - 1);
     const T* x = static_cast<const T*>(a.x) + row * a.pitch;
     const long long *indices = a.indices + row * a.k, target = a.targets ? a.targets[row] : -1;
     const float inv_tau = 1.0f / a.tau;
-    // (a lane's first entry stays in registers: lists are short)
-    const bool mine = lane < a.k;
-    const long long i0 = mine ? indices[lane] : -1;
-    const float v0 = mine ? value_at(a, row * a.k + lane) * inv_tau : 0.0f;
-    const bool fine0 = i0 >= 0 && i0 < a.V;
-    const float x0 = fine0 ? to_float(x[i0]) : minus_infinity();
+    float bad = target >= a.V ? 1.0f : 0.0f, top = minus_infinity(), reference = minus_infinity();
+    bool there[kHeld];
+    float v[kHeld], at[kHeld];
+    long long index[kHeld];
+#pragma unroll
+    for (int e = 0; e < kHeld; ++e) {
+        const int j = lane + e * LANES;
+        index[e] = j < a.k ? indices[j] : -1;
+        v[e] = j < a.k ? value_at(a, row * a.k + j) * inv_tau : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < kHeld; ++e) {
+        there[e] = index[e] >= 0;
+        if (index[e] >= a.V) bad = 1.0f;
+        at[e] = there[e] && index[e] < a.V ? to_float(x[index[e]]) : minus_infinity();
+    }
     List l;
     l.target = target >= 0 && target < a.V ? to_float(x[target]) : 0.0f;
     l.label = target >= 0;
-    float bad = (mine && i0 >= a.V) || target >= a.V ? 1.0f : 0.0f, top = i0 >= 0 ? v0 : minus_infinity(), reference = x0;
-    for (int j = lane + LANES; j < a.k; j += LANES) {
+#pragma unroll
+    for (int e = 0; e < kHeld; ++e) {
+        if (there[e]) top = largest_of(top, v[e]);
+        reference = largest_of(reference, at[e]);
+    }
+    for (int j = lane + kHeld * LANES; j < a.k; j += LANES) {
         const long long i = indices[j];
         if (i >= a.V) bad = 1.0f;
         if (i >= 0) top = largest_of(top, value_at(a, row * a.k + j) * inv_tau);
@@ -189,21 +229,27 @@ __device__ __forceinline__ List read_list(const DistilArgs& a, long long row, fl
     l.top = top = over_row<LANES>(top, Largest(), slots + kWarps);
     l.reference = reference = over_row<LANES>(reference, Largest(), slots + 2 * kWarps);
     l.some = top != minus_infinity();  // (a list of nothing but minus infinity says nothing)
-    float sum = l.some && i0 >= 0 ? expf(v0 - top) : 0.0f;
-    if (l.some)
-        for (int j = lane + LANES; j < a.k; j += LANES)
+    float sum = 0.0f;
+    if (l.some) {
+#pragma unroll
+        for (int e = 0; e < kHeld; ++e)
+            if (there[e]) sum += expf(v[e] - top);
+        for (int j = lane + kHeld * LANES; j < a.k; j += LANES)
             if (indices[j] >= 0) sum += expf(value_at(a, row * a.k + j) * inv_tau - top);
+    }
     sum = over_row<LANES>(sum, Plus(), slots + 3 * kWarps);
     l.inv_sum = 1.0f / sum;
     const float log_sum = logf(sum);
-    auto term = [&](float v, float at) {
-        const float t = v - top, p = expf(t) * l.inv_sum;
-        return p != 0.0f ? p * ((t - log_sum) - (at - reference) * inv_tau) : 0.0f;
+    auto term = [&](float value, float logit) {
+        const float t = value - top, p = expf(t) * l.inv_sum;
+        return p != 0.0f ? p * ((t - log_sum) - (logit - reference) * inv_tau) : 0.0f;
     };
     float terms = 0.0f;
     if (l.some && !l.bad) {
-        if (fine0) terms = term(v0, x0);
-        for (int j = lane + LANES; j < a.k; j += LANES)
+#pragma unroll
+        for (int e = 0; e < kHeld; ++e)
+            if (there[e]) terms += term(v[e], at[e]);
+        for (int j = lane + kHeld * LANES; j < a.k; j += LANES)
             if (indices[j] >= 0) terms += term(value_at(a, row * a.k + j) * inv_tau, to_float(x[indices[j]]));
     }
     l.terms = over_row<LANES>(terms, Plus(), slots + 4 * kWarps);
@@ -233,8 +279,8 @@ constexpr int kShortEntries = 128;  // of a list, in the backward pass
 // 8192 x 40001 bf16 178 us); those at a row's cut ends, element by element, come last.
 // meanwhile: what is done with the first four under way.
 template <class T, class F>
-__device__ __forceinline__ void read_pieces(const Pieces<T>& p, int first, int last, int thread, int threads, float c, float c1, bool second,
-                                            Sums& sums, F meanwhile) {
+__device__ __forceinline__ void read_pieces(const Pieces<T>& p, int first, int last, int thread, int threads, const Way& way, Sums& sums,
+                                            F meanwhile) {
     constexpr int H = Pieces<T>::N / 2;
     if (first >= last) {
         meanwhile();
@@ -257,22 +303,22 @@ __device__ __forceinline__ void read_pieces(const Pieces<T>& p, int first, int l
         j += kAhead * threads;
         more = j + (kAhead - 1) * threads < end;
         if (more) load();
-        add_values(sums, v, c, c1, second);
+        add_values(sums, v, way);
     }
     for (; j < end; j += threads) {
         float2 v[H];
         Pieces<T>::unpack(p.load(j), v);
-        add_values(sums, v, c, c1, second);
+        add_values(sums, v, way);
     }
     if (begin > first && thread == 0) {
         float2 v[H];
         p.edge(first, minus_infinity(), v);
-        add_values(sums, v, c, c1, second);
+        add_values(sums, v, way);
     }
     if (end < last && last - 1 >= begin && thread == 1) {
         float2 v[H];
         p.edge(last - 1, minus_infinity(), v);
-        add_values(sums, v, c, c1, second);
+        add_values(sums, v, way);
     }
 }
 
@@ -280,8 +326,7 @@ template <class T, int LANES>
 __global__ void __launch_bounds__(kDistilThreads, 3) distil_short_kernel(const __grid_constant__ DistilArgs a) {
     stream_order_begin();
     constexpr int kRows = kDistilThreads / LANES;
-    const float c = kLog2e / a.tau, c1 = kLog2e;
-    const bool second = a.targets && a.tau != 1.0f;
+    const Way way(a);
     const int lane = threadIdx.x & (LANES - 1);
     for (long long row0 = static_cast<long long>(blockIdx.x) * kRows; row0 < a.rows; row0 += static_cast<long long>(gridDim.x) * kRows) {
         const bool there = row0 + threadIdx.x / LANES < a.rows;  // (lanes without a row of their own go along with the last one)
@@ -289,12 +334,12 @@ __global__ void __launch_bounds__(kDistilThreads, 3) distil_short_kernel(const _
         const Pieces<T> p(static_cast<const T*>(a.x) + row * a.pitch, a.V);
         Sums sums = {minus_infinity(), 0.0f, 0.0f};
         List list;
-        read_pieces(p, 0, p.count, lane, LANES, c, c1, second, sums, [&] {
+        read_pieces(p, 0, p.count, lane, LANES, way, sums, [&] {
             __syncwarp();
             list = read_list<T, LANES>(a, row, nullptr);
         });
         __syncwarp();
-        sums.over_lanes(LANES, c, c1);
+        sums.over_lanes(LANES, way.c, way.c1);
         if (lane == 0 && there) finish_row(a, row, list, sums);
     }
 }
@@ -306,8 +351,7 @@ __global__ void __launch_bounds__(kDistilThreads, 4) distil_long_kernel(const __
     __shared__ Sums of_warps[kDistilWarps], of_ranks[kMostRanks];
     __shared__ float slots[5 * kDistilWarps];
     __shared__ List list;
-    const float c = kLog2e / a.tau, c1 = kLog2e;
-    const bool second = a.targets && a.tau != 1.0f;
+    const Way way(a);
     const uint32_t rank = cluster_rank(), ranks = cluster_size();
     const long long row = blockIdx.x / ranks;
     if (ranks > 1) cluster_barrier();  // (the first CTA is there to be written to)
@@ -315,18 +359,18 @@ __global__ void __launch_bounds__(kDistilThreads, 4) distil_long_kernel(const __
     const Pieces<T> p(static_cast<const T*>(a.x) + row * a.pitch, a.V);
     Sums sums = {minus_infinity(), 0.0f, 0.0f};
     read_pieces(p, static_cast<int>(static_cast<long long>(p.count) * rank / ranks), static_cast<int>(static_cast<long long>(p.count) * (rank + 1) / ranks),
-                threadIdx.x, kDistilThreads, c, c1, second, sums, [&] {
+                threadIdx.x, kDistilThreads, way, sums, [&] {
                     if (rank != 0) return;
                     const List l = read_list<T, kDistilThreads>(a, row, slots);
                     if (threadIdx.x == 0) list = l;
                 });
     __syncwarp();
-    sums.over_lanes(32, c, c1);
+    sums.over_lanes(32, way.c, way.c1);
     if (lane == 0) of_warps[warp] = sums;
     __syncthreads();
     if (warp == 0) {
         sums = lane < kDistilWarps ? of_warps[lane] : Sums{minus_infinity(), 0.0f, 0.0f};
-        sums.over_lanes(kDistilWarps, c, c1);
+        sums.over_lanes(kDistilWarps, way.c, way.c1);
         if (ranks > 1 && lane == 0) {
             const uint32_t to = in_cta(&of_ranks[rank], 0);
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(sums.m) : "memory");
@@ -339,10 +383,147 @@ __global__ void __launch_bounds__(kDistilThreads, 4) distil_long_kernel(const __
         cluster_barrier();
         if (rank == 0 && warp == 0) {
             sums = lane < static_cast<int>(ranks) ? of_ranks[lane] : Sums{minus_infinity(), 0.0f, 0.0f};
-            sums.over_lanes(kMostRanks, c, c1);
+            sums.over_lanes(kMostRanks, way.c, way.c1);
         }
     }
     if (rank == 0 && threadIdx.x == 0) finish_row(a, row, list, sums);
+}
+
+// Many long rows: blocks that take rows in turn and have the next 16 KB pieces of them under way whatever the row that they are of, so that
+// nothing waits while a row ends.  A warp fetches, eight add up, one reads the lists and makes the losses.
+constexpr int kRingStages = 6, kRingPieces = 1024, kRingBytes = kRingPieces * 16;
+constexpr int kRingThreads = kDistilThreads + 64;
+constexpr int kRingEntries = 128;  // of a list that one warp reads while a row comes
+struct RingBarriers {
+    uint64_t full[kRingStages], empty[kRingStages], added[2], taken[2];
+};
+constexpr int kRingSmem = kRingStages * kRingBytes + 128;
+__device__ __forceinline__ void fetch_bytes(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+template <class T>
+__global__ void __launch_bounds__(kRingThreads, 2) distil_ring_kernel(const __grid_constant__ DistilArgs a, int* status) {
+    extern __shared__ char raw[];
+    char* ring = raw + ((128 - (smem_u32(raw) & 127)) & 127);
+    __shared__ RingBarriers B;
+    __shared__ Sums of_warps[2][kDistilWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kRingStages; ++s) {
+            mbar_init(&B.full[s], 1);
+            mbar_init(&B.empty[s], kDistilWarps);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&B.added[s], kDistilWarps);
+            mbar_init(&B.taken[s], 1);
+        }
+        mbar_fence_init();
+    }
+    __syncthreads();
+    stream_order_begin();
+    constexpr int H = Pieces<T>::N / 2;
+    const Way way(a);
+    auto give_up = [&] { atomicExch(status, static_cast<int>(kDeviceTimeout)); };
+    // a row's whole pieces (those at its cut ends are the last warp's)
+    auto whole_of = [](const Pieces<T>& p, int& begin, int& end) {
+        begin = p.whole(0) ? 0 : 1;
+        end = p.whole(p.count - 1) ? p.count : p.count - 1;
+    };
+    auto pieces_of = [&](long long row) { return Pieces<T>(static_cast<const T*>(a.x) + row * a.pitch, a.V); };
+    RingPlace<kRingStages> at;
+    if (warp == kDistilWarps) {
+        if (elected()) {
+            long long i = 0;
+            bool fine = true;
+            for (long long row = blockIdx.x; row < a.rows && fine; row += gridDim.x) {
+                const Pieces<T> p = pieces_of(row);
+                int j, end;
+                whole_of(p, j, end);
+                for (; j < end; j += kRingPieces, ++i, at.next()) {
+                    if (i >= kRingStages && !mbar_wait_bounded(&B.empty[at.stage], at.parity ^ 1)) {
+                        fine = false;
+                        give_up();
+                        break;
+                    }
+                    const uint32_t bytes = static_cast<uint32_t>(end - j < kRingPieces ? end - j : kRingPieces) * 16;
+                    mbar_expect_tx(&B.full[at.stage], bytes);
+                    fetch_bytes(ring + at.stage * kRingBytes, p.row + p.first(j), bytes, &B.full[at.stage]);
+                }
+            }
+            for (long long k = i < kRingStages ? 0 : i - kRingStages; k < i; ++k)  // (no copy is in flight when the block ends)
+                if (!mbar_wait_bounded(&B.full[k % kRingStages], (k / kRingStages) & 1)) give_up();
+        }
+    } else if (warp < kDistilWarps) {
+        int n = 0;
+        bool fine = true;
+        for (long long row = blockIdx.x; row < a.rows && fine; row += gridDim.x, ++n) {
+            const Pieces<T> p = pieces_of(row);
+            int j, end;
+            whole_of(p, j, end);
+            Sums sums = {minus_infinity(), 0.0f, 0.0f};
+            for (; j < end && fine; j += kRingPieces, at.next()) {
+                fine = __all_sync(0xffffffffu, mbar_wait_bounded(&B.full[at.stage], at.parity));
+                if (!fine) break;
+                const uint4* from = reinterpret_cast<const uint4*>(ring + at.stage * kRingBytes) + threadIdx.x;
+                const int left = end - j - static_cast<int>(threadIdx.x);
+                static_assert(kRingPieces == kAhead * kDistilThreads, "four pieces per thread");
+                if (left > (kAhead - 1) * kDistilThreads) {
+                    float2 v[kAhead * H];
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) Pieces<T>::unpack(from[u * kDistilThreads], v + u * H);
+                    add_values(sums, v, way);
+                } else {
+#pragma unroll 1
+                    for (int u = 0; u * kDistilThreads < left; ++u) {
+                        float2 v[H];
+                        Pieces<T>::unpack(from[u * kDistilThreads], v);
+                        add_values(sums, v, way);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) arrive(&B.empty[at.stage]);
+            }
+            sums.over_lanes(32, way.c, way.c1);
+            if (n >= 2 && fine) fine = __all_sync(0xffffffffu, mbar_wait_bounded(&B.taken[n & 1], (n / 2 - 1) & 1));
+            if (lane == 0 && fine) {
+                of_warps[n & 1][warp] = sums;
+                arrive(&B.added[n & 1]);
+            }
+        }
+        if (!fine) give_up();
+    } else {
+        int n = 0;
+        for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, ++n) {
+            const Pieces<T> p = pieces_of(row);
+            // the elements at the row's ends that are in no whole piece
+            int begin, end;
+            whole_of(p, begin, end);
+            const int head = begin ? (p.first(1) < a.V ? p.first(1) : a.V) : 0, tail = end < p.count && end >= begin ? p.first(end) : a.V;
+            const int mine = lane < 16 ? lane : tail + lane - 16;
+            const bool there = lane < 16 ? mine < head : mine < a.V;
+            const float e = there ? to_float(p.row[mine]) : minus_infinity();
+            const float one = e == minus_infinity() ? 0.0f : exp2_fast(e - e);  // (not a number for infinity, as in a whole piece)
+            Sums sums = {e, one, one};
+            const List list = read_list<T, 32>(a, row, nullptr);
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&B.added[n & 1], (n / 2) & 1))) {
+                give_up();
+                break;
+            }
+            if (lane < kDistilWarps) {
+                const Sums w = of_warps[n & 1][lane];
+                sums.join(w.m, w.s, w.s1, way.c, way.c1);
+            }
+            __syncwarp();
+            if (lane == 0) arrive(&B.taken[n & 1]);
+            sums.over_lanes(32, way.c, way.c1);
+            if (lane == 0) finish_row(a, row, list, sums);
+        }
+    }
 }
 
 // The rows' losses in a fixed order
@@ -535,6 +716,15 @@ extern "C" LDN_API int ldn_distillation(const void* x, long long pitch, long lon
                 return with_lanes(lanes, [&](auto n) {
                     return launch_after(distil_short_kernel<T, decltype(n)::value>, short_blocks(rows, lanes, ctx), kDistilThreads, 0, st, a);
                 });
+            if (rows >= 4LL * ctx->sm_count && k <= kRingEntries) {
+                constexpr auto kernel = distil_ring_kernel<T>;
+                static OncePerDevice once;
+                int s = once([] { return allow_smem(kernel, kRingSmem); });
+                Scratch scratch;  // (for the status word)
+                if (s == kOk) s = scratch.take(st, 0);
+                if (s != kOk) return s;
+                return launch_after(kernel, static_cast<unsigned>(2 * ctx->sm_count), kRingThreads, kRingSmem, st, a, scratch.status);
+            }
             // as many CTAs per row as it takes to fill the device twice, each with 4096 classes at least
             int ranks = 1;
             while (ranks < kMostRanks && rows * ranks < 2LL * ctx->sm_count && V / (2 * ranks) >= 4096) ranks *= 2;

@@ -70,7 +70,9 @@ __device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, uint
 
 // What a pair of CTAs takes: whole tiles in turn, then its range of the units of the others.
 __host__ __device__ __forceinline__ long long range_begin(const TileArgs& a, int pair) {
-    return static_cast<long long>(a.tiles - a.whole) * a.units * pair / a.pairs;
+    const long long all = static_cast<long long>(a.tiles - a.whole) * a.units;
+    if (all < (1 << 24)) return static_cast<unsigned>(all) * static_cast<unsigned>(pair) / static_cast<unsigned>(a.pairs);  // (129 pairs at most)
+    return all * pair / a.pairs;
 }
 struct Segments {
     int next_whole, tile, first, last, slot, later;
@@ -415,8 +417,8 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 
 // The parts of a tile that several pairs share, added up in the order of their terms; a block has four rows of a tile, a thread four columns.
 // Which pairs have a part is found by a thread each, and four parts are under way at a time (found and loaded one after the other, 15 parts
-// of 64 rows took 29 us).
-constexpr int kFixRows = 4, kMostPairs = 128;
+// of 64 rows took 29 us; four at a time 11, eight 14).
+constexpr int kFixRows = 4, kFixAhead = 4, kMostPairs = 128;
 template <GatedForm F>
 constexpr int kFixRuns = F == GatedForm::Forward ? 32 : 64;  // of four columns
 template <class T, GatedForm F>
@@ -452,10 +454,10 @@ __global__ void __launch_bounds__(kFixRows * kFixRuns<F>) gated_parts_kernel(con
     if (m >= a.M || n >= a.N) return;
     const float* from = a.partials + static_cast<size_t>(row) * kSide + 4 * run;
     float v0[4] = {}, v1[4] = {};
-    for (int q0 = first; q0 <= last; q0 += 4) {
-        float4 s[4], t[4];
+    for (int q0 = first; q0 <= last; q0 += kFixAhead) {
+        float4 s[kFixAhead], t[kFixAhead];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kFixAhead; ++j) {
             const int slot = q0 + j <= last ? slots[q0 + j] : -1;
             s[j] = t[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (slot >= 0) {
@@ -465,7 +467,7 @@ __global__ void __launch_bounds__(kFixRows * kFixRuns<F>) gated_parts_kernel(con
             }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kFixAhead; ++j) {
             v0[0] += s[j].x; v0[1] += s[j].y; v0[2] += s[j].z; v0[3] += s[j].w;
             if constexpr (kGated) { v1[0] += t[j].x; v1[1] += t[j].y; v1[2] += t[j].z; v1[3] += t[j].w; }
         }

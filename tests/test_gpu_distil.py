@@ -185,3 +185,25 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             attempt()
     assert ldn._lib.lib.ldn_kernel_launches() == before
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows, V, k", [(600, 8193, 5), (1000, 3001, 128), (777, 10007, 129), (4000, 8200, 33), (650, 33000, 1)])
+def test_many_long_rows(rows, V, k, dtype):
+    check(*made(rows, V, k, dtype, ragged=True), 1.0, 0.3)
+    check(*made(rows, V, k, dtype, layout="slice"), 2.0, 0.0)
+    x, values, indices, targets, up = made(rows, V, k, dtype, masked=True, layout="shifted")
+    x[1], x[2, V // 2:], x[rows - 1, :V - 1] = -math.inf, -math.inf, -math.inf
+    x[3, 0], x[4, V - 1], x[5, 17] = math.nan, math.inf, math.nan
+    indices[1], targets[1] = -1, -1
+    indices[2], targets[2] = torch.arange(k, device="cuda"), 1
+    indices[rows - 1], targets[rows - 1] = -1, V - 1
+    indices[rows - 1, 0] = V - 1
+    losses = ldn.distillation_loss(x, values, indices, targets, 2.0, 0.3, "none")
+    assert losses[3:6].isnan().all() and losses[1] == 0
+    keep = [0, 2] + list(range(6, rows))
+    want, bound, _, _ = oracle.loss_and_gradient(x[keep], values[keep], indices[keep], targets[keep], 2.0, 0.3, up[keep])
+    # (the last row's only class may be one that is no choice: a row of nothing but minus infinity with a label is not a number)
+    some = torch.tensor([bool((x[i] > -math.inf).any()) for i in keep], device="cuda")
+    assert torch.equal(losses[keep].isfinite(), some) and losses[keep][~some].isnan().all()
+    assert head_oracle.near(losses[keep][some], want[some], bound[some])
