@@ -426,17 +426,25 @@ LDN_API int ldn_int8_linear_float(const void* x, long long pitch, int x_type, co
 #define LDN_SIGMOID 5
 LDN_API int ldn_gated_linear(const void* x, long long pitch, long long rows, int K, int H, int type, const void* w_gate,
                              long long pitch_gate, const void* w_up, long long pitch_up, const void* b_gate, const void* b_up,
-                             int param_type, int activation, void* y, float* g, float* u, long long pitch_saved, ldn_stream_t stream);
+                             int param_type, int activation, void* y, float* g, float* u, long long pitch_saved, void* images,
+                             ldn_stream_t stream);
+
+/*
+ * Bytes of `images`, in which ldn_gated_linear may leave float32 operands as it multiplies them, so that the backward pass need not make
+ * them again (6 bytes per element of x and of both weights, at a multiple of 256 bytes); 0 where it has none to leave: pass NULL then.
+ */
+LDN_API unsigned long long ldn_gated_image_bytes(long long rows, int K, int H, int type);
 
 /*
  * Gradients of ldn_gated_linear: with dg = grad_y u act'(g) and du = grad_y act(g) (rounded to `type` in products),
  *   grad_x = dg w_gate + du w_up,  grad_w_gate = dg' x,  grad_w_up = du' x,  grad_b_gate and grad_b_up the column sums of dg and du.
  * grad_y and the results are contiguous; grad_x, both of the weights' gradients, and either of the biases' may be NULL.  Sums are taken
- * in a fixed order (no atomics).  rows == 0 sets the weights' and biases' to zero.
+ * in a fixed order (no atomics).  rows == 0 sets the weights' and biases' to zero.  images: what the forward pass left of the same x and
+ * weights, or NULL.
  */
 LDN_API int ldn_gated_linear_backward(const void* grad_y, const void* x, long long pitch, long long rows, int K, int H, int type,
                                       const void* w_gate, long long pitch_gate, const void* w_up, long long pitch_up, const float* g,
-                                      const float* u, long long pitch_saved, int activation, void* grad_x, void* grad_w_gate,
+                                      const float* u, long long pitch_saved, const void* images, int activation, void* grad_x, void* grad_w_gate,
                                       void* grad_w_up, void* grad_b_gate, void* grad_b_up, int param_type, ldn_stream_t stream);
 
 /*

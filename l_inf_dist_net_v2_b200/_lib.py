@@ -61,8 +61,8 @@ SIGNATURES = {
     "ldn_layer_norm_quantized": [_p, _l, _l, _i, _i, _p, _p, _i, _f, _p, _l, _p, _s],
     "ldn_int8_linear": [_p, _l, _p, _p, _l, _p, _p, _l, _i, _i, _i, _p, _i, _s],
     "ldn_int8_linear_float": [_p, _l, _i, _p, _l, _p, _p, _l, _i, _i, _i, _p, _i, _s],
-    "ldn_gated_linear": [_p, _l, _l, _i, _i, _i, _p, _l, _p, _l, _p, _p, _i, _i, _p, _p, _p, _l, _s],
-    "ldn_gated_linear_backward": [_p, _p, _l, _l, _i, _i, _i, _p, _l, _p, _l, _p, _p, _l, _i, _p, _p, _p, _p, _p, _i, _s],
+    "ldn_gated_linear": [_p, _l, _l, _i, _i, _i, _p, _l, _p, _l, _p, _p, _i, _i, _p, _p, _p, _l, _p, _s],
+    "ldn_gated_linear_backward": [_p, _p, _l, _l, _i, _i, _i, _p, _l, _p, _l, _p, _p, _l, _p, _i, _p, _p, _p, _p, _p, _i, _s],
     "ldn_sandwich_norm": [_p, _l, _p, _l, _p, _l, _i, _l, _i, _i] + [_p] * 5 + [_i, _f, _p, _p, _p, _s],
     "ldn_sandwich_norm_backward": [_p, _p, _p, _l, _p, _p, _l, _i, _l, _i, _i] + [_p] * 4 + [_i] + [_p] * 9 + [_s],
     "ldn_distillation": [_p, _l, _l, _i, _i, _p, _i, _p, _i, _p, _f, _f, _f, _p, _p, _f, _p, _s],
@@ -76,7 +76,8 @@ SIGNATURES = {
     "ldn_probe_pipe": [_i, _i, _c_float_p, ctypes.c_void_p, _s],
 }
 OTHER_SYMBOLS = ["ldn_status_string", "ldn_version", "ldn_set_max_ctas", "ldn_kernel_launches", "ldn_set_trace_buffer",
-                 "ldn_enable_kernel_timing", "ldn_last_tile_kernel_ms", "ldn_set_fused_scratch_limit", "ldn_set_bound_one_pass_limit"]
+                 "ldn_enable_kernel_timing", "ldn_last_tile_kernel_ms", "ldn_set_fused_scratch_limit", "ldn_set_bound_one_pass_limit",
+                 "ldn_gated_image_bytes"]
 
 
 class LdnError(RuntimeError):
@@ -109,6 +110,8 @@ def load(path=LIB_PATH):
     lib.ldn_last_tile_kernel_ms.restype = ctypes.c_float
     lib.ldn_set_trace_buffer.argtypes = [ctypes.c_void_p]
     lib.ldn_set_trace_buffer.restype = None
+    lib.ldn_gated_image_bytes.argtypes = [_l, _i, _i, _i]
+    lib.ldn_gated_image_bytes.restype = ctypes.c_ulonglong
     lib.ldn_kernel_launches.argtypes = []
     lib.ldn_kernel_launches.restype = ctypes.c_ulonglong
     return lib

@@ -67,6 +67,8 @@ int param_type(const MaybeTensor& weight, const MaybeTensor& bias) {
     return weight.has_value() ? type_of(*weight) : bias.has_value() ? type_of(*bias) : LDN_F32;
 }
 MaybeTensor whole(const MaybeTensor& t) { return t.has_value() ? MaybeTensor(t->contiguous()) : t; }
+Tensor or_none(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
+MaybeTensor or_null(const Tensor& t) { return t.defined() ? MaybeTensor(t) : c10::nullopt; }
 void* ptr(const MaybeTensor& t) { return t.has_value() && t->defined() ? t->data_ptr() : nullptr; }
 
 // A tensor's rows: its memory as it is where rows are evenly spaced, else a copy
@@ -437,17 +439,21 @@ Gated gated_of(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const 
 }
 long long weight_pitch(const Rows& w) { return w.rows == 1 ? (w.C + 7) / 8 * 8 : w.pitch; }
 
-Tensor gated_forward(const Tensor& x, const Gated& a, Tensor* kept) {
+Tensor gated_forward(const Tensor& x, const Gated& a, Tensor* kept, Tensor* images) {
     std::vector<int64_t> shape = x.sizes().vec();
     const int64_t H = a.w_gate.rows, pitch = (H + 15) / 16 * 16;
     shape.back() = H;
     Tensor y = at::empty(shape, x.options());
     if (kept) *kept = at::empty({2, a.x.rows, pitch}, x.options().dtype(at::kFloat));
     float* g = kept ? floats(*kept) : nullptr;
+    if (images) {
+        const int64_t bytes = static_cast<int64_t>(ldn_gated_image_bytes(a.x.rows, a.x.C, static_cast<int>(H), type_of(x)));
+        if (bytes) *images = at::empty({bytes}, x.options().dtype(at::kByte));
+    }
     check(ldn_gated_linear(a.x.t.data_ptr(), a.x.pitch, a.x.rows, a.x.C, static_cast<int>(H), type_of(x), a.w_gate.t.data_ptr(),
                            weight_pitch(a.w_gate), a.w_up.t.data_ptr(), weight_pitch(a.w_up), ptr(a.b_gate), ptr(a.b_up),
                            param_type(a.b_gate, a.b_up), a.activation, y.data_ptr(), g, g ? g + a.x.rows * pitch : nullptr,
-                           pitch, stream()),
+                           pitch, images && images->defined() ? images->data_ptr() : nullptr, stream()),
           "gated_linear");
     return y;
 }
@@ -456,12 +462,12 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
     static Tensor forward(AutogradContext* ctx, Tensor x, Tensor w_gate, Tensor w_up, MaybeTensor b_gate, MaybeTensor b_up,
                           int64_t activation) {
         const c10::cuda::CUDAGuard guard(x.device());
-        Tensor kept;
-        Tensor y = gated_forward(x, gated_of(x, w_gate, w_up, b_gate, b_up, activation), &kept);
+        Tensor kept, images;
+        Tensor y = gated_forward(x, gated_of(x, w_gate, w_up, b_gate, b_up, activation), &kept, &images);
         ctx->saved_data["activation"] = activation;
         ctx->saved_data["biases"] = (b_gate.has_value() ? 1 : 0) + (b_up.has_value() ? 2 : 0);
         ctx->saved_data["param_type"] = param_type(b_gate, b_up);
-        ctx->save_for_backward({x, w_gate, w_up, kept});
+        ctx->save_for_backward({x, w_gate, w_up, kept, images});
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -487,7 +493,7 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
         const float* g = floats(kept);
         check(ldn_gated_linear_backward(dy.data_ptr(), a.x.t.data_ptr(), a.x.pitch, a.x.rows, a.x.C, static_cast<int>(H), type_of(x),
                                         a.w_gate.t.data_ptr(), weight_pitch(a.w_gate), a.w_up.t.data_ptr(), weight_pitch(a.w_up), g,
-                                        g + a.x.rows * kept.size(2), kept.size(2), a.activation, ptr(gx), ptr(gwg),
+                                        g + a.x.rows * kept.size(2), kept.size(2), ptr(or_null(saved[4])), a.activation, ptr(gx), ptr(gwg),
                                         ptr(gwu), ptr(gbg), ptr(gbu), params, stream()),
               "gated_linear_backward");
         const char* what = "gated_linear";
@@ -520,7 +526,7 @@ Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, c
     TORCH_CHECK(!b_gate.has_value() || !b_up.has_value() || b_gate->scalar_type() == b_up->scalar_type(), "the biases must have one type");
     if (wants_grad({&x, &w_gate, &w_up, at_of(b_gate), at_of(b_up)})) return GatedLinearFn::apply(x, w_gate, w_up, b_gate, b_up, activation);
     const c10::cuda::CUDAGuard guard(x.device());
-    return gated_forward(x, gated_of(x, w_gate, w_up, b_gate, b_up, activation), nullptr);
+    return gated_forward(x, gated_of(x, w_gate, w_up, b_gate, b_up, activation), nullptr, nullptr);
 }
 
 // ---- the residual stream between two norms ----------------------------------------------------------------------------------------
@@ -547,8 +553,6 @@ void sandwich_forward(const Tensor& x, const Tensor& residual, const MaybeTensor
                             static_cast<float>(eps), h.data_ptr(), y.data_ptr(), stats, stream()),
           "sandwich_norm");
 }
-Tensor or_none(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
-MaybeTensor or_null(const Tensor& t) { return t.defined() ? MaybeTensor(t) : c10::nullopt; }
 
 struct SandwichFn : public torch::autograd::Function<SandwichFn> {
     static variable_list forward(AutogradContext* ctx, Tensor x, Tensor residual, MaybeTensor gate, MaybeTensor scale, MaybeTensor post_weight,

@@ -134,6 +134,16 @@ struct Operands {
         }
         return count++;
     }
+    // (in images that are there already)
+    void found(char* at) {
+        for (int i = 0; i < copies; ++i) {
+            Images& o = images[copied[i]];
+            o.base = at;
+            at += pad256(static_cast<size_t>(o.count) * o.apart * 2);
+        }
+        copies = 0;
+        bytes = 0;
+    }
     int launch(char* scratch, const DeviceCtx* ctx, cudaStream_t st) {
         if (!copies) return kOk;
         long long most = 0;
@@ -286,10 +296,19 @@ bool on32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 
 using namespace ldn;
 
+extern "C" LDN_API unsigned long long ldn_gated_image_bytes(long long rows, int K, int H, int type) {
+    GatedArgs a = {};
+    a.T = rows;
+    if (type != LDN_F32 || rows < 1 || !row_fits(K) || !row_fits(H) || gated_is_few(a, type)) return 0;
+    Operands o{type};
+    for (const long long n : {rows, static_cast<long long>(H), static_cast<long long>(H)}) o.add(nullptr, K, n, K);
+    return o.bytes;
+}
+
 extern "C" LDN_API int ldn_gated_linear(const void* x, long long pitch, long long rows, int K, int H, int type, const void* w_gate,
                                         long long pitch_gate, const void* w_up, long long pitch_up, const void* b_gate, const void* b_up,
                                         int param_type, int activation, void* y, float* g, float* u, long long pitch_saved,
-                                        ldn_stream_t stream) {
+                                        void* images, ldn_stream_t stream) {
     if (!gated_fits(rows, K, H, type, param_type, b_gate, b_up, activation, pitch_gate, pitch_up) || !g != !u) return kBadArgument;
     if (g && (pitch_saved < H || pitch_saved % 16 || !on32(g) || !on32(u))) return kBadArgument;
     if (rows == 0) return kOk;
@@ -305,9 +324,11 @@ extern "C" LDN_API int ldn_gated_linear(const void* x, long long pitch, long lon
     o.add(x, pitch, rows, K);
     o.add(w_gate, pitch_gate, H, K);
     o.add(w_up, pitch_up, H, K);
+    const bool keep = images && type == LDN_F32;
+    const size_t operands = keep ? 0 : o.bytes;
     Scratch scratch;
-    r = scratch.take(st, o.bytes + gated_tiles_scratch(GatedForm::Forward, rows, H, K, type, ctx));
-    if (r == kOk) r = o.launch(scratch.base, ctx, st);
+    r = scratch.take(st, operands + gated_tiles_scratch(GatedForm::Forward, rows, H, K, type, ctx));
+    if (r == kOk) r = o.launch(keep ? static_cast<char*>(images) : scratch.base, ctx, st);
     if (r != kOk) return r;
     TileArgs t = {};
     t.M = rows;
@@ -315,13 +336,13 @@ extern "C" LDN_API int ldn_gated_linear(const void* x, long long pitch, long lon
     t.b_gate = b_gate; t.b_up = b_up; t.wide = a.wide; t.activation = activation;
     t.out0 = y; t.out1 = g; t.out2 = u;
     t.pitch = H; t.pitch_saved = pitch_saved;
-    return launch_gated_tiles(GatedForm::Forward, t, K, o.images[0], o.images[1], o.images[2], type, scratch.base + o.bytes, scratch.status,
+    return launch_gated_tiles(GatedForm::Forward, t, K, o.images[0], o.images[1], o.images[2], type, scratch.base + operands, scratch.status,
                               ctx, st);
 }
 
 extern "C" LDN_API int ldn_gated_linear_backward(const void* grad_y, const void* x, long long pitch, long long rows, int K, int H, int type,
                                                  const void* w_gate, long long pitch_gate, const void* w_up, long long pitch_up, const float* g,
-                                                 const float* u, long long pitch_saved, int activation, void* grad_x, void* grad_w_gate,
+                                                 const float* u, long long pitch_saved, const void* images, int activation, void* grad_x, void* grad_w_gate,
                                                  void* grad_w_up, void* grad_b_gate, void* grad_b_up, int param_type, ldn_stream_t stream) {
     if (!gated_fits(rows, K, H, type, param_type, grad_b_gate, grad_b_up, activation, pitch_gate, pitch_up) || !grad_w_gate != !grad_w_up ||
         pitch_saved < H || pitch_saved % 16)
@@ -342,8 +363,10 @@ extern "C" LDN_API int ldn_gated_linear_backward(const void* grad_y, const void*
     const DeviceCtx* ctx;
     if ((r = get_device_ctx(&ctx)) != kOk) return r;
     Operands o{type};
-    const int at_gate = grad_x ? o.add(w_gate, pitch_gate, H, K) : 0, at_up = grad_x ? o.add(w_up, pitch_up, H, K) : 0;
-    const int at_x = grad_w_gate ? o.add(x, pitch, rows, K) : 0;
+    const bool kept = images && type == LDN_F32;  // (all three, as the forward pass made them)
+    const int at_x = grad_w_gate || kept ? o.add(x, pitch, rows, K) : 0;
+    const int at_gate = grad_x || kept ? o.add(w_gate, pitch_gate, H, K) : 0, at_up = grad_x || kept ? o.add(w_up, pitch_up, H, K) : 0;
+    if (kept) o.found(static_cast<char*>(const_cast<void*>(images)));
     const int parts = type == LDN_F32 ? 3 : 1;
     Images d;  // dg and du
     d.rows = rows;

@@ -111,14 +111,14 @@ LONG = 2 ** 31 - 1
                                     dict(K=LONG), dict(H=LONG), dict(g=ctypes.c_void_p(AT.value + 4))])
 def test_gated_arguments(change):
     a = dict(x=AT, pitch=4, rows=2, K=4, H=20, type=0, w_gate=AT, pitch_gate=4, w_up=AT, pitch_up=4, b_gate=AT, b_up=None, param_type=0,
-             activation=3, y=AT, g=AT, u=AT, pitch_saved=32, stream=None)
+             activation=3, y=AT, g=AT, u=AT, pitch_saved=32, images=None, stream=None)
     assert lib.ldn_gated_linear(*{**a, **change}.values()) == BAD
 
 
 @pytest.mark.parametrize("change", [dict(K=0), dict(type=-1), dict(activation=2), dict(grad_y=None), dict(g=None), dict(u=None), dict(x=None),
                                     dict(w_gate=None), dict(grad_w_up=None), dict(pitch_saved=20), dict(param_type=2)])
 def test_gated_backward_arguments(change):
-    a = dict(grad_y=AT, x=AT, pitch=4, rows=2, K=4, H=20, type=0, w_gate=AT, pitch_gate=4, w_up=AT, pitch_up=4, g=AT, u=AT, pitch_saved=32,
+    a = dict(grad_y=AT, x=AT, pitch=4, rows=2, K=4, H=20, type=0, w_gate=AT, pitch_gate=4, w_up=AT, pitch_up=4, g=AT, u=AT, pitch_saved=32, images=None,
              activation=3, grad_x=AT, grad_w_gate=AT, grad_w_up=AT, grad_b_gate=AT, grad_b_up=AT, param_type=0, stream=None)
     assert lib.ldn_gated_linear_backward(*{**a, **change}.values()) == BAD
 
@@ -158,6 +158,6 @@ def test_distillation_backward_arguments(change):
 
 
 def test_calls_without_rows_do_nothing():
-    assert lib.ldn_gated_linear(None, 4, 0, 4, 4, 0, None, 4, None, 4, None, None, 0, 3, None, None, None, 0, None) == 0
+    assert lib.ldn_gated_linear(None, 4, 0, 4, 4, 0, None, 4, None, 4, None, None, 0, 3, None, None, None, 0, None, None) == 0
     assert lib.ldn_sandwich_norm(None, 4, None, 4, None, 0, 0, 0, 4, 0, None, None, None, None, None, 0, 1e-5, None, None, None, None) == 0
     assert lib.ldn_distillation_backward(None, 4, 0, 4, 0, None, 0, None, 2, None, 1.0, 1.0, 0.0, None, None, 0, 1.0, None, None) == 0
