@@ -119,76 +119,42 @@ __global__ void __launch_bounds__(kRowThreads) sandwich_grad_rows_kernel(const _
 
 constexpr int kColumns = 32, kColumnLanes = 8;
 
-// N elements of a row, as one load or one by one
-template <class T, int N>
-__device__ __forceinline__ void load_run(const T* p, float (&v)[N]) {
-    if constexpr (N == 1) {
-        v[0] = to_float(*p);
-    } else {
-        const uint4 raw = *reinterpret_cast<const uint4*>(p);
-        const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = to_float(e[i]);
-    }
-}
-// Column sums over a block of rows, behind the rows' means, where a row's registers have no room for them: a thread has N neighbouring
-// columns (a piece of 16 bytes, or one where rows are cut) and every eighth row, two or four of them under way.
-template <class T, Gate G, int N>
+// Column sums over a block of rows, behind the rows' means: a thread has a column and every eighth row, four of them under way.
+template <class T, Gate G>
 __global__ void __launch_bounds__(kColumns * kColumnLanes) sandwich_grad_columns_kernel(const __grid_constant__ SandwichGradArgs a) {
     stream_order_begin();
-    constexpr int kAhead = N == 1 ? 4 : 2;
-    __shared__ float sums[kColumnLanes][kColumns * N];
-    const int lane = threadIdx.x % kColumns, part = threadIdx.x / kColumns, c = (blockIdx.x * kColumns + lane) * N;
+    constexpr int kAhead = 4;
+    __shared__ float sums[4][kColumnLanes][kColumns];
+    const int lane = threadIdx.x % kColumns, part = threadIdx.x / kColumns, c = blockIdx.x * kColumns + lane;
     const long long first = a.rows * blockIdx.y / gridDim.y, last = a.rows * (blockIdx.y + 1) / gridDim.y;
     const T* gates = static_cast<const T*>(a.gate);
-    float s[4][N] = {}, weight[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) weight[i] = c + i < a.C ? param_or<T>(a.p.weight, a.p.wide, c + i, 1.0f) : 0.0f;
+    float s[4] = {};
     if (c < a.C)
         for (long long row0 = first + part; row0 < last; row0 += kAhead * kColumnLanes) {
-            float h[kAhead][N], x[kAhead][N], dy[kAhead][N] = {}, dh[kAhead][N] = {}, g[kAhead][N];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const long long row = row0 + u * kColumnLanes, at = row * a.C + c;
                 if (row >= last) continue;
-                load_run<T, N>(static_cast<const T*>(a.h) + at, h[u]);
-                load_run<T, N>(static_cast<const T*>(a.x) + row * a.pitch + c, x[u]);
-                if (a.grad_y) load_run<T, N>(static_cast<const T*>(a.grad_y) + at, dy[u]);
-                if (a.grad_h) load_run<T, N>(static_cast<const T*>(a.grad_h) + at, dh[u]);
-                if constexpr (G == Gate::All) load_run<T, N>(gates + row * a.pitch_gate + c, g[u]);
-            }
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const long long row = row0 + u * kColumnLanes;
-                if (row >= last) continue;
-                const float mean1 = a.stats[row], rstd1 = a.stats[a.rows + row], mean2 = a.stats[2 * a.rows + row], rstd2 = a.stats[3 * a.rows + row];
-                const float m1 = a.row_sums[row], m2 = a.row_sums[a.rows + row], row_gate = G == Gate::Row ? to_float(gates[row]) : 1.0f;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float z2 = (h[u][i] - mean2) * rstd2, z1 = (x[u][i] - mean1) * rstd1;
-                    float d = dh[u][i] + rstd2 * (dy[u][i] * weight[i] - m1 - z2 * m2);
-                    d *= G == Gate::All ? g[u][i] : row_gate;
-                    s[0][i] += dy[u][i] * z2;
-                    s[1][i] += dy[u][i];
-                    s[2][i] += d * z1;
-                    s[3][i] += d;
-                }
+                const float rstd2 = a.stats[3 * a.rows + row];
+                const float z2 = (to_float(static_cast<const T*>(a.h)[at]) - a.stats[2 * a.rows + row]) * rstd2;
+                const float z1 = (to_float(static_cast<const T*>(a.x)[row * a.pitch + c]) - a.stats[row]) * a.stats[a.rows + row];
+                const float g = a.grad_y ? to_float(static_cast<const T*>(a.grad_y)[at]) : 0.0f;
+                float d = stream_gradient<T>(a, at, c, z2, rstd2, a.row_sums[row], a.row_sums[a.rows + row]);
+                if (G == Gate::Row) d *= to_float(gates[row]);
+                if (G == Gate::All) d *= to_float(gates[row * a.pitch_gate + c]);
+                s[0] += g * z2;
+                s[1] += g;
+                s[2] += d * z1;
+                s[3] += d;
             }
         }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < N; ++i) sums[part][lane * N + i] = s[k][i];
-        __syncthreads();
-        for (int i = threadIdx.x; i < kColumns * N; i += kColumns * kColumnLanes) {
-            const int column = blockIdx.x * kColumns * N + i;
-            if (column >= a.C) continue;
-            float all = 0.0f;
-#pragma unroll
-            for (int r = 0; r < kColumnLanes; ++r) all += sums[r][i];
-            a.parts[(static_cast<long long>(blockIdx.y) * 4 + k) * a.C + column] = all;
-        }
+    for (int k = 0; k < 4; ++k) sums[k][part][lane] = s[k];
+    __syncthreads();
+    if (part < 4 && c < a.C) {
+        float all = 0.0f;
+        for (int i = 0; i < kColumnLanes; ++i) all += sums[part][i][lane];
+        a.parts[(static_cast<long long>(blockIdx.y) * 4 + part) * a.C + c] = all;
     }
 }
 
@@ -300,11 +266,9 @@ extern "C" LDN_API int ldn_sandwich_norm_backward(const void* grad_y, const void
     SandwichGradArgs a = {grad_y, grad_h, x, h, gate, pitch, pitch_gate, rows, C, f.p, stats, grad_x, grad_residual, grad_gate, nullptr, nullptr};
     const int columns = (C + kColumns - 1) / kColumns;
     const bool sums = grad_scale || grad_post_weight || grad_post_bias || grad_weight || grad_bias;
-    const int on_chip = sandwich_grad_in_registers(kind, a, type, ctx, sums, &f.count);
-    const bool registers = on_chip == kRowsAndSums;
-    const int run = sandwich_runs(kind, a, type) ? 16 / size_of(type) : 1, blocks_x = (C + kColumns * run - 1) / (kColumns * run);
+    const bool registers = sandwich_grad_in_registers(kind, a, type, ctx, &f.count);
     if (!registers) {
-        const long long most = (4LL * ctx->sm_count + blocks_x - 1) / blocks_x, needed = (rows + 63) / 64;
+        const long long most = (4LL * ctx->sm_count + columns - 1) / columns, needed = (rows + 63) / 64;
         f.count = static_cast<int>(most < needed ? most : needed);
     }
     const size_t row_bytes = registers ? 0 : pad256(static_cast<size_t>(rows) * 2 * sizeof(float));
@@ -315,7 +279,7 @@ extern "C" LDN_API int ldn_sandwich_norm_backward(const void* grad_y, const void
         a.row_sums = reinterpret_cast<float*>(scratch.base);
         if (sums) f.parts = a.parts = reinterpret_cast<float*>(scratch.base + row_bytes);
     }
-    if (on_chip != kNothing && (r = launch_sandwich_grad_in_registers(kind, a, type, ctx, st)) != kOk) return r;
+    if (registers && (r = launch_sandwich_grad_in_registers(kind, a, type, ctx, st)) != kOk) return r;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         int s = kOk;
@@ -323,13 +287,10 @@ extern "C" LDN_API int ldn_sandwich_norm_backward(const void* grad_y, const void
             s = with_gate(kind, [&](auto g) {
                 constexpr Gate G = decltype(g)::value;
                 const long long most = 32LL * ctx->sm_count;
-                int q = kOk;
-                if (on_chip == kNothing)
-                    q = launch_after(sandwich_grad_rows_kernel<T, G>, static_cast<unsigned>(rows < most ? rows : most), kRowThreads, 0, st, a);
+                const int q = launch_after(sandwich_grad_rows_kernel<T, G>, static_cast<unsigned>(rows < most ? rows : most), kRowThreads, 0, st, a);
                 if (q != kOk || !sums) return q;
-                const dim3 grid(blocks_x, static_cast<unsigned>(f.count));
-                return run > 1 ? launch_after(sandwich_grad_columns_kernel<T, G, 16 / sizeof(T)>, grid, kColumns * kColumnLanes, 0, st, a)
-                               : launch_after(sandwich_grad_columns_kernel<T, G, 1>, grid, kColumns * kColumnLanes, 0, st, a);
+                return launch_after(sandwich_grad_columns_kernel<T, G>, dim3(columns, static_cast<unsigned>(f.count)), kColumns * kColumnLanes, 0,
+                                    st, a);
             });
         if (s != kOk || !sums) return s;
         return launch_after(sandwich_fold_kernel<T>, columns, kColumns * 4 * kFoldLanes, 0, st, f);

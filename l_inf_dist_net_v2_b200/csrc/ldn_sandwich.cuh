@@ -33,18 +33,17 @@ struct SandwichGradArgs {
     SandwichParams p;
     const float* stats;
     void *grad_x, *grad_residual, *grad_gate;  // any may be null
-    float* row_sums;  // [2][rows]: mean(a), mean(a z2), where the column sums have a kernel of their own
+    float* row_sums;  // [2][rows]: mean(a), mean(a z2); simple kernels
     float* parts;     // [block of rows][4][C]: sums of dy z2, dy, d gate z1, d gate; may be null
 };
 
 // Rows held in registers (ldn_sandwich_rows.cu); false: these rows do not fit, or their tensors' pieces do not match
 bool sandwich_in_registers(Gate gate, const SandwichArgs& a, int type, const DeviceCtx* ctx, cudaStream_t st, int* status);
-// Backward: nothing, the rows with their two means in row_sums, or the rows and, where `sums` are wanted, the column sums
-enum OnChip { kNothing, kRows, kRowsAndSums };
-int sandwich_grad_in_registers(Gate gate, const SandwichGradArgs& a, int type, const DeviceCtx* ctx, bool sums, int* blocks);
+// (rows of T: how many blocks of column sums they have, or, with a stream, their launch)
+template <class T>
+int sandwich_grad_rows(Gate gate, const SandwichGradArgs& a, const DeviceCtx* ctx, int* blocks, const cudaStream_t* st);
+bool sandwich_grad_in_registers(Gate gate, const SandwichGradArgs& a, int type, const DeviceCtx* ctx, int* blocks);
 int launch_sandwich_grad_in_registers(Gate gate, const SandwichGradArgs& a, int type, const DeviceCtx* ctx, cudaStream_t st);
-// All rows of the backward pass are whole pieces of 16 bytes
-bool sandwich_runs(Gate gate, const SandwichGradArgs& a, int type);
 
 #ifdef __CUDACC__
 template <class T>

@@ -214,3 +214,11 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             attempt()
     assert ldn._lib.lib.ldn_kernel_launches() == before
+
+
+@pytest.mark.parametrize("rows, C", [(300, 5121), (200, 8192), (150, 10975), (130, 16385), (100, 33000), (20, 40960), (5, 41001)])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_many_rows_that_blocks_share(rows, C, dtype):
+    for gate in ("none", "row", "all"):
+        check(*made(rows, C, dtype, gate, F32 if gate == "row" else dtype))
+    check(*made(rows, C, dtype, "all", F32, layout="shifted"), use=("y",))
