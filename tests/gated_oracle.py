@@ -23,11 +23,11 @@ def act(g, name):
 
 def sum_unit(terms, dtype):
     """How far a sum of `terms` products may be off, in units of the sum of their magnitudes.  Products of 16 bits: an instruction adds 16 of
-    them to the accumulator and drops less than its last place, 2^-23.  Of 32 bits: 512 terms at a time (32 instructions with whole
-    magnitudes and five times as many with 2^-8 of them at most: less than 48), then additions in 32 bits; 2^-26 of each product
-    is left out."""
+    them to the accumulator and drops less than its last place, 2^-23.  Of 32 bits: 256 terms at a time (16 instructions with whole
+    magnitudes and five times as many with 2^-8 of them at most: less than 24), then additions in 32 bits; 2^-26 of each product
+    is left out.  A handful of rows: chains of terms / 128 additions and a dozen more."""
     if dtype == torch.float32:
-        return 48 * 2.0 ** -23 + (terms / 512 + 2) * EPS32 + 2.0 ** -26
+        return 24 * 2.0 ** -23 + (terms / 128 + 16) * EPS32 + 2.0 ** -26
     return (terms / 16 + 16) * 2.0 ** -23
 
 
