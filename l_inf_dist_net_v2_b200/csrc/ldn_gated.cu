@@ -4,7 +4,7 @@
 // The backward pass needs both projections again.  They are kept in 32 bits: rounded to bfloat16 they took the weights' gradients from
 // 2.4e-3 to 3.1e-3 of 64 bits (1.7e-3 is their own rounding), and making them again would cost a third of a training step's products.
 // What enters the products as dg and du has the rows' type: the tensor cores multiply no other at that rate.  Bound by memory: dy, both
-// projections, both gradients once.
+// projections, both gradients once (16384 x 5120 bf16: 226 us, 5.2 TB/s; 512 x 2048 float32: 9).
 #include "ldn_gated.cuh"
 
 namespace ldn {
@@ -59,7 +59,8 @@ __device__ __forceinline__ void store_split8(unsigned short* to, long long apart
 #pragma unroll
     for (int i = 0; i < 3; ++i) *reinterpret_cast<uint4*>(to + i * apart) = packed8(image[i]);
 }
-// Rows of any pitch and alignment as images: of 16 bits a copy, of 32 three parts.  A thread has eight columns.
+// Rows of any pitch and alignment as images: of 16 bits a copy, of 32 three parts.  A thread has eight columns.  Bound by memory: x and both
+// weights of 512, 5120 -> 2048 in float32, 94 MB in and 141 out, 34 us, 6.9 TB/s.
 template <class T>
 __global__ void __launch_bounds__(kCopyThreads) images_kernel(const __grid_constant__ Sources sources) {
     stream_order_begin();

@@ -2,6 +2,7 @@
 //
 // Bound by memory: 2 H K elements of the weights.  A block has some outputs, and its threads share their terms in pieces of 16 bytes, so
 // that every output's two weight rows are under way at once in whole lines; the rows themselves come from the first-level cache.
+// 1, 5120 -> 5120 bf16: 20.2 us, 5.2 TB/s; 1, 5120 -> 2048 float32: 16.7 us, 5.0; 8, 5120 -> 5120 float32: 69 us, 3.0.
 #include "ldn_gated.cuh"
 
 namespace ldn {

