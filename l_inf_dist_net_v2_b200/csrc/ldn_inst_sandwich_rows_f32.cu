@@ -1,0 +1,7 @@
+#include "ldn_sandwich_forward.cuh"
+
+namespace ldn {
+
+template bool sandwich_rows<float>(Gate, const SandwichArgs&, const DeviceCtx*, cudaStream_t, int*);
+
+}  // namespace ldn

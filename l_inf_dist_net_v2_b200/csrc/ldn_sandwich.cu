@@ -232,7 +232,7 @@ extern "C" LDN_API int ldn_sandwich_norm(const void* x, long long pitch, const v
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const SandwichArgs a = {x, residual, gate, pitch, pitch_residual, pitch_gate, rows, C,
                             {scale, post_weight, post_bias, weight, bias, param_type == LDN_F32}, eps, h, y, stats};
-    if (sandwich_in_registers(static_cast<Gate>(gate_kind), a, type, ctx, st, &r)) return r;
+    if (with_type(type, [&](auto t) { return sandwich_rows<decltype(t)>(static_cast<Gate>(gate_kind), a, ctx, st, &r) ? 1 : 0; })) return r;
     const long long most = 32LL * ctx->sm_count;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
@@ -266,7 +266,10 @@ extern "C" LDN_API int ldn_sandwich_norm_backward(const void* grad_y, const void
     SandwichGradArgs a = {grad_y, grad_h, x, h, gate, pitch, pitch_gate, rows, C, f.p, stats, grad_x, grad_residual, grad_gate, nullptr, nullptr};
     const int columns = (C + kColumns - 1) / kColumns;
     const bool sums = grad_scale || grad_post_weight || grad_post_bias || grad_weight || grad_bias;
-    const bool registers = sandwich_grad_in_registers(kind, a, type, ctx, &f.count);
+    auto in_registers = [&](int* blocks, const cudaStream_t* st) {
+        return with_type(type, [&](auto t) { return sandwich_grad_rows<decltype(t)>(kind, a, ctx, blocks, st); });
+    };
+    const bool registers = in_registers(&f.count, nullptr) == kOk;
     if (!registers) {
         const long long most = (4LL * ctx->sm_count + columns - 1) / columns, needed = (rows + 63) / 64;
         f.count = static_cast<int>(most < needed ? most : needed);
@@ -279,7 +282,7 @@ extern "C" LDN_API int ldn_sandwich_norm_backward(const void* grad_y, const void
         a.row_sums = reinterpret_cast<float*>(scratch.base);
         if (sums) f.parts = a.parts = reinterpret_cast<float*>(scratch.base + row_bytes);
     }
-    if (registers && (r = launch_sandwich_grad_in_registers(kind, a, type, ctx, st)) != kOk) return r;
+    if (registers && (r = in_registers(nullptr, &st)) != kOk) return r;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         int s = kOk;

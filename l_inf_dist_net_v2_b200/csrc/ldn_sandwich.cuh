@@ -37,13 +37,12 @@ struct SandwichGradArgs {
     float* parts;     // [block of rows][4][C]: sums of dy z2, dy, d gate z1, d gate; may be null
 };
 
-// Rows held in registers (ldn_sandwich_rows.cu); false: these rows do not fit, or their tensors' pieces do not match
-bool sandwich_in_registers(Gate gate, const SandwichArgs& a, int type, const DeviceCtx* ctx, cudaStream_t st, int* status);
-// (rows of T: how many blocks of column sums they have, or, with a stream, their launch)
+// Rows of T held in registers (ldn_sandwich_forward.cuh, ldn_sandwich_grad.cuh).  False: these rows do not fit, or their tensors' pieces do not match
+template <class T>
+bool sandwich_rows(Gate gate, const SandwichArgs& a, const DeviceCtx* ctx, cudaStream_t st, int* status);
+// kOk: they do; blocks: how many parts of column sums they make, where not null; st: their launch, where not null
 template <class T>
 int sandwich_grad_rows(Gate gate, const SandwichGradArgs& a, const DeviceCtx* ctx, int* blocks, const cudaStream_t* st);
-bool sandwich_grad_in_registers(Gate gate, const SandwichGradArgs& a, int type, const DeviceCtx* ctx, int* blocks);
-int launch_sandwich_grad_in_registers(Gate gate, const SandwichGradArgs& a, int type, const DeviceCtx* ctx, cudaStream_t st);
 
 #ifdef __CUDACC__
 template <class T>

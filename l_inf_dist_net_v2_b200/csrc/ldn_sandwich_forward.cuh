@@ -1,4 +1,5 @@
 // The residual stream between two norms, forward, with rows in registers (ldn_sandwich_rows.cuh).
+#pragma once
 #include "ldn_sandwich_rows.cuh"
 
 namespace ldn {
@@ -177,8 +178,7 @@ sandwich_registers_kernel(const __grid_constant__ SandwichArgs a, int lanes, int
     if constexpr (W == Share::Cluster) cluster_barrier();  // (no block ends while another may still write to it)
 }
 
-bool plan_forward(Gate gate, const SandwichArgs& a, int type, RowPlan* p, Share* who, int* ranks) {
-    const int size = size_of(type);
+bool plan_forward(Gate gate, const SandwichArgs& a, int size, RowPlan* p, Share* who, int* ranks) {
     const bool aligned = on16(a.x) && on16(a.residual) && on16(a.h) && on16(a.y) && (gate != Gate::All || on16(a.gate));
     const bool match = rows_match(size, a.C, a.pitch, aligned) && rows_match(size, a.C, a.pitch_residual, aligned) &&
                        (gate != Gate::All || rows_match(size, a.C, a.pitch_gate, aligned));
@@ -188,39 +188,30 @@ bool plan_forward(Gate gate, const SandwichArgs& a, int type, RowPlan* p, Share*
 }
 }  // namespace
 
-bool sandwich_in_registers(Gate gate, const SandwichArgs& a, int type, const DeviceCtx* ctx, cudaStream_t st, int* status) {
+template <class T>
+bool sandwich_rows(Gate gate, const SandwichArgs& a, const DeviceCtx* ctx, cudaStream_t st, int* status) {
     RowPlan p;
     Share who;
     int ranks;
-    if (!plan_forward(gate, a, type, &p, &who, &ranks)) return false;
+    if (!plan_forward(gate, a, sizeof(T), &p, &who, &ranks)) return false;
     bool fits = false;
-    *status = with_type(type, [&](auto t) {
-        using T = decltype(t);
-        return with_gate(gate, [&](auto g) {
-            return with_items<T, true>(p, who, [&](auto items, auto share, auto shift) {
-                constexpr Gate G = decltype(g)::value;
-                constexpr int kItems = decltype(items)::value;
-                constexpr Share W = decltype(share)::value;
-                constexpr auto kernel = sandwich_registers_kernel<T, G, kItems, W, decltype(shift)::value>;
-                constexpr int R = rows_forward(kItems * kPiece<T>, sizeof(T), W == Share::Group, decltype(shift)::value);
-                long long resident;
-                int depth;
-                RowShape s;
-                fits = resident_rows<kernel>(p, R, kForwardStreams<G>, 0, ranks, ctx, &resident, &depth) &&
-                       shape_of(p, a.rows, R, kForwardStreams<G>, 0, ranks, resident, depth, &s);
-                return fits ? launch_after_in_clusters(kernel, ranks, s.blocks * ranks, p.threads, s.smem, st, a, p.lanes, s.depth, ranks)
-                            : static_cast<int>(kOk);
-            });
+    *status = with_gate(gate, [&](auto g) {
+        return with_items<T, true>(p, who, [&](auto items, auto share, auto shift) {
+            constexpr Gate G = decltype(g)::value;
+            constexpr int kItems = decltype(items)::value;
+            constexpr Share W = decltype(share)::value;
+            constexpr auto kernel = sandwich_registers_kernel<T, G, kItems, W, decltype(shift)::value>;
+            constexpr int R = rows_forward(kItems * kPiece<T>, sizeof(T), W == Share::Group, decltype(shift)::value);
+            long long resident;
+            int depth;
+            RowShape s;
+            fits = resident_rows<kernel, W>(p, R, kForwardStreams<G>, 0, ranks, ctx, &resident, &depth) &&
+                   shape_of(p, a.rows, R, kForwardStreams<G>, 0, ranks, resident, depth, &s);
+            return fits ? launch_after_in_clusters(kernel, ranks, s.blocks * ranks, p.threads, s.smem, st, a, p.lanes, s.depth, ranks)
+                        : static_cast<int>(kOk);
         });
     });
     return fits;
-}
-
-bool sandwich_grad_in_registers(Gate gate, const SandwichGradArgs& a, int type, const DeviceCtx* ctx, int* blocks) {
-    return with_type(type, [&](auto t) { return sandwich_grad_rows<decltype(t)>(gate, a, ctx, blocks, nullptr); }) == kOk;
-}
-int launch_sandwich_grad_in_registers(Gate gate, const SandwichGradArgs& a, int type, const DeviceCtx* ctx, cudaStream_t st) {
-    return with_type(type, [&](auto t) { return sandwich_grad_rows<decltype(t)>(gate, a, ctx, nullptr, &st); });
 }
 
 }  // namespace ldn

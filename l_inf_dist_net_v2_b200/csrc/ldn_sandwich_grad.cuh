@@ -332,7 +332,7 @@ int with_backward(Gate gate, const SandwichGradArgs& a, const DeviceCtx* ctx, F 
             long long resident;
             int depth;
             RowShape s;
-            if (!resident_rows<kernel>(p, 1, kBackwardStreams<G>, params, ranks, ctx, &resident, &depth) ||
+            if (!resident_rows<kernel, W>(p, 1, kBackwardStreams<G>, params, ranks, ctx, &resident, &depth) ||
                 !shape_of(p, a.rows, 1, kBackwardStreams<G>, params, ranks, resident, depth, &s))
                 return static_cast<int>(kBadArgument);
             if constexpr (W == Share::Group) {

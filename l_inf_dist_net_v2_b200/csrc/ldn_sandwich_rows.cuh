@@ -7,8 +7,8 @@
 // eight, and rows that far apart start alike), and rows that are taken together share the barriers of their sums.  The scale and the first
 // norm's parameters are two numbers per column, scale weight and scale bias.
 //
-// 16384 x 5120 bf16 with a gate of its shape: forward 182 us, 4.6 TB/s, backward 276, 4.9 (228 with the sums over rows left out: what the warps
-// wait for); 8192 x 5120 float32 150 and 269; 524288 x 96 bf16 with a gate per row 131 and 236; 16383 x 4097 bf16, cut rows, 219 and 392;
+// 16384 x 5120 bf16 with a gate of its shape: forward 180 us, 4.7 TB/s, backward 287, 4.7 (228 with the sums over rows left out: what the warps
+// wait for); 8192 x 5120 float32 150 and 269; 524288 x 96 bf16 with a gate per row 131 and 236; 16383 x 4097 bf16, cut rows, 221 and 391;
 // 8192 x 8192 bf16 213 and 374; 3457 x 8118 float32, shared by blocks, 229 and 345.
 #pragma once
 #include "ldn_sandwich.cuh"
@@ -153,7 +153,8 @@ struct RowShape {
     size_t smem;
 };
 // (sums' slots and rows' numbers)
-constexpr int kStaticBytes = (2 * SumOf<Share::Cluster>::kSlots + 5 * kNumberRows) * sizeof(float) + 256;
+template <Share W>
+constexpr int kStaticBytes = (2 * SumOf<W>::kSlots + 5 * kNumberRows) * sizeof(float) + 256;
 // Elements of a thread, threads of a block, and who has a row.  Whole blocks: 16 elements per thread of 16 bits (the instructions around an
 // element count: 16384 x 5120 with 8 took 203 and 415 us), 8 of 32.  Longer rows: the blocks of a cluster; forward, where rows of 16 bits
 // are whole, blocks with 32 elements per thread, which read their parameters again (8192 x 8192 bf16 221 us, in clusters 299; 4096 x 8192
@@ -176,10 +177,10 @@ bool plan_row(int C, int size, bool shift, bool forward, RowPlan* p, Share* who,
     return true;
 }
 // What is on an SM: `per_sm` blocks that its registers hold, or fewer, so that rows are under way behind those that are worked on.
-// extra: bytes of a block beside its rows
-bool fill(const RowPlan& p, int R, int streams, long long extra, const DeviceCtx* ctx, int* per_sm, int* depth) {
+// extra, fixed: bytes of a block beside its rows
+bool fill(const RowPlan& p, int R, int streams, long long extra, int fixed, const DeviceCtx* ctx, int* per_sm, int* depth) {
     const long long row_bytes = static_cast<long long>(R) * streams * p.items * p.threads * 16;
-    auto room = [&] { return ctx->max_smem_optin / *per_sm - 1024 - kStaticBytes - extra; };
+    auto room = [&] { return ctx->max_smem_optin / *per_sm - 1024 - fixed - extra; };
     *depth = ring_depth(row_bytes, room());
     while (*depth < 2 && *per_sm > 1) {
         --*per_sm;
@@ -228,10 +229,10 @@ int with_gate(Gate gate, F f) {
     }
 }
 // The blocks of rows (or clusters of them) that the device holds at a time, and how many rows each has under way; false: not one
-template <auto KERNEL>
+template <auto KERNEL, Share W>
 bool resident_rows(const RowPlan& p, int R, int streams, long long extra, int ranks, const DeviceCtx* ctx, long long* resident, int* depth) {
     static OncePerDevice once;
-    if (once([&] { return allow_smem(KERNEL, ctx->max_smem_optin - kStaticBytes); }) != kOk) return false;
+    if (once([&] { return allow_smem(KERNEL, ctx->max_smem_optin - kStaticBytes<W>); }) != kOk) return false;
     static std::atomic<int> of_sm[64][33], of_device[64][33][kMostRanks + 1];
     auto asked = [](std::atomic<int>& known, auto ask) {
         int count = known.load(std::memory_order_acquire);
@@ -245,7 +246,7 @@ bool resident_rows(const RowPlan& p, int R, int streams, long long extra, int ra
     };
     int per_sm = asked(of_sm[ctx->device][p.threads / 32],
                        [&](int* n) { return cudaOccupancyMaxActiveBlocksPerMultiprocessor(n, KERNEL, p.threads, 0); });
-    if (!fill(p, R, streams, extra, ctx, &per_sm, depth)) return false;
+    if (!fill(p, R, streams, extra, kStaticBytes<W>, ctx, &per_sm, depth)) return false;
     *resident = static_cast<long long>(per_sm) * ctx->sm_count;
     if (ranks > 1)
         *resident = asked(of_device[ctx->device][p.threads / 32][ranks], [&](int* n) {
