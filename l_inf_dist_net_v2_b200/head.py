@@ -13,9 +13,9 @@ import torch.nn as nn
 
 from . import norm_dist_cuda as _C
 
-__all__ = ["layer_norm", "dropout", "dropout_add_layer_norm", "quantize_rows", "layer_norm_quantized", "int8_linear", "gated_linear", "sandwich_norm",
-           "LayerNorm", "GatedLinear", "SandwichNorm", "GatedHead",
-           "Dropout", "Int8Linear", "ResidualHead", "QuantizedHead"]
+__all__ = ["layer_norm", "dropout", "dropout_add_layer_norm", "quantize_rows", "layer_norm_quantized", "int8_linear", "gated_linear",
+           "sandwich_norm", "LayerNorm", "GatedLinear", "SandwichNorm", "GatedHead", "Dropout", "Int8Linear", "ResidualHead",
+           "QuantizedHead"]
 
 _ACTIVATIONS = {"none": 0, "relu": 1, "tanh": 2}
 _GATES = {"relu": 1, "silu": 3, "gelu": 4, "sigmoid": 5}
@@ -95,9 +95,10 @@ def gated_linear(x, weight_gate, weight_up, bias_gate=None, bias_up=None, activa
     """act(x @ weight_gate.T + bias_gate) * (x @ weight_up.T + bias_up): both projections, the activation and the product in one kernel,
     with the gradients of all five.  activation: "silu", "gelu" (of the normal distribution's function), "sigmoid" or "relu".
 
-    Weights are (outputs, terms) of the type of x, biases of that type or float32; sums have 32 bits.  Both projections are kept in 32 bits
-    for the backward pass, and of float32 operands the 6 bytes per element that they are multiplied as.  Rows of 16-bit tensors that start at multiples of 16 bytes are read where they lie, others are copied
-    first; float32 is multiplied on the tensor cores as three bfloat16 numbers (24 bits), where an infinity gives not-a-numbers."""
+    Weights are (outputs, terms) of the type of x, biases of that type or float32; sums have 32 bits.  Kept for the backward pass are both
+    projections in 32 bits and, of float32 operands, the 6 bytes per element that they are multiplied as.  Rows of 16-bit tensors that
+    start at multiples of 16 bytes are read where they lie, others are copied first; float32 is multiplied on the tensor cores as
+    three bfloat16 numbers (24 bits), where an infinity gives not-a-numbers."""
     if activation not in _GATES:
         raise ValueError(f"activation must be one of {sorted(_GATES)}, not {activation!r}")
     return _native().gated_linear(x, weight_gate, weight_up, bias_gate, bias_up, _GATES[activation])
@@ -219,7 +220,8 @@ class GatedLinear(nn.Module):
 
 
 class SandwichNorm(nn.Module):
-    """`sandwich_norm` with its parameters: the norm behind a block, the scale that its rows join the stream with, and the next block's norm."""
+    """`sandwich_norm` with its parameters: the norm behind a block, the scale that its rows join the stream with, and the next block's
+    norm."""
 
     def __init__(self, features, scale=1.0, eps=1e-5):
         super().__init__()

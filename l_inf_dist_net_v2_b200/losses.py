@@ -62,13 +62,14 @@ def distillation_loss(logits, teacher_values, teacher_indices, targets=None, tem
 
         (1 - mix) temperature^2 sum p (log p - log q) + mix cross_entropy(logits, target),
 
-    p = softmax(teacher_values / temperature) over the row's entries and q = softmax(logits / temperature) over all classes, with the gradient
-    of the logits (the teacher has none).  `teacher_values` and `teacher_indices` (..., k), k up to 1024, say which classes the entries
-    are of, in any order; an entry with an index below 0 is absent, entries of one class add up.  A row without entries has no first term, a
-    row with a target below 0 no second.  An index or target beyond the classes makes its row's loss and gradient not-a-numbers.
+    p = softmax(teacher_values / temperature) over the row's entries and q = softmax(logits / temperature) over all classes, with the
+    gradient of the logits (the teacher has none).  `teacher_values` and `teacher_indices` (..., k), k up to 1024, say which classes the
+    entries are of, in any order; an entry with an index below 0 is absent, entries of one class add up.  A row without entries has no
+    first term, a row with a target below 0 no second.  An index or target beyond the classes makes its row's loss and gradient
+    not-a-numbers.
 
-    reduction: "mean" over all rows, "sum" or "none"; the loss is float32.  Logits are float32, float16 or bfloat16 and may hold minus infinity
-    for classes that are no choice; sums have 32 bits and are made in one pass over the logits each way."""
+    reduction: "mean" over all rows, "sum" or "none"; the loss is float32.  Logits are float32, float16 or bfloat16 and may hold minus
+    infinity for classes that are no choice; sums have 32 bits and are made in one pass over the logits each way."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, not {reduction!r}")
     if mix and targets is None:
@@ -77,7 +78,8 @@ def distillation_loss(logits, teacher_values, teacher_indices, targets=None, tem
     if ext is None:
         raise RuntimeError("distillation_loss needs the compiled binding (python l_inf_dist_net_v2_b200/build.py) and runs under no "
                            "function transform and not in torch.compile")
-    return ext.distillation_loss(logits, teacher_values, teacher_indices, targets if mix else None, temperature, mix, _REDUCTIONS[reduction])
+    return ext.distillation_loss(logits, teacher_values, teacher_indices, targets if mix else None, temperature, mix,
+                                 _REDUCTIONS[reduction])
 
 
 class distillation:
