@@ -46,7 +46,9 @@ void plan(GatedForm form, long long M, int N, int terms, int type, const DeviceC
     a->units = a->side_units * (form == GatedForm::GradRows ? 2 : 1);
     const long long least = parted ? 1 : 4, shares = (static_cast<long long>(a->tiles) * a->units + least - 1) / least;
     const int held = resident_pairs(ctx), resident = held < kMostPairs ? held : kMostPairs;
-    a->pairs = static_cast<int>(shares < resident ? shares : resident);
+    // (a tile each at least: 85, 9 -> 7429 bf16 has 59 of one step; by 15 pairs it took 54 us, by 59 21)
+    const long long wanted = shares > a->tiles ? shares : a->tiles;
+    a->pairs = static_cast<int>(wanted < resident ? wanted : resident);
     const int rest = a->tiles % a->pairs;
     a->whole = a->tiles;
     if (rest) {
