@@ -6,6 +6,7 @@
 // What enters the products as dg and du has the rows' type: the tensor cores multiply no other at that rate.  Bound by memory: dy, both
 // projections, both gradients once (16384 x 5120 bf16: 226 us, 5.2 TB/s; 512 x 2048 float32: 9).
 #include "ldn_gated.cuh"
+#include "ldn_words.cuh"
 
 namespace ldn {
 namespace {
@@ -87,7 +88,10 @@ __global__ void __launch_bounds__(kCopyThreads) images_kernel(const __grid_const
         } else {
             // a piece that starts anywhere, from the two words of memory that it lies in, where both are the tensor's
             const unsigned off = static_cast<unsigned>(reinterpret_cast<uintptr_t>(from) & 15u);
-            if (c + 8 <= s.C && (row > 0 || c > 0 || off == 0) && (c + 16 <= s.C || row + 1 < s.rows)) {
+            const int words = words_of_piece(off, c, s.C, row, s.rows, s.pitch);
+            if (words == 1) {
+                *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+            } else if (words == 2) {
                 const uint4* at = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(from) - off);
                 const uint4 a = at[0], b = at[1];
                 const unsigned w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};

@@ -200,3 +200,21 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             call()
     assert ldn._lib.lib.ldn_kernel_launches() == before
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("step", [0, 1, 3, 7, 8, 13])
+@pytest.mark.parametrize("T, K", [(5, 40), (70, 104), (9, 99), (300, 16)])
+def test_rows_that_are_repeated_or_overlap(T, K, step, dtype):
+    _, wg, wu, bg, bu, dy = made(T, K, 24, dtype)
+    f = dict(device="cuda", generator=torch.Generator(device="cuda").manual_seed(step))
+    for start in (0, 3):
+        flat = torch.randn(start + (T - 1) * step + K, **f).to(dtype)[start:]
+        x = flat[:K].expand(T, K) if step == 0 else flat.unfold(0, K, step)
+        assert x.shape == (T, K) and x.stride() == (step, 1)
+        runs = []
+        for rows in (x, x.contiguous()):
+            leaves = [t.detach().requires_grad_() for t in (rows, wg, wu, bg, bu)]
+            y = ldn.gated_linear(*leaves)
+            runs.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
+        assert all(torch.equal(a, b) for a, b in zip(*runs))
