@@ -432,10 +432,15 @@ struct Gated {
     MaybeTensor b_gate, b_up;
     int activation;
 };
+// A weight's rows; of rows that are repeated or overlap a copy, as the library takes none of them
+Rows weight_rows(const Tensor& w) {
+    const Rows rows = rows_of(w);
+    return rows.rows > 1 && rows.pitch < rows.C ? rows_of(w.contiguous()) : rows;
+}
 // (the same in both passes)
 Gated gated_of(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const MaybeTensor& b_gate, const MaybeTensor& b_up,
                int64_t activation) {
-    return {rows_of(x), rows_of(w_gate), rows_of(w_up), whole(b_gate), whole(b_up), static_cast<int>(activation)};
+    return {rows_of(x), weight_rows(w_gate), weight_rows(w_up), whole(b_gate), whole(b_up), static_cast<int>(activation)};
 }
 long long weight_pitch(const Rows& w) { return w.rows == 1 ? (w.C + 7) / 8 * 8 : w.pitch; }
 

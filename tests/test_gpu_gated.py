@@ -218,3 +218,21 @@ def test_rows_that_are_repeated_or_overlap(T, K, step, dtype):
             y = ldn.gated_linear(*leaves)
             runs.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
         assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("step", [0, 1, 8])
+@pytest.mark.parametrize("T, K", [(1, 40), (3, 1), (70, 104), (20, 16), (33, 1)])
+def test_weights_whose_rows_are_repeated_or_overlap(T, K, step, dtype):
+    x, wg, wu, bg, bu, dy = made(T, K, 24, dtype)
+    flat = torch.randn(23 * step + K, device="cuda").to(dtype)
+    w = flat.expand(24, K) if step == 0 else flat.unfold(0, K, step)
+    assert w.shape == (24, K)
+    for one, other in ((w, wu), (wg, w), (w, w)):
+        runs = []
+        for a, b in ((one, other), (one.contiguous(), other.contiguous())):
+            leaves = [t.detach().requires_grad_() for t in (x, a, b, bg, bu)]
+            y = ldn.gated_linear(*leaves)
+            runs.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
+        assert all(torch.equal(a, b) for a, b in zip(*runs))
+    assert ldn.gated_linear(x, w[:1], w[:1]).shape == (T, 1)
