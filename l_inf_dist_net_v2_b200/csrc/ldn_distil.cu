@@ -260,17 +260,18 @@ __device__ __forceinline__ List read_list(const DistilArgs& a, long long row, fl
 // The rest, by one lane: the loss, and what the backward pass needs
 __device__ __forceinline__ void finish_row(const DistilArgs& a, long long row, const List& l, const Sums& sums) {
     const float s1 = a.tau == 1.0f ? sums.s : sums.s1;
+    const bool list = l.some && a.part != 0.0f, label = l.label && a.mix != 0.0f;  // (a term without weight is none, infinite ones too)
     float loss = 0.0f;
     // (a preferred class that is no choice: infinity, whatever the others are)
-    if (l.some) loss = a.part * a.tau * a.tau * (l.reference == minus_infinity() ? -minus_infinity() : l.terms - ((l.reference - sums.m) / a.tau - logf(sums.s)));
-    if (l.label) loss += a.mix * (logf(s1) - (l.target - sums.m));
+    if (list) loss = a.part * a.tau * a.tau * (l.reference == minus_infinity() ? -minus_infinity() : l.terms - ((l.reference - sums.m) / a.tau - logf(sums.s)));
+    if (label) loss += a.mix * (logf(s1) - (l.target - sums.m));
     a.losses[row] = l.bad ? not_a_number() : loss;
     if (a.stats) {
         a.stats[row] = sums.m;
         a.stats[a.rows + row] = l.bad ? not_a_number() : 1.0f / sums.s;
         a.stats[2 * a.rows + row] = l.bad ? not_a_number() : 1.0f / s1;
         a.stats[3 * a.rows + row] = l.top;
-        a.stats[4 * a.rows + row] = l.bad ? not_a_number() : l.some ? l.inv_sum : 0.0f;
+        a.stats[4 * a.rows + row] = l.bad ? not_a_number() : list ? l.inv_sum : 0.0f;
     }
 }
 
@@ -566,7 +567,7 @@ __device__ __forceinline__ void gradient_of_row(const DistilArgs& a, long long r
     const float up = a.up[row * a.up_step] * a.up_scale;
     const float inv_sum = a.stats[4 * a.rows + row], top = a.stats[3 * a.rows + row], inv_tau = 1.0f / a.tau;
     const long long target = a.targets ? a.targets[row] : -1;
-    const bool list = inv_sum != 0.0f, label = target >= 0;  // (a list that is not a number is there)
+    const bool list = inv_sum != 0.0f, label = target >= 0 && a.mix != 0.0f;  // (a list that is not a number is there)
     const float by_list = list ? up * a.part * a.tau : 0.0f, by_label = label ? up * a.mix : 0.0f;
     RowGradient g;
     g.m = a.stats[row];

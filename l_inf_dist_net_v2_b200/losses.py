@@ -65,8 +65,8 @@ def distillation_loss(logits, teacher_values, teacher_indices, targets=None, tem
     p = softmax(teacher_values / temperature) over the row's entries and q = softmax(logits / temperature) over all classes, with the
     gradient of the logits (the teacher has none).  `teacher_values` and `teacher_indices` (..., k), k up to 1024, say which classes the
     entries are of, in any order; an entry with an index below 0 is absent, entries of one class add up.  A row without entries has no
-    first term, a row with a target below 0 no second.  An index or target beyond the classes makes its row's loss and gradient
-    not-a-numbers.
+    first term, a row with a target below 0 no second; a term that `mix` gives no weight is none, infinite ones too.  An index or target
+    beyond the classes makes its row's loss and gradient not-a-numbers.
 
     reduction: "mean" over all rows, "sum" or "none"; the loss is float32.  Logits are float32, float16 or bfloat16 and may hold minus
     infinity for classes that are no choice; sums have 32 bits and are made in one pass over the logits each way."""

@@ -207,3 +207,43 @@ def test_many_long_rows(rows, V, k, dtype):
     some = torch.tensor([bool((x[i] > -math.inf).any()) for i in keep], device="cuda")
     assert torch.equal(losses[keep].isfinite(), some) and losses[keep][~some].isnan().all()
     assert head_oracle.near(losses[keep][some], want[some], bound[some])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows, V", [(40, 12), (9, 1001), (6, 5003), (700, 8193), (6, 40001)])
+def test_a_term_without_weight_is_none(rows, V, dtype):
+    """With mix = 1 what the teacher says does not count, a class that is no choice and values that are no numbers among it."""
+    x, values, indices, targets, up = made(rows, V, 4, dtype)
+    x[0, indices[0, 0]] = x[2, indices[2, 1]] = -math.inf
+    targets[0], targets[2] = indices[0, 1], indices[2, 0]
+    values[1, 0], values[1, 1] = math.nan, math.inf
+    values[3] = -math.inf
+    targets[4] = -1
+    for tau in (1.0, 2.0, 3.0):
+        leaf = x.detach().requires_grad_()
+        losses = ldn.distillation_loss(leaf, values, indices, targets, tau, 1.0, "none")
+        want, bound, dx, off = oracle.loss_and_gradient(x, torch.zeros_like(values), torch.full_like(indices, -1), targets, tau, 1.0, up)
+        assert want.isfinite().all() and head_oracle.near(losses.detach(), want, bound)
+        assert head_oracle.near(torch.autograd.grad(losses, leaf, up)[0], dx, off)
+        assert ldn.distillation_loss(x, values, indices, targets, tau, 1.0).isfinite()
+    indices[5 % rows, 2] = V  # (an index beyond the classes is wrong whatever it counts)
+    leaf = x.detach().requires_grad_()
+    losses = ldn.distillation_loss(leaf, values, indices, targets, 2.0, 1.0, "none")
+    dx, = torch.autograd.grad(losses, leaf, torch.ones_like(losses))
+    assert losses[5 % rows].isnan() and dx[5 % rows].isnan().all() and losses.isnan().sum() == 1
+
+
+@pytest.mark.parametrize("V", [12, 5003])
+def test_labels_without_weight_are_none_in_the_library(V):
+    x, values, indices, targets, up = made(6, V, 4, F32)
+    x[0, targets[0]] = -math.inf
+    indices[0] = torch.where(indices[0] == targets[0], -1, indices[0])
+    losses, stats, grad = torch.empty(6, device="cuda"), torch.empty(5, 6, device="cuda"), torch.empty_like(x)
+    lib, at = ldn._lib.lib, [t.data_ptr() for t in (x, values, indices, targets)]
+    assert lib.ldn_distillation(at[0], V, 6, V, 0, at[1], 0, at[2], 4, at[3], 2.0, 1.0, 0.0, losses.data_ptr(), stats.data_ptr(), 1.0, None, None) == 0
+    assert lib.ldn_distillation_backward(at[0], V, 6, V, 0, at[1], 0, at[2], 4, at[3], 2.0, 1.0, 0.0, stats.data_ptr(), up.data_ptr(), 1, 1.0,
+                                         grad.data_ptr(), None) == 0
+    leaf = x.detach().requires_grad_()
+    want = ldn.distillation_loss(leaf, values, indices, temperature=2.0, reduction="none")
+    assert want.isfinite().all() and torch.equal(losses, want.detach())
+    assert torch.equal(grad, torch.autograd.grad(want, leaf, up)[0])
