@@ -480,8 +480,8 @@ LDN_API int ldn_sandwich_norm_backward(const void* grad_y, const void* grad_h, c
  *   losses[row] = part * tau^2 * sum p (log p - log q) + mix * (log sum e^x - x[target]).
  * Rows without entries (or with nothing but minus infinity in them) have no first term, rows with a target below 0, and all where
  * targets is NULL, no second; a term whose part or mix is 0 is none, whatever it would be.  An index or target of V or more makes a
- * row's loss and gradient not-a-numbers.  1 <= k <= 1024; the same index may come several times.  value_type: type of the values.
- * stats: 5 x rows floats for the backward pass, or NULL.
+ * row's loss and gradient not-a-numbers.  1 <= k <= 1024; the same index may come several times (p and log p are each entry's own, and
+ * the gradient adds them up).  value_type: type of the values.  stats: 5 x rows floats for the backward pass, or NULL.
  * loss: receives loss_scale * the sum of the losses, in a fixed order, or NULL.
  */
 LDN_API int ldn_distillation(const void* x, long long pitch, long long rows, int V, int type, const void* values, int value_type,

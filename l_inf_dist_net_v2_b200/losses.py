@@ -64,7 +64,9 @@ def distillation_loss(logits, teacher_values, teacher_indices, targets=None, tem
 
     p = softmax(teacher_values / temperature) over the row's entries and q = softmax(logits / temperature) over all classes, with the
     gradient of the logits (the teacher has none).  `teacher_values` and `teacher_indices` (..., k), k up to 1024, say which classes the
-    entries are of, in any order; an entry with an index below 0 is absent, entries of one class add up.  A row without entries has no
+    entries are of, in any order; an entry with an index below 0 is absent.  Entries of one class add up beside log q
+    and in the gradient, while log p is each entry's own: a class that is listed several times lowers the loss by a number that does
+    not depend on the logits (twice alike, with nothing else to choose: -temperature^2 log 2).  A row without entries has no
     first term, a row with a target below 0 no second; a term that `mix` gives no weight is none, infinite ones too.  An index or target
     beyond the classes makes its row's loss and gradient not-a-numbers.
 

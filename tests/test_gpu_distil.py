@@ -247,3 +247,30 @@ def test_labels_without_weight_are_none_in_the_library(V):
     want = ldn.distillation_loss(leaf, values, indices, temperature=2.0, reduction="none")
     assert want.isfinite().all() and torch.equal(losses, want.detach())
     assert torch.equal(grad, torch.autograd.grad(want, leaf, up)[0])
+
+
+@pytest.mark.parametrize("V", [10, 1001, 5003])
+def test_entries_of_one_class_against_their_dense_sum(V):
+    """With P the sum of a class's p, made densely in 64 bits: the gradient is that of P, the loss the divergence of P and, as log p is each
+    entry's own, sum p log p - sum P log P less."""
+    tau, k = 2.0, 6
+    x, values, indices, _, up = made(8, V, k, F32)
+    indices[:, 3] = indices[:, 0]
+    indices[:, 5] = indices[:, 0]
+    indices[1] = indices[1, 0]
+    indices[2, 4] = -1
+    x[0] = -math.inf  # two equal entries of one class, which is all that there is to choose
+    x[0, 7], indices[0], values[0, :2] = 0.5, torch.tensor([7, 7, -1, -1, -1, -1], device="cuda"), 1.25
+    leaf = x.detach().requires_grad_()
+    losses = ldn.distillation_loss(leaf, values, indices, temperature=tau, reduction="none")
+    dx, = torch.autograd.grad(losses, leaf, up)
+    there = indices >= 0
+    p = torch.softmax(torch.where(there, values.double() / tau, -math.inf), 1)
+    P = torch.zeros(8, V, device="cuda", dtype=torch.float64).scatter_add_(1, indices.clamp_min(0), torch.where(there, p, 0.0))
+    log_q = torch.log_softmax(x.double() / tau, 1)
+    dense = (torch.xlogy(P, P) - torch.where(P > 0, P * log_q, 0.0)).sum(1)
+    want = tau ** 2 * (dense + torch.xlogy(p, p).sum(1) - torch.xlogy(P, P).sum(1))
+    _, bound, _, off = oracle.loss_and_gradient(x, values, indices, None, tau, 0.0, up)
+    assert head_oracle.near(losses.detach(), want, bound)
+    assert head_oracle.near(dx, up.double()[:, None] * tau * (log_q.exp() - P), off)
+    assert abs(losses[0] + tau ** 2 * math.log(2)) <= 2.0 ** -20 and losses[0] < 0
