@@ -450,9 +450,9 @@ LDN_API int ldn_gated_linear_backward(const void* grad_y, const void* x, long lo
 /*
  * A block's result joined to the residual stream between two norms: with norm(v) = (v - mean) / sqrt(mean((v - mean)^2) + eps),
  *   h = residual + gate * scale * (norm(x) * post_weight + post_bias), rounded to the rows' type,   y = norm(h) * weight + bias.
- * gate_kind: LDN_GATE_NONE (1), LDN_GATE_ROW (a number per row, contiguous) or LDN_GATE_ALL (a number per element, rows pitch_gate apart), of
- * the rows' type.  scale and the norms' parameters (any may be NULL) have C elements of param_type: LDN_F32, or the rows' type.
- * stats: 4 x rows floats for the backward pass, or NULL.  y and h are contiguous.
+ * gate_kind: LDN_GATE_NONE (the gate is 1 and `gate` is not read), LDN_GATE_ROW (a number per row, contiguous) or LDN_GATE_ALL (a number
+ * per element, rows pitch_gate apart), of the rows' type.  scale and the norms' parameters (any may be NULL) have C elements of
+ * param_type: LDN_F32, or the rows' type.  stats: 4 x rows floats for the backward pass, or NULL.  y and h are contiguous.
  */
 #define LDN_GATE_NONE 0
 #define LDN_GATE_ROW 1

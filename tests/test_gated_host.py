@@ -2,6 +2,8 @@
 import copy
 import ctypes
 import math
+import os
+import re
 
 import pytest
 import torch
@@ -161,3 +163,13 @@ def test_calls_without_rows_do_nothing():
     assert lib.ldn_gated_linear(None, 4, 0, 4, 4, 0, None, 4, None, 4, None, None, 0, 3, None, None, None, 0, None, None) == 0
     assert lib.ldn_sandwich_norm(None, 4, None, 4, None, 0, 0, 0, 4, 0, None, None, None, None, None, 0, 1e-5, None, None, None, None) == 0
     assert lib.ldn_distillation_backward(None, 4, 0, 4, 0, None, 0, None, 2, None, 1.0, 1.0, 0.0, None, None, 0, 1.0, None, None) == 0
+
+
+def test_the_kinds_of_gates_are_what_the_header_says():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with open(os.path.join(root, "include", "ldn_b200.h")) as f:
+        header = f.read()
+    kinds = dict(re.findall(r"#define (LDN_GATE_\w+) (\d+)", header))
+    assert kinds == dict(LDN_GATE_NONE="0", LDN_GATE_ROW="1", LDN_GATE_ALL="2")
+    for name, number in re.findall(r"(LDN_GATE_\w+) \((\d+)\)", header):  # (as comments number them)
+        assert kinds[name] == number
