@@ -1,5 +1,7 @@
 """The gated head and its distillation as a program uses them: whole steps, in mixed precision, recorded, recomputed, from several threads."""
 import copy
+import os
+import re
 import threading
 
 import pytest
@@ -192,3 +194,25 @@ def test_another_stream_and_several_threads():
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_the_example_of_the_documentation():
+    """The code of INTEGRATION.md's section on the gated head, as it is written, on what its names stand for."""
+    with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")) as f:
+        section = f.read().split("## 7. ")[1].split("\n## ")[0]
+    code, = re.findall(r"```python\n(.*?)```", section, re.S)
+    f = _gen(5)
+    names = dict(torch=torch, ldn=ldn, x=torch.randn(12, 96, **f), residual=torch.randn(12, 96, **f), weight=torch.ones(96, device="cuda"),
+                 bias=torch.zeros(96, device="cuda"), w1=torch.ones(96, device="cuda"), b1=torch.zeros(96, device="cuda"),
+                 s=torch.full((96,), 0.1, device="cuda"), g=torch.rand(12, 1, **f), images=torch.rand(12, 3, 32, 32, **f))
+    for name in ("gate", "up"):
+        names["weight_" + name], names["bias_" + name] = torch.randn(40, 96, **f), torch.randn(40, **f)
+    with torch.device("cuda"):
+        names["teacher"] = torch.nn.Sequential(torch.nn.Flatten(), torch.nn.LazyLinear(10))
+    with torch.no_grad():
+        logits = names["teacher"](names["images"])
+    names["logits"], (names["values"], names["indices"]), names["targets"] = logits, logits.topk(3), logits.argmax(1)
+    with torch.device("cuda"):
+        exec(code, names)
+    assert names["y"].shape == names["h"].shape == (12, 96) and names["loss"].isfinite()
+    assert all(p.grad is not None and p.grad.isfinite().all() for p in names["model"].head.parameters())
