@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kColumns * kColumnLanes) sandwich_grad_columns
                 const long long row = row0 + u * kColumnLanes, at = row * a.C + c;
                 if (row >= last) continue;
                 const float rstd2 = a.stats[3 * a.rows + row];
-                const float z2 = (to_float(static_cast<const T*>(a.h)[at]) - a.stats[2 * a.rows + row]) * rstd2;
+                const float z2 = a.grad_y ? (to_float(static_cast<const T*>(a.h)[at]) - a.stats[2 * a.rows + row]) * rstd2 : 0.0f;
                 const float z1 = (to_float(static_cast<const T*>(a.x)[row * a.pitch + c]) - a.stats[row]) * a.stats[a.rows + row];
                 const float g = a.grad_y ? to_float(static_cast<const T*>(a.grad_y)[at]) : 0.0f;
                 float d = stream_gradient<T>(a, at, c, z2, rstd2, a.row_sums[row], a.row_sums[a.rows + row]);

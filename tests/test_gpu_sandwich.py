@@ -222,3 +222,25 @@ def test_many_rows_that_blocks_share(rows, C, dtype):
     for gate in ("none", "row", "all"):
         check(*made(rows, C, dtype, gate, F32 if gate == "row" else dtype))
     check(*made(rows, C, dtype, "all", F32, layout="shifted"), use=("y",))
+
+
+@pytest.mark.parametrize("gate", ["none", "row", "all"])
+@pytest.mark.parametrize("C, layout", [(96, "plain"), (33, "plain"), (1024, "plain"), (4097, "plain"), (16384, "plain"), (60000, "plain"), (520, "shifted")])
+def test_without_the_gradient_of_y_it_does_not_matter_what_h_is(C, layout, gate):
+    """h with infinities and what is not a number: the gradients of h alone are those of any other h."""
+    for dtype in TYPES:
+        t, _, dh = made(9, C, dtype, gate, F32, layout)
+        held = {k: v if v is None else v.detach() for k, v in t.items()}
+        want = oracle.backward(None, dh, held["x"], held["x"], held["gate"], held["scale"], held["pw"], held["pb"], held["w"], 0.0)
+        t["residual"] = t["residual"].clone()
+        t["residual"][2, C // 2], t["residual"][4, 0], t["residual"][5, C - 1] = float("inf"), float("-inf"), float("nan")
+        t = {k: v if v is None else v.detach().requires_grad_() for k, v in t.items()}
+        h = call(t, 0.0)[1]
+        assert not h[2, C // 2].isfinite() and not h[5, C - 1].isfinite()
+        leaves = {k: v for k, v in t.items() if v is not None}
+        for name, g in zip(leaves, torch.autograd.grad(h, list(leaves.values()), dh)):
+            if name in ("w", "b"):
+                assert not g.any(), name
+            else:
+                assert head_oracle.near(g, want[name][0].view_as(g), want[name][1].view_as(g)), name
+        assert torch.equal(torch.autograd.grad(call(t, 0.0)[1], t["residual"], dh)[0], dh)
