@@ -92,10 +92,8 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
 #pragma unroll
                 for (int i = 0; i < ITEMS; ++i) {
                     copy_piece<T, SHIFT>(slot_of(stage, j, 0, i), from_x.of(j, i * apart), column(i), bytes[i], a.x);
-                    if (a.grad_y) {
-                        copy_piece<T, SHIFT>(slot_of(stage, j, 1, i), from_h.of(j, i * apart), column(i), bytes[i], a.h);
-                        copy_piece<T, SHIFT>(slot_of(stage, j, 2, i), from_dy.of(j, i * apart), column(i), bytes[i], a.grad_y);
-                    }
+                    copy_piece<T, SHIFT>(slot_of(stage, j, 1, i), from_h.of(j, i * apart), column(i), bytes[i], a.h);
+                    if (a.grad_y) copy_piece<T, SHIFT>(slot_of(stage, j, 2, i), from_dy.of(j, i * apart), column(i), bytes[i], a.grad_y);
                     if (a.grad_h) copy_piece<T, SHIFT>(slot_of(stage, j, 3, i), from_dh.of(j, i * apart), column(i), bytes[i], a.grad_h);
                     if constexpr (G == Gate::All)
                         copy_piece<T, SHIFT>(slot_of(stage, j, 4, i), from_gate.of(j, i * apart), column(i), bytes[i], a.gate);
@@ -109,12 +107,11 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
         from_dh.on(R);
         if constexpr (G == Gate::All) from_gate.on(R);
     };
-    // (zeros for pieces behind the row's end, and for a gradient that does not come; without that of y, h and its statistics are zeros too:
-    // they do not matter, whatever they are)
+    // (zeros for pieces behind the row's end, and for a gradient that does not come)
     for (int d = 0; d < depth * R * S; ++d)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
-            if (!bytes[i] || (!a.grad_y && (d % S == 1 || d % S == 2)) || (!a.grad_h && d % S == 3)) own[(d * ITEMS + i) * blockDim.x] = make_uint4(0u, 0u, 0u, 0u);
+            if (!bytes[i] || (!a.grad_y && d % S == 2) || (!a.grad_h && d % S == 3)) own[(d * ITEMS + i) * blockDim.x] = make_uint4(0u, 0u, 0u, 0u);
     for (int d = 0; d < depth; ++d) fetch(d);
     constexpr int kNumbers = G == Gate::Row ? 5 : 4;
     __shared__ float numbers[kNumbers][kNumberRows];
@@ -127,7 +124,7 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
         float mean1[R], rstd1[R], mean2[R], rstd2[R], gate[R], s[2 * R], t[K * R];
         RowNumbers<kNumbers, R * kNumberRows> of_rows(numbers, R * per_block);
         of_rows.at_turn(turn, a.rows, [&](int i) { return row_of(turn, i); }, [&](int k, long long row) {
-            return k < 4 ? (k < 2 || a.grad_y ? a.stats[k * a.rows + row] : 0.0f) : to_float(static_cast<const T*>(a.gate)[row]);
+            return k < 4 ? a.stats[k * a.rows + row] : to_float(static_cast<const T*>(a.gate)[row]);
         });
 #pragma unroll
         for (int j = 0; j < R; ++j) {
