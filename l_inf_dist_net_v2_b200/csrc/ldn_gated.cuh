@@ -49,6 +49,7 @@ struct TileArgs {
     int tiles_m, tiles_n;
     int tiles, whole, pairs;  // of the tiles, how many a pair of CTAs takes as a whole; the rest are shared out in units
     int units, side_units, side_steps;
+    bool drained;  // sums of 16-bit products leave the accumulator after every unit
     const void *b_gate, *b_up;
     bool wide;
     int activation;

@@ -9,7 +9,7 @@ int resident_pairs(const DeviceCtx* ctx) {
     static std::atomic<int> known[64];
     const int have = known[ctx->device].load(std::memory_order_acquire);
     if (have > 0) return have;
-    constexpr auto kernel = gated_tiles_kernel<__nv_bfloat16, GatedForm::Forward>;
+    constexpr auto kernel = gated_tiles_kernel<__nv_bfloat16, GatedForm::Forward, false>;
     cudaLaunchAttribute attr[1] = {};
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
@@ -35,7 +35,8 @@ int steps_over(long long n, int size) { return static_cast<int>((n + size - 1) /
 // (both in clocks: a step takes 512, a pair stores and another kernel reads 1 KB per row of a part at 4000 bytes per clock).
 void plan(GatedForm form, long long M, int N, int terms, int type, const DeviceCtx* ctx, TileArgs* a) {
     const bool parted = type == LDN_F32;
-    const int unit_steps = parted ? kUnitSteps<float> : 1;
+    a->drained = !parted && static_cast<long long>(terms) * (form == GatedForm::GradRows ? 2 : 1) > kMostTerms;
+    const int unit_steps = parted ? kUnitSteps<float, false> : a->drained ? kUnitSteps<__half, true> : 1;
     a->M = M;
     a->N = N;
     a->tiles_m = steps_over(M, kSide);
@@ -44,7 +45,7 @@ void plan(GatedForm form, long long M, int N, int terms, int type, const DeviceC
     a->side_steps = steps_over(terms, kStepTerms);
     a->side_units = steps_over(a->side_steps, unit_steps);
     a->units = a->side_units * (form == GatedForm::GradRows ? 2 : 1);
-    const long long least = parted ? 1 : 4, shares = (static_cast<long long>(a->tiles) * a->units + least - 1) / least;
+    const long long least = parted || a->drained ? 1 : 4, shares = (static_cast<long long>(a->tiles) * a->units + least - 1) / least;
     const int held = resident_pairs(ctx), resident = held < kMostPairs ? held : kMostPairs;
     // (a tile each at least: 85, 9 -> 7429 bf16 has 59 of one step; by 15 pairs it took 54 us, by 59 21)
     const long long wanted = shares > a->tiles ? shares : a->tiles;
@@ -66,9 +67,9 @@ int map_of(CUtensorMap* map, const Images& o, bool across) {
     return make_image_map(map, o.base, o.columns, o.rows, o.count, o.pitch, o.count > 1 ? o.apart : o.pitch, across ? kStepTerms : 128);
 }
 
-template <class T, GatedForm F>
+template <class T, GatedForm F, bool LONG>
 int launch(const TileArgs& a, const CUtensorMap& map_a, const CUtensorMap& map_b0, const CUtensorMap& map_b1, cudaStream_t st) {
-    constexpr auto kernel = gated_tiles_kernel<T, F>;
+    constexpr auto kernel = gated_tiles_kernel<T, F, LONG>;
     static OncePerDevice once;
     int r = once([] { return allow_smem(kernel, kTileSmem); });
     if (r != kOk) return r;
@@ -98,11 +99,17 @@ int launch_gated_tiles(GatedForm form, TileArgs a, int terms, const Images& op_a
     if (r != kOk) return r;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        switch (form) {
-            case GatedForm::Forward: return launch<T, GatedForm::Forward>(a, map_a, map_b0, map_b1, st);
-            case GatedForm::GradRows: return launch<T, GatedForm::GradRows>(a, map_a, map_b0, map_b1, st);
-            default: return launch<T, GatedForm::GradWeights>(a, map_a, map_b0, map_b1, st);
-        }
+        auto go = [&](auto drained) {
+            constexpr bool kLong = decltype(drained)::value;
+            switch (form) {
+                case GatedForm::Forward: return launch<T, GatedForm::Forward, kLong>(a, map_a, map_b0, map_b1, st);
+                case GatedForm::GradRows: return launch<T, GatedForm::GradRows, kLong>(a, map_a, map_b0, map_b1, st);
+                default: return launch<T, GatedForm::GradWeights, kLong>(a, map_a, map_b0, map_b1, st);
+            }
+        };
+        if constexpr (!kParted<T>)
+            if (a.drained) return go(std::true_type());
+        return go(std::false_type());
     });
 }
 

@@ -7,8 +7,10 @@
 //
 // 32-bit operands are the sums of three bfloat16 images, 24 bits, and the six products of images down to 2^-18 are taken (what is left
 // out is 2^-24 of a term or less): at the rate of 16-bit products a sixth, four times that of the 32-bit pipe.  The accumulator drops
-// bits towards zero, 3.5e-8 of it per instruction on average, so sums stay in it for 256 terms at a time, small images first, and
-// are added up in registers.
+// bits towards zero, 7e-8 of it per instruction on average, so sums stay in it for 256 terms at a time, small images first, and
+// are added up in registers.  Sums of 16-bit products stay in it for 16384 terms (positive ones come 1e-4 too small at most, a fifth of what
+// float16 rounds to); longer ones leave it after every 4096 (LONG): of 262144 terms they came 1.1e-3 too small, now 4e-5 (gradients of 2048 x
+// 2048 weights in float16: 4.67 and 4.83 ms).
 //
 // What does not fill all pairs at the end is shared out among them in equal ranges of terms; a second kernel adds up the parts, in order.
 //
@@ -35,8 +37,9 @@ template <class T>
 constexpr int kParts = kParted<T> ? 3 : 1;
 // steps of a unit: of what is shared out, and at 32 bits of what stays in the accumulator (512 x 5120 -> 2048 in float32 with gradients,
 // 2 / 4 / 8 steps: 381 / 374 / 382 us)
-template <class T>
-constexpr int kUnitSteps = kParted<T> ? 4 : 1;
+template <class T, bool LONG>
+constexpr int kUnitSteps = kParted<T> ? 4 : LONG ? 64 : 1;
+constexpr int kMostTerms = 16384;  // of 16 bits that stay in the accumulator
 // the products of images, smallest first
 __device__ __forceinline__ int part_of_a(int pass) { return (0x001102 >> 4 * pass) & 15; }
 __device__ __forceinline__ int part_of_b(int pass) { return (0x010120 >> 4 * pass) & 15; }
@@ -191,11 +194,12 @@ __device__ __forceinline__ void finish(const TileArgs& a, int which, long long m
     }
 }
 
-template <class T, GatedForm F>
+template <class T, GatedForm F, bool LONG>
 __global__ void __launch_bounds__(kProductThreads, 1)
 gated_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b0,
                    const __grid_constant__ CUtensorMap map_b1, const __grid_constant__ TileArgs a) {
     constexpr bool kGated = F == GatedForm::Forward, kAcrossA = F == GatedForm::GradWeights, kAcrossB = !kGated;
+    constexpr bool kDrained = kParted<T> || LONG;  // sums leave the accumulator after every unit
     constexpr int kPasses = kParted<T> ? 6 : 1, kAheadA = kAcrossA ? 128 : 2, kAheadB = kAcrossB ? 128 : 2;
     constexpr uint32_t kKind = kind_of<T>(kAcrossA, kAcrossB);
     extern __shared__ char raw[];
@@ -227,8 +231,8 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     auto give_up = [&]() { atomicExch(a.status, static_cast<int>(kDeviceTimeout)); };
     // steps of a unit on its side (the two sides: dg with the gate's weights, du with the other's)
     auto steps_of = [&](int unit) {
-        const int left = a.side_steps - (unit < a.side_units ? unit : unit - a.side_units) * kUnitSteps<T>;
-        return left < kUnitSteps<T> ? left : kUnitSteps<T>;
+        const int left = a.side_steps - (unit < a.side_units ? unit : unit - a.side_units) * kUnitSteps<T, LONG>;
+        return left < kUnitSteps<T, LONG> ? left : kUnitSteps<T, LONG>;
     };
     Segments seg(a, pair);
     if (warp == 0) {
@@ -243,7 +247,7 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 const int n = kGated ? p.n * 128 : p.n * kSide + rank * 128;
                 for (int u = seg.first; u < seg.last && fine; ++u) {
                     const int side = u >= a.side_units, steps = steps_of(u);
-                    const int term0 = (u - (side ? a.side_units : 0)) * kUnitSteps<T> * kStepTerms;
+                    const int term0 = (u - (side ? a.side_units : 0)) * kUnitSteps<T, LONG> * kStepTerms;
                     const CUtensorMap* map_b = (kGated ? rank : side) ? &map_b1 : &map_b0;
                     const int first_image = (F == GatedForm::GradRows ? side : which) * kParts<T>;
 #pragma unroll 1
@@ -286,14 +290,14 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     } else if (warp == 1) {
         if (rank == 0 && elected()) {
             bool fine = true;
-            int batch = 0;  // sums that leave together: a segment's, of 32-bit operands a unit's
+            int batch = 0;  // sums that leave together: a segment's, or a unit's
             RingPlace<kStages> at;
             const uint64_t a0 = kAcrossA ? operand_across(stage) : operand(stage);
             const uint64_t b0 = kAcrossB ? operand_across(stage + kHalfBytes) : operand(stage + kHalfBytes);
             while (fine && seg.next(a)) {
                 bool add = false;
                 for (int u = seg.first; u < seg.last && fine; ++u) {
-                    if (kParted<T> || u == seg.first) {
+                    if (kDrained || u == seg.first) {
                         if (batch >= 2 && !wait_bounded_cluster(&B->taken[batch & 1], (batch / 2 - 1) & 1)) {
                             fine = false;
                             break;
@@ -313,7 +317,7 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                         add = true;
                         arrive_when_done<2>(&B->empty[at.stage]);
                     }
-                    if (fine && (kParted<T> || u == seg.last - 1)) {
+                    if (fine && (kDrained || u == seg.last - 1)) {
                         arrive_when_done<2>(&B->sums[batch & 1]);
                         ++batch;
                     }
@@ -351,7 +355,7 @@ gated_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             const long long m = static_cast<long long>(which ? p.m - a.tiles_m : p.m) * kSide + row;
             const int n = kGated ? p.n * 128 + 64 * half : p.n * kSide + 128 * half;  // of this warp's first run
             float* part = a.partials + (static_cast<size_t>(seg.slot) * kSide + row) * kSide;
-            if constexpr (kParted<T>) {
+            if constexpr (kDrained) {
                 float acc[8][16];
 #pragma unroll
                 for (int r = 0; r < 8; ++r)

@@ -236,3 +236,40 @@ def test_weights_whose_rows_are_repeated_or_overlap(T, K, step, dtype):
             runs.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
         assert all(torch.equal(a, b) for a, b in zip(*runs))
     assert ldn.gated_linear(x, w[:1], w[:1]).shape == (T, 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("T, K, H", [(16385, 72, 40), (20000, 200, 300), (40, 16400, 72), (300, 20001, 130), (24, 40, 8193), (300, 72, 10000)])
+def test_sums_of_more_terms_than_stay_in_the_accumulator(T, K, H, dtype):
+    check(*made(T, K, H, dtype), "silu")
+
+
+# (sums leave the accumulator after 4096 terms: 256 instructions that drop less than 2^-23 of it each; then they are added up in 32 bits, and so
+# are the parts of a tile that several pairs of CTAs share)
+def drained(terms):
+    return 256 * 2.0 ** -23 + (terms / 4096 + 80) * head_oracle.EPS32
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_long_sums_are_not_smaller_for_it(dtype):
+    """Sums of positive products alone, with relu of one as the gate: y = u, du = dy and dg = dy u exactly where u is a power of two."""
+    f = dict(device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    T, C = 262144, 2048
+    x, dy = (torch.rand(T, C, **f) + 0.5).to(dtype), ((torch.rand(T, C, **f) + 0.5) * 2.0 ** -6).to(dtype)
+    zero, one = torch.zeros(C, C, device="cuda", dtype=dtype), torch.ones(C, device="cuda", dtype=dtype)
+    wu = zero.clone().requires_grad_()
+    got, = torch.autograd.grad(ldn.gated_linear(x, zero, wu, one, one, activation="relu"), wu, dy)
+    want = torch.cat([dy[:, i:i + 8].double().t() @ x.double() for i in range(0, 64, 8)])
+    assert head_oracle.near(got[:64], want, drained(T) * want)
+    del x, dy, got
+    T, K, H = 600, 131072, 1100
+    x, wu = (torch.rand(T, K, **f) + 0.5).to(dtype), ((torch.rand(H, K, **f) + 0.5) * 2.0 ** -7).to(dtype)
+    got = ldn.gated_linear(x, torch.zeros_like(wu), wu, torch.ones(H, device="cuda", dtype=dtype), activation="relu")
+    want = x[:64].double() @ wu.double().t()
+    assert head_oracle.near(got[:64], want, (drained(K) + 4 * head_oracle.EPS32) * want)
+    T, K, H = 300, 600, 131072
+    dy, w = ((torch.rand(T, H, **f) + 0.5) * 2.0 ** -7).to(dtype), (torch.rand(H, K, **f) + 0.5).to(dtype)
+    x, one = torch.zeros(T, K, device="cuda", dtype=dtype, requires_grad=True), torch.ones(H, device="cuda", dtype=dtype)
+    got, = torch.autograd.grad(ldn.gated_linear(x, w, w, one, one, activation="relu"), x, dy)
+    want = 2 * dy[:64].double() @ w.double()
+    assert head_oracle.near(got[:64], want, drained(2 * H) * want)
