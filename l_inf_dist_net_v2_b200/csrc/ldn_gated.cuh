@@ -66,9 +66,35 @@ int launch_gated_tiles(GatedForm form, TileArgs a, int terms, const Images& op_a
 #ifdef __CUDACC__
 // 1 / (1 + e^-g); the quotient's error is 2 units at most, and it is 0 where e^-g has no number
 __device__ __forceinline__ float logistic(float g) { return __fdividef(1.0f, 1.0f + expf(-g)); }
+// The normal distribution's function, and e^(-g^2 / 2).  With t = |g|, the smaller of the function's two sides is e^(-t^2 / 2) q(t), q falling
+// from 1/2 to 0.4 / t: u P(u) with u = 1 / (1 + 0.24 t), P of degree 9 fitted to q(t) / u over u(0 .. 20) for the least relative error, 4e-9.
+// What t^2 is rounded by is put back.  A dozen units of 2^-24 of itself at most, on either side (0.5 (1 + erf) leaves nothing of it
+// below -5.5).
+struct Normal {
+    float cdf, bell;
+};
+__device__ __forceinline__ Normal normal_of(float g) {
+    float t;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(t) : "f"(fabsf(g)), "f"(20.0f));  // (both are 0 there)
+    const float u = __fdividef(1.0f, fmaf(0.24f, t, 1.0f));
+    float p = 0.025488367f;
+    p = fmaf(p, u, -0.12448445f);
+    p = fmaf(p, u, 0.20524898f);
+    p = fmaf(p, u, -0.14414364f);
+    p = fmaf(p, u, 0.14150542f);
+    p = fmaf(p, u, 0.028033895f);
+    p = fmaf(p, u, 0.0878384f);
+    p = fmaf(p, u, 0.08890992f);
+    p = fmaf(p, u, 0.0958613f);
+    p = fmaf(p, u, 0.0957418f);
+    const float square = __fmul_rn(t, t), rest = fmaf(t, t, -square);
+    float bell = expf(-0.5f * square);
+    bell = fmaf(bell, -0.5f * rest, bell);
+    const float low = bell * (u * p);
+    return {g < 0.0f ? low : 1.0f - low, bell};
+}
 // (called: see tanh_called of the integer product)
-static __device__ __noinline__ float normal_cdf(float g) { return 0.5f * (1.0f + erff(g * 0.70710678118654752f)); }
-__device__ __forceinline__ float normal_pdf(float g) { return 0.39894228040143268f * expf(-0.5f * g * g); }
+static __device__ __noinline__ float normal_cdf(float g) { return normal_of(g).cdf; }
 
 // act(g) of N numbers
 template <int N>
@@ -91,8 +117,8 @@ __device__ __forceinline__ void activate(float (&g)[N], int activation) {
 __device__ __forceinline__ float2 activation_and_slope(float g, int activation) {
     if (activation == LDN_RELU) return make_float2(g < 0.0f ? 0.0f : g, g > 0.0f ? 1.0f : 0.0f);
     if (activation == LDN_GELU) {
-        const float c = normal_cdf(g);
-        return make_float2(g * c, c + g * normal_pdf(g));
+        const Normal n = normal_of(g);
+        return make_float2(g * n.cdf, n.cdf + g * (0.39894228040143268f * n.bell));
     }
     const float s = logistic(g);
     return activation == LDN_SIGMOID ? make_float2(s, s * (1.0f - s)) : make_float2(g * s, s * (1.0f + g * (1.0f - s)));

@@ -273,3 +273,28 @@ def test_long_sums_are_not_smaller_for_it(dtype):
     got, = torch.autograd.grad(ldn.gated_linear(x, w, w, one, one, activation="relu"), x, dy)
     want = 2 * dy[:64].double() @ w.double()
     assert head_oracle.near(got[:64], want, drained(2 * H) * want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("T", [1, 40])
+def test_gelu_keeps_its_digits_far_below_zero(T, dtype):
+    """The gate is a bias alone, so that the function and its slope come by themselves.  The normal distribution's function is off by a dozen units
+    of itself, e^(-g^2 / 2) by eight; products and sums round once each (and a bias's gradient T / 8 + 64 times)."""
+    g = torch.cat([torch.linspace(-14, 10, 8000), torch.tensor([-0.0, 0.0, -30.0, 30.0, 1e30, -1e30])]).cuda()
+    H, unit, least = g.numel(), head_oracle.EPS32, 64 * 2.0 ** -149
+    x, w, one = torch.zeros(T, 8, device="cuda", dtype=dtype), torch.zeros(H, 8, device="cuda", dtype=dtype), torch.ones(H, device="cuda")
+    leaf = g.clone().requires_grad_()
+    y = ldn.gated_linear(x, w, w, leaf, one, activation="gelu")
+    got, = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    g = g.double()
+    cdf = 0.5 * torch.special.erfc(-g * 0.5 ** 0.5)
+    bell = g * torch.exp(-g * g / 2) / (2 * torch.pi) ** 0.5
+    want = (g * cdf).expand(T, H)
+    held = want.abs() <= torch.finfo(dtype).max  # (1e30 is infinity in float16)
+    assert head_oracle.near(y.detach()[held], want[held], 16 * unit * want[held].abs() + least)
+    assert (y.detach()[~held] == float("inf")).all() and (dtype == torch.float16 or held.all())
+    bound = unit * (16 * cdf + 12 * bell.abs() + (T / 8 + 64) * (T > 1) * (cdf + bell).abs()) + least
+    assert head_oracle.near(got, T * (cdf + bell), T * bound)
+    ends = torch.tensor([float("inf"), float("nan")], device="cuda")
+    y = ldn.gated_linear(x, w[:2], w[:2], ends, one[:2], activation="gelu")
+    assert (y[:, 0] == float("inf")).all() and y[:, 1].isnan().all()
