@@ -120,8 +120,10 @@ __device__ __forceinline__ float2 activation_and_slope(float g, int activation) 
         const Normal n = normal_of(g);
         return make_float2(g * n.cdf, n.cdf + g * (0.39894228040143268f * n.bell));
     }
-    const float s = logistic(g);
-    return activation == LDN_SIGMOID ? make_float2(s, s * (1.0f - s)) : make_float2(g * s, s * (1.0f + g * (1.0f - s)));
+    // (s and 1 - s from e^-|g|, so that the smaller one keeps its digits)
+    const float e = expf(-fabsf(g)), larger_one = __fdividef(1.0f, 1.0f + e), smaller_one = e * larger_one;
+    const float s = g < 0.0f ? smaller_one : larger_one, rest = g < 0.0f ? larger_one : smaller_one;
+    return activation == LDN_SIGMOID ? make_float2(s, s * rest) : make_float2(g * s, s * (1.0f + g * rest));
 }
 #endif
 

@@ -298,3 +298,19 @@ def test_gelu_keeps_its_digits_far_below_zero(T, dtype):
     ends = torch.tensor([float("inf"), float("nan")], device="cuda")
     y = ldn.gated_linear(x, w[:2], w[:2], ends, one[:2], activation="gelu")
     assert (y[:, 0] == float("inf")).all() and y[:, 1].isnan().all()
+
+
+@pytest.mark.parametrize("T", [1, 40])
+def test_the_slope_of_a_gate_that_is_wide_open_keeps_its_digits(T):
+    """As for gelu; s and 1 - s are off by eight units of themselves, their product by two more."""
+    g, unit = torch.linspace(-80, 80, 8001).cuda(), head_oracle.EPS32
+    H = g.numel()
+    x, w, one = torch.zeros(T, 8, device="cuda"), torch.zeros(H, 8, device="cuda"), torch.ones(H, device="cuda")
+    chain = 18 + (T / 8 + 64) * (T > 1)
+    e = torch.exp(-g.double().abs())
+    s = torch.where(g < 0, e, 1.0) / (1 + e)
+    rest = torch.where(g < 0, 1.0, e) / (1 + e)
+    for name, want, size in (("sigmoid", s * rest, s * rest), ("silu", s * (1 + g.double() * rest), s * (1 + g.double().abs() * rest))):
+        leaf = g.clone().requires_grad_()
+        got, = torch.autograd.grad(ldn.gated_linear(x, w, w, leaf, one, activation=name).sum(), leaf)
+        assert head_oracle.near(got, T * want, T * chain * unit * size), name
