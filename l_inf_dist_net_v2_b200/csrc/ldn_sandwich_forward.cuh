@@ -10,7 +10,7 @@ __global__ void __launch_bounds__(W == Share::Group ? kGroupThreads : most_threa
 sandwich_registers_kernel(const __grid_constant__ SandwichArgs a, int lanes, int depth, int ranks) {
     stream_order_begin();
     constexpr bool GROUP = W == Share::Group, kKeep = ITEMS * kPiece<T> <= 16;  // (the columns' parameters stay in registers)
-    constexpr int V = kPiece<T>, S = kForwardStreams<G>, R = rows_forward(ITEMS * V, sizeof(T), GROUP, SHIFT);
+    constexpr int V = kPiece<T>, S = kForwardStreams<G>, R = rows_forward(ITEMS * V);
     __shared__ alignas(16) float slots[2 * SumOf<W>::kSlots];
     extern __shared__ uint4 ring[];  // [depth][row][stream][item][thread]
     const int rank = W == Share::Cluster ? static_cast<int>(cluster_rank()) : 0;
@@ -201,7 +201,7 @@ bool sandwich_rows(Gate gate, const SandwichArgs& a, const DeviceCtx* ctx, cudaS
             constexpr int kItems = decltype(items)::value;
             constexpr Share W = decltype(share)::value;
             constexpr auto kernel = sandwich_registers_kernel<T, G, kItems, W, decltype(shift)::value>;
-            constexpr int R = rows_forward(kItems * kPiece<T>, sizeof(T), W == Share::Group, decltype(shift)::value);
+            constexpr int R = rows_forward(kItems * kPiece<T>);
             long long resident;
             int depth;
             RowShape s;

@@ -8,8 +8,8 @@
 // norm's parameters are two numbers per column, scale weight and scale bias.
 //
 // 16384 x 5120 bf16 with a gate of its shape: forward 180 us, 4.7 TB/s, backward 287, 4.7 (228 with the sums over rows left out: what the warps
-// wait for); 8192 x 5120 float32 150 and 269; 524288 x 96 bf16 with a gate per row 131 and 236; 16383 x 4097 bf16, cut rows, 221 and 391;
-// 8192 x 8192 bf16 213 and 374; 3457 x 8118 float32, shared by blocks, 229 and 345.
+// wait for); 8192 x 5120 float32 150 and 269; 524288 x 96 bf16 with a gate per row 146 and 236; 16383 x 4097 bf16, cut rows, 221 and 391;
+// 8192 x 8192 bf16 215 and 376; 3457 x 8118 float32, shared by blocks, 229 and 345.
 #pragma once
 #include "ldn_sandwich.cuh"
 #include "ldn_rows.cuh"
@@ -25,11 +25,10 @@ constexpr int kBackwardStreams = G == Gate::All ? 5 : 4;
 constexpr int kMostRanks = 8;  // blocks of a cluster that share a row
 // Threads of a block of rows (of 320, the compiler has as many registers for each as of 384)
 __host__ __device__ constexpr int most_threads(int elements) { return elements <= 8 ? 640 : elements <= 16 ? 384 : 512; }
-// Rows that a block, or each of its groups, takes at a time forward; backward one (524288 x 96 bf16 with a gate per row, 1 / 2 / 4 rows of a
-// group: 172 / 145 / 131 us, backward 236 / 306; 1000000 x 17, cut rows: 107 / 111 / 141; 200000 x 40 f32: 45 / 43 / 49)
-__host__ __device__ constexpr int rows_forward(int elements, int size, bool group, bool shift) {
-    return group ? (elements <= 8 && size == 2 && !shift ? 4 : 2) : elements > 16 ? 1 : 2;
-}
+// Rows that a block, or each of its groups, takes at a time forward; backward one (524288 x 96 bf16 with a gate per row, 1 / 2 rows of a
+// group: 172 / 146 us, backward 236 / 306; 1000000 x 17, cut rows: 107 / 111; 200000 x 40 f32: 45 / 43, four 49; groups of one lane, 4000000 x 8
+// bf16 without a gate and with one per row, 2 / 4 rows: 57 / 63 and 142 / 138)
+__host__ __device__ constexpr int rows_forward(int elements) { return elements > 16 ? 1 : 2; }
 
 // scale weight and scale bias of a piece's columns (1 and 0 outside the row)
 template <class T, bool SHIFT>
