@@ -96,8 +96,9 @@ def gated_linear(x, weight_gate, weight_up, bias_gate=None, bias_up=None, activa
     with the gradients of all five.  activation: "silu", "gelu" (of the normal distribution's function), "sigmoid" or "relu".
 
     Weights are (outputs, terms) of the type of x, biases of that type or float32; sums have 32 bits.  Kept for the backward pass are both
-    projections in 32 bits and, of float32 operands, the 6 bytes per element that they are multiplied as.  Rows of 16-bit tensors that
-    start at multiples of 16 bytes are read where they lie, others are copied first; float32 is multiplied on the tensor cores as
+    projections in 32 bits and, of float32 operands, the 6 bytes per element that they are multiplied as.  The projections' gradients are
+    rounded to the type of x before the backward pass multiplies them.  Rows of 16-bit tensors that start at multiples of 16 bytes are
+    read where they lie; others, and rows that are repeated or overlap, are copied first.  float32 is multiplied on the tensor cores as
     three bfloat16 numbers (24 bits), where an infinity gives not-a-numbers."""
     if activation not in _GATES:
         raise ValueError(f"activation must be one of {sorted(_GATES)}, not {activation!r}")
