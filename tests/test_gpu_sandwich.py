@@ -244,3 +244,23 @@ def test_without_the_gradient_of_y_it_does_not_matter_what_h_is(C, layout, gate)
             else:
                 assert head_oracle.near(g, want[name][0].view_as(g), want[name][1].view_as(g)), name
         assert torch.equal(torch.autograd.grad(call(t, 0.0)[1], t["residual"], dh)[0], dh)
+
+
+@pytest.mark.parametrize("gate", ["none", "row", "all"])
+@pytest.mark.parametrize("rows, C, dtype", [(20003, 1001, F32), (40000, 1024, BF16), (9001, 5120, F16), (90000, 500, F32), (300000, 96, F32),
+                                            (5001, 9000, F32)])
+def test_without_the_gradient_of_y_of_many_rows(rows, C, dtype, gate):
+    """More rows than the zeros in h's place are for: they are taken some at a time, and have the gradients of a y that has none."""
+    t, _, dh = made(rows, C, dtype, gate, F32)
+    t = {k: v if v is None else v.detach().requires_grad_() for k, v in t.items()}
+    y, h = call(t)
+    leaves = {k: v for k, v in t.items() if v is not None}
+    alone = torch.autograd.grad(h, list(leaves.values()), dh, retain_graph=True)
+    exact = oracle.backward(None, dh, *[None if v is None else v.detach() for v in (t["x"], h, t["gate"], t["scale"], t["pw"], t["pb"], t["w"])], 1e-5)
+    for name, g in zip(leaves, alone):
+        want, bound = exact[name]
+        assert head_oracle.near(g, want.view_as(g), bound.view_as(g)), name
+    both = torch.autograd.grad((y, h), list(leaves.values()), (torch.zeros_like(y), dh))
+    for name, g, same in zip(leaves, alone, both):
+        if name in ("x", "residual", "gate"):
+            assert torch.equal(g, same), name
