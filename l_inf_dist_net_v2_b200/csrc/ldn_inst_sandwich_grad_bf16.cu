@@ -2,6 +2,6 @@
 
 namespace ldn {
 
-template int sandwich_grad_rows<__nv_bfloat16>(Gate, const SandwichGradArgs&, const DeviceCtx*, int*, const cudaStream_t*);
+template int sandwich_grad_rows<__nv_bfloat16, true>(Gate, const SandwichGradArgs&, const DeviceCtx*, int*, const cudaStream_t*);
 
 }  // namespace ldn

@@ -2,6 +2,6 @@
 
 namespace ldn {
 
-template int sandwich_grad_rows<__half>(Gate, const SandwichGradArgs&, const DeviceCtx*, int*, const cudaStream_t*);
+template int sandwich_grad_rows<__half, true>(Gate, const SandwichGradArgs&, const DeviceCtx*, int*, const cudaStream_t*);
 
 }  // namespace ldn

@@ -1,0 +1,7 @@
+#include "ldn_sandwich_grad.cuh"
+
+namespace ldn {
+
+template int sandwich_grad_rows<__nv_bfloat16, false>(Gate, const SandwichGradArgs&, const DeviceCtx*, int*, const cudaStream_t*);
+
+}  // namespace ldn

@@ -158,19 +158,6 @@ __global__ void __launch_bounds__(kColumns * kColumnLanes) sandwich_grad_columns
     }
 }
 
-// In place of h where only its own gradient comes: zeros, and statistics that are zeros beside those of x (two numbers per row, `apart`).  The
-// kernels with rows in registers multiply the gradient of y that does not come, zeros, with the normalised stream, which may be no
-// numbers.  (Asked for in those kernels, it moved their registers: 16383 x 4097 bf16 with both gradients 392 -> 447 us.)  Rows that fill half of
-// the second-level cache at a time, so that the zeros take no more memory and are read from there.
-constexpr long long kZeroBytes = 64 << 20;
-__global__ void __launch_bounds__(kRowThreads) no_stream_kernel(uint4* zeros, long long pieces, float* stats, const float* of_x, long long apart,
-                                                               long long rows) {
-    stream_order_begin();
-    const long long first = static_cast<long long>(blockIdx.x) * kRowThreads + threadIdx.x, step = static_cast<long long>(gridDim.x) * kRowThreads;
-    for (long long i = first; i < pieces; i += step) zeros[i] = make_uint4(0u, 0u, 0u, 0u);
-    for (long long i = first; i < 4 * rows; i += step) stats[i] = i < rows ? of_x[i] : i < 2 * rows ? of_x[apart + i - rows] : 0.0f;
-}
-
 struct FoldArgs {
     const float* parts;
     int count, C;
@@ -279,64 +266,26 @@ extern "C" LDN_API int ldn_sandwich_norm_backward(const void* grad_y, const void
     SandwichGradArgs a = {grad_y, grad_h, x, h, gate, pitch, pitch_gate, rows, C, f.p, stats, grad_x, grad_residual, grad_gate, nullptr, nullptr};
     const int columns = (C + kColumns - 1) / kColumns;
     const bool sums = grad_scale || grad_post_weight || grad_post_bias || grad_weight || grad_bias;
-    auto in_registers = [&](const SandwichGradArgs& of, int* blocks, const cudaStream_t* st) {
-        return with_type(type, [&](auto t) { return sandwich_grad_rows<decltype(t)>(kind, of, ctx, blocks, st); });
+    auto in_registers = [&](int* blocks, const cudaStream_t* st) {
+        return with_type(type, [&](auto t) {
+            using T = decltype(t);
+            return grad_y ? sandwich_grad_rows<T, true>(kind, a, ctx, blocks, st) : sandwich_grad_rows<T, false>(kind, a, ctx, blocks, st);
+        });
     };
-    const bool registers = in_registers(a, &f.count, nullptr) == kOk, no_stream = registers && !grad_y;
-    const long long size = size_of(type), fit = kZeroBytes / (size * C) / 8 * 8;  // (rows that far apart start alike)
-    const long long turn = !no_stream ? rows : rows < fit ? rows : fit > 8 ? fit : rows < 8 ? rows : 8;
-    if (turn < rows) {
-        SandwichGradArgs some = a;
-        int of_turn = 0, of_last = 0;
-        some.rows = turn;
-        if ((r = in_registers(some, &of_turn, nullptr)) != kOk) return r;
-        some.rows = rows % turn;
-        if (some.rows && (r = in_registers(some, &of_last, nullptr)) != kOk) return r;
-        f.count = static_cast<int>(rows / turn) * of_turn + of_last;
-    }
+    const bool registers = in_registers(&f.count, nullptr) == kOk;
     if (!registers) {
         const long long most = (4LL * ctx->sm_count + columns - 1) / columns, needed = (rows + 63) / 64;
         f.count = static_cast<int>(most < needed ? most : needed);
     }
     const size_t row_bytes = registers ? 0 : pad256(static_cast<size_t>(rows) * 2 * sizeof(float));
-    const size_t part_bytes = sums ? pad256(static_cast<size_t>(f.count) * 4 * C * sizeof(float)) : 0;
-    const size_t zero_bytes = no_stream ? pad256(static_cast<size_t>(turn) * C * size) : 0;
-    const size_t stat_bytes = no_stream ? static_cast<size_t>(turn) * 4 * sizeof(float) : 0;
+    const size_t part_bytes = sums ? static_cast<size_t>(f.count) * 4 * C * sizeof(float) : 0;
     Scratch scratch;
-    if (row_bytes + part_bytes + zero_bytes) {
-        if ((r = scratch.take(st, row_bytes + part_bytes + zero_bytes + stat_bytes)) != kOk) return r;
+    if (row_bytes + part_bytes) {
+        if ((r = scratch.take(st, row_bytes + part_bytes)) != kOk) return r;
         a.row_sums = reinterpret_cast<float*>(scratch.base);
         if (sums) f.parts = a.parts = reinterpret_cast<float*>(scratch.base + row_bytes);
     }
-    if (no_stream) {
-        char* zeros = scratch.base + row_bytes + part_bytes;
-        float* of_both = reinterpret_cast<float*>(zeros + zero_bytes);
-        const long long pieces = static_cast<long long>(zero_bytes / 16), needed = (pieces + kRowThreads - 1) / kRowThreads, most = 16LL * ctx->sm_count;
-        const long long of_gate = kind == Gate::All ? C : 1;
-        auto moved = [&](auto*& p, long long elements) {
-            if (p) p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(reinterpret_cast<uintptr_t>(p) + elements * size);
-        };
-        SandwichGradArgs some = a;
-        some.h = zeros;
-        some.stats = of_both;
-        for (long long row = 0; row < rows; row += turn) {
-            some.rows = rows - row < turn ? rows - row : turn;
-            r = launch_after(no_stream_kernel, static_cast<unsigned>(needed < most ? needed : most), kRowThreads, 0, st, reinterpret_cast<uint4*>(zeros),
-                             row ? 0 : pieces, of_both, stats + row, rows, some.rows);
-            int blocks = 0;
-            if (r == kOk) r = in_registers(some, &blocks, &st);
-            if (r != kOk) return r;
-            if (some.parts) some.parts += static_cast<long long>(blocks) * 4 * C;
-            moved(some.x, turn * pitch);
-            moved(some.gate, turn * (kind == Gate::All ? pitch_gate : 1));
-            moved(some.grad_h, turn * C);
-            moved(some.grad_x, turn * C);
-            moved(some.grad_residual, turn * C);
-            moved(some.grad_gate, turn * of_gate);
-        }
-    } else if (registers && (r = in_registers(a, nullptr, &st)) != kOk) {
-        return r;
-    }
+    if (registers && (r = in_registers(nullptr, &st)) != kOk) return r;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         int s = kOk;

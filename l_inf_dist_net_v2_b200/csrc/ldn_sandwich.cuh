@@ -40,8 +40,8 @@ struct SandwichGradArgs {
 // Rows of T held in registers (ldn_sandwich_forward.cuh, ldn_sandwich_grad.cuh).  False: these rows do not fit, or their tensors' pieces do not match
 template <class T>
 bool sandwich_rows(Gate gate, const SandwichArgs& a, const DeviceCtx* ctx, cudaStream_t st, int* status);
-// kOk: they do; blocks: how many parts of column sums they make, where not null; st: their launch, where not null
-template <class T>
+// kOk: they do; blocks: how many parts of column sums they make, where not null; st: their launch, where not null.  OF_Y: grad_y is not null
+template <class T, bool OF_Y>
 int sandwich_grad_rows(Gate gate, const SandwichGradArgs& a, const DeviceCtx* ctx, int* blocks, const cudaStream_t* st);
 
 #ifdef __CUDACC__

@@ -10,12 +10,14 @@ __device__ __forceinline__ float at_of(const float2 (&v)[N], int e) {
     return e % 2 ? v[e / 2].y : v[e / 2].x;
 }
 
-template <class T, Gate G, int ITEMS, Share W, bool SHIFT>
+// OF_Y: a gradient of y comes; without it neither h nor its statistics are read (what they are does not matter then, infinities neither)
+template <class T, Gate G, int ITEMS, Share W, bool SHIFT, bool OF_Y>
 __global__ void __launch_bounds__(W == Share::Group ? kGroupThreads : most_threads(ITEMS * kPiece<T>), 1)
 sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int lanes, int depth, int ranks) {
     stream_order_begin();
     constexpr bool GROUP = W == Share::Group;
-    constexpr int V = kPiece<T>, S = kBackwardStreams<G>, R = 1;
+    constexpr int V = kPiece<T>, S = kBackwardStreams<G, OF_Y>, R = 1;
+    constexpr int kOfH = 1, kOfDy = 2, kOfDh = OF_Y ? 3 : 1, kOfGate = OF_Y ? 4 : 2;  // streams' numbers (x has 0)
     constexpr int K = G == Gate::Row ? 4 : 2;  // sums of a row in the second round (a power of two)
     __shared__ alignas(16) float slots[2 * SumOf<W>::kSlots];
     extern __shared__ uint4 ring[];  // [depth][row][stream][item][thread], then blocks: [3][item][V / 4][thread]; at the end, groups: [warp][4][C] floats
@@ -92,18 +94,23 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
 #pragma unroll
                 for (int i = 0; i < ITEMS; ++i) {
                     copy_piece<T, SHIFT>(slot_of(stage, j, 0, i), from_x.of(j, i * apart), column(i), bytes[i], a.x);
-                    copy_piece<T, SHIFT>(slot_of(stage, j, 1, i), from_h.of(j, i * apart), column(i), bytes[i], a.h);
-                    if (a.grad_y) copy_piece<T, SHIFT>(slot_of(stage, j, 2, i), from_dy.of(j, i * apart), column(i), bytes[i], a.grad_y);
-                    if (a.grad_h) copy_piece<T, SHIFT>(slot_of(stage, j, 3, i), from_dh.of(j, i * apart), column(i), bytes[i], a.grad_h);
+                    if constexpr (OF_Y) {
+                        copy_piece<T, SHIFT>(slot_of(stage, j, kOfH, i), from_h.of(j, i * apart), column(i), bytes[i], a.h);
+                        // (asked for although it comes: the compiler's order without is slower, 9999 x 1001 f16 87 us instead of 81)
+                        if (a.grad_y) copy_piece<T, SHIFT>(slot_of(stage, j, kOfDy, i), from_dy.of(j, i * apart), column(i), bytes[i], a.grad_y);
+                    }
+                    if (a.grad_h) copy_piece<T, SHIFT>(slot_of(stage, j, kOfDh, i), from_dh.of(j, i * apart), column(i), bytes[i], a.grad_h);
                     if constexpr (G == Gate::All)
-                        copy_piece<T, SHIFT>(slot_of(stage, j, 4, i), from_gate.of(j, i * apart), column(i), bytes[i], a.gate);
+                        copy_piece<T, SHIFT>(slot_of(stage, j, kOfGate, i), from_gate.of(j, i * apart), column(i), bytes[i], a.gate);
                 }
             }
         copies_commit();
         to_fetch -= R;
         from_x.on(R);
-        from_h.on(R);
-        from_dy.on(R);
+        if constexpr (OF_Y) {
+            from_h.on(R);
+            from_dy.on(R);
+        }
         from_dh.on(R);
         if constexpr (G == Gate::All) from_gate.on(R);
     };
@@ -111,9 +118,9 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
     for (int d = 0; d < depth * R * S; ++d)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
-            if (!bytes[i] || (!a.grad_y && d % S == 2) || (!a.grad_h && d % S == 3)) own[(d * ITEMS + i) * blockDim.x] = make_uint4(0u, 0u, 0u, 0u);
+            if (!bytes[i] || (OF_Y && !a.grad_y && d % S == kOfDy) || (!a.grad_h && d % S == kOfDh)) own[(d * ITEMS + i) * blockDim.x] = make_uint4(0u, 0u, 0u, 0u);
     for (int d = 0; d < depth; ++d) fetch(d);
-    constexpr int kNumbers = G == Gate::Row ? 5 : 4;
+    constexpr int kStats = OF_Y ? 4 : 2, kNumbers = G == Gate::Row ? kStats + 1 : kStats;
     __shared__ float numbers[kNumbers][kNumberRows];
     int stage = 0;
     const long long block_first = static_cast<long long>(block) * per_block;
@@ -124,15 +131,15 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
         float mean1[R], rstd1[R], mean2[R], rstd2[R], gate[R], s[2 * R], t[K * R];
         RowNumbers<kNumbers, R * kNumberRows> of_rows(numbers, R * per_block);
         of_rows.at_turn(turn, a.rows, [&](int i) { return row_of(turn, i); }, [&](int k, long long row) {
-            return k < 4 ? a.stats[k * a.rows + row] : to_float(static_cast<const T*>(a.gate)[row]);
+            return k < kStats ? a.stats[k * a.rows + row] : to_float(static_cast<const T*>(a.gate)[row]);
         });
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             const int index = j * per_block + (GROUP ? threadIdx.x / lanes : 0);
             mean1[j] = of_rows.of(0, turn, index);
             rstd1[j] = of_rows.of(1, turn, index);
-            mean2[j] = of_rows.of(2, turn, index);
-            rstd2[j] = of_rows.of(3, turn, index);
+            mean2[j] = OF_Y ? of_rows.of(2, turn, index) : 0.0f;
+            rstd2[j] = OF_Y ? of_rows.of(3, turn, index) : 0.0f;
             gate[j] = G == Gate::Row ? of_rows.of(kNumbers - 1, turn, index) : 1.0f;
         }
         copies_wait(depth);
@@ -141,50 +148,54 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
             const uint4 raw = live(j) ? *slot_of(stage, j, stream, i) : make_uint4(0u, 0u, 0u, 0u);
             unpack<T>(SHIFT ? masked(raw, mask[i]) : raw, v);
         };
+        if constexpr (OF_Y) {
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            float2 s0 = both(0.0f), s1 = both(0.0f);
+            for (int j = 0; j < R; ++j) {
+                float2 s0 = both(0.0f), s1 = both(0.0f);
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) {
-                float2 h[V / 2], dy[V / 2], w2[V / 2];
-                piece_of(j, 1, i, h);
-                piece_of(j, 2, i, dy);
-                param_piece(2, i, w2);
+                for (int i = 0; i < ITEMS; ++i) {
+                    float2 h[V / 2], dy[V / 2], w2[V / 2];
+                    piece_of(j, kOfH, i, h);
+                    piece_of(j, kOfDy, i, dy);
+                    param_piece(2, i, w2);
 #pragma unroll
-                for (int e = 0; e < V / 2; ++e) {
-                    // (rstd behind the sum: outside the row the gradient is 0 and h - mean a number, but (0 - mean) rstd may be infinite)
-                    const float2 u = __fmul2_rn(dy[e], __fadd2_rn(h[e], both(-mean2[j])));
-                    sums[0][i][e] = __ffma2_rn(u, both(rstd2[j]), sums[0][i][e]);
-                    sums[1][i][e] = __fadd2_rn(sums[1][i][e], dy[e]);
-                    s0 = __ffma2_rn(dy[e], w2[e], s0);
-                    s1 = __ffma2_rn(u, w2[e], s1);
+                    for (int e = 0; e < V / 2; ++e) {
+                        // (rstd behind the sum: outside the row the gradient is 0 and h - mean a number, but (0 - mean) rstd may be infinite)
+                        const float2 u = __fmul2_rn(dy[e], __fadd2_rn(h[e], both(-mean2[j])));
+                        sums[0][i][e] = __ffma2_rn(u, both(rstd2[j]), sums[0][i][e]);
+                        sums[1][i][e] = __fadd2_rn(sums[1][i][e], dy[e]);
+                        s0 = __ffma2_rn(dy[e], w2[e], s0);
+                        s1 = __ffma2_rn(u, w2[e], s1);
+                    }
                 }
+                s[2 * j] = s0.x + s0.y;
+                s[2 * j + 1] = s1.x + s1.y;
             }
-            s[2 * j] = s0.x + s0.y;
-            s[2 * j + 1] = s1.x + s1.y;
+            reduce(s, [&](float all) { return all * inv_C; });
         }
-        reduce(s, [&](float all) { return all * inv_C; });
         float2 by[R][ITEMS][V / 2];  // what goes into the first norm's gradient
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             float2 t0 = both(0.0f), t1 = both(0.0f), tg = both(0.0f);
-            const float m1 = s[2 * j], m2 = s[2 * j + 1] * rstd2[j] * rstd2[j];
+            const float m1 = OF_Y ? s[2 * j] : 0.0f, m2 = OF_Y ? s[2 * j + 1] * rstd2[j] * rstd2[j] : 0.0f;
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
                 const int c = column(i);
                 float2 d[V / 2], h[V / 2], x[V / 2], n[V / 2], w[V / 2];
-                piece_of(j, 1, i, h);
-                piece_of(j, 2, i, d);
-                param_piece(2, i, w);
+                if constexpr (OF_Y) {
+                    piece_of(j, kOfH, i, h);
+                    piece_of(j, kOfDy, i, d);
+                    param_piece(2, i, w);
 #pragma unroll
-                for (int e = 0; e < V / 2; ++e)
-                    d[e] = __ffma2_rn(__fadd2_rn(h[e], both(-mean2[j])), both(-m2), __ffma2_rn(d[e], w[e], both(-m1)));
-                piece_of(j, 3, i, h);
+                    for (int e = 0; e < V / 2; ++e)
+                        d[e] = __ffma2_rn(__fadd2_rn(h[e], both(-mean2[j])), both(-m2), __ffma2_rn(d[e], w[e], both(-m1)));
+                }
+                piece_of(j, kOfDh, i, h);
                 piece_of(j, 0, i, x);
                 param_piece(0, i, w);
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e) {
-                    d[e] = __ffma2_rn(d[e], both(rstd2[j]), h[e]);
+                    d[e] = OF_Y ? __ffma2_rn(d[e], both(rstd2[j]), h[e]) : h[e];
                     x[e] = __fadd2_rn(x[e], both(-mean1[j]));  // (rstd behind the sums, as above)
                 }
                 if (live(j) && a.grad_residual) store_piece<T, SHIFT>(to_onto.of(j, i * apart), c, a.C, pack<T>(d));
@@ -196,7 +207,7 @@ sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int l
                 if constexpr (G == Gate::All) {
                     if (live(j) && a.grad_gate) store_piece<T, SHIFT>(to_gate.of(j, i * apart), c, a.C, pack<T>(n));
                     float2 g[V / 2];
-                    piece_of(j, 4, i, g);
+                    piece_of(j, kOfGate, i, g);
 #pragma unroll
                     for (int e = 0; e < V / 2; ++e) d[e] = __fmul2_rn(d[e], g[e]);
                 } else if constexpr (G == Gate::Row) {
@@ -316,7 +327,7 @@ bool plan_backward(Gate gate, const SandwichGradArgs& a, int size, RowPlan* p, S
     return match && plan_row(a.C, size, shift, false, p, who, ranks);
 }
 // The backward kernel for these rows, with its shape: f(kernel, shape); kBadArgument where there is none
-template <class T, class F>
+template <class T, bool OF_Y, class F>
 int with_backward(Gate gate, const SandwichGradArgs& a, const DeviceCtx* ctx, F f) {
     RowPlan p;
     Share who;
@@ -327,13 +338,13 @@ int with_backward(Gate gate, const SandwichGradArgs& a, const DeviceCtx* ctx, F 
             constexpr Gate G = decltype(g)::value;
             constexpr int kItems = decltype(items)::value;
             constexpr Share W = decltype(share)::value;
-            constexpr auto kernel = sandwich_grad_registers_kernel<T, G, kItems, W, decltype(shift)::value>;
+            constexpr auto kernel = sandwich_grad_registers_kernel<T, G, kItems, W, decltype(shift)::value, OF_Y>;
             const long long params = W == Share::Group ? 0 : 3LL * kItems * (kPiece<T> / 4) * p.threads * 16;
             long long resident;
             int depth;
             RowShape s;
-            if (!resident_rows<kernel, W>(p, 1, kBackwardStreams<G>, params, ranks, ctx, &resident, &depth) ||
-                !shape_of(p, a.rows, 1, kBackwardStreams<G>, params, ranks, resident, depth, &s))
+            if (!resident_rows<kernel, W>(p, 1, kBackwardStreams<G, OF_Y>, params, ranks, ctx, &resident, &depth) ||
+                !shape_of(p, a.rows, 1, kBackwardStreams<G, OF_Y>, params, ranks, resident, depth, &s))
                 return static_cast<int>(kBadArgument);
             if constexpr (W == Share::Group) {
                 const size_t columns = static_cast<size_t>(kGroupThreads / 32) * 4 * a.C * sizeof(float);
@@ -346,9 +357,9 @@ int with_backward(Gate gate, const SandwichGradArgs& a, const DeviceCtx* ctx, F 
 
 }  // namespace
 
-template <class T>
+template <class T, bool OF_Y>
 int sandwich_grad_rows(Gate gate, const SandwichGradArgs& a, const DeviceCtx* ctx, int* blocks, const cudaStream_t* st) {
-    return with_backward<T>(gate, a, ctx, [&](auto kernel, const RowShape& s) {
+    return with_backward<T, OF_Y>(gate, a, ctx, [&](auto kernel, const RowShape& s) {
         if (blocks) *blocks = s.blocks;
         if (!st) return static_cast<int>(kOk);
         return launch_after_in_clusters(kernel, s.ranks, s.blocks * s.ranks, s.p.threads, s.smem, *st, a, s.p.lanes, s.depth, s.ranks);

@@ -20,8 +20,8 @@ namespace {
 
 template <Gate G>
 constexpr int kForwardStreams = G == Gate::All ? 3 : 2;
-template <Gate G>
-constexpr int kBackwardStreams = G == Gate::All ? 5 : 4;
+template <Gate G, bool OF_Y>
+constexpr int kBackwardStreams = (G == Gate::All ? 5 : 4) - (OF_Y ? 0 : 2);
 constexpr int kMostRanks = 8;  // blocks of a cluster that share a row
 // Threads of a block of rows (of 320, the compiler has as many registers for each as of 384)
 __host__ __device__ constexpr int most_threads(int elements) { return elements <= 8 ? 640 : elements <= 16 ? 384 : 512; }

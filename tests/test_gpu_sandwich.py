@@ -250,7 +250,7 @@ def test_without_the_gradient_of_y_it_does_not_matter_what_h_is(C, layout, gate)
 @pytest.mark.parametrize("rows, C, dtype", [(20003, 1001, F32), (40000, 1024, BF16), (9001, 5120, F16), (90000, 500, F32), (300000, 96, F32),
                                             (5001, 9000, F32)])
 def test_without_the_gradient_of_y_of_many_rows(rows, C, dtype, gate):
-    """More rows than the zeros in h's place are for: they are taken some at a time, and have the gradients of a y that has none."""
+    """They have the gradients of a y whose gradient is zero."""
     t, _, dh = made(rows, C, dtype, gate, F32)
     t = {k: v if v is None else v.detach().requires_grad_() for k, v in t.items()}
     y, h = call(t)
