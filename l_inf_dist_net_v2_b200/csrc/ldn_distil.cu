@@ -30,7 +30,7 @@ struct DistilArgs {
     const long long* targets;  // [rows], may be null
     float tau, part, mix;
     float* losses;  // [rows]
-    float* stats;   // [5][rows]: largest logit, 1 / sums at tau and at 1, the list's largest value / tau, 1 / its sum
+    float* stats;   // [5][rows]: largest logit, 1 / sums at tau and at 1, the list's largest value, 1 / its sum
     // backward
     const float* up;
     int up_step;      // 0: one number for all rows
@@ -184,7 +184,7 @@ struct Largest {
     __device__ __forceinline__ float operator()(float a, float b) const { return largest_of(a, b); }
 };
 
-// What of a row's loss does not wait for its sums: with t = value / tau - top, p = e^t / sum, and the largest of the list's logits as reference,
+// What of a row's loss does not wait for its sums: with t = (value - top) / tau (values may be the type's lowest), p = e^t / sum, and the largest of the list's logits as reference,
 // terms = sum p (t - log sum - (x - reference) / tau)
 struct List {
     float top, inv_sum, terms, reference, target;
@@ -206,7 +206,7 @@ __device__ __forceinline__ List read_list(const DistilArgs& a, long long row, fl
     for (int e = 0; e < kHeld; ++e) {
         const int j = lane + e * LANES;
         index[e] = j < a.k ? indices[j] : -1;
-        v[e] = j < a.k ? value_at(a, row * a.k + j) * inv_tau : 0.0f;
+        v[e] = j < a.k ? value_at(a, row * a.k + j) : 0.0f;
     }
 #pragma unroll
     for (int e = 0; e < kHeld; ++e) {
@@ -225,7 +225,7 @@ __device__ __forceinline__ List read_list(const DistilArgs& a, long long row, fl
     for (int j = lane + kHeld * LANES; j < a.k; j += LANES) {
         const long long i = indices[j];
         if (i >= a.V) bad = 1.0f;
-        if (i >= 0) top = largest_of(top, value_at(a, row * a.k + j) * inv_tau);
+        if (i >= 0) top = largest_of(top, value_at(a, row * a.k + j));
         if (i >= 0 && i < a.V) reference = largest_of(reference, to_float(x[i]));
     }
     l.bad = over_row<LANES>(bad, Largest(), slots) != 0.0f;
@@ -236,15 +236,15 @@ __device__ __forceinline__ List read_list(const DistilArgs& a, long long row, fl
     if (l.some) {
 #pragma unroll
         for (int e = 0; e < kHeld; ++e)
-            if (there[e]) sum += expf(v[e] - top);
+            if (there[e]) sum += expf((v[e] - top) * inv_tau);
         for (int j = lane + kHeld * LANES; j < a.k; j += LANES)
-            if (indices[j] >= 0) sum += expf(value_at(a, row * a.k + j) * inv_tau - top);
+            if (indices[j] >= 0) sum += expf((value_at(a, row * a.k + j) - top) * inv_tau);
     }
     sum = over_row<LANES>(sum, Plus(), slots + 3 * kWarps);
     l.inv_sum = 1.0f / sum;
     const float log_sum = logf(sum);
     auto term = [&](float value, float logit) {
-        const float t = value - top, p = expf(t) * l.inv_sum;
+        const float t = (value - top) * inv_tau, p = expf(t) * l.inv_sum;
         return p != 0.0f ? p * ((t - log_sum) - (logit - reference) * inv_tau) : 0.0f;
     };
     float terms = 0.0f;
@@ -253,7 +253,7 @@ __device__ __forceinline__ List read_list(const DistilArgs& a, long long row, fl
         for (int e = 0; e < kHeld; ++e)
             if (there[e]) terms += term(v[e], at[e]);
         for (int j = lane + kHeld * LANES; j < a.k; j += LANES)
-            if (indices[j] >= 0) terms += term(value_at(a, row * a.k + j) * inv_tau, to_float(x[indices[j]]));
+            if (indices[j] >= 0) terms += term(value_at(a, row * a.k + j), to_float(x[indices[j]]));
     }
     l.terms = over_row<LANES>(terms, Plus(), slots + 4 * kWarps);
     return l;
@@ -592,7 +592,7 @@ __device__ __forceinline__ void gradient_of_row(const DistilArgs& a, long long r
     for (int j = thread; j < room; j += THREADS) {
         const long long i = j < a.k ? a.indices[row * a.k + j] : j == a.k ? target : -1;
         index[j] = i >= 0 && i < a.V ? static_cast<int>(i) : -1;
-        minus[j] = j == a.k ? by_label : j < a.k && i >= 0 && list ? by_list * (expf(value_at(a, row * a.k + j) * inv_tau - top) * inv_sum) : 0.0f;
+        minus[j] = j == a.k ? by_label : j < a.k && i >= 0 && list ? by_list * (expf((value_at(a, row * a.k + j) - top) * inv_tau) * inv_sum) : 0.0f;
     }
     if (!there) last_piece = first;
     const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(to)) & 15u) == 0;

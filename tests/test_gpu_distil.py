@@ -274,3 +274,21 @@ def test_entries_of_one_class_against_their_dense_sum(V):
     assert head_oracle.near(losses.detach(), want, bound)
     assert head_oracle.near(dx, up.double()[:, None] * tau * (log_q.exp() - P), off)
     assert abs(losses[0] + tau ** 2 * math.log(2)) <= 2.0 ** -20 and losses[0] < 0
+
+
+@pytest.mark.parametrize("rows, V", [(6, 12), (6, 5003), (700, 8193)])
+def test_a_teacher_of_the_lowest_values_and_at_low_temperatures(rows, V):
+    """p depends on the values' differences alone: rows of the type's lowest value are rows of equal ones at any temperature, and what the largest
+    is does not cost digits (its difference from the others is exact here, and rounds once as it is divided)."""
+    x, values, indices, _, up = made(rows, V, 5, F32)
+    for tau in (0.5, 0.25, 2.0 ** -10):
+        teachers = [torch.full_like(values, torch.finfo(F32).min), torch.full_like(values, torch.finfo(F32).max),
+                    4096.0 + torch.arange(5, device="cuda").mul(-2.0 ** -11).expand_as(values)]
+        alike = [torch.zeros_like(values), torch.zeros_like(values), teachers[2] - 4096.0]
+        for teacher, same in zip(teachers, alike):
+            leaf = x.detach().requires_grad_()
+            losses = ldn.distillation_loss(leaf, teacher, indices, temperature=tau, reduction="none")
+            want, bound, dx, off = oracle.loss_and_gradient(x, same, indices, None, tau, 0.0, up)
+            assert head_oracle.near(losses.detach(), want, bound)
+            # (a power below 2^-126, the smallest normal number, is 0: q is off by that much, and the gradient by up tau times it)
+            assert head_oracle.near(torch.autograd.grad(losses, leaf, up)[0], dx, off + 2.0 ** -126 * tau * up.double().abs()[:, None])
