@@ -10,7 +10,8 @@ __device__ __forceinline__ float at_of(const float2 (&v)[N], int e) {
     return e % 2 ? v[e / 2].y : v[e / 2].x;
 }
 
-// OF_Y: a gradient of y comes; without it neither h nor its statistics are read (what they are does not matter then, infinities neither)
+// OF_Y: a gradient of y comes; without it neither h nor its statistics are read (what they are does not matter then, infinities neither): one round
+// of sums and two streams fewer, 16384 x 5120 bf16 with a gate of its shape 175 us where both gradients take 287.
 template <class T, Gate G, int ITEMS, Share W, bool SHIFT, bool OF_Y>
 __global__ void __launch_bounds__(W == Share::Group ? kGroupThreads : most_threads(ITEMS * kPiece<T>), 1)
 sandwich_grad_registers_kernel(const __grid_constant__ SandwichGradArgs a, int lanes, int depth, int ranks) {
